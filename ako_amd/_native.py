@@ -31,7 +31,25 @@ AKO_ERR_HIP = 3
 AKO_ERR_NO_DEVICE = 4
 
 DTYPE_CODES: dict[torch.dtype, int] = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+#: Page types beyond the rows' own: e4m3 with scale codes.
+E4M3_CODE = 3
 ROPE_STYLE_CODES = {"neox": 0, "interleaved": 1}
+
+
+class PagedCache(ctypes.Structure):
+    """``ako_paged_t`` of the header."""
+
+    _fields_ = [
+        ("k_pages", ctypes.c_void_p), ("v_pages", ctypes.c_void_p),
+        ("k_scales", ctypes.c_void_p), ("v_scales", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p), ("seq_lens", ctypes.c_void_p), ("cu_seqlens", ctypes.c_void_p),
+        ("k_strides", ctypes.c_int64 * 3), ("v_strides", ctypes.c_int64 * 3),
+        ("k_scale_strides", ctypes.c_int64 * 3), ("v_scale_strides", ctypes.c_int64 * 3),
+        ("num_pages", ctypes.c_int64), ("kv_heads", ctypes.c_int64), ("page_size", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64), ("n_seqs", ctypes.c_int64), ("table_width", ctypes.c_int64),
+        ("table_stride", ctypes.c_int64), ("tokens", ctypes.c_int64), ("page_dtype", ctypes.c_int32),
+    ]
+
 
 #: Every symbol the header declares, with its (restype, argtypes).
 _i64, _int, _ptr, _f32 = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_float
@@ -68,6 +86,15 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
          _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _int, _int, _int, _ptr],
     ),
     "ako_swiglu_fwd": (_int, [_ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _int, _ptr]),
+    "ako_rope_qk_paged_fwd": (
+        _int,
+        [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _ptr, _ptr, _ptr, _i64, _i64, _int, _int, _int, _ptr],
+    ),
+    "ako_paged_read_fwd": (_int, [_ptr, _ptr, _ptr, _int, _ptr]),
+    "ako_paged_attention_fwd": (
+        _int, [_ptr, _ptr, _ptr, _ptr, _i64, _f32, _i64, _i64, _ptr, _i64, _int, _ptr],
+    ),
+    "ako_paged_attention_workspace": (_i64, [_ptr, _i64, _int]),
     "ako_set_tuning": (_int, [_int, _int, _int]),
     "ako_time_next_launch": (_int, [_ptr, _ptr]),
 }

@@ -13,6 +13,7 @@
 #include <string>
 
 #include "ako_hip.h"
+#include "common.h"
 #include "launch.h"
 
 namespace {
@@ -557,6 +558,315 @@ int ako_swiglu_fwd(const void* gate, const void* up, void* y, int64_t rows, int6
   const bool contiguous = rows == 1 || (gate_row_stride == n && up_row_stride == n && y_row_stride == n);
   ako::SwigluArgs a{gate, up, y, rows, n, gate_row_stride, up_row_stride, y_row_stride, dtype, contiguous};
   return hip_status(ako::launch_swiglu(a, static_cast<hipStream_t>(stream)), fn);
+}
+
+// ------------------------------------------------- paged key/value cache --
+extern "C++" {
+namespace {
+
+// Positions are 32-bit, with room for a tile past the last one.
+constexpr int64_t kMaxPositions = kMaxInt - 65536;
+
+bool valid_page_dtype(int page_dtype, int dtype) { return page_dtype == dtype || page_dtype == AKO_DTYPE_E4M3; }
+
+// Checks what every call over a paged cache needs and fills the launchers'
+// arguments. `empty` is set when there are no rows: the call is then done.
+int paged_common(const char* fn, const ako_paged_t* c, int64_t heads, int dtype, ako::PagedArgs* out, bool* empty) {
+  if (!c) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: null cache", fn);
+  if (!valid_dtype(dtype)) return fail(AKO_ERR_UNSUPPORTED, "%s: unknown dtype code %d", fn, dtype);
+  if (!valid_page_dtype(c->page_dtype, dtype))
+    return fail(AKO_ERR_UNSUPPORTED, "%s: pages of dtype code %d for rows of %s", fn, c->page_dtype, dtype_name(dtype));
+  if (c->num_pages < 0 || c->n_seqs < 0 || c->table_width < 0 || c->tokens < 0 || heads < 0)
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: negative size", fn);
+  if (c->head_dim < 16 || c->head_dim > 256 || c->head_dim % 16)
+    return fail(AKO_ERR_UNSUPPORTED, "%s: head_dim must be a multiple of 16 up to 256, got %lld", fn, (long long)c->head_dim);
+  if (c->kv_heads < 1 || c->page_size < 1)
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: kv_heads and page_size must be at least 1", fn);
+  if (c->page_size > kMaxPositions || c->table_width > kMaxPositions / c->page_size)
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: the block table names 2^31-65537 positions or more", fn);
+  if (c->kv_heads > kMaxInt / 1024 || heads > kMaxInt / 1024 || c->num_pages > kMaxInt || c->n_seqs > kMaxInt / 2 ||
+      c->tokens > kMaxInt / 2 / std::max<int64_t>(1, std::max(heads, c->kv_heads)))
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: too many heads, pages, sequences or rows", fn);
+  if (!c->cu_seqlens && c->tokens > 0 && (c->n_seqs == 0 || c->tokens % c->n_seqs))
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: %lld rows are no multiple of %lld sequences", fn, (long long)c->tokens,
+                (long long)c->n_seqs);
+  *empty = c->tokens == 0;
+  const bool mx = c->page_dtype == AKO_DTYPE_E4M3;
+  for (int i = 0; i < 3; ++i)
+    if (c->k_strides[i] < 0 || c->v_strides[i] < 0 || (mx && (c->k_scale_strides[i] < 0 || c->v_scale_strides[i] < 0)))
+      return fail(AKO_ERR_INVALID_ARGUMENT, "%s: negative page stride", fn);
+  if (c->table_stride < 0 || (c->table_stride < c->table_width && c->n_seqs > 1))
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: block table rows overlap", fn);
+  if (*empty) return AKO_OK;
+  if (c->num_pages > 0 && (!c->k_pages || !c->v_pages || (mx && (!c->k_scales || !c->v_scales))))
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: null pages or scales", fn);
+  if (!mx && (c->k_scales || c->v_scales))
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: scales are for e4m3 pages", fn);
+  if (c->n_seqs > 0 && (!c->seq_lens || (c->table_width > 0 && !c->block_table)))
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: null block table or lengths", fn);
+  ako::PagedArgs& a = *out;
+  a.k = c->k_pages;
+  a.v = c->v_pages;
+  a.ks = c->k_scales;
+  a.vs = c->v_scales;
+  a.mx = mx;
+  a.table = c->block_table;
+  a.lens = c->seq_lens;
+  a.cu = c->cu_seqlens;
+  for (int i = 0; i < 3; ++i) {
+    a.kst[i] = c->k_strides[i];
+    a.vst[i] = c->v_strides[i];
+    a.ksst[i] = mx ? c->k_scale_strides[i] : 0;
+    a.vsst[i] = mx ? c->v_scale_strides[i] : 0;
+  }
+  a.table_stride = c->table_stride;
+  a.table_width = c->table_width;
+  a.n_seqs = c->n_seqs;
+  a.num_pages = c->num_pages;
+  a.kv_heads = c->kv_heads;
+  a.page_size = c->page_size;
+  a.head_dim = c->head_dim;
+  a.tokens = c->tokens;
+  return AKO_OK;
+}
+
+// The memory a cache call reads or writes: pages and scales, then the step's
+// own index tensors.
+struct PagedSpans {
+  Span pages[4], index[3];
+  int n_pages = 0, n_index = 0;
+  bool ok = true;
+
+  PagedSpans(const ako_paged_t* c, int dtype) {
+    const bool mx = c->page_dtype == AKO_DTYPE_E4M3;
+    const int eb = mx ? 1 : ako::dtype_bytes(dtype);
+    const int64_t codes = ako::ceil_div(c->head_dim, 32);
+    if (c->num_pages > 0) {
+      add(span_4d(c->k_pages, c->num_pages, c->kv_heads, c->page_size, c->head_dim, c->k_strides, eb));
+      add(span_4d(c->v_pages, c->num_pages, c->kv_heads, c->page_size, c->head_dim, c->v_strides, eb));
+      if (mx) {
+        add(span_4d(c->k_scales, c->num_pages, c->kv_heads, c->page_size, codes, c->k_scale_strides, 1));
+        add(span_4d(c->v_scales, c->num_pages, c->kv_heads, c->page_size, codes, c->v_scale_strides, 1));
+      }
+    }
+    if (c->n_seqs > 0) {
+      if (c->table_width > 0) add_index(span_2d(c->block_table, c->n_seqs, c->table_width, c->table_stride, 4));
+      add_index(span_2d(c->seq_lens, 1, c->n_seqs, c->n_seqs, 4));
+    }
+    if (c->cu_seqlens) add_index(span_2d(c->cu_seqlens, 1, c->n_seqs + 1, c->n_seqs + 1, 4));
+  }
+  bool meets(const Span& s) const {
+    for (int i = 0; i < n_pages; ++i)
+      if (overlap(pages[i], s)) return true;
+    return meets_index(s);
+  }
+  bool meets_index(const Span& s) const {
+    for (int i = 0; i < n_index; ++i)
+      if (overlap(index[i], s)) return true;
+    return false;
+  }
+
+ private:
+  void add(const Span& s) {
+    ok = ok && s.ok;
+    pages[n_pages++] = s;
+  }
+  void add_index(const Span& s) {
+    ok = ok && s.ok;
+    index[n_index++] = s;
+  }
+};
+
+// Whether rows of `width` bytes at a and at b (same shape and strides, in
+// bytes) never share a byte: apart altogether, or interleaved in one
+// allocation with every row of one between rows of the other.
+bool rows_apart(const Span& sa, const Span& sb, int64_t n0, int64_t n1, int64_t n2, int64_t width, const int64_t* st_a,
+                const int64_t* st_b, int eb) {
+  if (!overlap(sa, sb)) return true;
+  for (int i = 0; i < 3; ++i)
+    if (st_a[i] != st_b[i]) return false;
+  const uint64_t gap = sa.lo < sb.lo ? sb.lo - sa.lo : sa.lo - sb.lo;
+  struct Dim { __int128 stride; int64_t count; } dims[4] = {
+      {__int128(st_a[0]) * eb, n0}, {__int128(st_a[1]) * eb, n1}, {__int128(st_a[2]) * eb, n2}, {__int128(gap), 2}};
+  for (int i = 0; i < 4; ++i)
+    for (int j = i + 1; j < 4; ++j)
+      if (dims[j].stride < dims[i].stride) std::swap(dims[i], dims[j]);
+  __int128 reach = __int128(width) * eb;
+  for (const Dim& d : dims) {
+    if (d.count <= 1) continue;
+    if (d.stride < reach) return false;
+    reach += d.stride * (d.count - 1);
+  }
+  return true;
+}
+
+}  // namespace
+}  // extern "C++"
+
+int ako_rope_qk_paged_fwd(const void* q, const void* k, const void* v, const void* cos_table, const void* sin_table,
+                          void* q_out, const ako_paged_t* cache, int64_t q_heads, const int64_t* q_strides,
+                          const int64_t* k_strides, const int64_t* v_strides, int64_t table_rows,
+                          int64_t table_row_stride, int dtype, int table_dtype, int style, void* stream) {
+  const char* fn = "ako_rope_qk_paged_fwd";
+  ako::PagedWriteArgs a{};
+  bool empty = false;
+  if (const int rc = paged_common(fn, cache, q_heads, dtype, &a.c, &empty)) return rc;
+  if (!valid_dtype(table_dtype)) return fail(AKO_ERR_UNSUPPORTED, "%s: unknown table dtype code %d", fn, table_dtype);
+  if (style != AKO_ROPE_NEOX && style != AKO_ROPE_INTERLEAVED)
+    return fail(AKO_ERR_UNSUPPORTED, "%s: unknown RoPE style %d", fn, style);
+  if (table_rows < 0) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: negative size", fn);
+  if (empty) return AKO_OK;
+  const int64_t d = cache->head_dim, kvh = cache->kv_heads, n = cache->num_pages, ps = cache->page_size;
+  const int64_t per = cache->cu_seqlens ? cache->tokens : cache->tokens / cache->n_seqs;
+  const int64_t seqs = cache->cu_seqlens ? 1 : cache->n_seqs;
+  if ((q_heads > 0 && (!q || !q_out)) || !k || !v || !q_strides || !k_strides || !v_strides ||
+      (table_rows > 0 && (!cos_table || !sin_table)))
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: null pointer argument", fn);
+  if (table_row_stride < 0 || (table_rows > 1 && table_row_stride < d / 2))
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: table row stride %lld < head_dim/2", fn, (long long)table_row_stride);
+  for (int i = 0; i < 3; ++i)
+    if (q_strides[i] < 0 || k_strides[i] < 0 || v_strides[i] < 0)
+      return fail(AKO_ERR_INVALID_ARGUMENT, "%s: negative stride", fn);
+  const int eb = ako::dtype_bytes(dtype), tb = ako::dtype_bytes(table_dtype);
+  const PagedSpans held(cache, dtype);
+  Span in[5];
+  int n_in = 0;
+  if (q_heads > 0) in[n_in++] = span_4d(q, seqs, per, q_heads, d, q_strides, eb);
+  in[n_in++] = span_4d(k, seqs, per, kvh, d, k_strides, eb);
+  in[n_in++] = span_4d(v, seqs, per, kvh, d, v_strides, eb);
+  if (table_rows > 0) {
+    in[n_in++] = span_2d(cos_table, table_rows, d / 2, table_row_stride, tb);
+    in[n_in++] = span_2d(sin_table, table_rows, d / 2, table_row_stride, tb);
+  }
+  const Span qo = span_2d(q_out, 1, cache->tokens * q_heads * d, 0, eb);
+  bool ok = held.ok && qo.ok;
+  for (int i = 0; i < n_in; ++i) ok = ok && in[i].ok;
+  if (!ok) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: sizes and strides overflow the address space", fn);
+  for (int i = 0; i < n_in; ++i) {
+    if (q_heads > 0 && overlap(qo, in[i])) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: q_out overlaps an input", fn);
+    for (int j = 0; j < held.n_pages; ++j)
+      if (overlap(held.pages[j], in[i])) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: the pages overlap an input", fn);
+  }
+  if (q_heads > 0 && held.meets(qo))
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: q_out overlaps the cache or its indexes", fn);
+  for (int j = 0; j < held.n_pages; ++j)
+    if (held.meets_index(held.pages[j]))
+      return fail(AKO_ERR_INVALID_ARGUMENT, "%s: the pages overlap the block table or the lengths", fn);
+  if (n > 0) {
+    const bool mx = cache->page_dtype == AKO_DTYPE_E4M3;
+    const int pb = mx ? 1 : eb;
+    const int64_t codes = ako::ceil_div(d, 32);
+    bool apart = distinct_rows(n, kvh, ps, d, cache->k_strides) && distinct_rows(n, kvh, ps, d, cache->v_strides) &&
+                 rows_apart(held.pages[0], held.pages[1], n, kvh, ps, d, cache->k_strides, cache->v_strides, pb);
+    if (mx)
+      apart = apart && distinct_rows(n, kvh, ps, codes, cache->k_scale_strides) &&
+              distinct_rows(n, kvh, ps, codes, cache->v_scale_strides) &&
+              rows_apart(held.pages[2], held.pages[3], n, kvh, ps, codes, cache->k_scale_strides, cache->v_scale_strides, 1) &&
+              !overlap(held.pages[0], held.pages[2]) && !overlap(held.pages[0], held.pages[3]) &&
+              !overlap(held.pages[1], held.pages[2]) && !overlap(held.pages[1], held.pages[3]);
+    if (!apart) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: rows of the cache overlap", fn);
+  }
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.q_out = q_out;
+  a.cos = cos_table;
+  a.sin = sin_table;
+  for (int i = 0; i < 3; ++i) {
+    a.qs[i] = q_strides[i];
+    a.kns[i] = k_strides[i];
+    a.vns[i] = v_strides[i];
+  }
+  a.st = table_row_stride;
+  a.table_rows = table_rows;
+  a.q_heads = q_heads;
+  a.dtype = dtype;
+  a.table_dtype = table_dtype;
+  a.neox = style == AKO_ROPE_NEOX;
+  return hip_status(ako::launch_paged_write(a, static_cast<hipStream_t>(stream)), fn);
+}
+
+int ako_paged_read_fwd(const ako_paged_t* cache, void* k_out, void* v_out, int dtype, void* stream) {
+  const char* fn = "ako_paged_read_fwd";
+  ako::PagedReadArgs a{};
+  bool empty = false;
+  if (const int rc = paged_common(fn, cache, 0, dtype, &a.c, &empty)) return rc;
+  if (empty) return AKO_OK;
+  if (!k_out || !v_out) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: null pointer argument", fn);
+  const int64_t n = cache->tokens * cache->kv_heads * cache->head_dim;
+  const Span ko = span_2d(k_out, 1, n, 0, ako::dtype_bytes(dtype)), vo = span_2d(v_out, 1, n, 0, ako::dtype_bytes(dtype));
+  const PagedSpans held(cache, dtype);
+  if (!ko.ok || !vo.ok || !held.ok)
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: sizes and strides overflow the address space", fn);
+  if (overlap(ko, vo) || held.meets(ko) || held.meets(vo))
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: an output overlaps another buffer", fn);
+  a.k_out = k_out;
+  a.v_out = v_out;
+  a.dtype = dtype;
+  return hip_status(ako::launch_paged_read(a, static_cast<hipStream_t>(stream)), fn);
+}
+
+extern "C++" {
+namespace {
+
+int attention_common(const char* fn, const ako_paged_t* cache, int64_t q_heads, int dtype, ako::PagedAttentionArgs* a,
+                     bool* empty) {
+  if (const int rc = paged_common(fn, cache, q_heads, dtype, &a->c, empty)) return rc;
+  if (q_heads % cache->kv_heads)
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: %lld query heads are no multiple of %lld", fn, (long long)q_heads,
+                (long long)cache->kv_heads);
+  *empty = *empty || q_heads == 0;
+  a->q_heads = q_heads;
+  a->dtype = dtype;
+  return AKO_OK;
+}
+
+}  // namespace
+}  // extern "C++"
+
+int ako_paged_attention_fwd(const void* q, const int64_t* q_strides, void* out, const ako_paged_t* cache, int64_t q_heads,
+                            float scale, int64_t window, int64_t sinks, void* workspace, int64_t workspace_bytes, int dtype,
+                            void* stream) {
+  const char* fn = "ako_paged_attention_fwd";
+  ako::PagedAttentionArgs a{};
+  bool empty = false;
+  if (const int rc = attention_common(fn, cache, q_heads, dtype, &a, &empty)) return rc;
+  if (!(scale - scale == 0.0f)) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: scale must be finite", fn);
+  if (window < 0 || sinks < 0) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: window and sinks must be >= 0", fn);
+  if (empty) return AKO_OK;
+  if (!q || !out || !q_strides) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: null pointer argument", fn);
+  if (q_strides[0] < 0 || q_strides[1] < 0 || q_strides[2] < 0)
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: negative stride", fn);
+  const int64_t need = ako::paged_attention_workspace(a);
+  if (workspace_bytes < need || (need > 0 && (!workspace || !aligned(workspace, 16))))
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: needs a 16-byte aligned workspace of %lld bytes, got %lld", fn,
+                (long long)need, (long long)workspace_bytes);
+  const int64_t d = cache->head_dim;
+  const int64_t per = cache->cu_seqlens ? cache->tokens : cache->tokens / cache->n_seqs;
+  const Span qi = span_4d(q, cache->cu_seqlens ? 1 : cache->n_seqs, per, q_heads, d, q_strides, ako::dtype_bytes(dtype));
+  const Span o = span_2d(out, 1, cache->tokens * q_heads * d, 0, ako::dtype_bytes(dtype));
+  const Span w = span_bytes(workspace, need);
+  const PagedSpans held(cache, dtype);
+  if (!qi.ok || !o.ok || !w.ok || !held.ok)
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: sizes and strides overflow the address space", fn);
+  if (overlap(o, qi) || held.meets(o)) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: out overlaps an input", fn);
+  if (overlap(w, qi) || overlap(w, o) || held.meets(w))
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: the workspace overlaps another buffer", fn);
+  a.q = q;
+  a.out = out;
+  for (int i = 0; i < 3; ++i) a.qs[i] = q_strides[i];
+  a.window = window;
+  a.sinks = sinks;
+  a.scale = scale;
+  a.workspace = workspace;
+  return hip_status(ako::launch_paged_attention(a, static_cast<hipStream_t>(stream)), fn);
+}
+
+int64_t ako_paged_attention_workspace(const ako_paged_t* cache, int64_t q_heads, int dtype) {
+  ako::PagedAttentionArgs a{};
+  bool empty = false;
+  if (attention_common("ako_paged_attention_workspace", cache, q_heads, dtype, &a, &empty)) return -1;
+  return empty ? 0 : ako::paged_attention_workspace(a);
 }
 
 }  // extern "C"

@@ -158,4 +158,56 @@ struct SwigluArgs {
 };
 hipError_t launch_swiglu(const SwigluArgs& a, hipStream_t stream);
 
+// A paged key/value cache and the token rows of one step (ako_paged_t).
+struct PagedArgs {
+  const void* k;
+  const void* v;
+  const void* ks;  // scale codes of e4m3 pages
+  const void* vs;
+  const int* table;
+  const int* lens;
+  const int* cu;  // null: tokens / n_seqs rows each
+  int64_t kst[3], vst[3], ksst[3], vsst[3];  // page, head, slot
+  int64_t table_stride, table_width, n_seqs;
+  int64_t num_pages, kv_heads, page_size, head_dim;
+  int64_t tokens;
+  bool mx;  // e4m3 pages with scale codes
+};
+
+struct PagedWriteArgs {
+  PagedArgs c;
+  const void* q;
+  const void* k;
+  const void* v;
+  void* q_out;
+  const void* cos;
+  const void* sin;
+  int64_t qs[3], kns[3], vns[3];  // batch, token, head
+  int64_t st, table_rows, q_heads;
+  int dtype, table_dtype;
+  bool neox;
+};
+hipError_t launch_paged_write(const PagedWriteArgs& a, hipStream_t stream);
+
+struct PagedReadArgs {
+  PagedArgs c;
+  void* k_out;
+  void* v_out;
+  int dtype;
+};
+hipError_t launch_paged_read(const PagedReadArgs& a, hipStream_t stream);
+
+struct PagedAttentionArgs {
+  PagedArgs c;
+  const void* q;
+  void* out;
+  int64_t qs[3];  // batch, token, head
+  int64_t q_heads, window, sinks;  // window 0: none
+  float scale;
+  int dtype;
+  void* workspace;  // paged_attention_workspace bytes
+};
+int64_t paged_attention_workspace(const PagedAttentionArgs& a);
+hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t stream);
+
 }  // namespace ako

@@ -14,8 +14,10 @@
 #include <ATen/hip/HIPContext.h>
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <string>
 #include <utility>
+#include <vector>
 
 #include "ako_hip.h"
 
@@ -42,6 +44,10 @@ std::string dtype_str(at::ScalarType st) {
     case at::kHalf: return "torch.float16";
     case at::kBFloat16: return "torch.bfloat16";
     case at::kDouble: return "torch.float64";
+    case at::kFloat8_e4m3fn: return "torch.float8_e4m3fn";
+    case at::kInt: return "torch.int32";
+    case at::kLong: return "torch.int64";
+    case at::kByte: return "torch.uint8";
     default: return std::string("torch.") + c10::toString(st);
   }
 }
@@ -344,6 +350,221 @@ at::Tensor swiglu(const at::Tensor& gate, const at::Tensor& up) {
   return y;
 }
 
+// ------------------------------------------------- paged key/value cache --
+// The checks and messages of ako_amd/ops/paged_ref.py (cache_error, rows_error,
+// write_error, read_error, attention_error), in the same order.
+using OptTensor = c10::optional<at::Tensor>;
+
+const at::Tensor* get(const OptTensor& t) { return t.has_value() && t->defined() ? &*t : nullptr; }
+
+constexpr int64_t kMaxPositions = 2147483647 - 65536;
+
+struct PagedArg {
+  const at::Tensor &k, &v, &table, &lens;
+  const at::Tensor *ks, *vs, *cu;
+  std::string pre;  // "function: "
+  bool mx() const { return k.scalar_type() == at::kFloat8_e4m3fn; }
+  int64_t n() const { return table.size(0); }
+  [[noreturn]] void refuse(const std::string& msg) const { value_error(pre + msg); }
+
+  void check_cache() const {
+    if (k.dim() != 4 || !v.sizes().equals(k.sizes()) || v.scalar_type() != k.scalar_type())
+      refuse("k_pages " + shape_str(k.sizes()) + " " + dtype_str(k.scalar_type()) + " and v_pages " + shape_str(v.sizes()) +
+             " " + dtype_str(v.scalar_type()) + " must be (pages, kv_heads, page_size, head_dim) alike");
+    const int64_t d = k.size(3);
+    if (d < 16 || d > 256 || d % 16) refuse("head_dim must be a multiple of 16 up to 256, got " + std::to_string(d));
+    if (k.size(1) < 1 || k.size(2) < 1) refuse("kv_heads and page_size must be at least 1");
+    if (!mx() && dtype_code_or(k.scalar_type()) < 0)
+      refuse("pages must be float32/float16/bfloat16/float8_e4m3fn, got " + dtype_str(k.scalar_type()));
+    if (k.stride(3) != 1 || v.stride(3) != 1) refuse("page rows must be contiguous in head_dim");
+    if (mx()) {
+      const int64_t want[4] = {k.size(0), k.size(1), k.size(2), (d + 31) / 32};
+      for (int i = 0; i < 2; ++i) {
+        const at::Tensor* t = i ? vs : ks;
+        const char* name = i ? "v_scales" : "k_scales";
+        if (!t || !t->sizes().equals(at::IntArrayRef(want, 4)) || t->scalar_type() != at::kByte)
+          refuse(std::string("e4m3 pages need ") + name + " of shape " + shape_str(at::IntArrayRef(want, 4)) +
+                 " and dtype uint8");
+        if (t->size(3) > 1 && t->stride(3) != 1) refuse(std::string(name) + " must be contiguous in the last dimension");
+      }
+    } else if (ks || vs) {
+      refuse("k_scales and v_scales are for float8_e4m3fn pages");
+    }
+    if (table.dim() != 2 || table.scalar_type() != at::kInt) refuse("block_table must be a 2-D int32 tensor");
+    if (table.size(1) > 1 && table.stride(1) != 1) refuse("block_table rows must be contiguous");
+    if (table.size(1) > kMaxPositions / k.size(2))
+      refuse("block_table names more than " + std::to_string(kMaxPositions) + " positions");
+    if (lens.dim() != 1 || lens.size(0) != n() || lens.scalar_type() != at::kInt || !lens.is_contiguous())
+      refuse("seq_lens must be a contiguous int32 tensor of shape (" + std::to_string(n()) + ",)");
+    if (cu && (cu->dim() != 1 || cu->size(0) != n() + 1 || cu->scalar_type() != at::kInt || !cu->is_contiguous()))
+      refuse("cu_seqlens must be a contiguous int32 tensor of shape (" + std::to_string(n() + 1) + ",)");
+    same_device("v_pages", &v);
+    same_device("k_scales", ks);
+    same_device("v_scales", vs);
+    same_device("block_table", &table);
+    same_device("seq_lens", &lens);
+    same_device("cu_seqlens", cu);
+  }
+  void same_device(const char* name, const at::Tensor* t) const {
+    if (t && t->device() != k.device()) refuse(std::string(name) + " must be on the device of the pages");
+  }
+
+  void check_rows(const char* name, const at::Tensor& x, int64_t heads) const {
+    if (x.dim() != (cu ? 3 : 4))
+      refuse(std::string(name) + " must be (batch, seq, heads, head_dim), or (tokens, heads, head_dim) with cu_seqlens, got " +
+             shape_str(x.sizes()));
+    if (x.size(-1) != k.size(3) || (heads >= 0 && x.size(-2) != heads))
+      refuse(std::string(name) + " " + shape_str(x.sizes()) + " does not match the pages " + shape_str(k.sizes()));
+    if (!cu && x.size(0) != n())
+      refuse(std::string(name) + " has " + std::to_string(x.size(0)) + " sequences, the block table " + std::to_string(n()));
+    if (dtype_code_or(x.scalar_type()) < 0)
+      refuse(std::string(name) + " must be float32/float16/bfloat16, got " + dtype_str(x.scalar_type()));
+    if (!mx() && x.scalar_type() != k.scalar_type())
+      refuse(std::string(name) + " is " + dtype_str(x.scalar_type()) + ", the pages " + dtype_str(k.scalar_type()));
+    if (x.device() != k.device()) refuse(std::string(name) + " must be on the device of the pages");
+  }
+
+  ako_paged_t c(int64_t tokens) const {
+    ako_paged_t c{};
+    c.k_pages = k.data_ptr();
+    c.v_pages = v.data_ptr();
+    c.block_table = static_cast<const int32_t*>(table.data_ptr());
+    c.seq_lens = static_cast<const int32_t*>(lens.data_ptr());
+    c.cu_seqlens = cu ? static_cast<const int32_t*>(cu->data_ptr()) : nullptr;
+    for (int i = 0; i < 3; ++i) {
+      c.k_strides[i] = k.stride(i);
+      c.v_strides[i] = v.stride(i);
+    }
+    if (mx()) {
+      c.k_scales = ks->data_ptr();
+      c.v_scales = vs->data_ptr();
+      for (int i = 0; i < 3; ++i) {
+        c.k_scale_strides[i] = ks->stride(i);
+        c.v_scale_strides[i] = vs->stride(i);
+      }
+    }
+    c.num_pages = k.size(0);
+    c.kv_heads = k.size(1);
+    c.page_size = k.size(2);
+    c.head_dim = k.size(3);
+    c.n_seqs = n();
+    c.table_width = table.size(1);
+    c.table_stride = n() > 1 ? table.stride(0) : table.size(1);
+    c.tokens = tokens;
+    c.page_dtype = mx() ? AKO_DTYPE_E4M3 : dtype_code_or(k.scalar_type());
+    return c;
+  }
+};
+
+int64_t row_count(const at::Tensor& x) { return x.dim() == 4 ? x.size(0) * x.size(1) : x.size(0); }
+
+struct RowStrides {
+  int64_t s[3];
+  explicit RowStrides(const at::Tensor& x) {
+    const bool four = x.dim() == 4;
+    s[0] = four ? x.stride(0) : 0;
+    s[1] = x.stride(four ? 1 : 0);
+    s[2] = x.stride(four ? 2 : 1);
+  }
+};
+
+at::Tensor rope_qk_paged(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cos,
+                         const at::Tensor& sin, const at::Tensor& k_pages, const at::Tensor& v_pages,
+                         const at::Tensor& block_table, const at::Tensor& seq_lens, const std::string& style,
+                         const OptTensor& k_scales, const OptTensor& v_scales, const OptTensor& cu_seqlens) {
+  const char* fn = "rope_qk_paged_hip";
+  const int index = gpu_index(q, fn);
+  const PagedArg p{k_pages, v_pages, block_table, seq_lens, get(k_scales), get(v_scales), get(cu_seqlens),
+                   std::string(fn) + ": "};
+  p.check_cache();
+  if (style != "neox" && style != "interleaved")
+    p.refuse("Unknown RoPE style '" + style + "', expected one of ('neox', 'interleaved')");
+  const at::Tensor* rows[3] = {&q, &k, &v};
+  const char* names[3] = {"q", "k", "v"};
+  for (int i = 0; i < 3; ++i) {
+    const at::Tensor& x = *rows[i];
+    p.check_rows(names[i], x, i ? k_pages.size(1) : -1);
+    bool alike = x.scalar_type() == q.scalar_type() && x.dim() == q.dim();
+    for (int64_t j = 0; alike && j + 2 < x.dim(); ++j) alike = x.size(j) == q.size(j);
+    if (!alike)
+      p.refuse(std::string(names[i]) + " " + shape_str(x.sizes()) + " " + dtype_str(x.scalar_type()) +
+               " does not match q " + shape_str(q.sizes()) + " " + dtype_str(q.scalar_type()));
+  }
+  if (cos.dim() != 2 || cos.size(1) != k_pages.size(3) / 2 || !sin.sizes().equals(cos.sizes()))
+    p.refuse("tables must be (positions, " + std::to_string(k_pages.size(3) / 2) + "), got " + shape_str(cos.sizes()) +
+             " and " + shape_str(sin.sizes()));
+  if (cos.device() != q.device() || sin.device() != q.device()) p.refuse("tables must be on the device of the pages");
+  const at::Tensor qv = head_view(q), kv = head_view(k), vv = head_view(v);
+  const Tables t = tables(cos, sin, index);
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  const ako_paged_t c = p.c(row_count(q));
+  const RowStrides qs(qv), ks(kv), vs(vv);
+  check(on_device(index, [&](hipStream_t s) {
+          return ako_rope_qk_paged_fwd(qv.data_ptr(), kv.data_ptr(), vv.data_ptr(), t.cos.data_ptr(), t.sin.data_ptr(),
+                                       out.data_ptr(), &c, q.size(-2), qs.s, ks.s, vs.s, t.cos.size(0), t.stride,
+                                       dtype_code_or(q.scalar_type()), t.dtype, style_code(style), s);
+        }), fn);
+  return out;
+}
+
+std::pair<at::Tensor, at::Tensor> paged_read(const at::Tensor& k_pages, const at::Tensor& v_pages,
+                                             const at::Tensor& block_table, const at::Tensor& seq_lens, int64_t rows,
+                                             const c10::optional<at::ScalarType>& dtype, const OptTensor& k_scales,
+                                             const OptTensor& v_scales, const OptTensor& cu_seqlens) {
+  const char* fn = "paged_read_hip";
+  const int index = gpu_index(k_pages, fn);
+  const PagedArg p{k_pages, v_pages, block_table, seq_lens, get(k_scales), get(v_scales), get(cu_seqlens),
+                   std::string(fn) + ": "};
+  p.check_cache();
+  if (rows < 0) p.refuse("rows must be at least 0, got " + std::to_string(rows));
+  const at::ScalarType to = dtype.value_or(k_pages.scalar_type());
+  if (dtype_code_or(to) < 0) p.refuse("dtype must be float32/float16/bfloat16, got " + dtype_str(to));
+  if (!p.mx() && to != k_pages.scalar_type())
+    p.refuse("dtype is " + dtype_str(to) + ", the pages " + dtype_str(k_pages.scalar_type()));
+  std::vector<int64_t> shape{rows, k_pages.size(1), k_pages.size(3)};
+  if (!p.cu) shape.insert(shape.begin(), p.n());
+  at::Tensor k = at::empty(shape, k_pages.options().dtype(to)), v = at::empty_like(k);
+  const ako_paged_t c = p.c(row_count(k));
+  check(on_device(index, [&](hipStream_t s) {
+          return ako_paged_read_fwd(&c, k.data_ptr(), v.data_ptr(), dtype_code_or(to), s);
+        }), fn);
+  return {k, v};
+}
+
+at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
+                           const at::Tensor& block_table, const at::Tensor& seq_lens, const c10::optional<double>& scale_in,
+                           const c10::optional<int64_t>& window, int64_t sinks, const OptTensor& k_scales,
+                           const OptTensor& v_scales, const OptTensor& cu_seqlens) {
+  const char* fn = "paged_attention_hip";
+  const int index = gpu_index(q, fn);
+  const PagedArg p{k_pages, v_pages, block_table, seq_lens, get(k_scales), get(v_scales), get(cu_seqlens),
+                   std::string(fn) + ": "};
+  p.check_cache();
+  p.check_rows("q", q, -1);
+  const int64_t heads = q.size(-2);
+  const double scale = scale_in.has_value() ? *scale_in : 1.0 / std::sqrt(static_cast<double>(k_pages.size(3)));
+  if (heads % k_pages.size(1))
+    p.refuse(std::to_string(heads) + " query heads are no multiple of " + std::to_string(k_pages.size(1)) + " key heads");
+  if (!std::isfinite(scale)) p.refuse(std::string("scale must be finite, got ") + (std::isnan(scale) ? "nan" : scale > 0 ? "inf" : "-inf"));
+  if ((window.has_value() && *window < 1) || sinks < 0)
+    p.refuse("window must be at least 1 (or None) and sinks at least 0, got " +
+             (window.has_value() ? std::to_string(*window) : std::string("None")) + " and " + std::to_string(sinks));
+  const at::Tensor qv = head_view(q);
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  const ako_paged_t c = p.c(row_count(q));
+  const int dt = dtype_code_or(q.scalar_type());
+  const int64_t need = ako_paged_attention_workspace(&c, heads, dt);
+  at::Tensor space;
+  if (need > 0) space = at::empty({need}, q.options().dtype(at::kByte));
+  const RowStrides qs(qv);
+  check(on_device(index, [&](hipStream_t s) {
+          return ako_paged_attention_fwd(qv.data_ptr(), qs.s, out.data_ptr(), &c, heads, static_cast<float>(scale),
+                                         window.value_or(0), sinks, need > 0 ? space.data_ptr() : nullptr,
+                                         need > 0 ? need : 0, dt, s);
+        }), fn);
+  return out;
+}
+
 // The stream this binding launches on, for tests: torch's current stream.
 int64_t current_stream(int64_t index) {
   return reinterpret_cast<int64_t>(at::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(index)).stream());
@@ -369,6 +590,14 @@ PYBIND11_MODULE(_ako_torch, m) {
   m.def("rope_qk_cache", &rope_qk_cache, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("cos"),
         py::arg("sin"), py::arg("pos"), py::arg("k_cache"), py::arg("v_cache"), py::arg("style") = "neox");
   m.def("swiglu", &swiglu, py::arg("gate"), py::arg("up"));
+  m.def("rope_qk_paged", &rope_qk_paged, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("cos"), py::arg("sin"),
+        py::arg("k_pages"), py::arg("v_pages"), py::arg("block_table"), py::arg("seq_lens"), py::arg("style"),
+        py::arg("k_scales"), py::arg("v_scales"), py::arg("cu_seqlens"));
+  m.def("paged_read", &paged_read, py::arg("k_pages"), py::arg("v_pages"), py::arg("block_table"), py::arg("seq_lens"),
+        py::arg("rows"), py::arg("dtype"), py::arg("k_scales"), py::arg("v_scales"), py::arg("cu_seqlens"));
+  m.def("paged_attention", &paged_attention, py::arg("q"), py::arg("k_pages"), py::arg("v_pages"),
+        py::arg("block_table"), py::arg("seq_lens"), py::arg("scale"), py::arg("window"), py::arg("sinks"),
+        py::arg("k_scales"), py::arg("v_scales"), py::arg("cu_seqlens"));
   m.def("current_stream", &current_stream);
   m.def("row_walk", &row_walk, py::arg("t"));
 }

@@ -40,7 +40,8 @@ extern "C" {
 typedef enum {
   AKO_DTYPE_F32 = 0,
   AKO_DTYPE_F16 = 1,
-  AKO_DTYPE_BF16 = 2
+  AKO_DTYPE_BF16 = 2,
+  AKO_DTYPE_E4M3 = 3 /* pages of a paged cache only: OCP e4m3 with scale codes */
 } ako_dtype_t;
 
 typedef enum {
@@ -201,6 +202,96 @@ int ako_swiglu_fwd(const void* gate, const void* up, void* y,
                    int64_t rows, int64_t n,
                    int64_t gate_row_stride, int64_t up_row_stride, int64_t y_row_stride,
                    int dtype, void* stream);
+
+/*
+ * A paged key/value cache and the token rows of one step. The reference has
+ * no counterpart (its decoder re-concatenates dense caches,
+ * ako/models/decoder.py:84-93); the step's semantics are those of
+ * ako/models/decoder.py:173-185 with the caches in pages.
+ *
+ * Keys and values lie in pools of pages, [num_pages, kv_heads, page_size,
+ * head_dim] in any strides with head_dim contiguous. Position p of sequence i
+ * is slot p % page_size of page block_table[i][p / page_size]; an entry
+ * outside [0, num_pages) is a page that is not there. seq_lens[i] counts the
+ * positions of sequence i with this step's tokens. A step has `tokens` rows:
+ * with cu_seqlens, rows cu_seqlens[i] .. cu_seqlens[i+1]-1 are the last
+ * positions of sequence i (cu_seqlens[0] = 0, ascending; rows from
+ * cu_seqlens[n_seqs] on are padding); without, sequence i has the rows
+ * i*(tokens/n_seqs) .. (i+1)*(tokens/n_seqs)-1. A row whose position would be
+ * negative (a sequence shorter than its rows) is padding too. block_table,
+ * seq_lens and cu_seqlens are read on the device, so that a captured step can
+ * be replayed as they change; whatever they hold, no kernel reads or writes
+ * outside the tensors.
+ *
+ * page_dtype is the rows' own dtype, or AKO_DTYPE_E4M3: one byte per element
+ * and, for each 32 elements of a row, an E8M0 scale code c (2^(c-127)) in
+ * k_scales / v_scales [num_pages, kv_heads, page_size, ceil(head_dim/32)],
+ * last dimension contiguous. A block is written with the smallest code >= 1
+ * under which none of its finite elements passes 448, elements rounded to
+ * nearest even; infinities and NaN are written as NaN.
+ *
+ * head_dim is a multiple of 16 up to 256. Stride triples are page, head, slot.
+ */
+typedef struct {
+  void* k_pages;
+  void* v_pages;
+  void* k_scales;            /* NULL unless page_dtype is AKO_DTYPE_E4M3 */
+  void* v_scales;
+  const int32_t* block_table; /* [n_seqs, table_width], rows table_stride apart */
+  const int32_t* seq_lens;    /* [n_seqs] */
+  const int32_t* cu_seqlens;  /* [n_seqs + 1], or NULL */
+  int64_t k_strides[3], v_strides[3];
+  int64_t k_scale_strides[3], v_scale_strides[3];
+  int64_t num_pages, kv_heads, page_size, head_dim;
+  int64_t n_seqs, table_width, table_stride;
+  int64_t tokens;
+  int32_t page_dtype;
+} ako_paged_t;
+
+/*
+ * RoPE of the step's q and k at their positions: rotated q to q_out
+ * ([tokens, q_heads, head_dim], dense), rotated k and unrotated v to their
+ * slots. k and v have cache->kv_heads heads. Stride triples of q, k and v are
+ * sequence, token, head; with cu_seqlens the first is not used. The tables
+ * hold positions 0 .. table_rows-1. The rows of q_out of padding are zero; a
+ * row whose page is not there, or whose position the block table or the
+ * tables do not cover, is written to no slot and its row of q_out is NaN. Rows
+ * of one step must not share a slot.
+ */
+int ako_rope_qk_paged_fwd(const void* q, const void* k, const void* v,
+                          const void* cos_table, const void* sin_table, void* q_out,
+                          const ako_paged_t* cache, int64_t q_heads,
+                          const int64_t* q_strides, const int64_t* k_strides,
+                          const int64_t* v_strides, int64_t table_rows, int64_t table_row_stride,
+                          int dtype, int table_dtype, int style, void* stream);
+
+/*
+ * The keys and values stored at the rows' positions, as dense [tokens,
+ * kv_heads, head_dim] tensors of dtype (which must be page_dtype unless that
+ * is AKO_DTYPE_E4M3). Rows that are padding or have no page are zero.
+ */
+int ako_paged_read_fwd(const ako_paged_t* cache, void* k_out, void* v_out, int dtype, void* stream);
+
+/*
+ * Attention of the step's rows over what their sequences hold. Head h of q
+ * attends to head h / (q_heads / kv_heads) of the cache; a row at position p
+ * sees the positions j <= p with (window == 0, or j > p - window, or
+ * j < sinks), except those whose page is not there:
+ *   out = to_dtype( sum_j softmax_j(scale * q.k_j) v_j ),
+ * zero where a row sees nothing (padding). Positions a row does not see have
+ * no influence on it, whatever they hold. out is [tokens, q_heads, head_dim],
+ * dense; q's strides are sequence, token, head. e4m3 pages are read as values
+ * of dtype. workspace holds ako_paged_attention_workspace bytes of device
+ * memory, 16-byte aligned, that nothing else uses until the work on `stream`
+ * is done.
+ */
+int ako_paged_attention_fwd(const void* q, const int64_t* q_strides, void* out,
+                            const ako_paged_t* cache, int64_t q_heads, float scale,
+                            int64_t window, int64_t sinks, void* workspace,
+                            int64_t workspace_bytes, int dtype, void* stream);
+
+/* Bytes of workspace for such a call (0: none); -1 for arguments it refuses. */
+int64_t ako_paged_attention_workspace(const ako_paged_t* cache, int64_t q_heads, int dtype);
 
 /*
  * Launch-shape override for tuning sweeps and tests (no counterpart in the

@@ -584,7 +584,7 @@ int paged_common(const char* fn, const ako_paged_t* c, int64_t heads, int dtype,
     return fail(AKO_ERR_INVALID_ARGUMENT, "%s: kv_heads and page_size must be at least 1", fn);
   if (c->page_size > kMaxPositions || c->table_width > kMaxPositions / c->page_size)
     return fail(AKO_ERR_INVALID_ARGUMENT, "%s: the block table names 2^31-65537 positions or more", fn);
-  if (c->kv_heads > kMaxInt / 1024 || heads > kMaxInt / 1024 || c->num_pages > kMaxInt || c->n_seqs > kMaxInt / 2 ||
+  if (c->kv_heads > kMaxInt / 65536 || heads > kMaxInt / 65536 || c->num_pages > kMaxInt || c->n_seqs > kMaxInt / 2 ||
       c->tokens > kMaxInt / 2 / std::max<int64_t>(1, std::max(heads, c->kv_heads)))
     return fail(AKO_ERR_INVALID_ARGUMENT, "%s: too many heads, pages, sequences or rows", fn);
   if (!c->cu_seqlens && c->tokens > 0 && (c->n_seqs == 0 || c->tokens % c->n_seqs))

@@ -47,7 +47,7 @@ inline PagedDev paged_dev(const PagedArgs& a) {
   d.n_seqs = static_cast<int>(a.n_seqs);
   d.num_pages = static_cast<int>(a.num_pages);
   d.page_size = static_cast<int>(a.page_size);
-  d.capacity = static_cast<int>(a.table_width * a.page_size);
+  d.capacity = a.num_pages > 0 ? static_cast<int>(a.table_width * a.page_size) : 0;
   d.tokens = static_cast<int>(a.tokens);
   d.seq = a.cu || a.n_seqs == 0 ? 0 : static_cast<int>(a.tokens / a.n_seqs);
   d.by_seq = make_fastdiv(d.seq > 0 ? d.seq : 1);

@@ -3,7 +3,24 @@
 // Token row t at position p of its sequence sees the keys j <= p, and with a
 // window w only those with j > p - w or j < sinks:
 //   out = sum_j e^(scale q.k_j - m) v_j / sum_j e^(scale q.k_j - m),  m = max_j scale q.k_j
-// in 32 bits, zero where nothing is visible.
+// in 32 bits, zero where nothing is visible. Keys are walked once, in tiles,
+// with a running maximum m, total l and weighted sum o (rescaled by e^(m_old - m_new)
+// where a tile raises m). The query rows of the heads that share a key head
+// are laid side by side, row r = (token of the sequence) * group + (head in group),
+// so that a tile of rows reads each key once for all of them.
+//
+// Products are formed transposed, S^T = K Q^T and O^T = V^T P^T: a lane then
+// holds scores of one query only, its maximum and total are one lane's
+// numbers, and the scores as they come out of the first product are the
+// operand of the second without moving between lanes. The matrix
+// instruction's k index is only a name for a key, so it is named by where the
+// first product leaves its scores; V^T is read with the same names. V^T comes
+// from rows of V in LDS through transposing reads.
+//
+// Weights e^(..) are at most 1 and are rounded to the rows' type for the second
+// product (half a step each, as the result is); totals add the 32-bit
+// weights. Long key ranges are split over workgroups and joined by a second
+// kernel in order of the split, so results do not depend on scheduling.
 
 #include <algorithm>
 #include <limits>
@@ -12,132 +29,634 @@
 
 namespace ako {
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
 struct AttnDev {
   PagedDev c;
   const void* q;
   void* out;
+  float* part_o;   // [splits][rows][head_dim], rows = tokens * q_heads
+  float2* part_ml; // [splits][rows]: maximum and total
   int64_t qs[3];
-  int q_heads, group, head_dim;
+  int64_t rows;
+  int q_heads, kv_heads, group, head_dim;
   int window, sinks;
-  float scale_log2;  // scale * log2(e)
-  FastDiv by_heads, by_group;
+  int tile0;              // first row tile of the launch
+  int splits, min_tiles;  // at most `splits` parts of a row tile's keys, of at least min_tiles tiles
+  int seq_tiles;          // row tiles per sequence (uniform steps)
+  float scale_log2;       // scale * log2(e): exponentials are of base 2
+  FastDiv by_kv_heads, by_group, by_splits, by_seq_tiles;
 };
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int m = 1; m < kWave; m *= 2) v = __builtin_fmaxf(v, __shfl_xor(v, m));
-  return v;
+// A workgroup's rows: those of one sequence (or padding) that share a key head.
+struct RowTile {
+  int seq;     // -1: padding, nothing is visible
+  int token0;  // first token row of the sequence
+  int rows;    // rows of the sequence for one key head
+  int row0;    // the tile's first
+  int pos0;    // position of token0, negative where the sequence is shorter than its rows
+};
+
+// Row tiles of a packed step are numbered with sequence i's first at
+// cu[i] * group / R + i: no two sequences share a number, whatever their lengths,
+// and a number is resolved without a sum over the sequences before it. What
+// lies behind the last sequence counts as one more, padding.
+template <int R>
+__device__ __forceinline__ bool find_rows(const AttnDev& a, int tile, RowTile& t) {
+  const PagedDev& p = a.c;
+  if (p.cu == nullptr) {
+    if (p.seq == 0) return false;
+    const int s = fast_div(tile, a.by_seq_tiles);
+    t.seq = s;
+    t.token0 = s * p.seq;
+    t.rows = p.seq * a.group;
+    t.row0 = (tile - s * a.seq_tiles) * R;
+    t.pos0 = max(p.lens[s], 0) - p.seq;
+    return true;
+  }
+  const auto start = [&](int i) { return min(max(p.cu[i], 0), p.tokens) * a.group / R + i; };
+  const int s = last_at_most(p.n_seqs, tile, start);
+  const int first = min(max(p.cu[s], 0), p.tokens);
+  const int end = s < p.n_seqs ? min(max(p.cu[s + 1], 0), p.tokens) : p.tokens;
+  t.token0 = first;
+  t.rows = (end - first) * a.group;
+  t.row0 = (tile - (first * a.group / R + s)) * R;
+  t.seq = s < p.n_seqs ? s : -1;
+  t.pos0 = s < p.n_seqs ? max(p.lens[s], 0) - (end - first) : -1;
+  return t.row0 >= 0 && t.row0 < t.rows;
 }
 
-// One wavefront per (token, query head): 64 keys at a time, one key per lane
-// for the products, then one slice of the head per lane for the sum.
-template <typename T, bool MX>
-__global__ __launch_bounds__(kWave) void paged_attention_simple(AttnDev a) {
-  __shared__ float qv[256], pv[kWave];
-  __shared__ int64_t row[kWave];
-  __shared__ int64_t srow[kWave];
-  const int lane = threadIdx.x;
-  const int token = fast_div(blockIdx.x, a.by_heads), h = blockIdx.x - token * a.q_heads;
-  const int kvh = fast_div(h, a.by_group);
-  const TokenPlace at = token_place(a.c, token);
-  const int b = a.c.cu ? 0 : static_cast<int>(fast_div(token, a.c.by_seq));
-  const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + (token - b * a.c.seq) * a.qs[1] + h * a.qs[2];
-  for (int d = lane; d < a.head_dim; d += kWave) qv[d] = to_f32(q[d]);
-  __syncthreads();
-  float m = -__builtin_inff(), l = 0.0f, acc[4] = {};
-  const int end = at.seq < 0 ? 0 : min(at.pos + 1, a.c.capacity);
-  const int low = a.window > 0 ? max(0, at.pos - a.window + 1) : 0;
-  for (int j0 = 0; j0 < end; j0 += kWave) {
-    if (j0 + kWave <= low && j0 >= a.sinks) continue;
-    const int j = j0 + lane;
-    int slot = 0, page = -1;
-    const bool seen = j < end && (j >= low || j < a.sinks);
-    if (seen) page = page_of(a.c, at.seq, j, slot);
-    float s = -__builtin_inff();
-    if (page >= 0) {
-      s = 0.0f;
-      const int64_t kr = page * a.c.kst[0] + kvh * a.c.kst[1] + slot * a.c.kst[2];
-      const int64_t sr = MX ? page * a.c.ksst[0] + kvh * a.c.ksst[1] + slot * a.c.ksst[2] : 0;
-      for (int d = 0; d < a.head_dim; d += 8) {
-        Eight<T> x;
-        if constexpr (MX) x = from_e4m3<T>(load_bytes8(static_cast<const uint8_t*>(a.c.k) + kr + d), e8m0_scale(a.c.ks[sr + d / 32]));
-        else x = load_eight<T>(static_cast<const T*>(a.c.k) + kr + d);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s = __builtin_fmaf(qv[d + i], to_f32(x[i]), s);
-      }
-      s *= a.scale_log2;
-    }
-    row[lane] = page < 0 ? -1 : page * a.c.vst[0] + kvh * a.c.vst[1] + slot * a.c.vst[2];
-    srow[lane] = page < 0 || !MX ? 0 : page * a.c.vsst[0] + kvh * a.c.vsst[1] + slot * a.c.vsst[2];
-    const float top = wave_max(s), mn = __builtin_fmaxf(m, top);
-    const float base = mn == -__builtin_inff() ? 0.0f : mn;
-    const float p = page < 0 ? 0.0f : __builtin_amdgcn_exp2f(s - base), keep = __builtin_amdgcn_exp2f(m - base);
-    pv[lane] = p;
-    l = l * keep + wave_sum(p);
-    m = mn;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] *= keep;
-    for (int k = 0; k < kWave; ++k) {
-      if (row[k] < 0) continue;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int d = lane + kWave * i;
-        if (d >= a.head_dim) continue;
-        float v;
-        if constexpr (MX) {
-          const unsigned w = static_cast<const uint8_t*>(a.c.v)[row[k] + d];
-          v = to_f32(static_cast<T>(FromE4m3<T>::lo(w, e8m0_scale(a.c.vs[srow[k] + d / 32]))[0]));
-        } else {
-          v = to_f32(static_cast<const T*>(a.c.v)[row[k] + d]);
-        }
-        acc[i] = __builtin_fmaf(pv[k], v, acc[i]);
-      }
-    }
-    __syncthreads();
+// The key tiles that a row tile sees, in order: those of the sinks, then those
+// from the first row's window on.
+struct KeyTiles {
+  int sink_tiles, low, end;  // low: a multiple of the tile
+  int count;
+};
+template <int KT>
+__device__ __forceinline__ KeyTiles key_tiles(const AttnDev& a, int first_pos, int last_pos) {
+  KeyTiles k{0, 0, 0, 0};
+  k.end = min(last_pos + 1, a.c.capacity);
+  if (k.end <= 0) return k;
+  if (a.window > 0) {
+    k.low = max(0, max(first_pos, 0) - a.window + 1) / KT * KT;
+    k.low = min(k.low, k.end / KT * KT);
+    k.sink_tiles = (min(a.sinks, k.low) + KT - 1) / KT;
   }
-  T* out = static_cast<T*>(a.out) + (int64_t(token) * a.q_heads + h) * a.head_dim;
-  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+  k.count = k.sink_tiles + (k.end - k.low + KT - 1) / KT;
+  return k;
+}
+
+// ---- matrix products ----------------------------------------------------------
+// Sixteen rows of A times sixteen columns of B, eight elements of the inner
+// dimension per lane. kShift: weights (and so totals and sums) are held times
+// 2^kShift; a power of two that the final division removes. fp16's weights
+// would be subnormal, with fewer bits, below 2^-14 of the largest; times 2^15
+// the largest is still far from fp16's end and the last bit is lost below 2^-29.
+template <typename T> struct Mfma;
+template <> struct Mfma<__bf16> {
+  static constexpr float kShift = 0.0f;
+  static __device__ __forceinline__ f32x4 mul(const Eight<__bf16>& a, const Eight<__bf16>& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+};
+template <> struct Mfma<_Float16> {
+  static constexpr float kShift = 15.0f;
+  static __device__ __forceinline__ f32x4 mul(const Eight<_Float16>& a, const Eight<_Float16>& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+};
+template <> struct Mfma<float> {
+  static constexpr float kShift = 0.0f;
+  static __device__ __forceinline__ f32x4 mul(const Eight<float>& a, const Eight<float>& b, f32x4 c) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int d = lane + kWave * i;
-    if (d < a.head_dim) out[d] = from_f32<T>(acc[i] * inv);
+    for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// Orders LDS accesses of one wavefront's lanes to each other's data. The LDS
+// serves a wavefront in order; only the compiler has to be held.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+__device__ __forceinline__ float max_over_groups(float v) {  // over the lanes l % 16
+  v = __builtin_fmaxf(v, __shfl_xor(v, 16));
+  return __builtin_fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float sum_over_groups(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+template <typename T>
+__device__ __forceinline__ bool not_finite(const Eight<T>& x) {
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) bad |= !(__builtin_fabsf(to_f32(x[i])) < __builtin_inff());
+  return bad;
+}
+
+// ---- up to 16 rows per workgroup -------------------------------------------------
+// Decode steps, where the cache's bytes are all that counts, and every step in
+// 32 bits. A wavefront takes key tiles of its own: K goes from memory straight into
+// the operand's registers (lane: key l % 16, and of each chunk of the head the
+// part l / 16), V through registers into the wavefront's own piece of LDS, so that
+// no barrier stands in the loop. The next tile's loads are issued as soon as
+// the registers of this tile's are free. The wavefronts' results are joined in LDS
+// at the end.
+template <typename T, bool MX, int DP>
+struct RowsShape {
+  static constexpr int kBlocks = sizeof(T) == 4 ? 1 : 2;    // 16-key blocks per tile
+  static constexpr int kKeys = 16 * kBlocks;
+  static constexpr int kChunk = MX ? 16 : 16 / sizeof(T);   // elements in 16 loaded bytes
+  static constexpr int kChunks = DP / (4 * kChunk);         // of K, per lane and key
+  static constexpr int kRowLanes = DP / kChunk;             // lanes across a row of V
+  static constexpr int kRowKeys = kWave / kRowLanes;        // keys per load of V
+  static constexpr int kLoads = kKeys / kRowKeys;           // of V, per lane
+  static constexpr int kRowBytes = DP * sizeof(T);
+  static constexpr int kTileBytes = kKeys * kRowBytes;      // = 16 rows of DP floats, too
+};
+
+// LDS place of 16-byte packet p of key's row. Rows are multiples of 128 or 256
+// bytes, all on the same banks: packets are exchanged in pairs (a transposing
+// read takes 32 bytes of four keys' rows) so that eight keys' pairs lie on
+// different banks.
+template <int ROW_BYTES>
+__device__ __forceinline__ int lds_packet(int key, int p) {
+  constexpr int kPairs = ROW_BYTES / 32;
+  const int x = kPairs >= 8 ? key & 7 : (key >> 1) & (kPairs - 1);
+  return key * ROW_BYTES + ((p ^ (x << 1)) << 4);
+}
+
+template <typename T, bool MX, int DP, int WAVES, bool PAGE16>
+__global__ __launch_bounds__(WAVES* kWave) void attn_rows(AttnDev a) {
+  using S = RowsShape<T, MX, DP>;
+  constexpr int KT = S::kKeys, NB = S::kBlocks, NC = S::kChunks, C = S::kChunk, NV = S::kLoads;
+  constexpr int E = 16 / static_cast<int>(sizeof(T));  // elements of an LDS packet
+  __shared__ __align__(16) unsigned char lds[WAVES * S::kTileBytes];
+  __shared__ float2 lds_ml[WAVES][16];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+  const int col = lane % 16, g = lane / 16;
+  unsigned char* const vt = lds + wave * S::kTileBytes;
+
+  // Key heads run fastest over the workgroups, so that the XCDs share them out
+  // and the row tiles of one head meet in one XCD's L2.
+  const unsigned nth = fast_div(blockIdx.x, a.by_kv_heads);
+  const int kvh = blockIdx.x - nth * a.kv_heads;
+  const unsigned tile_id = fast_div(nth, a.by_splits);
+  const int split = nth - tile_id * a.splits;
+  RowTile t;
+  if (!find_rows<16>(a, a.tile0 + tile_id, t)) return;
+
+  const int live = min(16, t.rows - t.row0);
+  const int my_token = fast_div(t.row0 + col, a.by_group);  // of the sequence
+  const int my_head = kvh * a.group + (t.row0 + col - my_token * a.group);
+  const int first_pos = t.pos0 + static_cast<int>(fast_div(t.row0, a.by_group));
+  const int last_pos = t.pos0 + static_cast<int>(fast_div(t.row0 + live - 1, a.by_group));
+  const KeyTiles kt = t.seq < 0 ? KeyTiles{0, 0, 0, 0} : key_tiles<KT>(a, first_pos, last_pos);
+  const int parts = max(1, min(a.splits, kt.count / a.min_tiles));
+  const int begin = split < parts ? static_cast<int>(static_cast<int64_t>(kt.count) * split / parts) : 0;
+  const int end = split < parts ? static_cast<int>(static_cast<int64_t>(kt.count) * (split + 1) / parts) : 0;
+
+  // This lane's query row, in the order of the K operand.
+  const bool row_live = col < live;
+  const int hi = row_live ? t.pos0 + my_token : -1;
+  const int lo = a.window > 0 ? max(hi, 0) - a.window + 1 : 0;
+  Eight<T> q[NC * C / 8 > 0 ? NC * C / 8 : 1];
+  {
+    const int b = a.c.cu ? 0 : t.seq;
+    const T* x = static_cast<const T*>(a.q) + b * a.qs[0] + (t.token0 - b * a.c.seq + my_token) * a.qs[1] + my_head * a.qs[2];
+#pragma unroll
+    for (int i = 0; i < NC * C / 4; ++i) {  // four elements at a time
+      const int d = (i * 4 / C) * 4 * C + g * C + i * 4 % C;
+      Pack<T, 4> v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v.e[e] = from_f32<T>(0.0f);
+      if (row_live && d < a.head_dim) v = load_pack<T, 4>(x + d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[i / 2][i % 2 * 4 + e] = v.e[e];
+    }
+  }
+
+  float m = -__builtin_inff(), l = 0.0f;
+  f32x4 o[DP / 16];
+#pragma unroll
+  for (int i = 0; i < DP / 16; ++i) o[i] = f32x4{0, 0, 0, 0};
+
+  const int* const table = a.c.table + (t.seq < 0 ? 0 : t.seq * a.c.table_stride);
+  const auto tile_start = [&](int i) {
+    return i < kt.sink_tiles ? i * KT : kt.low + (i - kt.sink_tiles) * KT;
+  };
+  // Page of the 16 keys from `key` on (PAGE16: they share it), or of one key.
+  const auto page_at = [&](int key) { return table[fast_div(min(key, kt.end - 1), a.c.by_page)]; };
+
+  // Loaded bytes of a tile. Keys past the end are read as the last one, absent
+  // pages as page 0: every address is inside the pool, and `there` tells.
+  u32x4 kreg[NB][NC], vreg[NV];
+  unsigned kcode[NB][NC], vcode[NV];
+  int pages[NB];     // of this lane's keys (PAGE16: of the blocks)
+  unsigned there[NB];
+  const int vkey = lane / S::kRowLanes, vpart = lane % S::kRowLanes * C;
+  const int vd = vpart < a.head_dim ? vpart : 0;
+
+  const auto look_up = [&](int i, int (&to)[NB]) {
+    const int k0 = tile_start(i);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) to[b] = page_at(PAGE16 ? k0 + 16 * b : k0 + 16 * b + col);
+  };
+  const auto load_k = [&](int i) {
+    const int k0 = tile_start(i);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const int key = min(k0 + 16 * b + col, kt.end - 1);
+      const bool ok = pages[b] >= 0 && pages[b] < a.c.num_pages;
+      const int slot = key - static_cast<int>(fast_div(key, a.c.by_page)) * a.c.page_size;
+      const int64_t page = ok ? pages[b] : 0;
+      const int64_t row = page * a.c.kst[0] + kvh * a.c.kst[1] + slot * a.c.kst[2];
+      const int64_t srow = MX ? page * a.c.ksst[0] + kvh * a.c.ksst[1] + slot * a.c.ksst[2] : 0;
+      there[b] = static_cast<unsigned>(__ballot(ok && k0 + 16 * b + col < kt.end)) & 0xffffu;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        int d = c * 4 * C + g * C;
+        d = d < a.head_dim ? d : 0;
+        if constexpr (MX) {
+          kreg[b][c] = load_pack<uint8_t, 16>(static_cast<const uint8_t*>(a.c.k) + row + d).raw;
+          kcode[b][c] = a.c.ks[srow + d / 32];
+        } else {
+          kreg[b][c] = load_pack<T, E>(static_cast<const T*>(a.c.k) + row + d).raw;
+        }
+      }
+    }
+  };
+  const auto load_v = [&](int i) {
+    const int k0 = tile_start(i);
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int key = min(k0 + n * S::kRowKeys + vkey, kt.end - 1);
+      const int b = n * S::kRowKeys / 16;
+      int pg = pages[b];
+      if constexpr (!PAGE16) pg = __shfl(pages[b], (n * S::kRowKeys + vkey) % 16);
+      const int64_t page = pg >= 0 && pg < a.c.num_pages ? pg : 0;
+      const int slot = key - static_cast<int>(fast_div(key, a.c.by_page)) * a.c.page_size;
+      if constexpr (MX) {
+        vreg[n] = load_pack<uint8_t, 16>(static_cast<const uint8_t*>(a.c.v) + page * a.c.vst[0] + kvh * a.c.vst[1] + slot * a.c.vst[2] + vd).raw;
+        vcode[n] = a.c.vs[page * a.c.vsst[0] + kvh * a.c.vsst[1] + slot * a.c.vsst[2] + vd / 32];
+      } else {
+        vreg[n] = load_pack<T, E>(static_cast<const T*>(a.c.v) + page * a.c.vst[0] + kvh * a.c.vst[1] + slot * a.c.vst[2] + vd).raw;
+      }
+    }
+  };
+
+  int i = begin + wave;
+  if (i < end) {
+    look_up(i, pages);
+    load_v(i);
+    load_k(i);
+  }
+  for (; i < end; i += WAVES) {
+    const int k0 = tile_start(i);
+    // Whether every live row sees every key of the tile.
+    unsigned all = 0xffffu;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) all &= there[b];
+    const bool whole = all == 0xffffu && k0 + KT - 1 <= first_pos && (a.window <= 0 || k0 > last_pos - a.window || k0 + KT <= a.sinks);
+    unsigned here[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) here[b] = there[b];
+    const bool more = i + WAVES < end;
+    int next_pages[NB];
+    if (more) look_up(i + WAVES, next_pages);
+
+    // V into LDS; rows that are not there as zeros.
+    wave_fence();
+    bool strange = false;  // values that 0 would not cancel
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int key = n * S::kRowKeys + vkey;
+      const bool ok = whole || (here[n * S::kRowKeys / 16] >> (key % 16) & 1);
+      if constexpr (MX) {
+        const float s = e8m0_scale(vcode[n]);
+        Eight<T> x = from_e4m3<T>(u32x2{vreg[n][0], vreg[n][1]}, s), y = from_e4m3<T>(u32x2{vreg[n][2], vreg[n][3]}, s);
+        if (!whole) {
+          if (!ok) x = y = zero_eight<T>();
+          strange |= not_finite(x) || not_finite(y);
+        }
+#pragma unroll
+        for (int h = 0; h < 16 / E; ++h)
+          *reinterpret_cast<u32x4*>(vt + lds_packet<S::kRowBytes>(key, lane % S::kRowLanes * (16 / E) + h)) =
+              h * E < 8 ? x.p[h * E % 8 / E].raw : y.p[h * E % 8 / E].raw;
+      } else {
+        Pack<T, E> x;
+        x.raw = vreg[n];
+        if (!whole) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            if (!ok) x.e[e] = from_f32<T>(0.0f);
+            strange |= !(__builtin_fabsf(to_f32(x.e[e])) < __builtin_inff());
+          }
+        }
+        *reinterpret_cast<u32x4*>(vt + lds_packet<S::kRowBytes>(key, lane % S::kRowLanes)) = x.raw;
+      }
+    }
+    wave_fence();
+    // S^T: block b holds keys k0 + 16 b + 4 g + r of query `col`.
+    f32x4 s[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      s[b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const bool in = c * 4 * C + g * C < a.head_dim;
+        if constexpr (MX) {
+          const float sc = e8m0_scale(kcode[b][c]);
+          Eight<T> x = from_e4m3<T>(u32x2{kreg[b][c][0], kreg[b][c][1]}, sc), y = from_e4m3<T>(u32x2{kreg[b][c][2], kreg[b][c][3]}, sc);
+          if (a.head_dim != DP && !in) x = y = zero_eight<T>();
+          s[b] = Mfma<T>::mul(x, q[2 * c], s[b]);
+          s[b] = Mfma<T>::mul(y, q[2 * c + 1], s[b]);
+        } else if constexpr (E == 8) {
+          Eight<T> x;
+          x.p[0].raw = kreg[b][c];
+          if (a.head_dim != DP && !in) x = zero_eight<T>();
+          s[b] = Mfma<T>::mul(x, q[c], s[b]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = a.head_dim != DP && !in ? 0.0f : __builtin_bit_cast(float, static_cast<unsigned>(kreg[b][c][e]));
+            s[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, q[c / 2][c % 2 * 4 + e], s[b], 0, 0, 0);
+          }
+        }
+      }
+    }
+    if (more) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) pages[b] = next_pages[b];
+      load_v(i + WAVES);
+      load_k(i + WAVES);
+    }
+
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float v = s[b][r] * a.scale_log2;
+        if (!whole) {
+          const int n = 4 * g + r, key = k0 + 16 * b + n;
+          const bool seen = key <= hi && (key >= lo || key < a.sinks) && (here[b] >> n & 1);
+          v = seen ? v : -__builtin_inff();
+        }
+        s[b][r] = v;
+        top = __builtin_fmaxf(top, v);
+      }
+    }
+    const float mn = __builtin_fmaxf(m, max_over_groups(top));
+    const float base = mn == -__builtin_inff() ? 0.0f : mn;
+    if (__ballot(mn != m)) {
+      const float keep = __builtin_amdgcn_exp2f(m - base);
+      l *= keep;
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) o[d] *= keep;
+      m = mn;
+    }
+    const float from = base - Mfma<T>::kShift;
+    Eight<T> p;  // NB * 4 are used
+    float pf[NB][4];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        pf[b][r] = __builtin_amdgcn_exp2f(s[b][r] - from);
+        l += pf[b][r];
+        p[4 * b + r] = from_f32<T>(pf[b][r]);
+      }
+
+    // O^T += V^T P^T.
+    if (__builtin_expect(!whole && __ballot(strange) != 0, 0)) {
+      // Infinities or NaN among values that not every row sees: 0 times them
+      // is not 0, so each row adds only the keys that it sees.
+      for (int n = 0; n < KT; ++n) {
+        const int b = n / 16, owner = n % 16 / 4 * 16 + col;
+        float w = 0.0f;
+#pragma unroll
+        for (int bb = 0; bb < NB; ++bb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float v = __shfl(pf[bb][r], owner);
+            if (bb == b && r == n % 4) w = v;
+          }
+        const int key = k0 + n;
+        unsigned hb = here[0];
+#pragma unroll
+        for (int bb = 1; bb < NB; ++bb) hb = b == bb ? here[bb] : hb;
+        const bool seen = key <= hi && (key >= lo || key < a.sinks) && (hb >> (n % 16) & 1);
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int e = 16 * d + 4 * g + r;
+            const float v = to_f32(*reinterpret_cast<const T*>(vt + lds_packet<S::kRowBytes>(n, e / E) + e % E * sizeof(T)));
+            o[d][r] = seen ? __builtin_fmaf(w, v, o[d][r]) : o[d][r];
+          }
+      }
+    } else {
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) {
+        if constexpr (E == 8) {
+          // Lane i of 16 gives the address of 8 bytes (key i / 4, elements 4 (i % 4) ..) and receives column i of the four keys.
+          const int at = 16 * d + 4 * (col % 4), key = 4 * g + col / 4;
+          Eight<T> v;
+          u32x2 half[NB];
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+            half[b] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4*)(vt + lds_packet<S::kRowBytes>(16 * b + key, at / 8) + at % 8 * 2)));
+          v.p[0].raw = u32x4{half[0][0], half[0][1], half[NB - 1][0], half[NB - 1][1]};
+          o[d] = Mfma<T>::mul(v, p, o[d]);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int e = 16 * d + col;
+            const float v = *reinterpret_cast<const float*>(vt + lds_packet<S::kRowBytes>(4 * g + r, e / 4) + e % 4 * 4);
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, pf[0][r], o[d], 0, 0, 0);
+          }
+        }
+      }
+    }
+  }
+
+  wave_fence();
+  // Join the wavefronts: o as rows of DP floats in the wavefront's own LDS, 16-byte
+  // packets exchanged by the row's number against bank conflicts.
+  l = sum_over_groups(l);
+  if (g == 0) lds_ml[wave][col] = float2{m, l};
+  float* const mine = reinterpret_cast<float*>(vt);
+#pragma unroll
+  for (int d = 0; d < DP / 16; ++d) *reinterpret_cast<f32x4*>(mine + col * DP + (((4 * d + g) ^ col) << 2)) = o[d];
+  __syncthreads();
+  for (int n = threadIdx.x; n < 16 * DP / 4; n += WAVES * kWave) {
+    const int row = n / (DP / 4), d = n % (DP / 4) * 4;
+    if (row >= live || d >= a.head_dim) continue;
+    float M = -__builtin_inff(), L = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) M = __builtin_fmaxf(M, lds_ml[w][row].x);
+    const float base = M == -__builtin_inff() ? 0.0f : M;
+    f32x4 x = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const float keep = __builtin_amdgcn_exp2f(lds_ml[w][row].x - base);
+      L += lds_ml[w][row].y * keep;
+      const f32x4 y = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + w * S::kTileBytes) + row * DP + (((d / 4) ^ row) << 2));
+      if (lds_ml[w][row].y != 0.0f) x += y * keep;  // a wavefront without keys holds nothing
+    }
+    const int token = fast_div(t.row0 + row, a.by_group);
+    const int64_t at = int64_t(t.token0 + token) * a.q_heads + kvh * a.group + (t.row0 + row - token * a.group);
+    if (a.splits > 1) {
+      if (d == 0) a.part_ml[split * a.rows + at] = float2{M, L};
+      if (L != 0.0f) *reinterpret_cast<f32x4*>(a.part_o + (split * a.rows + at) * a.head_dim + d) = x;
+    } else {
+      const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+      Pack<T, 4> y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y.e[e] = from_f32<T>(x[e] * inv);
+      store_pack<T, 4>(static_cast<T*>(a.out) + at * a.head_dim + d, y);
+    }
+  }
+}
+
+// ---- joining the parts of split key ranges ---------------------------------------
+// One wavefront per row: out = sum_s e^(m_s - M) o_s / sum_s e^(m_s - M) l_s, in the
+// order of the parts. A part without keys has l = 0 and is not read further.
+constexpr int kMaxSplits = 64;
+
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join(const float* __restrict__ part_o, const float2* __restrict__ part_ml,
+                                                 T* __restrict__ out, int64_t row0, int64_t end, int64_t rows, int splits,
+                                                 int head_dim) {
+  const int64_t row = row0 + int64_t(blockIdx.x) * 4 + threadIdx.x / kWave;
+  const int lane = threadIdx.x % kWave;
+  if (row >= end) return;
+  const float2 ml = lane < splits ? part_ml[lane * rows + row] : float2{-__builtin_inff(), 0.0f};
+  float M = ml.x;
+#pragma unroll
+  for (int k = 1; k < kWave; k *= 2) M = __builtin_fmaxf(M, __shfl_xor(M, k));
+  const float w = __builtin_amdgcn_exp2f(ml.x - (M == -__builtin_inff() ? 0.0f : M));
+  const uint64_t some = __ballot(ml.y != 0.0f);
+  float L = 0.0f, x[4] = {};
+  for (int s = 0; s < splits; ++s) {
+    if (!(some >> s & 1)) continue;
+    const float keep = __shfl(w, s);
+    L += __shfl(ml.y, s) * keep;
+    const int d = lane * 4;
+    if (d < head_dim) {
+      const f32x4 y = *reinterpret_cast<const f32x4*>(part_o + (s * rows + row) * head_dim + d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] += y[e] * keep;
+    }
+  }
+  const float inv = some ? 1.0f / L : 0.0f;
+  if (lane * 4 < head_dim) {
+    Pack<T, 4> y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y.e[e] = from_f32<T>(x[e] * inv);
+    store_pack<T, 4>(out + row * head_dim + lane * 4, y);
   }
 }
 
 namespace {
 
-template <typename T>
+constexpr int kWaves = 4;
+
+// How a call is cut up: known from what the host knows of it, so that the
+// workspace can be sized before the call.
+struct Plan {
+  int64_t tiles;  // row tiles
+  int splits;
+};
+
+Plan plan(const PagedAttentionArgs& a) {
+  const int64_t group = a.q_heads / a.c.kv_heads;
+  Plan p;
+  if (a.c.cu) p.tiles = a.c.tokens * group / 16 + a.c.n_seqs + 1;
+  else p.tiles = a.c.n_seqs * ceil_div(a.c.tokens / a.c.n_seqs * group, 16);
+  const int64_t want = 1024, blocks = p.tiles * a.c.kv_heads;
+  const int64_t most = ceil_div(a.c.table_width * a.c.page_size, 256);
+  p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({ceil_div(want, blocks), most, kMaxSplits})));
+  return p;
+}
+
+template <typename T, bool MX, int DP>
 hipError_t run(const PagedAttentionArgs& a, hipStream_t stream) {
+  const Plan p = plan(a);
   AttnDev d{};
   d.c = paged_dev(a.c);
   d.q = a.q;
   d.out = a.out;
   for (int i = 0; i < 3; ++i) d.qs[i] = a.qs[i];
+  d.rows = a.c.tokens * a.q_heads;
+  d.part_o = static_cast<float*>(a.workspace);
+  d.part_ml = reinterpret_cast<float2*>(d.part_o + p.splits * d.rows * a.c.head_dim);
   d.q_heads = static_cast<int>(a.q_heads);
+  d.kv_heads = static_cast<int>(a.c.kv_heads);
   d.group = static_cast<int>(a.q_heads / a.c.kv_heads);
   d.head_dim = static_cast<int>(a.c.head_dim);
   const int64_t most = std::numeric_limits<int>::max();
   d.window = static_cast<int>(std::min(a.window, most));
   d.sinks = static_cast<int>(std::min(a.sinks, most));
+  d.splits = p.splits;
+  d.min_tiles = 256 / RowsShape<T, MX, DP>::kKeys;
+  d.seq_tiles = static_cast<int>(a.c.cu ? 1 : ceil_div(a.c.tokens / a.c.n_seqs * d.group, 16));
   d.scale_log2 = a.scale * 1.44269504088896340736f;
-  d.by_heads = make_fastdiv(d.q_heads);
+  d.by_kv_heads = make_fastdiv(d.kv_heads);
   d.by_group = make_fastdiv(d.group);
-  const dim3 grid(static_cast<unsigned>(a.c.tokens * a.q_heads));
-  if (a.c.mx) AKO_LAUNCH((paged_attention_simple<T, true>), grid, dim3(kWave), 0, stream, d);
-  else AKO_LAUNCH((paged_attention_simple<T, false>), grid, dim3(kWave), 0, stream, d);
-  return hipGetLastError();
+  d.by_splits = make_fastdiv(d.splits);
+  d.by_seq_tiles = make_fastdiv(d.seq_tiles);
+  // Work-items of a launch stay below 2^32.
+  const int64_t per_tile = p.splits * a.c.kv_heads, most_tiles = std::max<int64_t>(1, (int64_t(1) << 22) / per_tile);
+  for (int64_t t0 = 0; t0 < p.tiles; t0 += most_tiles) {
+    d.tile0 = static_cast<int>(t0);
+    const dim3 grid(static_cast<unsigned>(std::min(most_tiles, p.tiles - t0) * per_tile));
+    if (a.c.page_size % 16 == 0) AKO_LAUNCH((attn_rows<T, MX, DP, kWaves, true>), grid, dim3(kWaves * kWave), 0, stream, d);
+    else AKO_LAUNCH((attn_rows<T, MX, DP, kWaves, false>), grid, dim3(kWaves * kWave), 0, stream, d);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return err;
+  }
+  if (p.splits == 1) return hipSuccess;
+  constexpr int64_t kJoinRows = int64_t(1) << 24;  // per launch
+  for (int64_t r0 = 0; r0 < d.rows; r0 += kJoinRows) {
+    const int64_t n = std::min(kJoinRows, d.rows - r0);
+    AKO_LAUNCH((attn_join<T>), dim3(static_cast<unsigned>(ceil_div(n, 4))), dim3(256), 0, stream, d.part_o, d.part_ml,
+               static_cast<T*>(a.out), r0, r0 + n, d.rows, d.splits, d.head_dim);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return err;
+  }
+  return hipSuccess;
+}
+
+template <typename T, bool MX>
+hipError_t by_head_dim(const PagedAttentionArgs& a, hipStream_t stream) {
+  if (a.c.head_dim <= 64) return run<T, MX, 64>(a, stream);
+  if (a.c.head_dim <= 128) return run<T, MX, 128>(a, stream);
+  return run<T, MX, 256>(a, stream);
 }
 
 }  // namespace
 
-int64_t paged_attention_workspace(const PagedAttentionArgs&) { return 0; }
+int64_t paged_attention_workspace(const PagedAttentionArgs& a) {
+  const Plan p = plan(a);
+  if (p.splits == 1) return 0;
+  return p.splits * a.c.tokens * a.q_heads * (a.c.head_dim + 2) * static_cast<int64_t>(sizeof(float));
+}
 
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t stream) {
   switch (a.dtype) {
-    case kF32: return run<float>(a, stream);
-    case kF16: return run<_Float16>(a, stream);
-    case kBF16: return run<__bf16>(a, stream);
+    case kF32: return a.c.mx ? by_head_dim<float, true>(a, stream) : by_head_dim<float, false>(a, stream);
+    case kF16: return a.c.mx ? by_head_dim<_Float16, true>(a, stream) : by_head_dim<_Float16, false>(a, stream);
+    case kBF16: return a.c.mx ? by_head_dim<__bf16, true>(a, stream) : by_head_dim<__bf16, false>(a, stream);
     default: return hipErrorInvalidValue;
   }
 }

@@ -23,6 +23,7 @@
 // kernel in order of the split, so results do not depend on scheduling.
 
 #include <algorithm>
+#include <cmath>
 #include <limits>
 
 #include "paged.h"
@@ -47,7 +48,8 @@ struct AttnDev {
   int tile0;              // first row tile of the launch
   int splits, min_tiles;  // at most `splits` parts of a row tile's keys, of at least min_tiles tiles
   int seq_tiles;          // row tiles per sequence (uniform steps)
-  float scale_log2;       // scale * log2(e): exponentials are of base 2
+  float scale_log2;       // |scale| * log2(e), above 0: exponentials are of base 2
+  unsigned q_sign;        // sign bits to flip in a word of q (scale < 0)
   FastDiv by_kv_heads, by_group, by_splits, by_seq_tiles;
 };
 
@@ -137,6 +139,12 @@ template <> struct Mfma<float> {
   }
 };
 
+template <typename T>
+__device__ __forceinline__ void flip_sign(Eight<T>& x, unsigned bits) {
+#pragma unroll
+  for (int i = 0; i < 8 / Eight<T>::kPer; ++i) x.p[i].raw ^= bits;
+}
+
 // Orders LDS accesses of one wavefront's lanes to each other's data. The LDS
 // serves a wavefront in order; only the compiler has to be held.
 __device__ __forceinline__ void wave_fence() {
@@ -153,12 +161,30 @@ __device__ __forceinline__ float sum_over_groups(float v) {
   return v + __shfl_xor(v, 32);
 }
 
-template <typename T>
-__device__ __forceinline__ bool not_finite(const Eight<T>& x) {
-  bool bad = false;
+// Nonzero where a word of values holds an infinity or NaN (or might, once
+// multiplied by its scale): their exponents are all ones, and one more in the exponent's
+// last place then carries into the sign's, which was masked out. e4m3 has only NaN,
+// all ones below the sign; in fp16 scales from 2^8 on can take it past the end.
+template <typename T, bool MX>
+__device__ __forceinline__ unsigned odd_values(u32x4 w, unsigned code) {
+  constexpr unsigned kMask = MX ? 0x7f7f7f7fu : sizeof(T) == 4 ? 0x7f800000u : __is_same(T, __bf16) ? 0x7f807f80u : 0x7c007c00u;
+  constexpr unsigned kOne = MX ? 0x01010101u : sizeof(T) == 4 ? 0x00800000u : __is_same(T, __bf16) ? 0x00800080u : 0x04000400u;
+  constexpr unsigned kSign = MX ? 0x80808080u : sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+  unsigned odd = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) bad |= !(__builtin_fabsf(to_f32(x[i])) < __builtin_inff());
-  return bad;
+  for (int i = 0; i < 4; ++i) odd |= (w[i] & kMask) + kOne;
+  odd &= kSign;
+  if constexpr (MX && __is_same(T, _Float16)) odd |= code >= 127 + 8;
+  return odd;
+}
+
+// The keys of a tile of up to 64, from k0 on, that a row sees of those that are
+// there: j <= hi, and j >= lo or j < sinks.
+__device__ __forceinline__ uint64_t below(int n) {
+  return n <= 0 ? 0 : n >= 64 ? ~uint64_t(0) : (uint64_t(1) << n) - 1;
+}
+__device__ __forceinline__ uint64_t keys_seen(uint64_t there, int k0, int lo, int hi, int sinks) {
+  return there & below(hi + 1 - k0) & (~below(lo - k0) | below(sinks - k0));
 }
 
 // ---- up to 16 rows per workgroup -------------------------------------------------
@@ -226,8 +252,8 @@ __global__ __launch_bounds__(WAVES* kWave) void attn_rows(AttnDev a) {
   // This lane's query row, in the order of the K operand.
   const bool row_live = col < live;
   const int hi = row_live ? t.pos0 + my_token : -1;
-  const int lo = a.window > 0 ? max(hi, 0) - a.window + 1 : 0;
-  Eight<T> q[NC * C / 8 > 0 ? NC * C / 8 : 1];
+  const int lo = a.window > 0 ? max(0, max(hi, 0) - a.window + 1) : 0;
+  Eight<T> q[NC * C / 8];
   {
     const int b = a.c.cu ? 0 : t.seq;
     const T* x = static_cast<const T*>(a.q) + b * a.qs[0] + (t.token0 - b * a.c.seq + my_token) * a.qs[1] + my_head * a.qs[2];
@@ -241,6 +267,8 @@ __global__ __launch_bounds__(WAVES* kWave) void attn_rows(AttnDev a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) q[i / 2][i % 2 * 4 + e] = v.e[e];
     }
+#pragma unroll
+    for (int i = 0; i < NC * C / 8; ++i) flip_sign(q[i], a.q_sign);
   }
 
   float m = -__builtin_inff(), l = 0.0f;
@@ -260,7 +288,7 @@ __global__ __launch_bounds__(WAVES* kWave) void attn_rows(AttnDev a) {
   u32x4 kreg[NB][NC], vreg[NV];
   unsigned kcode[NB][NC], vcode[NV];
   int pages[NB];     // of this lane's keys (PAGE16: of the blocks)
-  unsigned there[NB];
+  unsigned there = 0;
   const int vkey = lane / S::kRowLanes, vpart = lane % S::kRowLanes * C;
   const int vd = vpart < a.head_dim ? vpart : 0;
 
@@ -279,7 +307,8 @@ __global__ __launch_bounds__(WAVES* kWave) void attn_rows(AttnDev a) {
       const int64_t page = ok ? pages[b] : 0;
       const int64_t row = page * a.c.kst[0] + kvh * a.c.kst[1] + slot * a.c.kst[2];
       const int64_t srow = MX ? page * a.c.ksst[0] + kvh * a.c.ksst[1] + slot * a.c.ksst[2] : 0;
-      there[b] = static_cast<unsigned>(__ballot(ok && k0 + 16 * b + col < kt.end)) & 0xffffu;
+      const unsigned bits = static_cast<unsigned>(__ballot(ok && k0 + 16 * b + col < kt.end)) & 0xffffu;
+      there = b == 0 ? bits : there | bits << 16;
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         int d = c * 4 * C + g * C;
@@ -321,46 +350,37 @@ __global__ __launch_bounds__(WAVES* kWave) void attn_rows(AttnDev a) {
   for (; i < end; i += WAVES) {
     const int k0 = tile_start(i);
     // Whether every live row sees every key of the tile.
-    unsigned all = 0xffffu;
-#pragma unroll
-    for (int b = 0; b < NB; ++b) all &= there[b];
-    const bool whole = all == 0xffffu && k0 + KT - 1 <= first_pos && (a.window <= 0 || k0 > last_pos - a.window || k0 + KT <= a.sinks);
-    unsigned here[NB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) here[b] = there[b];
+    const unsigned here = there;
+    const bool whole = here == (KT == 32 ? ~0u : 0xffffu) && k0 + KT - 1 <= first_pos &&
+                       (a.window <= 0 || k0 > last_pos - a.window || k0 + KT <= a.sinks);
+    const unsigned seen = whole ? ~0u : static_cast<unsigned>(keys_seen(here, k0, lo, hi, a.sinks));
     const bool more = i + WAVES < end;
     int next_pages[NB];
     if (more) look_up(i + WAVES, next_pages);
 
     // V into LDS; rows that are not there as zeros.
     wave_fence();
-    bool strange = false;  // values that 0 would not cancel
+    unsigned odd = 0;  // values that a weight of 0 would not cancel
+    if (!whole) {
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const int key = n * S::kRowKeys + vkey;
+        if (!(here >> key & 1)) vreg[n] = u32x4{0, 0, 0, 0};
+        odd |= odd_values<T, MX>(vreg[n], MX ? vcode[n] : 0);
+      }
+    }
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const int key = n * S::kRowKeys + vkey;
-      const bool ok = whole || (here[n * S::kRowKeys / 16] >> (key % 16) & 1);
       if constexpr (MX) {
         const float s = e8m0_scale(vcode[n]);
         Eight<T> x = from_e4m3<T>(u32x2{vreg[n][0], vreg[n][1]}, s), y = from_e4m3<T>(u32x2{vreg[n][2], vreg[n][3]}, s);
-        if (!whole) {
-          if (!ok) x = y = zero_eight<T>();
-          strange |= not_finite(x) || not_finite(y);
-        }
 #pragma unroll
         for (int h = 0; h < 16 / E; ++h)
           *reinterpret_cast<u32x4*>(vt + lds_packet<S::kRowBytes>(key, lane % S::kRowLanes * (16 / E) + h)) =
               h * E < 8 ? x.p[h * E % 8 / E].raw : y.p[h * E % 8 / E].raw;
       } else {
-        Pack<T, E> x;
-        x.raw = vreg[n];
-        if (!whole) {
-#pragma unroll
-          for (int e = 0; e < E; ++e) {
-            if (!ok) x.e[e] = from_f32<T>(0.0f);
-            strange |= !(__builtin_fabsf(to_f32(x.e[e])) < __builtin_inff());
-          }
-        }
-        *reinterpret_cast<u32x4*>(vt + lds_packet<S::kRowBytes>(key, lane % S::kRowLanes)) = x.raw;
+        *reinterpret_cast<u32x4*>(vt + lds_packet<S::kRowBytes>(key, lane % S::kRowLanes)) = vreg[n];
       }
     }
     wave_fence();
@@ -405,11 +425,7 @@ __global__ __launch_bounds__(WAVES* kWave) void attn_rows(AttnDev a) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         float v = s[b][r] * a.scale_log2;
-        if (!whole) {
-          const int n = 4 * g + r, key = k0 + 16 * b + n;
-          const bool seen = key <= hi && (key >= lo || key < a.sinks) && (here[b] >> n & 1);
-          v = seen ? v : -__builtin_inff();
-        }
+        if (!whole) v = seen >> (16 * b + 4 * g + r) & 1 ? v : -__builtin_inff();
         s[b][r] = v;
         top = __builtin_fmaxf(top, v);
       }
@@ -436,7 +452,7 @@ __global__ __launch_bounds__(WAVES* kWave) void attn_rows(AttnDev a) {
       }
 
     // O^T += V^T P^T.
-    if (__builtin_expect(!whole && __ballot(strange) != 0, 0)) {
+    if (__builtin_expect(!whole && __ballot(odd != 0) != 0, 0)) {
       // Infinities or NaN among values that not every row sees: 0 times them
       // is not 0, so each row adds only the keys that it sees.
       for (int n = 0; n < KT; ++n) {
@@ -449,18 +465,14 @@ __global__ __launch_bounds__(WAVES* kWave) void attn_rows(AttnDev a) {
             const float v = __shfl(pf[bb][r], owner);
             if (bb == b && r == n % 4) w = v;
           }
-        const int key = k0 + n;
-        unsigned hb = here[0];
-#pragma unroll
-        for (int bb = 1; bb < NB; ++bb) hb = b == bb ? here[bb] : hb;
-        const bool seen = key <= hi && (key >= lo || key < a.sinks) && (hb >> (n % 16) & 1);
+        const bool add = seen >> n & 1;
 #pragma unroll
         for (int d = 0; d < DP / 16; ++d)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int e = 16 * d + 4 * g + r;
             const float v = to_f32(*reinterpret_cast<const T*>(vt + lds_packet<S::kRowBytes>(n, e / E) + e % E * sizeof(T)));
-            o[d][r] = seen ? __builtin_fmaf(w, v, o[d][r]) : o[d][r];
+            o[d][r] = add ? __builtin_fmaf(w, v, o[d][r]) : o[d][r];
           }
       }
     } else {
@@ -528,6 +540,321 @@ __global__ __launch_bounds__(WAVES* kWave) void attn_rows(AttnDev a) {
   }
 }
 
+// ---- many rows per workgroup ---------------------------------------------------------
+// Chunks of a prompt in half types: 32 rows per wavefront, which share each key
+// tile through LDS. Bound by the matrix cores and, about as much, by the
+// exponentials beside them: two workgroups fit on a CU, so that one's
+// exponentials run under the other's products. A tile's loads are issued a whole
+// tile ahead, into registers, and go to the other half of LDS after the
+// products of the tile before.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f32x16 mfma32(const Eight<__bf16>& a, const Eight<__bf16>& b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32(const Eight<_Float16>& a, const Eight<_Float16>& b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// LDS place of packet p of a key's row of K, which is read 16 bytes of 32 rows at a
+// time: sixteen rows' packets lie on different banks.
+template <int ROW_BYTES>
+__device__ __forceinline__ int lds_packet_k(int key, int p) {
+  constexpr int kPackets = ROW_BYTES / 16;
+  const int x = kPackets >= 16 ? key & 15 : (key >> 1) & (kPackets - 1);
+  return key * ROW_BYTES + ((p ^ x) << 4);
+}
+
+template <typename T, bool MX, int DP, int WAVES, bool PAGE16>
+__global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(AttnDev a) {
+  constexpr int KT = DP <= 128 ? 64 : 32, R = 32 * WAVES, KB = KT / 32;
+  constexpr int ROW = DP * 2, TILE = KT * ROW;       // bytes
+  constexpr int C = MX ? 16 : 8;                     // elements of a 16-byte load
+  constexpr int LANES = DP / C;                      // lanes across a row
+  constexpr int PASS = WAVES * kWave / LANES, NP = KT / PASS;  // keys per pass of the workgroup, passes
+  __shared__ __align__(16) unsigned char lds[2][2][TILE];  // buffer, K and V
+  __shared__ int lds_odd[2][WAVES];  // per buffer: V holds infinities or NaN
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+  const int col = lane % 32, h = lane / 32;
+
+  const unsigned nth = fast_div(blockIdx.x, a.by_kv_heads);
+  const int kvh = blockIdx.x - nth * a.kv_heads;
+  const unsigned tile_id = fast_div(nth, a.by_splits);
+  const int split = nth - tile_id * a.splits;
+  RowTile t;
+  if (!find_rows<R>(a, a.tile0 + tile_id, t)) return;
+
+  const int last_row = min(t.row0 + R, t.rows) - 1;
+  const auto pos_of = [&](int row) { return t.pos0 + static_cast<int>(fast_div(row, a.by_group)); };
+  const KeyTiles kt = t.seq < 0 ? KeyTiles{0, 0, 0, 0} : key_tiles<KT>(a, pos_of(t.row0), pos_of(last_row));
+  const int parts = max(1, min(a.splits, kt.count / a.min_tiles));
+  const int begin = split < parts ? static_cast<int>(static_cast<int64_t>(kt.count) * split / parts) : 0;
+  const int end = split < parts ? static_cast<int>(static_cast<int64_t>(kt.count) * (split + 1) / parts) : 0;
+  const int first_all = pos_of(t.row0), last_all = pos_of(last_row);
+
+  // The wavefront's rows, and this lane's query.
+  const int wrow0 = t.row0 + 32 * wave;
+  const bool busy = wrow0 <= last_row;
+  const int wfirst = busy ? pos_of(wrow0) : 0, wlast = busy ? pos_of(min(wrow0 + 31, last_row)) : -1;
+  const bool row_live = wrow0 + col <= last_row;
+  const int my_token = fast_div(wrow0 + col, a.by_group);
+  const int my_head = kvh * a.group + (wrow0 + col - my_token * a.group);
+  const int hi = row_live ? t.pos0 + my_token : -1;
+  const int lo = a.window > 0 ? max(0, max(hi, 0) - a.window + 1) : 0;
+  Eight<T> q[DP / 16];
+  {
+    const int b = a.c.cu ? 0 : t.seq;
+    const T* x = static_cast<const T*>(a.q) + b * a.qs[0] + (t.token0 - b * a.c.seq + my_token) * a.qs[1] + my_head * a.qs[2];
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+      const int d = 16 * i + 8 * h;
+      q[i] = zero_eight<T>();
+      if (row_live && d < a.head_dim) q[i] = load_eight<T>(x + d);
+      flip_sign(q[i], a.q_sign);
+    }
+  }
+
+  float m = -__builtin_inff(), l = 0.0f;
+  f32x16 o[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[i][r] = 0.0f;
+
+  const int* const table = a.c.table + (t.seq < 0 ? 0 : t.seq * a.c.table_stride);
+  const auto tile_start = [&](int i) {
+    return i < kt.sink_tiles ? i * KT : kt.low + (i - kt.sink_tiles) * KT;
+  };
+  // Lane j holds the page of the tile's key j (keys past the end: of the last one).
+  const auto look_up = [&](int i) {
+    return table[fast_div(min(tile_start(i) + lane % KT, kt.end - 1), a.c.by_page)];
+  };
+  const auto present = [&](int pg, int i) {
+    return __ballot(pg >= 0 && pg < a.c.num_pages && lane < KT && tile_start(i) + lane < kt.end);
+  };
+
+  u32x4 kreg[NP], vreg[NP];
+  unsigned kcode[NP], vcode[NP];
+  const int key0 = threadIdx.x / LANES, part = threadIdx.x % LANES;
+  const bool part_in = part * C < a.head_dim;
+  const int pd = part_in ? part * C : 0;
+  const auto load_tile = [&](int i, int pg) {
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+      const int j = n * PASS + key0, key = min(tile_start(i) + j, kt.end - 1);
+      // A wavefront's keys of one pass lie inside 16.
+      int page = PAGE16 ? __builtin_amdgcn_readlane(pg, n * PASS + wave * (kWave / LANES)) : __shfl(pg, j);
+      page = page >= 0 && page < a.c.num_pages ? page : 0;
+      const int slot = key - static_cast<int>(fast_div(key, a.c.by_page)) * a.c.page_size;
+      const int64_t kr = page * a.c.kst[0] + kvh * a.c.kst[1] + slot * a.c.kst[2] + pd;
+      const int64_t vr = page * a.c.vst[0] + kvh * a.c.vst[1] + slot * a.c.vst[2] + pd;
+      if constexpr (MX) {
+        kreg[n] = load_pack<uint8_t, 16>(static_cast<const uint8_t*>(a.c.k) + kr).raw;
+        vreg[n] = load_pack<uint8_t, 16>(static_cast<const uint8_t*>(a.c.v) + vr).raw;
+        kcode[n] = a.c.ks[page * a.c.ksst[0] + kvh * a.c.ksst[1] + slot * a.c.ksst[2] + pd / 32];
+        vcode[n] = a.c.vs[page * a.c.vsst[0] + kvh * a.c.vsst[1] + slot * a.c.vsst[2] + pd / 32];
+      } else {
+        kreg[n] = load_pack<T, 8>(static_cast<const T*>(a.c.k) + kr).raw;
+        vreg[n] = load_pack<T, 8>(static_cast<const T*>(a.c.v) + vr).raw;
+      }
+    }
+  };
+  // A tile that some row of the workgroup does not see whole.
+  const auto is_edge = [&](int i, uint64_t here, int first, int last) {
+    const int k0 = tile_start(i);
+    return here != (KT == 64 ? ~uint64_t(0) : (uint64_t(1) << (KT % 64)) - 1) || k0 + KT - 1 > first ||
+           (a.window > 0 && k0 <= last - a.window && k0 + KT > a.sinks);
+  };
+  const auto store_tile = [&](int i, int buf, uint64_t here) {
+    const bool edge = is_edge(i, here, first_all, last_all);
+    unsigned odd = 0;
+    if (edge) {
+#pragma unroll
+      for (int n = 0; n < NP; ++n) {
+        if (!(here >> (n * PASS + key0) & 1)) vreg[n] = u32x4{0, 0, 0, 0};
+        odd |= odd_values<T, MX>(vreg[n], MX ? vcode[n] : 0);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+      const int j = n * PASS + key0;
+      Eight<T> k[C / 8], v[C / 8];
+      if constexpr (MX) {
+        const float sk = e8m0_scale(kcode[n]), sv = e8m0_scale(vcode[n]);
+        k[0] = from_e4m3<T>(u32x2{kreg[n][0], kreg[n][1]}, sk);
+        k[1] = from_e4m3<T>(u32x2{kreg[n][2], kreg[n][3]}, sk);
+        v[0] = from_e4m3<T>(u32x2{vreg[n][0], vreg[n][1]}, sv);
+        v[1] = from_e4m3<T>(u32x2{vreg[n][2], vreg[n][3]}, sv);
+      } else {
+        k[0].p[0].raw = kreg[n];
+        v[0].p[0].raw = vreg[n];
+      }
+#pragma unroll
+      for (int c = 0; c < C / 8; ++c) {
+        if (a.head_dim != DP && !part_in) k[c] = zero_eight<T>();
+        const int p = part * (C / 8) + c;
+        *reinterpret_cast<u32x4*>(lds[buf][0] + lds_packet_k<ROW>(j, p)) = k[c].p[0].raw;
+        *reinterpret_cast<u32x4*>(lds[buf][1] + lds_packet<ROW>(j, p)) = v[c].p[0].raw;
+      }
+    }
+    const bool any = __ballot(odd != 0) != 0;
+    if (lane == 0) lds_odd[buf][wave] = any;
+  };
+
+  uint64_t here = 0;
+  int pg = 0;
+  if (begin < end) {
+    pg = look_up(begin);
+    here = present(pg, begin);
+    load_tile(begin, pg);
+    if (begin + 1 < end) pg = look_up(begin + 1);
+    store_tile(begin, 0, here);
+  }
+  __syncthreads();
+  for (int i = begin; i < end; ++i) {
+    const int buf = (i - begin) & 1, k0 = tile_start(i);
+    uint64_t next = 0;
+    if (i + 1 < end) {
+      load_tile(i + 1, pg);
+      next = present(pg, i + 1);
+      if (i + 2 < end) pg = look_up(i + 2);
+    }
+    if (busy && k0 <= wlast) {
+      const bool edge = is_edge(i, here, wfirst, wlast);
+      const unsigned char* const kl = lds[buf][0];
+      const unsigned char* const vl = lds[buf][1];
+      // S^T: block b holds keys k0 + 32 b + 8 (r / 4) + 4 h + r % 4 of query `col`.
+      f32x16 s[KB];
+#pragma unroll
+      for (int b = 0; b < KB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+          Eight<T> x;
+          x.p[0].raw = *reinterpret_cast<const u32x4*>(kl + lds_packet_k<ROW>(32 * b + col, 2 * d + h));
+          s[b] = mfma32(x, q[d], s[b]);
+        }
+      uint64_t seen = 0;
+      if (edge) {
+        seen = keys_seen(here, k0, lo, hi, a.sinks);
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+          const unsigned bits = static_cast<unsigned>(seen >> (32 * b)) >> (4 * h);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[b][r] = bits >> (8 * (r / 4) + r % 4) & 1 ? s[b][r] : -__builtin_inff();
+        }
+      }
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int b = 0; b < KB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = __builtin_fmaxf(top, s[b][r]);
+      const float mn = __builtin_fmaxf(m, __builtin_fmaxf(top, __shfl_xor(top, 32)));
+      const float base = mn == -__builtin_inff() ? 0.0f : mn;
+      if (__ballot(mn != m)) {
+        const float keep = __builtin_amdgcn_exp2f((m - base) * a.scale_log2);
+        l *= keep;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[d][r] *= keep;
+        m = mn;
+      }
+      const float from = Mfma<T>::kShift - base * a.scale_log2;
+      Eight<T> p[KT / 16];
+#pragma unroll
+      for (int b = 0; b < KB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[b][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], a.scale_log2, from));
+          l += s[b][r];
+          p[2 * b + r / 8][r % 8] = from_f32<T>(s[b][r]);
+        }
+      int odd = 0;
+      if (edge)
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) odd |= lds_odd[buf][w];
+      if (__builtin_expect(__builtin_amdgcn_readfirstlane(odd) != 0, 0)) {
+        // Infinities or NaN among values that not every row sees: each row adds
+        // only the keys that it sees.
+#pragma nounroll
+        for (int j = 0; j < KT; ++j) {
+          // Key j is element (j % 32 / 8 * 4 + j % 4) of block j / 32 on the half j % 8 / 4: a half word of p.
+          const int word = (j / 32 * 16 + j % 32 / 8 * 4 + j % 4) / 2, owner = j % 8 / 4 * 32 + col;
+          unsigned bits = 0;
+#pragma unroll
+          for (int k = 0; k < KT / 4; ++k) bits = k == word ? static_cast<unsigned>(p[k / 4].p[0].raw[k % 4]) : bits;
+          bits = __shfl(bits, owner) >> (j % 2 * 16);
+          const float w = to_f32(__builtin_bit_cast(T, static_cast<unsigned short>(bits)));
+          const bool add = seen >> j & 1;
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d) {
+            __builtin_amdgcn_sched_barrier(0);  // few values at a time: this path must not cost the others registers
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int e = 32 * d + 8 * (r / 4) + 4 * h + r % 4;
+              const float v = to_f32(*reinterpret_cast<const T*>(vl + lds_packet<ROW>(j, e / 8) + e % 8 * 2));
+              o[d][r] = add ? __builtin_fmaf(w, v, o[d][r]) : o[d][r];
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < KT / 16; ++j)
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d) {
+            // 16 lanes read four keys' 16 elements: keys 16 j + 4 h + (0..3), then 8 further.
+            const int at = 32 * d + 16 * (lane / 16 % 2) + 4 * (lane % 4), key = 16 * j + 4 * h + lane % 16 / 4;
+            u32x2 x[2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+              x[n] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (__attribute__((address_space(3))) s16x4*)(const_cast<unsigned char*>(vl) + lds_packet<ROW>(key + 8 * n, at / 8) + at % 8 * 2)));
+            Eight<T> v;
+            v.p[0].raw = u32x4{x[0][0], x[0][1], x[1][0], x[1][1]};
+            o[d] = mfma32(v, p[j], o[d]);
+          }
+      }
+    }
+    if (i + 1 < end) store_tile(i + 1, buf ^ 1, next);
+    here = next;
+    __syncthreads();
+  }
+
+  if (!row_live) return;
+  l += __shfl_xor(l, 32);
+  const int64_t at = int64_t(t.token0 + my_token) * a.q_heads + my_head;
+  if (a.splits > 1) {
+    if (h == 0) a.part_ml[split * a.rows + at] = float2{m * a.scale_log2, l};
+    if (l != 0.0f) {
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+          const int e = 32 * d + 2 * r + 4 * h;
+          if (e < a.head_dim)
+            *reinterpret_cast<f32x4*>(a.part_o + (split * a.rows + at) * a.head_dim + e) =
+                f32x4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
+        }
+    }
+    return;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int e = 32 * d + 2 * r + 4 * h;
+      Pack<T, 4> y;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) y.e[k] = from_f32<T>(o[d][r + k] * inv);
+      if (e < a.head_dim) store_pack<T, 4>(static_cast<T*>(a.out) + at * a.head_dim + e, y);
+    }
+}
+
 // ---- joining the parts of split key ranges ---------------------------------------
 // One wavefront per row: out = sum_s e^(m_s - M) o_s / sum_s e^(m_s - M) l_s, in the
 // order of the parts. A part without keys has l = 0 and is not read further.
@@ -570,20 +897,26 @@ __global__ __launch_bounds__(256) void attn_join(const float* __restrict__ part_
 namespace {
 
 constexpr int kWaves = 4;
+constexpr int kChunkRows = 32 * kWaves;
 
 // How a call is cut up: known from what the host knows of it, so that the
 // workspace can be sized before the call.
 struct Plan {
+  bool chunk;     // attn_chunk's row tiles, else attn_rows'
   int64_t tiles;  // row tiles
-  int splits;
+  int seq_tiles, splits;
 };
 
 Plan plan(const PagedAttentionArgs& a) {
   const int64_t group = a.q_heads / a.c.kv_heads;
-  Plan p;
-  if (a.c.cu) p.tiles = a.c.tokens * group / 16 + a.c.n_seqs + 1;
-  else p.tiles = a.c.n_seqs * ceil_div(a.c.tokens / a.c.n_seqs * group, 16);
-  const int64_t want = 1024, blocks = p.tiles * a.c.kv_heads;
+  Plan p{};
+  // Rows that share a key head, per sequence (on average in a packed step).
+  const int64_t rows = a.c.n_seqs > 0 ? ceil_div(a.c.tokens * group, a.c.n_seqs) : 1;
+  p.chunk = a.dtype != kF32 && rows > 16;
+  const int64_t r = p.chunk ? kChunkRows : 16;
+  p.seq_tiles = static_cast<int>(a.c.cu ? 1 : ceil_div(rows, r));
+  p.tiles = a.c.cu ? a.c.tokens * group / r + a.c.n_seqs + 1 : a.c.n_seqs * p.seq_tiles;
+  const int64_t want = p.chunk ? 512 : 1024, blocks = p.tiles * a.c.kv_heads;
   const int64_t most = ceil_div(a.c.table_width * a.c.page_size, 256);
   p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({ceil_div(want, blocks), most, kMaxSplits})));
   return p;
@@ -608,20 +941,34 @@ hipError_t run(const PagedAttentionArgs& a, hipStream_t stream) {
   d.window = static_cast<int>(std::min(a.window, most));
   d.sinks = static_cast<int>(std::min(a.sinks, most));
   d.splits = p.splits;
-  d.min_tiles = 256 / RowsShape<T, MX, DP>::kKeys;
-  d.seq_tiles = static_cast<int>(a.c.cu ? 1 : ceil_div(a.c.tokens / a.c.n_seqs * d.group, 16));
-  d.scale_log2 = a.scale * 1.44269504088896340736f;
+  d.seq_tiles = p.seq_tiles;
+  // Not 0: times it a masked score, -inf, has to stay that.
+  d.scale_log2 = std::max(std::fabs(a.scale) * 1.44269504088896340736f, std::numeric_limits<float>::min());
+  d.q_sign = a.scale < 0.0f ? (sizeof(T) == 4 ? 0x80000000u : 0x80008000u) : 0u;
   d.by_kv_heads = make_fastdiv(d.kv_heads);
   d.by_group = make_fastdiv(d.group);
   d.by_splits = make_fastdiv(d.splits);
   d.by_seq_tiles = make_fastdiv(d.seq_tiles);
   // Work-items of a launch stay below 2^32.
   const int64_t per_tile = p.splits * a.c.kv_heads, most_tiles = std::max<int64_t>(1, (int64_t(1) << 22) / per_tile);
+  const bool page16 = a.c.page_size % 16 == 0;
   for (int64_t t0 = 0; t0 < p.tiles; t0 += most_tiles) {
     d.tile0 = static_cast<int>(t0);
-    const dim3 grid(static_cast<unsigned>(std::min(most_tiles, p.tiles - t0) * per_tile));
-    if (a.c.page_size % 16 == 0) AKO_LAUNCH((attn_rows<T, MX, DP, kWaves, true>), grid, dim3(kWaves * kWave), 0, stream, d);
-    else AKO_LAUNCH((attn_rows<T, MX, DP, kWaves, false>), grid, dim3(kWaves * kWave), 0, stream, d);
+    const dim3 grid(static_cast<unsigned>(std::min(most_tiles, p.tiles - t0) * per_tile)), block(kWaves * kWave);
+    bool launched = false;
+    if constexpr (sizeof(T) == 2) {
+      if (p.chunk) {
+        d.min_tiles = DP <= 128 ? 4 : 8;
+        if (page16) AKO_LAUNCH((attn_chunk<T, MX, DP, kWaves, true>), grid, block, 0, stream, d);
+        else AKO_LAUNCH((attn_chunk<T, MX, DP, kWaves, false>), grid, block, 0, stream, d);
+        launched = true;
+      }
+    }
+    if (!launched) {
+      d.min_tiles = 256 / RowsShape<T, MX, DP>::kKeys;
+      if (page16) AKO_LAUNCH((attn_rows<T, MX, DP, kWaves, true>), grid, block, 0, stream, d);
+      else AKO_LAUNCH((attn_rows<T, MX, DP, kWaves, false>), grid, block, 0, stream, d);
+    }
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
   }

@@ -178,6 +178,71 @@ __device__ __forceinline__ unsigned odd_values(u32x4 w, unsigned code) {
   return odd;
 }
 
+// Infinities and NaN among values that not every row sees: a weight of 0 would
+// not cancel them. They are taken out of V (zeros in their places), and for
+// each of the head's elements two words of `masks` (DP of them, then DP more) tell which of a
+// wavefront's keys held +infinity and which -infinity there, NaN in both. A row
+// then adds the infinities of those keys that it does see (add_odd).
+// Bit n * KPW + w is the key of load n that is w-th among the KPW of the wavefront.
+template <typename T, bool MX, int DP, int KPW, int LOADS>
+__device__ __forceinline__ void take_out_odd(u32x4 (&v)[LOADS], const unsigned (&code)[LOADS], unsigned* masks, int lane) {
+  constexpr int C = MX ? 16 : 16 / static_cast<int>(sizeof(T)), LANES = DP / C;
+  const int part = lane % LANES;
+  unsigned plus[C] = {}, minus[C] = {};
+#pragma unroll
+  for (int n = 0; n < LOADS; ++n) {
+    T x[C];
+    if constexpr (MX) {
+      const float s = e8m0_scale(code[n]);
+      const Eight<T> a = from_e4m3<T>(u32x2{v[n][0], v[n][1]}, s), b = from_e4m3<T>(u32x2{v[n][2], v[n][3]}, s);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = a[e];
+        x[8 + e] = b[e];
+      }
+    } else {
+      Pack<T, C> w;
+      w.raw = v[n];
+#pragma unroll
+      for (int e = 0; e < C; ++e) x[e] = w.e[e];
+    }
+#pragma unroll
+    for (int e = 0; e < C; ++e) {
+      const float f = to_f32(x[e]);
+      const bool odd = !(__builtin_fabsf(f) < __builtin_inff());
+      const uint64_t up = __ballot(odd && !(f < 0.0f)), down = __ballot(odd && !(f > 0.0f));
+#pragma unroll
+      for (int w = 0; w < KPW; ++w) {
+        plus[e] |= static_cast<unsigned>(up >> (w * LANES + part) & 1) << (n * KPW + w);
+        minus[e] |= static_cast<unsigned>(down >> (w * LANES + part) & 1) << (n * KPW + w);
+      }
+      constexpr int kBits = 128 / C, kPerWord = 32 / kBits;  // of an element of v[n]
+      const unsigned all = kBits == 32 ? ~0u : ((1u << (kBits % 32)) - 1) << (e % kPerWord * kBits % 32);
+      v[n][e / kPerWord] = odd ? v[n][e / kPerWord] & ~all : v[n][e / kPerWord];
+    }
+  }
+  if (lane < LANES) {
+#pragma unroll
+    for (int e = 0; e < C; ++e) {
+      masks[part * C + e] = plus[e];
+      masks[DP + part * C + e] = minus[e];
+    }
+  }
+}
+
+// Adds to elements e .. e + 3 the infinities that a row sees.
+__device__ __forceinline__ float odd_sum(unsigned plus, unsigned minus) {
+  return (plus ? __builtin_inff() : 0.0f) - (minus ? __builtin_inff() : 0.0f);
+}
+template <int DP>
+__device__ __forceinline__ f32x4 odd_sums(const unsigned* masks, int e, unsigned seen) {
+  const u32x4 p = *reinterpret_cast<const u32x4*>(masks + e), m = *reinterpret_cast<const u32x4*>(masks + DP + e);
+  f32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = odd_sum(p[i] & seen, m[i] & seen);
+  return r;
+}
+
 // The keys of a tile of up to 64, from k0 on, that a row sees of those that are
 // there: j <= hi, and j >= lo or j < sinks.
 __device__ __forceinline__ uint64_t below(int n) {
@@ -185,6 +250,43 @@ __device__ __forceinline__ uint64_t below(int n) {
 }
 __device__ __forceinline__ uint64_t keys_seen(uint64_t there, int k0, int lo, int hi, int sinks) {
   return there & below(hi + 1 - k0) & (~below(lo - k0) | below(sinks - k0));
+}
+
+// Where a wavefront's load of a few keys' rows starts: those of the keys kw ..
+// kw + 15 at most, kw + `mine` being this lane's. `pages` holds the page of the
+// tile's key j in lane j, `at` is kw's place in the tile, `end` the number of
+// keys that may be read.
+//
+// PAGE16 (pages of a multiple of 16 slots, and kw .. inside 16): the page and the
+// slot are the wavefront's, so the row's address is scalar and a lane adds a
+// 32-bit offset that is the same for every tile. Slots past `end` inside a page
+// are read with it; blocks past `end` are read as the last one. Otherwise each
+// lane finds its own key's page, and keys past `end` are read as the last.
+// Absent pages are read as page 0. Every address is inside the pool.
+struct RowPlace {
+  int page, slot;
+};
+template <bool PAGE16>
+__device__ __forceinline__ RowPlace row_place(const PagedDev& c, int pages, int kw, int at, int mine, int end) {
+  int page, key;
+  if constexpr (PAGE16) {
+    page = __builtin_amdgcn_readlane(pages, at);
+    key = kw < end ? kw : (end - 1) / 16 * 16 + kw % 16;
+  } else {
+    page = __shfl(pages, at + mine);
+    key = min(kw + mine, end - 1);
+  }
+  const int slot = key - static_cast<int>(fast_div(key, c.by_page)) * c.page_size;
+  return RowPlace{page >= 0 && page < c.num_pages ? page : 0, slot};
+}
+__device__ __forceinline__ const uint8_t* row_at(const void* pool, const int64_t (&st)[3], RowPlace r, int head, int elem) {
+  return static_cast<const uint8_t*>(pool) + (r.page * st[0] + head * st[1] + r.slot * st[2]) * elem;
+}
+// Sixteen bytes of a row of T (or, MX, of e4m3), aligned as its elements are.
+template <typename T, bool MX>
+__device__ __forceinline__ u32x4 load16(const uint8_t* p) {
+  if constexpr (MX) return load_pack<uint8_t, 16>(p).raw;
+  else return load_pack<T, 16 / static_cast<int>(sizeof(T))>(reinterpret_cast<const T*>(p)).raw;
 }
 
 // ---- up to 16 rows per workgroup -------------------------------------------------
@@ -220,12 +322,13 @@ __device__ __forceinline__ int lds_packet(int key, int p) {
 }
 
 template <typename T, bool MX, int DP, int WAVES, bool PAGE16>
-__global__ __launch_bounds__(WAVES* kWave) void attn_rows(AttnDev a) {
+__global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 ? 3 : DP * sizeof(T) <= 256 ? 2 : 1) void attn_rows(AttnDev a) {
   using S = RowsShape<T, MX, DP>;
   constexpr int KT = S::kKeys, NB = S::kBlocks, NC = S::kChunks, C = S::kChunk, NV = S::kLoads;
   constexpr int E = 16 / static_cast<int>(sizeof(T));  // elements of an LDS packet
   __shared__ __align__(16) unsigned char lds[WAVES * S::kTileBytes];
   __shared__ float2 lds_ml[WAVES][16];
+  __shared__ __align__(16) unsigned lds_odd[WAVES][2 * DP];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
   const int col = lane % 16, g = lane / 16;
   unsigned char* const vt = lds + wave * S::kTileBytes;
@@ -280,72 +383,61 @@ __global__ __launch_bounds__(WAVES* kWave) void attn_rows(AttnDev a) {
   const auto tile_start = [&](int i) {
     return i < kt.sink_tiles ? i * KT : kt.low + (i - kt.sink_tiles) * KT;
   };
-  // Page of the 16 keys from `key` on (PAGE16: they share it), or of one key.
-  const auto page_at = [&](int key) { return table[fast_div(min(key, kt.end - 1), a.c.by_page)]; };
+  // Lane j holds the page of the tile's key j (keys past the end: of the last one).
+  const auto look_up = [&](int i) {
+    return table[fast_div(min(tile_start(i) + lane % KT, kt.end - 1), a.c.by_page)];
+  };
 
-  // Loaded bytes of a tile. Keys past the end are read as the last one, absent
-  // pages as page 0: every address is inside the pool, and `there` tells.
+  // Loaded bytes of a tile, and which of its keys are there.
   u32x4 kreg[NB][NC], vreg[NV];
   unsigned kcode[NB][NC], vcode[NV];
-  int pages[NB];     // of this lane's keys (PAGE16: of the blocks)
   unsigned there = 0;
   const int vkey = lane / S::kRowLanes, vpart = lane % S::kRowLanes * C;
-  const int vd = vpart < a.head_dim ? vpart : 0;
-
-  const auto look_up = [&](int i, int (&to)[NB]) {
-    const int k0 = tile_start(i);
+  constexpr int EB = MX ? 1 : sizeof(T);
+  unsigned koff[NC], kcoff[NC];
 #pragma unroll
-    for (int b = 0; b < NB; ++b) to[b] = page_at(PAGE16 ? k0 + 16 * b : k0 + 16 * b + col);
-  };
-  const auto load_k = [&](int i) {
+  for (int c = 0; c < NC; ++c) {
+    const int d = c * 4 * C + g * C < a.head_dim ? c * 4 * C + g * C : 0;
+    koff[c] = ((PAGE16 ? col * static_cast<unsigned>(a.c.kst[2]) : 0) + d) * EB;
+    kcoff[c] = (PAGE16 ? col * static_cast<unsigned>(a.c.ksst[2]) : 0) + d / 32;
+  }
+  const int vd = vpart < a.head_dim ? vpart : 0;
+  const unsigned voff = ((PAGE16 ? vkey * static_cast<unsigned>(a.c.vst[2]) : 0) + vd) * EB;
+  const unsigned vcoff = (PAGE16 ? vkey * static_cast<unsigned>(a.c.vsst[2]) : 0) + vd / 32;
+
+  const auto load_k = [&](int i, int pages) {
     const int k0 = tile_start(i);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      const int key = min(k0 + 16 * b + col, kt.end - 1);
-      const bool ok = pages[b] >= 0 && pages[b] < a.c.num_pages;
-      const int slot = key - static_cast<int>(fast_div(key, a.c.by_page)) * a.c.page_size;
-      const int64_t page = ok ? pages[b] : 0;
-      const int64_t row = page * a.c.kst[0] + kvh * a.c.kst[1] + slot * a.c.kst[2];
-      const int64_t srow = MX ? page * a.c.ksst[0] + kvh * a.c.ksst[1] + slot * a.c.ksst[2] : 0;
-      const unsigned bits = static_cast<unsigned>(__ballot(ok && k0 + 16 * b + col < kt.end)) & 0xffffu;
-      there = b == 0 ? bits : there | bits << 16;
+      const RowPlace r = row_place<PAGE16>(a.c, pages, k0 + 16 * b, 16 * b, col, kt.end);
+      const uint8_t* const x = row_at(a.c.k, a.c.kst, r, kvh, EB);
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        int d = c * 4 * C + g * C;
-        d = d < a.head_dim ? d : 0;
-        if constexpr (MX) {
-          kreg[b][c] = load_pack<uint8_t, 16>(static_cast<const uint8_t*>(a.c.k) + row + d).raw;
-          kcode[b][c] = a.c.ks[srow + d / 32];
-        } else {
-          kreg[b][c] = load_pack<T, E>(static_cast<const T*>(a.c.k) + row + d).raw;
-        }
+      for (int c = 0; c < NC; ++c) kreg[b][c] = load16<T, MX>(x + koff[c]);
+      if constexpr (MX) {
+        const uint8_t* const y = row_at(a.c.ks, a.c.ksst, r, kvh, 1);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) kcode[b][c] = y[kcoff[c]];
       }
     }
+    there = static_cast<unsigned>(__ballot(pages >= 0 && pages < a.c.num_pages && lane < KT && k0 + lane < kt.end));
   };
-  const auto load_v = [&](int i) {
+  const auto load_v = [&](int i, int pages) {
     const int k0 = tile_start(i);
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
-      const int key = min(k0 + n * S::kRowKeys + vkey, kt.end - 1);
-      const int b = n * S::kRowKeys / 16;
-      int pg = pages[b];
-      if constexpr (!PAGE16) pg = __shfl(pages[b], (n * S::kRowKeys + vkey) % 16);
-      const int64_t page = pg >= 0 && pg < a.c.num_pages ? pg : 0;
-      const int slot = key - static_cast<int>(fast_div(key, a.c.by_page)) * a.c.page_size;
-      if constexpr (MX) {
-        vreg[n] = load_pack<uint8_t, 16>(static_cast<const uint8_t*>(a.c.v) + page * a.c.vst[0] + kvh * a.c.vst[1] + slot * a.c.vst[2] + vd).raw;
-        vcode[n] = a.c.vs[page * a.c.vsst[0] + kvh * a.c.vsst[1] + slot * a.c.vsst[2] + vd / 32];
-      } else {
-        vreg[n] = load_pack<T, E>(static_cast<const T*>(a.c.v) + page * a.c.vst[0] + kvh * a.c.vst[1] + slot * a.c.vst[2] + vd).raw;
-      }
+      const RowPlace r = row_place<PAGE16>(a.c, pages, k0 + n * S::kRowKeys, n * S::kRowKeys, vkey, kt.end);
+      vreg[n] = load16<T, MX>(row_at(a.c.v, a.c.vst, r, kvh, EB) + voff);
+      if constexpr (MX) vcode[n] = row_at(a.c.vs, a.c.vsst, r, kvh, 1)[vcoff];
     }
   };
 
   int i = begin + wave;
+  int pages = 0;  // of the next tile
   if (i < end) {
-    look_up(i, pages);
-    load_v(i);
-    load_k(i);
+    pages = look_up(i);
+    load_v(i, pages);
+    load_k(i, pages);
+    if (i + WAVES < end) pages = look_up(i + WAVES);
   }
   for (; i < end; i += WAVES) {
     const int k0 = tile_start(i);
@@ -355,8 +447,6 @@ __global__ __launch_bounds__(WAVES* kWave) void attn_rows(AttnDev a) {
                        (a.window <= 0 || k0 > last_pos - a.window || k0 + KT <= a.sinks);
     const unsigned seen = whole ? ~0u : static_cast<unsigned>(keys_seen(here, k0, lo, hi, a.sinks));
     const bool more = i + WAVES < end;
-    int next_pages[NB];
-    if (more) look_up(i + WAVES, next_pages);
 
     // V into LDS; rows that are not there as zeros.
     wave_fence();
@@ -368,6 +458,8 @@ __global__ __launch_bounds__(WAVES* kWave) void attn_rows(AttnDev a) {
         if (!(here >> key & 1)) vreg[n] = u32x4{0, 0, 0, 0};
         odd |= odd_values<T, MX>(vreg[n], MX ? vcode[n] : 0);
       }
+      odd = __ballot(odd != 0) != 0;
+      if (__builtin_expect(odd, 0)) take_out_odd<T, MX, DP, S::kRowKeys, NV>(vreg, vcode, lds_odd[wave], lane);
     }
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
@@ -413,10 +505,9 @@ __global__ __launch_bounds__(WAVES* kWave) void attn_rows(AttnDev a) {
       }
     }
     if (more) {
-#pragma unroll
-      for (int b = 0; b < NB; ++b) pages[b] = next_pages[b];
-      load_v(i + WAVES);
-      load_k(i + WAVES);
+      load_v(i + WAVES, pages);
+      load_k(i + WAVES, pages);
+      if (i + 2 * WAVES < end) pages = look_up(i + 2 * WAVES);
     }
 
     float top = -__builtin_inff();
@@ -452,52 +543,31 @@ __global__ __launch_bounds__(WAVES* kWave) void attn_rows(AttnDev a) {
       }
 
     // O^T += V^T P^T.
-    if (__builtin_expect(!whole && __ballot(odd != 0) != 0, 0)) {
-      // Infinities or NaN among values that not every row sees: 0 times them
-      // is not 0, so each row adds only the keys that it sees.
-      for (int n = 0; n < KT; ++n) {
-        const int b = n / 16, owner = n % 16 / 4 * 16 + col;
-        float w = 0.0f;
 #pragma unroll
-        for (int bb = 0; bb < NB; ++bb)
+    for (int d = 0; d < DP / 16; ++d) {
+      if constexpr (E == 8) {
+        // Lane i of 16 gives the address of 8 bytes (key i / 4, elements 4 (i % 4) ..) and receives column i of the four keys.
+        const int at = 16 * d + 4 * (col % 4), key = 4 * g + col / 4;
+        Eight<T> v;
+        u32x2 half[NB];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float v = __shfl(pf[bb][r], owner);
-            if (bb == b && r == n % 4) w = v;
-          }
-        const bool add = seen >> n & 1;
+        for (int b = 0; b < NB; ++b)
+          half[b] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) s16x4*)(vt + lds_packet<S::kRowBytes>(16 * b + key, at / 8) + at % 8 * 2)));
+        v.p[0].raw = u32x4{half[0][0], half[0][1], half[NB - 1][0], half[NB - 1][1]};
+        o[d] = Mfma<T>::mul(v, p, o[d]);
+      } else {
 #pragma unroll
-        for (int d = 0; d < DP / 16; ++d)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int e = 16 * d + 4 * g + r;
-            const float v = to_f32(*reinterpret_cast<const T*>(vt + lds_packet<S::kRowBytes>(n, e / E) + e % E * sizeof(T)));
-            o[d][r] = add ? __builtin_fmaf(w, v, o[d][r]) : o[d][r];
-          }
-      }
-    } else {
-#pragma unroll
-      for (int d = 0; d < DP / 16; ++d) {
-        if constexpr (E == 8) {
-          // Lane i of 16 gives the address of 8 bytes (key i / 4, elements 4 (i % 4) ..) and receives column i of the four keys.
-          const int at = 16 * d + 4 * (col % 4), key = 4 * g + col / 4;
-          Eight<T> v;
-          u32x2 half[NB];
-#pragma unroll
-          for (int b = 0; b < NB; ++b)
-            half[b] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4*)(vt + lds_packet<S::kRowBytes>(16 * b + key, at / 8) + at % 8 * 2)));
-          v.p[0].raw = u32x4{half[0][0], half[0][1], half[NB - 1][0], half[NB - 1][1]};
-          o[d] = Mfma<T>::mul(v, p, o[d]);
-        } else {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int e = 16 * d + col;
-            const float v = *reinterpret_cast<const float*>(vt + lds_packet<S::kRowBytes>(4 * g + r, e / 4) + e % 4 * 4);
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, pf[0][r], o[d], 0, 0, 0);
-          }
+        for (int r = 0; r < 4; ++r) {
+          const int e = 16 * d + col;
+          const float v = *reinterpret_cast<const float*>(vt + lds_packet<S::kRowBytes>(4 * g + r, e / 4) + e % 4 * 4);
+          o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, pf[0][r], o[d], 0, 0, 0);
         }
       }
+    }
+    if (__builtin_expect(odd, 0)) {
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) o[d] += odd_sums<DP>(lds_odd[wave], 16 * d + 4 * g, seen);
     }
   }
 
@@ -565,6 +635,21 @@ __device__ __forceinline__ int lds_packet_k(int key, int p) {
   return key * ROW_BYTES + ((p ^ x) << 4);
 }
 
+// Four keys' (from `key` on) 16 elements (from d on) transposed by 16 lanes: a lane
+// gives the address of 8 bytes and receives its column; then the same 8 keys on.
+template <typename T, int ROW_BYTES>
+__device__ __forceinline__ Eight<T> read_v(const unsigned char* v, int d, int key, int lane) {
+  const int at = d + 4 * (lane % 4), k = key + lane % 16 / 4;
+  u32x2 x[2];
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+    x[n] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) s16x4*)(const_cast<unsigned char*>(v) + lds_packet<ROW_BYTES>(k + 8 * n, at / 8) + at % 8 * 2)));
+  Eight<T> r;
+  r.p[0].raw = u32x4{x[0][0], x[0][1], x[1][0], x[1][1]};
+  return r;
+}
+
 template <typename T, bool MX, int DP, int WAVES, bool PAGE16>
 __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(AttnDev a) {
   constexpr int KT = DP <= 128 ? 64 : 32, R = 32 * WAVES, KB = KT / 32;
@@ -573,7 +658,8 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
   constexpr int LANES = DP / C;                      // lanes across a row
   constexpr int PASS = WAVES * kWave / LANES, NP = KT / PASS;  // keys per pass of the workgroup, passes
   __shared__ __align__(16) unsigned char lds[2][2][TILE];  // buffer, K and V
-  __shared__ int lds_odd[2][WAVES];  // per buffer: V holds infinities or NaN
+  __shared__ int lds_odd[2][WAVES];  // of edge tiles: whether infinities or NaN were taken out of V
+  __shared__ __align__(16) unsigned lds_masks[2][WAVES][2 * DP];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
   const int col = lane % 32, h = lane / 32;
 
@@ -635,27 +721,25 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
 
   u32x4 kreg[NP], vreg[NP];
   unsigned kcode[NP], vcode[NP];
+  constexpr int KPW = kWave / LANES;  // keys of a wavefront's load: at most 16, and they lie inside 16
+  constexpr int EB = MX ? 1 : 2;
   const int key0 = threadIdx.x / LANES, part = threadIdx.x % LANES;
   const bool part_in = part * C < a.head_dim;
-  const int pd = part_in ? part * C : 0;
-  const auto load_tile = [&](int i, int pg) {
+  const int pd = part_in ? part * C : 0, wkey = lane / LANES;
+  const unsigned koff = ((PAGE16 ? wkey * static_cast<unsigned>(a.c.kst[2]) : 0) + pd) * EB;
+  const unsigned voff = ((PAGE16 ? wkey * static_cast<unsigned>(a.c.vst[2]) : 0) + pd) * EB;
+  const unsigned kcoff = (PAGE16 ? wkey * static_cast<unsigned>(a.c.ksst[2]) : 0) + pd / 32;
+  const unsigned vcoff = (PAGE16 ? wkey * static_cast<unsigned>(a.c.vsst[2]) : 0) + pd / 32;
+  const auto load_tile = [&](int i, int pages) {
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
-      const int j = n * PASS + key0, key = min(tile_start(i) + j, kt.end - 1);
-      // A wavefront's keys of one pass lie inside 16.
-      int page = PAGE16 ? __builtin_amdgcn_readlane(pg, n * PASS + wave * (kWave / LANES)) : __shfl(pg, j);
-      page = page >= 0 && page < a.c.num_pages ? page : 0;
-      const int slot = key - static_cast<int>(fast_div(key, a.c.by_page)) * a.c.page_size;
-      const int64_t kr = page * a.c.kst[0] + kvh * a.c.kst[1] + slot * a.c.kst[2] + pd;
-      const int64_t vr = page * a.c.vst[0] + kvh * a.c.vst[1] + slot * a.c.vst[2] + pd;
+      const int at = n * PASS + wave * KPW;
+      const RowPlace r = row_place<PAGE16>(a.c, pages, tile_start(i) + at, at, wkey, kt.end);
+      kreg[n] = load16<T, MX>(row_at(a.c.k, a.c.kst, r, kvh, EB) + koff);
+      vreg[n] = load16<T, MX>(row_at(a.c.v, a.c.vst, r, kvh, EB) + voff);
       if constexpr (MX) {
-        kreg[n] = load_pack<uint8_t, 16>(static_cast<const uint8_t*>(a.c.k) + kr).raw;
-        vreg[n] = load_pack<uint8_t, 16>(static_cast<const uint8_t*>(a.c.v) + vr).raw;
-        kcode[n] = a.c.ks[page * a.c.ksst[0] + kvh * a.c.ksst[1] + slot * a.c.ksst[2] + pd / 32];
-        vcode[n] = a.c.vs[page * a.c.vsst[0] + kvh * a.c.vsst[1] + slot * a.c.vsst[2] + pd / 32];
-      } else {
-        kreg[n] = load_pack<T, 8>(static_cast<const T*>(a.c.k) + kr).raw;
-        vreg[n] = load_pack<T, 8>(static_cast<const T*>(a.c.v) + vr).raw;
+        kcode[n] = row_at(a.c.ks, a.c.ksst, r, kvh, 1)[kcoff];
+        vcode[n] = row_at(a.c.vs, a.c.vsst, r, kvh, 1)[vcoff];
       }
     }
   };
@@ -674,6 +758,9 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
         if (!(here >> (n * PASS + key0) & 1)) vreg[n] = u32x4{0, 0, 0, 0};
         odd |= odd_values<T, MX>(vreg[n], MX ? vcode[n] : 0);
       }
+      odd = __ballot(odd != 0) != 0;
+      if (__builtin_expect(odd, 0)) take_out_odd<T, MX, DP, KPW, NP>(vreg, vcode, lds_masks[buf][wave], lane);
+      if (lane == 0) lds_odd[buf][wave] = odd;
     }
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
@@ -697,8 +784,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
         *reinterpret_cast<u32x4*>(lds[buf][1] + lds_packet<ROW>(j, p)) = v[c].p[0].raw;
       }
     }
-    const bool any = __ballot(odd != 0) != 0;
-    if (lane == 0) lds_odd[buf][wave] = any;
+
   };
 
   uint64_t here = 0;
@@ -773,50 +859,29 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
           l += s[b][r];
           p[2 * b + r / 8][r % 8] = from_f32<T>(s[b][r]);
         }
-      int odd = 0;
-      if (edge)
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) odd |= lds_odd[buf][w];
-      if (__builtin_expect(__builtin_amdgcn_readfirstlane(odd) != 0, 0)) {
-        // Infinities or NaN among values that not every row sees: each row adds
-        // only the keys that it sees.
+      for (int j = 0; j < KT / 16; ++j)
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+          o[d] = mfma32(read_v<T, ROW>(vl, 32 * d + 16 * (lane / 16 % 2), 16 * j + 4 * h, lane), p[j], o[d]);
+      if (edge) {
 #pragma nounroll
-        for (int j = 0; j < KT; ++j) {
-          // Key j is element (j % 32 / 8 * 4 + j % 4) of block j / 32 on the half j % 8 / 4: a half word of p.
-          const int word = (j / 32 * 16 + j % 32 / 8 * 4 + j % 4) / 2, owner = j % 8 / 4 * 32 + col;
-          unsigned bits = 0;
+        for (int w = 0; w < WAVES; ++w) {
+          if (__builtin_expect(!__builtin_amdgcn_readfirstlane(lds_odd[buf][w]), 1)) continue;
+          unsigned bits = 0;  // the row's keys of wavefront w's loads
 #pragma unroll
-          for (int k = 0; k < KT / 4; ++k) bits = k == word ? static_cast<unsigned>(p[k / 4].p[0].raw[k % 4]) : bits;
-          bits = __shfl(bits, owner) >> (j % 2 * 16);
-          const float w = to_f32(__builtin_bit_cast(T, static_cast<unsigned short>(bits)));
-          const bool add = seen >> j & 1;
+          for (int n = 0; n < NP; ++n)
+            bits |= (static_cast<unsigned>(seen >> (n * PASS + w * KPW)) & ((1u << KPW) - 1)) << (n * KPW);
 #pragma unroll
-          for (int d = 0; d < DP / 32; ++d) {
-            __builtin_amdgcn_sched_barrier(0);  // few values at a time: this path must not cost the others registers
+          for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int e = 32 * d + 8 * (r / 4) + 4 * h + r % 4;
-              const float v = to_f32(*reinterpret_cast<const T*>(vl + lds_packet<ROW>(j, e / 8) + e % 8 * 2));
-              o[d][r] = add ? __builtin_fmaf(w, v, o[d][r]) : o[d][r];
+            for (int r = 0; r < 16; r += 4) {
+              const f32x4 x = odd_sums<DP>(lds_masks[buf][w], 32 * d + 2 * r + 4 * h, bits);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) o[d][r + k] += x[k];
+              __builtin_amdgcn_sched_barrier(0);  // rare: not worth registers
             }
-          }
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < KT / 16; ++j)
-#pragma unroll
-          for (int d = 0; d < DP / 32; ++d) {
-            // 16 lanes read four keys' 16 elements: keys 16 j + 4 h + (0..3), then 8 further.
-            const int at = 32 * d + 16 * (lane / 16 % 2) + 4 * (lane % 4), key = 16 * j + 4 * h + lane % 16 / 4;
-            u32x2 x[2];
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-              x[n] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                  (__attribute__((address_space(3))) s16x4*)(const_cast<unsigned char*>(vl) + lds_packet<ROW>(key + 8 * n, at / 8) + at % 8 * 2)));
-            Eight<T> v;
-            v.p[0].raw = u32x4{x[0][0], x[0][1], x[1][0], x[1][1]};
-            o[d] = mfma32(v, p[j], o[d]);
-          }
       }
     }
     if (i + 1 < end) store_tile(i + 1, buf ^ 1, next);
@@ -951,7 +1016,8 @@ hipError_t run(const PagedAttentionArgs& a, hipStream_t stream) {
   d.by_seq_tiles = make_fastdiv(d.seq_tiles);
   // Work-items of a launch stay below 2^32.
   const int64_t per_tile = p.splits * a.c.kv_heads, most_tiles = std::max<int64_t>(1, (int64_t(1) << 22) / per_tile);
-  const bool page16 = a.c.page_size % 16 == 0;
+  bool page16 = a.c.page_size % 16 == 0;
+  for (const auto* st : {a.c.kst, a.c.vst, a.c.ksst, a.c.vsst}) page16 = page16 && st[2] < (int64_t(1) << 24);
   for (int64_t t0 = 0; t0 < p.tiles; t0 += most_tiles) {
     d.tile0 = static_cast<int>(t0);
     const dim3 grid(static_cast<unsigned>(std::min(most_tiles, p.tiles - t0) * per_tile)), block(kWaves * kWave);

@@ -193,6 +193,11 @@ int ako_set_tuning(int op, int key, int value) {
       if (key == 1) { ako::g_swiglu_tuning.vecs_per_thread = value; return AKO_OK; }
       if (key == 2) { ako::g_swiglu_tuning.xcd_chunk = value; return AKO_OK; }
       break;
+    case 3:
+      if (value > 65536) return fail(AKO_ERR_INVALID_ARGUMENT, "paged attention tuning values are at most 65536");
+      if (key == 1) { ako::g_paged_tuning.items = value; return AKO_OK; }
+      if (key == 2) { ako::g_paged_tuning.min_keys = value; return AKO_OK; }
+      break;
     default:
       break;
   }
@@ -837,6 +842,8 @@ int ako_paged_attention_fwd(const void* q, const int64_t* q_strides, void* out, 
   if (!q || !out || !q_strides) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: null pointer argument", fn);
   if (q_strides[0] < 0 || q_strides[1] < 0 || q_strides[2] < 0)
     return fail(AKO_ERR_INVALID_ARGUMENT, "%s: negative stride", fn);
+  a.window = window;
+  a.sinks = sinks;
   const int64_t need = ako::paged_attention_workspace(a);
   if (workspace_bytes < need || (need > 0 && (!workspace || !aligned(workspace, 16))))
     return fail(AKO_ERR_INVALID_ARGUMENT, "%s: needs a 16-byte aligned workspace of %lld bytes, got %lld", fn,
@@ -855,8 +862,6 @@ int ako_paged_attention_fwd(const void* q, const int64_t* q_strides, void* out, 
   a.q = q;
   a.out = out;
   for (int i = 0; i < 3; ++i) a.qs[i] = q_strides[i];
-  a.window = window;
-  a.sinks = sinks;
   a.scale = scale;
   a.workspace = workspace;
   return hip_status(ako::launch_paged_attention(a, static_cast<hipStream_t>(stream)), fn);

@@ -77,6 +77,11 @@ struct SwigluTuning {
   TuningKey vecs_per_thread{0};  // key 1: packets per lane of dense launches (1, 2, 4 or 8)
   TuningKey xcd_chunk{0};        // key 2: consecutive workgroups per XCD run (1 = block order; 0 = runs of 4 for launches of 2048-65535 workgroups)
 };
+struct PagedTuning {
+  TuningKey items{0};     // key 1: work items wanted beyond one for each row tile (0 = by kernel)
+  TuningKey min_keys{0};  // key 2: least keys of a part of a split key range (0 = 256)
+};
+extern PagedTuning g_paged_tuning;
 extern RmsTuning g_rms_tuning;
 extern RopeTuning g_rope_tuning;
 extern SwigluTuning g_swiglu_tuning;

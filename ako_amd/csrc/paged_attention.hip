@@ -35,61 +35,29 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
+PagedTuning g_paged_tuning;
+
 struct AttnDev {
   PagedDev c;
   const void* q;
   void* out;
-  float* part_o;   // [splits][rows][head_dim], rows = tokens * q_heads
-  float2* part_ml; // [splits][rows]: maximum and total
+  // Parts of split key ranges: `slots` row tiles of unscaled sums, of maxima and
+  // totals, and per output row the first part's row among those and the number of parts.
+  float* part_o;
+  float2* part_ml;
+  int2* row_parts;
+  int slots;
   int64_t qs[3];
-  int64_t rows;
   int q_heads, kv_heads, group, head_dim;
   int window, sinks;
-  int tile0;              // first row tile of the launch
-  int splits, min_tiles;  // at most `splits` parts of a row tile's keys, of at least min_tiles tiles
-  int seq_tiles;          // row tiles per sequence (uniform steps)
+  int item0;        // first work item of the launch
+  int max_parts;    // 1: key ranges are not split
+  int min_tiles;    // least key tiles of a part
+  float per_item;   // 1 / work items wanted for each key head
   float scale_log2;       // |scale| * log2(e), above 0: exponentials are of base 2
   unsigned q_sign;        // sign bits to flip in a word of q (scale < 0)
-  FastDiv by_kv_heads, by_group, by_splits, by_seq_tiles;
+  FastDiv by_kv_heads, by_group;
 };
-
-// A workgroup's rows: those of one sequence (or padding) that share a key head.
-struct RowTile {
-  int seq;     // -1: padding, nothing is visible
-  int token0;  // first token row of the sequence
-  int rows;    // rows of the sequence for one key head
-  int row0;    // the tile's first
-  int pos0;    // position of token0, negative where the sequence is shorter than its rows
-};
-
-// Row tiles of a packed step are numbered with sequence i's first at
-// cu[i] * group / R + i: no two sequences share a number, whatever their lengths,
-// and a number is resolved without a sum over the sequences before it. What
-// lies behind the last sequence counts as one more, padding.
-template <int R>
-__device__ __forceinline__ bool find_rows(const AttnDev& a, int tile, RowTile& t) {
-  const PagedDev& p = a.c;
-  if (p.cu == nullptr) {
-    if (p.seq == 0) return false;
-    const int s = fast_div(tile, a.by_seq_tiles);
-    t.seq = s;
-    t.token0 = s * p.seq;
-    t.rows = p.seq * a.group;
-    t.row0 = (tile - s * a.seq_tiles) * R;
-    t.pos0 = max(p.lens[s], 0) - p.seq;
-    return true;
-  }
-  const auto start = [&](int i) { return min(max(p.cu[i], 0), p.tokens) * a.group / R + i; };
-  const int s = last_at_most(p.n_seqs, tile, start);
-  const int first = min(max(p.cu[s], 0), p.tokens);
-  const int end = s < p.n_seqs ? min(max(p.cu[s + 1], 0), p.tokens) : p.tokens;
-  t.token0 = first;
-  t.rows = (end - first) * a.group;
-  t.row0 = (tile - (first * a.group / R + s)) * R;
-  t.seq = s < p.n_seqs ? s : -1;
-  t.pos0 = s < p.n_seqs ? max(p.lens[s], 0) - (end - first) : -1;
-  return t.row0 >= 0 && t.row0 < t.rows;
-}
 
 // The key tiles that a row tile sees, in order: those of the sinks, then those
 // from the first row's window on.
@@ -111,8 +79,102 @@ __device__ __forceinline__ KeyTiles key_tiles(const AttnDev& a, int first_pos, i
   return k;
 }
 
+// A work item: a tile of rows of one sequence (or of padding) that share a key
+// head, and a part of the keys that they see.
+struct Item {
+  int seq;     // -1: padding, nothing is visible
+  int token0;  // first token row of the sequence
+  int rows;    // rows of the sequence for one key head
+  int row0;    // the tile's first
+  int pos0;    // position of token0, negative where the sequence is shorter than its rows
+  int part, parts;
+  int slot;    // of the parts' memory, for part 0 of key head 0
+};
+
+// Work item `item` of one key head. Items are laid out on the device, from the
+// lengths that are only known there: with T the key tiles of all row tiles,
+// a range of n tiles is cut into n / L parts, L = max(min_tiles, T * per_item). That
+// makes at most 1 / per_item items more than there are row tiles, which the host
+// launches; long sequences do not hold up a step of short ones, and where all
+// are long the items are 1 / per_item, a number of whole rounds of the chip
+// (one item more would cost another round). What lies behind the last packed sequence counts as one more, padding. Sequences are
+// looked at 64 at a time, one per lane.
+template <int R, int KT>
+__device__ __forceinline__ bool find_item(const AttnDev& a, int item, Item& t) {
+  const PagedDev& p = a.c;
+  const int lane = threadIdx.x % kWave;
+  const int n = p.cu ? p.n_seqs + 1 : p.seq > 0 ? p.n_seqs : 0;
+  struct Seq { int token0, rows, pos0, row_tiles, tiles; };
+  const auto look = [&](int i) {
+    Seq s{0, 0, -1, 0, 0};
+    if (i >= n) return s;
+    if (p.cu == nullptr) {
+      s.token0 = i * p.seq;
+      s.rows = p.seq * a.group;
+      s.pos0 = max(p.lens[i], 0) - p.seq;
+    } else {
+      s.token0 = min(max(p.cu[i], 0), p.tokens);
+      const int end = i < p.n_seqs ? min(max(p.cu[i + 1], 0), p.tokens) : p.tokens;
+      s.rows = max(0, end - s.token0) * a.group;
+      s.pos0 = (i < p.n_seqs ? max(p.lens[i], 0) : -1) - max(0, end - s.token0);
+    }
+    s.row_tiles = (s.rows + R - 1) / R;
+    if (s.row_tiles > 0)
+      s.tiles = key_tiles<KT>(a, s.pos0 + static_cast<int>(fast_div((s.row_tiles - 1) * R, a.by_group)),
+                              s.pos0 + static_cast<int>(fast_div(s.rows - 1, a.by_group))).count;
+    return s;
+  };
+  Seq s = look(lane);
+  int len = 1 << 30;
+  if (a.max_parts > 1) {
+    float total = static_cast<float>(s.row_tiles) * static_cast<float>(s.tiles);
+    for (int base = kWave; base < n; base += kWave) {
+      const Seq more = look(base + lane);
+      total += static_cast<float>(more.row_tiles) * static_cast<float>(more.tiles);
+    }
+    // Rounded up past the float sum's own error, so that the items stay in bound.
+    len = max(a.min_tiles, static_cast<int>(__builtin_fminf(wave_sum(total) * a.per_item * 1.0001f, 1e9f)) + 1);
+  }
+  int before = 0, slots_before = 0;
+  for (int base = 0; base < n; base += kWave) {
+    if (base > 0) s = look(base + lane);
+    const int parts = min(a.max_parts, max(1, s.tiles / len));
+    const int items = s.row_tiles * parts, slots = parts > 1 ? items : 0;
+    int upto = items, slots_upto = slots;
+#pragma unroll
+    for (int k = 1; k < kWave; k *= 2) {
+      const int x = __shfl_up(upto, k), y = __shfl_up(slots_upto, k);
+      if (lane >= k) {
+        upto += x;
+        slots_upto += y;
+      }
+    }
+    const uint64_t behind = __ballot(item < before + upto);
+    if (behind) {
+      const int l = __builtin_ctzll(behind);
+      t.parts = __builtin_amdgcn_readlane(parts, l);
+      t.token0 = __builtin_amdgcn_readlane(s.token0, l);
+      t.rows = __builtin_amdgcn_readlane(s.rows, l);
+      t.pos0 = __builtin_amdgcn_readlane(s.pos0, l);
+      t.seq = p.cu && base + l >= p.n_seqs ? -1 : base + l;
+      const int local = item - before - __builtin_amdgcn_readlane(upto - items, l);
+      // The last rows first: they see the most keys.
+      const int from_last = local / t.parts;
+      t.row0 = (__builtin_amdgcn_readlane(s.row_tiles, l) - 1 - from_last) * R;
+      t.part = local - from_last * t.parts;
+      t.slot = slots_before + __builtin_amdgcn_readlane(slots_upto - slots, l) + from_last * t.parts;
+      // Indexes that make no sense may have wrapped the sums.
+      return local >= 0 && t.row0 >= 0 &&
+             (t.parts == 1 || (t.slot >= 0 && (int64_t(t.slot) + t.parts) * a.kv_heads <= a.slots));
+    }
+    before += __builtin_amdgcn_readlane(upto, kWave - 1);
+    slots_before += __builtin_amdgcn_readlane(slots_upto, kWave - 1);
+  }
+  return false;
+}
+
 // ---- matrix products ----------------------------------------------------------
-// Sixteen rows of A times sixteen columns of B, eight elements of the inner
+// Sixteen rows of A times sixteen columns of B, a packet of 16 bytes of the inner
 // dimension per lane. kShift: weights (and so totals and sums) are held times
 // 2^kShift; a power of two that the final division removes. fp16's weights
 // would be subnormal, with fewer bits, below 2^-14 of the largest; times 2^15
@@ -120,30 +182,24 @@ __device__ __forceinline__ KeyTiles key_tiles(const AttnDev& a, int first_pos, i
 template <typename T> struct Mfma;
 template <> struct Mfma<__bf16> {
   static constexpr float kShift = 0.0f;
-  static __device__ __forceinline__ f32x4 mul(const Eight<__bf16>& a, const Eight<__bf16>& b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  static __device__ __forceinline__ f32x4 mul(const Pack<__bf16, 8>& a, const Pack<__bf16, 8>& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a.raw), __builtin_bit_cast(bf16x8, b.raw), c, 0, 0, 0);
   }
 };
 template <> struct Mfma<_Float16> {
   static constexpr float kShift = 15.0f;
-  static __device__ __forceinline__ f32x4 mul(const Eight<_Float16>& a, const Eight<_Float16>& b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  static __device__ __forceinline__ f32x4 mul(const Pack<_Float16, 8>& a, const Pack<_Float16, 8>& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a.raw), __builtin_bit_cast(f16x8, b.raw), c, 0, 0, 0);
   }
 };
 template <> struct Mfma<float> {
   static constexpr float kShift = 0.0f;
-  static __device__ __forceinline__ f32x4 mul(const Eight<float>& a, const Eight<float>& b, f32x4 c) {
+  static __device__ __forceinline__ f32x4 mul(const Pack<float, 4>& a, const Pack<float, 4>& b, f32x4 c) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.e[i], b.e[i], c, 0, 0, 0);
     return c;
   }
 };
-
-template <typename T>
-__device__ __forceinline__ void flip_sign(Eight<T>& x, unsigned bits) {
-#pragma unroll
-  for (int i = 0; i < 8 / Eight<T>::kPer; ++i) x.p[i].raw ^= bits;
-}
 
 // Orders LDS accesses of one wavefront's lanes to each other's data. The LDS
 // serves a wavefront in order; only the compiler has to be held.
@@ -188,44 +244,31 @@ template <typename T, bool MX, int DP, int KPW, int LOADS>
 __device__ __forceinline__ void take_out_odd(u32x4 (&v)[LOADS], const unsigned (&code)[LOADS], unsigned* masks, int lane) {
   constexpr int C = MX ? 16 : 16 / static_cast<int>(sizeof(T)), LANES = DP / C;
   const int part = lane % LANES;
-  unsigned plus[C] = {}, minus[C] = {};
 #pragma unroll
-  for (int n = 0; n < LOADS; ++n) {
-    T x[C];
-    if constexpr (MX) {
-      const float s = e8m0_scale(code[n]);
-      const Eight<T> a = from_e4m3<T>(u32x2{v[n][0], v[n][1]}, s), b = from_e4m3<T>(u32x2{v[n][2], v[n][3]}, s);
+  for (int e = 0; e < C; ++e) {
+    __builtin_amdgcn_sched_barrier(0);  // rare: element by element, to cost the loop around it no registers
+    unsigned plus = 0, minus = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = a[e];
-        x[8 + e] = b[e];
-      }
-    } else {
-      Pack<T, C> w;
-      w.raw = v[n];
-#pragma unroll
-      for (int e = 0; e < C; ++e) x[e] = w.e[e];
-    }
-#pragma unroll
-    for (int e = 0; e < C; ++e) {
-      const float f = to_f32(x[e]);
+    for (int n = 0; n < LOADS; ++n) {
+      constexpr int kBits = 128 / C, kPerWord = 32 / kBits;  // of an element of v[n]
+      const unsigned word = v[n][e / kPerWord], shift = e % kPerWord * kBits;
+      float f;
+      if constexpr (MX) f = to_f32(FromE4m3<T>::lo(word >> shift, e8m0_scale(code[n]))[0]);
+      else if constexpr (sizeof(T) == 4) f = __builtin_bit_cast(float, word);
+      else f = to_f32(__builtin_bit_cast(T, static_cast<unsigned short>(word >> shift)));
       const bool odd = !(__builtin_fabsf(f) < __builtin_inff());
       const uint64_t up = __ballot(odd && !(f < 0.0f)), down = __ballot(odd && !(f > 0.0f));
 #pragma unroll
       for (int w = 0; w < KPW; ++w) {
-        plus[e] |= static_cast<unsigned>(up >> (w * LANES + part) & 1) << (n * KPW + w);
-        minus[e] |= static_cast<unsigned>(down >> (w * LANES + part) & 1) << (n * KPW + w);
+        plus |= static_cast<unsigned>(up >> (w * LANES + part) & 1) << (n * KPW + w);
+        minus |= static_cast<unsigned>(down >> (w * LANES + part) & 1) << (n * KPW + w);
       }
-      constexpr int kBits = 128 / C, kPerWord = 32 / kBits;  // of an element of v[n]
-      const unsigned all = kBits == 32 ? ~0u : ((1u << (kBits % 32)) - 1) << (e % kPerWord * kBits % 32);
-      v[n][e / kPerWord] = odd ? v[n][e / kPerWord] & ~all : v[n][e / kPerWord];
+      const unsigned all = kBits == 32 ? ~0u : ((1u << (kBits % 32)) - 1) << shift;
+      v[n][e / kPerWord] = odd ? word & ~all : word;
     }
-  }
-  if (lane < LANES) {
-#pragma unroll
-    for (int e = 0; e < C; ++e) {
-      masks[part * C + e] = plus[e];
-      masks[DP + part * C + e] = minus[e];
+    if (lane < LANES) {
+      masks[part * C + e] = plus;
+      masks[DP + part * C + e] = minus;
     }
   }
 }
@@ -283,29 +326,29 @@ __device__ __forceinline__ const uint8_t* row_at(const void* pool, const int64_t
   return static_cast<const uint8_t*>(pool) + (r.page * st[0] + head * st[1] + r.slot * st[2]) * elem;
 }
 // Sixteen bytes of a row of T (or, MX, of e4m3), aligned as its elements are.
-template <typename T, bool MX>
+// ONCE: rows that no other workgroup reads, with the non-temporal hint.
+template <typename T, bool MX, bool ONCE>
 __device__ __forceinline__ u32x4 load16(const uint8_t* p) {
-  if constexpr (MX) return load_pack<uint8_t, 16>(p).raw;
-  else return load_pack<T, 16 / static_cast<int>(sizeof(T))>(reinterpret_cast<const T*>(p)).raw;
+  if constexpr (MX) return load_pack<uint8_t, 16, ONCE>(p).raw;
+  else return load_pack<T, 16 / static_cast<int>(sizeof(T)), ONCE>(reinterpret_cast<const T*>(p)).raw;
 }
 
 // ---- up to 16 rows per workgroup -------------------------------------------------
 // Decode steps, where the cache's bytes are all that counts, and every step in
-// 32 bits. A wavefront takes key tiles of its own: K goes from memory straight into
-// the operand's registers (lane: key l % 16, and of each chunk of the head the
-// part l / 16), V through registers into the wavefront's own piece of LDS, so that
-// no barrier stands in the loop. The next tile's loads are issued as soon as
-// the registers of this tile's are free. The wavefronts' results are joined in LDS
-// at the end.
+// 32 bits. A wavefront takes key tiles of its own, loads whole rows of K and V
+// (a kilobyte per instruction) into registers and from there into its own
+// piece of LDS, so that no barrier stands in the loop; the loads of a later tile
+// are issued as soon as those registers are free, and are in flight while this
+// tile is worked on. The wavefronts' results are joined in LDS at the end.
 template <typename T, bool MX, int DP>
 struct RowsShape {
   static constexpr int kBlocks = sizeof(T) == 4 ? 1 : 2;    // 16-key blocks per tile
   static constexpr int kKeys = 16 * kBlocks;
   static constexpr int kChunk = MX ? 16 : 16 / sizeof(T);   // elements in 16 loaded bytes
-  static constexpr int kChunks = DP / (4 * kChunk);         // of K, per lane and key
-  static constexpr int kRowLanes = DP / kChunk;             // lanes across a row of V
-  static constexpr int kRowKeys = kWave / kRowLanes;        // keys per load of V
-  static constexpr int kLoads = kKeys / kRowKeys;           // of V, per lane
+  static constexpr int kRowLanes = DP / kChunk;             // lanes across a row
+  static constexpr int kRowKeys = kWave / kRowLanes;        // keys per load
+  static constexpr int kLoads = kKeys / kRowKeys;           // of K and of V, per lane and tile
+  static constexpr int kAhead = MX ? 2 : 1;                 // tiles in flight
   static constexpr int kRowBytes = DP * sizeof(T);
   static constexpr int kTileBytes = kKeys * kRowBytes;      // = 16 rows of DP floats, too
 };
@@ -321,26 +364,34 @@ __device__ __forceinline__ int lds_packet(int key, int p) {
   return key * ROW_BYTES + ((p ^ (x << 1)) << 4);
 }
 
-template <typename T, bool MX, int DP, int WAVES, bool PAGE16>
-__global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 ? 3 : DP * sizeof(T) <= 256 ? 2 : 1) void attn_rows(AttnDev a) {
+// LDS place of packet p of a key's row of K, which is read 16 bytes of 32 rows at a
+// time: sixteen rows' packets lie on different banks.
+template <int ROW_BYTES>
+__device__ __forceinline__ int lds_packet_k(int key, int p) {
+  constexpr int kPackets = ROW_BYTES / 16;
+  const int x = kPackets >= 16 ? key & 15 : (key >> 1) & (kPackets - 1);
+  return key * ROW_BYTES + ((p ^ x) << 4);
+}
+
+template <typename T, bool MX, int DP, int WAVES, bool PAGE16, bool ONCE>
+__global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 && !MX ? 3 : DP * sizeof(T) <= 256 ? 2 : 1) void attn_rows(AttnDev a) {
   using S = RowsShape<T, MX, DP>;
-  constexpr int KT = S::kKeys, NB = S::kBlocks, NC = S::kChunks, C = S::kChunk, NV = S::kLoads;
+  constexpr int KT = S::kKeys, NB = S::kBlocks, C = S::kChunk, NV = S::kLoads, AHEAD = S::kAhead;
   constexpr int E = 16 / static_cast<int>(sizeof(T));  // elements of an LDS packet
-  __shared__ __align__(16) unsigned char lds[WAVES * S::kTileBytes];
+  __shared__ __align__(16) unsigned char lds[WAVES][2][S::kTileBytes];  // K and V
   __shared__ float2 lds_ml[WAVES][16];
   __shared__ __align__(16) unsigned lds_odd[WAVES][2 * DP];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
   const int col = lane % 16, g = lane / 16;
-  unsigned char* const vt = lds + wave * S::kTileBytes;
+  unsigned char* const kl = lds[wave][0];
+  unsigned char* const vt = lds[wave][1];
 
   // Key heads run fastest over the workgroups, so that the XCDs share them out
   // and the row tiles of one head meet in one XCD's L2.
   const unsigned nth = fast_div(blockIdx.x, a.by_kv_heads);
   const int kvh = blockIdx.x - nth * a.kv_heads;
-  const unsigned tile_id = fast_div(nth, a.by_splits);
-  const int split = nth - tile_id * a.splits;
-  RowTile t;
-  if (!find_rows<16>(a, a.tile0 + tile_id, t)) return;
+  Item t;
+  if (!find_item<16, KT>(a, a.item0 + nth, t)) return;
 
   const int live = min(16, t.rows - t.row0);
   const int my_token = fast_div(t.row0 + col, a.by_group);  // of the sequence
@@ -348,30 +399,25 @@ __global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 ? 3 : DP * size
   const int first_pos = t.pos0 + static_cast<int>(fast_div(t.row0, a.by_group));
   const int last_pos = t.pos0 + static_cast<int>(fast_div(t.row0 + live - 1, a.by_group));
   const KeyTiles kt = t.seq < 0 ? KeyTiles{0, 0, 0, 0} : key_tiles<KT>(a, first_pos, last_pos);
-  const int parts = max(1, min(a.splits, kt.count / a.min_tiles));
-  const int begin = split < parts ? static_cast<int>(static_cast<int64_t>(kt.count) * split / parts) : 0;
-  const int end = split < parts ? static_cast<int>(static_cast<int64_t>(kt.count) * (split + 1) / parts) : 0;
+  const int begin = static_cast<int>(static_cast<int64_t>(kt.count) * t.part / t.parts);
+  const int end = static_cast<int>(static_cast<int64_t>(kt.count) * (t.part + 1) / t.parts);
 
   // This lane's query row, in the order of the K operand.
   const bool row_live = col < live;
   const int hi = row_live ? t.pos0 + my_token : -1;
   const int lo = a.window > 0 ? max(0, max(hi, 0) - a.window + 1) : 0;
-  Eight<T> q[NC * C / 8];
+  constexpr int NQ = DP / (4 * E);  // packets of the row in this lane: elements (4 c + g) E ..
+  Pack<T, E> q[NQ];
   {
     const int b = a.c.cu ? 0 : t.seq;
     const T* x = static_cast<const T*>(a.q) + b * a.qs[0] + (t.token0 - b * a.c.seq + my_token) * a.qs[1] + my_head * a.qs[2];
 #pragma unroll
-    for (int i = 0; i < NC * C / 4; ++i) {  // four elements at a time
-      const int d = (i * 4 / C) * 4 * C + g * C + i * 4 % C;
-      Pack<T, 4> v;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v.e[e] = from_f32<T>(0.0f);
-      if (row_live && d < a.head_dim) v = load_pack<T, 4>(x + d);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) q[i / 2][i % 2 * 4 + e] = v.e[e];
+    for (int c = 0; c < NQ; ++c) {
+      const int d = (4 * c + g) * E;
+      q[c].raw = u32x4{0, 0, 0, 0};
+      if (row_live && d < a.head_dim) q[c] = load_pack<T, E>(x + d);
+      q[c].raw ^= a.q_sign;
     }
-#pragma unroll
-    for (int i = 0; i < NC * C / 8; ++i) flip_sign(q[i], a.q_sign);
   }
 
   float m = -__builtin_inff(), l = 0.0f;
@@ -389,91 +435,81 @@ __global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 ? 3 : DP * size
   };
 
   // Loaded bytes of a tile, and which of its keys are there.
-  u32x4 kreg[NB][NC], vreg[NV];
-  unsigned kcode[NB][NC], vcode[NV];
-  unsigned there = 0;
-  const int vkey = lane / S::kRowLanes, vpart = lane % S::kRowLanes * C;
-  constexpr int EB = MX ? 1 : sizeof(T);
-  unsigned koff[NC], kcoff[NC];
-#pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int d = c * 4 * C + g * C < a.head_dim ? c * 4 * C + g * C : 0;
-    koff[c] = ((PAGE16 ? col * static_cast<unsigned>(a.c.kst[2]) : 0) + d) * EB;
-    kcoff[c] = (PAGE16 ? col * static_cast<unsigned>(a.c.ksst[2]) : 0) + d / 32;
-  }
-  const int vd = vpart < a.head_dim ? vpart : 0;
-  const unsigned voff = ((PAGE16 ? vkey * static_cast<unsigned>(a.c.vst[2]) : 0) + vd) * EB;
-  const unsigned vcoff = (PAGE16 ? vkey * static_cast<unsigned>(a.c.vsst[2]) : 0) + vd / 32;
-
-  const auto load_k = [&](int i, int pages) {
-    const int k0 = tile_start(i);
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const RowPlace r = row_place<PAGE16>(a.c, pages, k0 + 16 * b, 16 * b, col, kt.end);
-      const uint8_t* const x = row_at(a.c.k, a.c.kst, r, kvh, EB);
-#pragma unroll
-      for (int c = 0; c < NC; ++c) kreg[b][c] = load16<T, MX>(x + koff[c]);
-      if constexpr (MX) {
-        const uint8_t* const y = row_at(a.c.ks, a.c.ksst, r, kvh, 1);
-#pragma unroll
-        for (int c = 0; c < NC; ++c) kcode[b][c] = y[kcoff[c]];
-      }
-    }
-    there = static_cast<unsigned>(__ballot(pages >= 0 && pages < a.c.num_pages && lane < KT && k0 + lane < kt.end));
+  struct Loaded {
+    u32x4 k[NV], v[NV];
+    unsigned kcode[NV], vcode[NV];
+    unsigned there;
   };
-  const auto load_v = [&](int i, int pages) {
+  constexpr int EB = MX ? 1 : sizeof(T);
+  const int vkey = lane / S::kRowLanes, vpart = lane % S::kRowLanes;
+  const bool part_in = vpart * C < a.head_dim;
+  const int pd = part_in ? vpart * C : 0;
+  const unsigned koff = ((PAGE16 ? vkey * static_cast<unsigned>(a.c.kst[2]) : 0) + pd) * EB;
+  const unsigned voff = ((PAGE16 ? vkey * static_cast<unsigned>(a.c.vst[2]) : 0) + pd) * EB;
+  const unsigned kcoff = (PAGE16 ? vkey * static_cast<unsigned>(a.c.ksst[2]) : 0) + pd / 32;
+  const unsigned vcoff = (PAGE16 ? vkey * static_cast<unsigned>(a.c.vsst[2]) : 0) + pd / 32;
+  const auto load = [&](Loaded& x, int i, int pages) {
     const int k0 = tile_start(i);
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const RowPlace r = row_place<PAGE16>(a.c, pages, k0 + n * S::kRowKeys, n * S::kRowKeys, vkey, kt.end);
-      vreg[n] = load16<T, MX>(row_at(a.c.v, a.c.vst, r, kvh, EB) + voff);
-      if constexpr (MX) vcode[n] = row_at(a.c.vs, a.c.vsst, r, kvh, 1)[vcoff];
+      x.k[n] = load16<T, MX, ONCE>(row_at(a.c.k, a.c.kst, r, kvh, EB) + koff);
+      x.v[n] = load16<T, MX, ONCE>(row_at(a.c.v, a.c.vst, r, kvh, EB) + voff);
+      if constexpr (MX) {
+        x.kcode[n] = row_at(a.c.ks, a.c.ksst, r, kvh, 1)[kcoff];
+        x.vcode[n] = row_at(a.c.vs, a.c.vsst, r, kvh, 1)[vcoff];
+      }
+    }
+    x.there = static_cast<unsigned>(__ballot(pages >= 0 && pages < a.c.num_pages && lane < KT && k0 + lane < kt.end));
+  };
+  // Packet `part` of a row into LDS, as T.
+  const auto to_lds = [&](u32x4 w, unsigned code, auto place) {
+    if constexpr (MX) {
+      const float s = e8m0_scale(code);
+      const Eight<T> x = from_e4m3<T>(u32x2{w[0], w[1]}, s), y = from_e4m3<T>(u32x2{w[2], w[3]}, s);
+#pragma unroll
+      for (int h = 0; h < 16 / E; ++h)
+        *reinterpret_cast<u32x4*>(place(vpart * (16 / E) + h)) = h * E < 8 ? x.p[h * E % 8 / E].raw : y.p[h * E % 8 / E].raw;
+    } else {
+      *reinterpret_cast<u32x4*>(place(vpart)) = w;
     }
   };
 
-  int i = begin + wave;
-  int pages = 0;  // of the next tile
-  if (i < end) {
-    pages = look_up(i);
-    load_v(i, pages);
-    load_k(i, pages);
-    if (i + WAVES < end) pages = look_up(i + WAVES);
-  }
-  for (; i < end; i += WAVES) {
+  Loaded loaded[AHEAD];
+  int pages = 0;  // of the next tile to load
+  const auto work = [&](Loaded& x, int i) {
     const int k0 = tile_start(i);
     // Whether every live row sees every key of the tile.
-    const unsigned here = there;
+    const unsigned here = x.there;
     const bool whole = here == (KT == 32 ? ~0u : 0xffffu) && k0 + KT - 1 <= first_pos &&
                        (a.window <= 0 || k0 > last_pos - a.window || k0 + KT <= a.sinks);
     const unsigned seen = whole ? ~0u : static_cast<unsigned>(keys_seen(here, k0, lo, hi, a.sinks));
-    const bool more = i + WAVES < end;
 
-    // V into LDS; rows that are not there as zeros.
+    // K and V into LDS; rows of V that are not there as zeros.
     wave_fence();
     unsigned odd = 0;  // values that a weight of 0 would not cancel
     if (!whole) {
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
-        const int key = n * S::kRowKeys + vkey;
-        if (!(here >> key & 1)) vreg[n] = u32x4{0, 0, 0, 0};
-        odd |= odd_values<T, MX>(vreg[n], MX ? vcode[n] : 0);
+        if (!(here >> (n * S::kRowKeys + vkey) & 1)) x.v[n] = u32x4{0, 0, 0, 0};
+        odd |= odd_values<T, MX>(x.v[n], MX ? x.vcode[n] : 0);
       }
       odd = __ballot(odd != 0) != 0;
-      if (__builtin_expect(odd, 0)) take_out_odd<T, MX, DP, S::kRowKeys, NV>(vreg, vcode, lds_odd[wave], lane);
+      if (__builtin_expect(odd, 0)) take_out_odd<T, MX, DP, S::kRowKeys, NV>(x.v, x.vcode, lds_odd[wave], lane);
     }
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const int key = n * S::kRowKeys + vkey;
-      if constexpr (MX) {
-        const float s = e8m0_scale(vcode[n]);
-        Eight<T> x = from_e4m3<T>(u32x2{vreg[n][0], vreg[n][1]}, s), y = from_e4m3<T>(u32x2{vreg[n][2], vreg[n][3]}, s);
-#pragma unroll
-        for (int h = 0; h < 16 / E; ++h)
-          *reinterpret_cast<u32x4*>(vt + lds_packet<S::kRowBytes>(key, lane % S::kRowLanes * (16 / E) + h)) =
-              h * E < 8 ? x.p[h * E % 8 / E].raw : y.p[h * E % 8 / E].raw;
-      } else {
-        *reinterpret_cast<u32x4*>(vt + lds_packet<S::kRowBytes>(key, lane % S::kRowLanes)) = vreg[n];
-      }
+      if (a.head_dim != DP && !part_in) x.k[n] = u32x4{0, 0, 0, 0};
+      to_lds(x.k[n], MX ? x.kcode[n] : 0, [&](int p) { return kl + lds_packet_k<S::kRowBytes>(key, p); });
+      to_lds(x.v[n], MX ? x.vcode[n] : 0, [&](int p) { return vt + lds_packet<S::kRowBytes>(key, p); });
+    }
+    if (i + AHEAD * WAVES < end) {
+      // Loads return in order: the pages of the tile behind it are asked for
+      // first, so that using them does not wait for the tile.
+      const int now = pages;
+      if (i + (AHEAD + 1) * WAVES < end) pages = look_up(i + (AHEAD + 1) * WAVES);
+      load(x, i + AHEAD * WAVES, now);
     }
     wave_fence();
     // S^T: block b holds keys k0 + 16 b + 4 g + r of query `col`.
@@ -482,32 +518,11 @@ __global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 ? 3 : DP * size
     for (int b = 0; b < NB; ++b) {
       s[b] = f32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const bool in = c * 4 * C + g * C < a.head_dim;
-        if constexpr (MX) {
-          const float sc = e8m0_scale(kcode[b][c]);
-          Eight<T> x = from_e4m3<T>(u32x2{kreg[b][c][0], kreg[b][c][1]}, sc), y = from_e4m3<T>(u32x2{kreg[b][c][2], kreg[b][c][3]}, sc);
-          if (a.head_dim != DP && !in) x = y = zero_eight<T>();
-          s[b] = Mfma<T>::mul(x, q[2 * c], s[b]);
-          s[b] = Mfma<T>::mul(y, q[2 * c + 1], s[b]);
-        } else if constexpr (E == 8) {
-          Eight<T> x;
-          x.p[0].raw = kreg[b][c];
-          if (a.head_dim != DP && !in) x = zero_eight<T>();
-          s[b] = Mfma<T>::mul(x, q[c], s[b]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = a.head_dim != DP && !in ? 0.0f : __builtin_bit_cast(float, static_cast<unsigned>(kreg[b][c][e]));
-            s[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, q[c / 2][c % 2 * 4 + e], s[b], 0, 0, 0);
-          }
-        }
+      for (int c = 0; c < NQ; ++c) {
+        Pack<T, E> k;
+        k.raw = *reinterpret_cast<const u32x4*>(kl + lds_packet_k<S::kRowBytes>(16 * b + col, 4 * c + g));
+        s[b] = Mfma<T>::mul(k, q[c], s[b]);
       }
-    }
-    if (more) {
-      load_v(i + WAVES, pages);
-      load_k(i + WAVES, pages);
-      if (i + 2 * WAVES < end) pages = look_up(i + 2 * WAVES);
     }
 
     float top = -__builtin_inff();
@@ -531,7 +546,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 ? 3 : DP * size
       m = mn;
     }
     const float from = base - Mfma<T>::kShift;
-    Eight<T> p;  // NB * 4 are used
+    Pack<T, E> p;
     float pf[NB][4];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -539,7 +554,8 @@ __global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 ? 3 : DP * size
       for (int r = 0; r < 4; ++r) {
         pf[b][r] = __builtin_amdgcn_exp2f(s[b][r] - from);
         l += pf[b][r];
-        p[4 * b + r] = from_f32<T>(pf[b][r]);
+        if constexpr (E == 8) p.e[4 * b + r] = from_f32<T>(pf[b][r]);
+        else p.e[r] = pf[b][r];
       }
 
     // O^T += V^T P^T.
@@ -548,27 +564,42 @@ __global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 ? 3 : DP * size
       if constexpr (E == 8) {
         // Lane i of 16 gives the address of 8 bytes (key i / 4, elements 4 (i % 4) ..) and receives column i of the four keys.
         const int at = 16 * d + 4 * (col % 4), key = 4 * g + col / 4;
-        Eight<T> v;
         u32x2 half[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b)
           half[b] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
               (__attribute__((address_space(3))) s16x4*)(vt + lds_packet<S::kRowBytes>(16 * b + key, at / 8) + at % 8 * 2)));
-        v.p[0].raw = u32x4{half[0][0], half[0][1], half[NB - 1][0], half[NB - 1][1]};
+        Pack<T, E> v;
+        v.raw = u32x4{half[0][0], half[0][1], half[NB - 1][0], half[NB - 1][1]};
         o[d] = Mfma<T>::mul(v, p, o[d]);
       } else {
+        Pack<T, E> v;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int e = 16 * d + col;
-          const float v = *reinterpret_cast<const float*>(vt + lds_packet<S::kRowBytes>(4 * g + r, e / 4) + e % 4 * 4);
-          o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, pf[0][r], o[d], 0, 0, 0);
+          v.e[r] = *reinterpret_cast<const T*>(vt + lds_packet<S::kRowBytes>(4 * g + r, e / E) + e % E * sizeof(T));
         }
+        o[d] = Mfma<T>::mul(v, p, o[d]);
       }
     }
     if (__builtin_expect(odd, 0)) {
 #pragma unroll
       for (int d = 0; d < DP / 16; ++d) o[d] += odd_sums<DP>(lds_odd[wave], 16 * d + 4 * g, seen);
     }
+  };
+
+  const int first = begin + wave;
+#pragma unroll
+  for (int n = 0; n < AHEAD; ++n)
+    if (first + n * WAVES < end) {
+      const int now = n == 0 ? look_up(first) : pages;
+      if (first + (n + 1) * WAVES < end) pages = look_up(first + (n + 1) * WAVES);
+      load(loaded[n], first + n * WAVES, now);
+    }
+  for (int i = first; i < end; i += AHEAD * WAVES) {
+    work(loaded[0], i);
+    if constexpr (AHEAD == 2)
+      if (i + WAVES < end) work(loaded[1], i + WAVES);
   }
 
   wave_fence();
@@ -592,14 +623,16 @@ __global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 ? 3 : DP * size
     for (int w = 0; w < WAVES; ++w) {
       const float keep = __builtin_amdgcn_exp2f(lds_ml[w][row].x - base);
       L += lds_ml[w][row].y * keep;
-      const f32x4 y = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + w * S::kTileBytes) + row * DP + (((d / 4) ^ row) << 2));
+      const f32x4 y = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds[w][1]) + row * DP + (((d / 4) ^ row) << 2));
       if (lds_ml[w][row].y != 0.0f) x += y * keep;  // a wavefront without keys holds nothing
     }
     const int token = fast_div(t.row0 + row, a.by_group);
     const int64_t at = int64_t(t.token0 + token) * a.q_heads + kvh * a.group + (t.row0 + row - token * a.group);
-    if (a.splits > 1) {
-      if (d == 0) a.part_ml[split * a.rows + at] = float2{M, L};
-      if (L != 0.0f) *reinterpret_cast<f32x4*>(a.part_o + (split * a.rows + at) * a.head_dim + d) = x;
+    const int slot_row = ((t.slot + t.part) * a.kv_heads + kvh) * 16 + row;
+    if (a.max_parts > 1 && t.part == 0 && d == 0) a.row_parts[at] = int2{slot_row, t.parts};
+    if (t.parts > 1) {
+      if (d == 0) a.part_ml[slot_row] = float2{M, L};
+      if (L != 0.0f) *reinterpret_cast<f32x4*>(a.part_o + int64_t(slot_row) * a.head_dim + d) = x;
     } else {
       const float inv = L == 0.0f ? 0.0f : 1.0f / L;
       Pack<T, 4> y;
@@ -624,15 +657,6 @@ __device__ __forceinline__ f32x16 mfma32(const Eight<__bf16>& a, const Eight<__b
 }
 __device__ __forceinline__ f32x16 mfma32(const Eight<_Float16>& a, const Eight<_Float16>& b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-
-// LDS place of packet p of a key's row of K, which is read 16 bytes of 32 rows at a
-// time: sixteen rows' packets lie on different banks.
-template <int ROW_BYTES>
-__device__ __forceinline__ int lds_packet_k(int key, int p) {
-  constexpr int kPackets = ROW_BYTES / 16;
-  const int x = kPackets >= 16 ? key & 15 : (key >> 1) & (kPackets - 1);
-  return key * ROW_BYTES + ((p ^ x) << 4);
 }
 
 // Four keys' (from `key` on) 16 elements (from d on) transposed by 16 lanes: a lane
@@ -665,17 +689,14 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
 
   const unsigned nth = fast_div(blockIdx.x, a.by_kv_heads);
   const int kvh = blockIdx.x - nth * a.kv_heads;
-  const unsigned tile_id = fast_div(nth, a.by_splits);
-  const int split = nth - tile_id * a.splits;
-  RowTile t;
-  if (!find_rows<R>(a, a.tile0 + tile_id, t)) return;
+  Item t;
+  if (!find_item<R, KT>(a, a.item0 + nth, t)) return;
 
   const int last_row = min(t.row0 + R, t.rows) - 1;
   const auto pos_of = [&](int row) { return t.pos0 + static_cast<int>(fast_div(row, a.by_group)); };
   const KeyTiles kt = t.seq < 0 ? KeyTiles{0, 0, 0, 0} : key_tiles<KT>(a, pos_of(t.row0), pos_of(last_row));
-  const int parts = max(1, min(a.splits, kt.count / a.min_tiles));
-  const int begin = split < parts ? static_cast<int>(static_cast<int64_t>(kt.count) * split / parts) : 0;
-  const int end = split < parts ? static_cast<int>(static_cast<int64_t>(kt.count) * (split + 1) / parts) : 0;
+  const int begin = static_cast<int>(static_cast<int64_t>(kt.count) * t.part / t.parts);
+  const int end = static_cast<int>(static_cast<int64_t>(kt.count) * (t.part + 1) / t.parts);
   const int first_all = pos_of(t.row0), last_all = pos_of(last_row);
 
   // The wavefront's rows, and this lane's query.
@@ -696,7 +717,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
       const int d = 16 * i + 8 * h;
       q[i] = zero_eight<T>();
       if (row_live && d < a.head_dim) q[i] = load_eight<T>(x + d);
-      flip_sign(q[i], a.q_sign);
+      q[i].p[0].raw ^= a.q_sign;
     }
   }
 
@@ -735,8 +756,8 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
     for (int n = 0; n < NP; ++n) {
       const int at = n * PASS + wave * KPW;
       const RowPlace r = row_place<PAGE16>(a.c, pages, tile_start(i) + at, at, wkey, kt.end);
-      kreg[n] = load16<T, MX>(row_at(a.c.k, a.c.kst, r, kvh, EB) + koff);
-      vreg[n] = load16<T, MX>(row_at(a.c.v, a.c.vst, r, kvh, EB) + voff);
+      kreg[n] = load16<T, MX, false>(row_at(a.c.k, a.c.kst, r, kvh, EB) + koff);
+      vreg[n] = load16<T, MX, false>(row_at(a.c.v, a.c.vst, r, kvh, EB) + voff);
       if constexpr (MX) {
         kcode[n] = row_at(a.c.ks, a.c.ksst, r, kvh, 1)[kcoff];
         vcode[n] = row_at(a.c.vs, a.c.vsst, r, kvh, 1)[vcoff];
@@ -892,8 +913,10 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
   if (!row_live) return;
   l += __shfl_xor(l, 32);
   const int64_t at = int64_t(t.token0 + my_token) * a.q_heads + my_head;
-  if (a.splits > 1) {
-    if (h == 0) a.part_ml[split * a.rows + at] = float2{m * a.scale_log2, l};
+  const int slot_row = ((t.slot + t.part) * a.kv_heads + kvh) * R + 32 * wave + col;
+  if (a.max_parts > 1 && t.part == 0 && h == 0) a.row_parts[at] = int2{slot_row, t.parts};
+  if (t.parts > 1) {
+    if (h == 0) a.part_ml[slot_row] = float2{m * a.scale_log2, l};
     if (l != 0.0f) {
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
@@ -901,7 +924,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
         for (int r = 0; r < 16; r += 4) {
           const int e = 32 * d + 2 * r + 4 * h;
           if (e < a.head_dim)
-            *reinterpret_cast<f32x4*>(a.part_o + (split * a.rows + at) * a.head_dim + e) =
+            *reinterpret_cast<f32x4*>(a.part_o + int64_t(slot_row) * a.head_dim + e) =
                 f32x4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
         }
     }
@@ -921,41 +944,57 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
 }
 
 // ---- joining the parts of split key ranges ---------------------------------------
-// One wavefront per row: out = sum_s e^(m_s - M) o_s / sum_s e^(m_s - M) l_s, in the
-// order of the parts. A part without keys has l = 0 and is not read further.
-constexpr int kMaxSplits = 64;
+// One wavefront per row whose keys were split: out = sum_s e^(m_s - M) o_s /
+// sum_s e^(m_s - M) l_s over its parts, which are `stride` rows apart. Bound by
+// latency: LANES lanes hold a part's row, the groups of lanes take every
+// (64 / LANES)-th part and eight of them at a time, and are added up at the end; an
+// order that depends on nothing but the number of parts. A part without keys
+// has l = 0 and is not read further.
+constexpr int kMaxParts = kWave;
 
-template <typename T>
+template <typename T, int LANES>
 __global__ __launch_bounds__(256) void attn_join(const float* __restrict__ part_o, const float2* __restrict__ part_ml,
-                                                 T* __restrict__ out, int64_t row0, int64_t end, int64_t rows, int splits,
-                                                 int head_dim) {
+                                                 const int2* __restrict__ row_parts, T* __restrict__ out, int64_t row0,
+                                                 int64_t end, int stride, int64_t part_rows, int head_dim) {
+  constexpr int G = kWave / LANES, U = 8;
   const int64_t row = row0 + int64_t(blockIdx.x) * 4 + threadIdx.x / kWave;
   const int lane = threadIdx.x % kWave;
   if (row >= end) return;
-  const float2 ml = lane < splits ? part_ml[lane * rows + row] : float2{-__builtin_inff(), 0.0f};
+  const int2 where = row_parts[row];
+  const int n = where.y;
+  // Rows that no item covered (a step whose indexes make no sense) hold anything.
+  if (n <= 1 || n > kMaxParts || where.x < 0 || where.x + int64_t(n - 1) * stride >= part_rows) return;
+  const float2 ml = lane < n ? part_ml[where.x + int64_t(lane) * stride] : float2{-__builtin_inff(), 0.0f};
   float M = ml.x;
 #pragma unroll
   for (int k = 1; k < kWave; k *= 2) M = __builtin_fmaxf(M, __shfl_xor(M, k));
   const float w = __builtin_amdgcn_exp2f(ml.x - (M == -__builtin_inff() ? 0.0f : M));
   const uint64_t some = __ballot(ml.y != 0.0f);
-  float L = 0.0f, x[4] = {};
-  for (int s = 0; s < splits; ++s) {
-    if (!(some >> s & 1)) continue;
-    const float keep = __shfl(w, s);
-    L += __shfl(ml.y, s) * keep;
-    const int d = lane * 4;
-    if (d < head_dim) {
-      const f32x4 y = *reinterpret_cast<const f32x4*>(part_o + (s * rows + row) * head_dim + d);
+  const float L = wave_sum(ml.y != 0.0f ? ml.y * w : 0.0f);
+  const int d = lane % LANES * 4;
+  f32x4 x = {0, 0, 0, 0};
+  for (int s0 = 0; s0 < n; s0 += U * G) {  // the same for all lanes, which read each other's weights
+    f32x4 y[U];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] += y[e] * keep;
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + lane / LANES + u * G;
+      y[u] = f32x4{0, 0, 0, 0};
+      if (s < n && (some >> s & 1) && d < head_dim)
+        y[u] = *reinterpret_cast<const f32x4*>(part_o + (where.x + int64_t(s) * stride) * head_dim + d);
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) x += y[u] * __shfl(w, (s0 + lane / LANES + u * G) % kWave);
   }
+#pragma unroll
+  for (int k = LANES; k < kWave; k *= 2)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] += __shfl_xor(x[e], k);
   const float inv = some ? 1.0f / L : 0.0f;
-  if (lane * 4 < head_dim) {
+  if (lane < LANES && d < head_dim) {
     Pack<T, 4> y;
 #pragma unroll
     for (int e = 0; e < 4; ++e) y.e[e] = from_f32<T>(x[e] * inv);
-    store_pack<T, 4>(out + row * head_dim + lane * 4, y);
+    store_pack<T, 4>(out + row * head_dim + d, y);
   }
 }
 
@@ -967,9 +1006,13 @@ constexpr int kChunkRows = 32 * kWaves;
 // How a call is cut up: known from what the host knows of it, so that the
 // workspace can be sized before the call.
 struct Plan {
-  bool chunk;     // attn_chunk's row tiles, else attn_rows'
-  int64_t tiles;  // row tiles
-  int seq_tiles, splits;
+  bool chunk;         // attn_chunk's row tiles, else attn_rows'
+  bool once;          // attn_rows reads (nearly) every key in one workgroup only
+  int rows;           // of a row tile
+  int64_t row_tiles;  // for one key head, at most
+  int64_t items;      // work items wanted for one key head beyond one for each row tile
+  int max_parts, min_keys;
+  int64_t slots;      // row tiles of parts, of all key heads, at most
 };
 
 Plan plan(const PagedAttentionArgs& a) {
@@ -978,13 +1021,30 @@ Plan plan(const PagedAttentionArgs& a) {
   // Rows that share a key head, per sequence (on average in a packed step).
   const int64_t rows = a.c.n_seqs > 0 ? ceil_div(a.c.tokens * group, a.c.n_seqs) : 1;
   p.chunk = a.dtype != kF32 && rows > 16;
-  const int64_t r = p.chunk ? kChunkRows : 16;
-  p.seq_tiles = static_cast<int>(a.c.cu ? 1 : ceil_div(rows, r));
-  p.tiles = a.c.cu ? a.c.tokens * group / r + a.c.n_seqs + 1 : a.c.n_seqs * p.seq_tiles;
-  const int64_t want = p.chunk ? 512 : 1024, blocks = p.tiles * a.c.kv_heads;
-  const int64_t most = ceil_div(a.c.table_width * a.c.page_size, 256);
-  p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({ceil_div(want, blocks), most, kMaxSplits})));
+  p.once = a.dtype != kF32 || rows <= 16;
+  p.rows = p.chunk ? kChunkRows : 16;
+  p.row_tiles = a.c.cu ? a.c.tokens * group / p.rows + a.c.n_seqs + 1 : a.c.n_seqs * ceil_div(rows, p.rows);
+  const int forced_items = g_paged_tuning.items, forced_keys = g_paged_tuning.min_keys;
+  p.items = ceil_div(forced_items > 0 ? forced_items : p.chunk ? 512 : 1024, a.c.kv_heads);
+  p.min_keys = forced_keys > 0 ? forced_keys : 256;
+  // No more than without a window: the workspace is asked for without knowing it.
+  const int64_t capacity = a.c.table_width * a.c.page_size;
+  const int64_t keys = a.window > 0 ? std::min(capacity, std::min(a.window, capacity) + std::min(a.sinks, capacity)) : capacity;
+  p.max_parts = static_cast<int>(std::min<int64_t>(kMaxParts, keys / p.min_keys));
+  if (p.max_parts <= 1) {
+    p.max_parts = 1;
+    p.items = 0;
+  } else {
+    p.items = std::min(p.items, p.row_tiles * p.max_parts);
+    p.slots = p.items * a.c.kv_heads;  // a range that is cut has at most length / L parts
+  }
   return p;
+}
+
+int64_t workspace_bytes(const PagedAttentionArgs& a, const Plan& p) {
+  if (p.max_parts == 1) return 0;
+  return p.slots * p.rows * (a.c.head_dim + 2) * static_cast<int64_t>(sizeof(float)) +
+         a.c.tokens * a.q_heads * static_cast<int64_t>(sizeof(int2));
 }
 
 template <typename T, bool MX, int DP>
@@ -995,9 +1055,10 @@ hipError_t run(const PagedAttentionArgs& a, hipStream_t stream) {
   d.q = a.q;
   d.out = a.out;
   for (int i = 0; i < 3; ++i) d.qs[i] = a.qs[i];
-  d.rows = a.c.tokens * a.q_heads;
   d.part_o = static_cast<float*>(a.workspace);
-  d.part_ml = reinterpret_cast<float2*>(d.part_o + p.splits * d.rows * a.c.head_dim);
+  d.part_ml = reinterpret_cast<float2*>(d.part_o + p.slots * p.rows * a.c.head_dim);
+  d.row_parts = reinterpret_cast<int2*>(d.part_ml + p.slots * p.rows);
+  d.slots = static_cast<int>(p.slots);
   d.q_heads = static_cast<int>(a.q_heads);
   d.kv_heads = static_cast<int>(a.c.kv_heads);
   d.group = static_cast<int>(a.q_heads / a.c.kv_heads);
@@ -1005,45 +1066,50 @@ hipError_t run(const PagedAttentionArgs& a, hipStream_t stream) {
   const int64_t most = std::numeric_limits<int>::max();
   d.window = static_cast<int>(std::min(a.window, most));
   d.sinks = static_cast<int>(std::min(a.sinks, most));
-  d.splits = p.splits;
-  d.seq_tiles = p.seq_tiles;
+  d.max_parts = p.max_parts;
+  const int tile = p.chunk ? (DP <= 128 ? 64 : 32) : sizeof(T) == 4 ? 16 : 32;
+  d.min_tiles = std::max(1, p.min_keys / tile);
+  d.per_item = p.items > 0 ? 1.0f / static_cast<float>(p.items) : 0.0f;
   // Not 0: times it a masked score, -inf, has to stay that.
   d.scale_log2 = std::max(std::fabs(a.scale) * 1.44269504088896340736f, std::numeric_limits<float>::min());
   d.q_sign = a.scale < 0.0f ? (sizeof(T) == 4 ? 0x80000000u : 0x80008000u) : 0u;
   d.by_kv_heads = make_fastdiv(d.kv_heads);
   d.by_group = make_fastdiv(d.group);
-  d.by_splits = make_fastdiv(d.splits);
-  d.by_seq_tiles = make_fastdiv(d.seq_tiles);
-  // Work-items of a launch stay below 2^32.
-  const int64_t per_tile = p.splits * a.c.kv_heads, most_tiles = std::max<int64_t>(1, (int64_t(1) << 22) / per_tile);
+  // Rows' offsets inside 16 slots are 32-bit there.
   bool page16 = a.c.page_size % 16 == 0;
   for (const auto* st : {a.c.kst, a.c.vst, a.c.ksst, a.c.vsst}) page16 = page16 && st[2] < (int64_t(1) << 24);
-  for (int64_t t0 = 0; t0 < p.tiles; t0 += most_tiles) {
-    d.tile0 = static_cast<int>(t0);
-    const dim3 grid(static_cast<unsigned>(std::min(most_tiles, p.tiles - t0) * per_tile)), block(kWaves * kWave);
+  // Work-items of a launch stay below 2^32.
+  const int64_t items = p.row_tiles + p.items, per_launch = std::max<int64_t>(1, (int64_t(1) << 22) / a.c.kv_heads);
+  for (int64_t i0 = 0; i0 < items; i0 += per_launch) {
+    d.item0 = static_cast<int>(i0);
+    const dim3 grid(static_cast<unsigned>(std::min(per_launch, items - i0) * a.c.kv_heads)), block(kWaves * kWave);
     bool launched = false;
     if constexpr (sizeof(T) == 2) {
       if (p.chunk) {
-        d.min_tiles = DP <= 128 ? 4 : 8;
         if (page16) AKO_LAUNCH((attn_chunk<T, MX, DP, kWaves, true>), grid, block, 0, stream, d);
         else AKO_LAUNCH((attn_chunk<T, MX, DP, kWaves, false>), grid, block, 0, stream, d);
         launched = true;
       }
     }
     if (!launched) {
-      d.min_tiles = 256 / RowsShape<T, MX, DP>::kKeys;
-      if (page16) AKO_LAUNCH((attn_rows<T, MX, DP, kWaves, true>), grid, block, 0, stream, d);
-      else AKO_LAUNCH((attn_rows<T, MX, DP, kWaves, false>), grid, block, 0, stream, d);
+      if (p.once) {
+        if (page16) AKO_LAUNCH((attn_rows<T, MX, DP, kWaves, true, true>), grid, block, 0, stream, d);
+        else AKO_LAUNCH((attn_rows<T, MX, DP, kWaves, false, true>), grid, block, 0, stream, d);
+      } else if constexpr (sizeof(T) == 4) {
+        if (page16) AKO_LAUNCH((attn_rows<T, MX, DP, kWaves, true, false>), grid, block, 0, stream, d);
+        else AKO_LAUNCH((attn_rows<T, MX, DP, kWaves, false, false>), grid, block, 0, stream, d);
+      }
     }
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
   }
-  if (p.splits == 1) return hipSuccess;
+  if (p.max_parts == 1) return hipSuccess;
+  const int64_t rows = a.c.tokens * a.q_heads;
   constexpr int64_t kJoinRows = int64_t(1) << 24;  // per launch
-  for (int64_t r0 = 0; r0 < d.rows; r0 += kJoinRows) {
-    const int64_t n = std::min(kJoinRows, d.rows - r0);
-    AKO_LAUNCH((attn_join<T>), dim3(static_cast<unsigned>(ceil_div(n, 4))), dim3(256), 0, stream, d.part_o, d.part_ml,
-               static_cast<T*>(a.out), r0, r0 + n, d.rows, d.splits, d.head_dim);
+  for (int64_t r0 = 0; r0 < rows; r0 += kJoinRows) {
+    const int64_t n = std::min(kJoinRows, rows - r0);
+    AKO_LAUNCH((attn_join<T, DP / 4>), dim3(static_cast<unsigned>(ceil_div(n, 4))), dim3(256), 0, stream, d.part_o, d.part_ml,
+               d.row_parts, static_cast<T*>(a.out), r0, r0 + n, d.kv_heads * p.rows, p.slots * p.rows, d.head_dim);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
   }
@@ -1059,11 +1125,7 @@ hipError_t by_head_dim(const PagedAttentionArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-int64_t paged_attention_workspace(const PagedAttentionArgs& a) {
-  const Plan p = plan(a);
-  if (p.splits == 1) return 0;
-  return p.splits * a.c.tokens * a.q_heads * (a.c.head_dim + 2) * static_cast<int64_t>(sizeof(float));
-}
+int64_t paged_attention_workspace(const PagedAttentionArgs& a) { return workspace_bytes(a, plan(a)); }
 
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t stream) {
   switch (a.dtype) {

@@ -295,36 +295,62 @@ __device__ __forceinline__ uint64_t keys_seen(uint64_t there, int k0, int lo, in
   return there & below(hi + 1 - k0) & (~below(lo - k0) | below(sinks - k0));
 }
 
-// Where a wavefront's load of a few keys' rows starts: those of the keys kw ..
-// kw + 15 at most, kw + `mine` being this lane's. `pages` holds the page of the
-// tile's key j in lane j, `at` is kw's place in the tile, `end` the number of
-// keys that may be read.
+// Where a tile's rows lie: lane j finds the byte offsets of key j's rows once for
+// the tile, and a load takes them from there. `mine` is a lane's key among the
+// KPW consecutive ones that a load covers, from the tile's key `at` on.
 //
-// PAGE16 (pages of a multiple of 16 slots, and kw .. inside 16): the page and the
-// slot are the wavefront's, so the row's address is scalar and a lane adds a
-// 32-bit offset that is the same for every tile. Slots past `end` inside a page
-// are read with it; blocks past `end` are read as the last one. Otherwise each
-// lane finds its own key's page, and keys past `end` are read as the last.
-// Absent pages are read as page 0. Every address is inside the pool.
-struct RowPlace {
-  int page, slot;
+// PAGE16 (pages of a multiple of 16 slots; KPW divides 16): a load's keys lie in
+// one page, so its address is scalar, that of key `at`, and lanes add a 32-bit
+// offset that is the same for every tile. Slots past `end` inside a page are
+// read with it; blocks of 16 keys past `end` are read as the last block. Otherwise
+// each lane takes its own key's offset, and keys past `end` are read as the
+// last. Absent pages are read as page 0. Every address is inside the pool.
+template <bool MX>
+struct RowOffsets {
+  int64_t k, v, ks, vs;
 };
-template <bool PAGE16>
-__device__ __forceinline__ RowPlace row_place(const PagedDev& c, int pages, int kw, int at, int mine, int end) {
-  int page, key;
-  if constexpr (PAGE16) {
-    page = __builtin_amdgcn_readlane(pages, at);
-    key = kw < end ? kw : (end - 1) / 16 * 16 + kw % 16;
-  } else {
-    page = __shfl(pages, at + mine);
-    key = min(kw + mine, end - 1);
-  }
+template <typename T, bool MX, bool PAGE16>
+__device__ __forceinline__ RowOffsets<MX> row_offsets(const PagedDev& c, int page, int key, int end) {
+  constexpr int EB = MX ? 1 : sizeof(T);
+  if constexpr (PAGE16) key = key < end ? key : (end - 1) / 16 * 16 + key % 16;
+  else key = min(key, end - 1);
   const int slot = key - static_cast<int>(fast_div(key, c.by_page)) * c.page_size;
-  return RowPlace{page >= 0 && page < c.num_pages ? page : 0, slot};
+  page = page >= 0 && page < c.num_pages ? page : 0;
+  RowOffsets<MX> r;
+  r.k = (page * c.kst[0] + slot * c.kst[2]) * EB;
+  r.v = (page * c.vst[0] + slot * c.vst[2]) * EB;
+  if constexpr (MX) {
+    r.ks = page * c.ksst[0] + slot * c.ksst[2];
+    r.vs = page * c.vsst[0] + slot * c.vsst[2];
+  }
+  return r;
 }
-__device__ __forceinline__ const uint8_t* row_at(const void* pool, const int64_t (&st)[3], RowPlace r, int head, int elem) {
-  return static_cast<const uint8_t*>(pool) + (r.page * st[0] + head * st[1] + r.slot * st[2]) * elem;
+template <bool PAGE16>
+__device__ __forceinline__ int64_t offset_at(int64_t offsets, int at, int mine) {
+  const int lo = static_cast<int>(offsets), hi = static_cast<int>(offsets >> 32);
+  unsigned l;
+  int h;
+  if constexpr (PAGE16) {
+    l = __builtin_amdgcn_readlane(lo, at);
+    h = __builtin_amdgcn_readlane(hi, at);
+  } else {
+    l = __shfl(lo, at + mine);
+    h = __shfl(hi, at + mine);
+  }
+  return static_cast<int64_t>(static_cast<uint64_t>(static_cast<unsigned>(h)) << 32 | l);
 }
+
+// A key head's part of the pools.
+struct HeadPools {
+  const uint8_t *k, *v, *ks, *vs;
+};
+template <typename T, bool MX>
+__device__ __forceinline__ HeadPools head_pools(const PagedDev& c, int head) {
+  constexpr int EB = MX ? 1 : sizeof(T);
+  return HeadPools{static_cast<const uint8_t*>(c.k) + head * c.kst[1] * EB, static_cast<const uint8_t*>(c.v) + head * c.vst[1] * EB,
+                   MX ? c.ks + head * c.ksst[1] : nullptr, MX ? c.vs + head * c.vsst[1] : nullptr};
+}
+
 // Sixteen bytes of a row of T (or, MX, of e4m3), aligned as its elements are.
 // ONCE: rows that no other workgroup reads, with the non-temporal hint.
 template <typename T, bool MX, bool ONCE>
@@ -448,16 +474,18 @@ __global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 && !MX ? 3 : DP
   const unsigned voff = ((PAGE16 ? vkey * static_cast<unsigned>(a.c.vst[2]) : 0) + pd) * EB;
   const unsigned kcoff = (PAGE16 ? vkey * static_cast<unsigned>(a.c.ksst[2]) : 0) + pd / 32;
   const unsigned vcoff = (PAGE16 ? vkey * static_cast<unsigned>(a.c.vsst[2]) : 0) + pd / 32;
+  const HeadPools pools = head_pools<T, MX>(a.c, kvh);
   const auto load = [&](Loaded& x, int i, int pages) {
     const int k0 = tile_start(i);
+    const RowOffsets<MX> r = row_offsets<T, MX, PAGE16>(a.c, pages, k0 + lane % KT, kt.end);
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
-      const RowPlace r = row_place<PAGE16>(a.c, pages, k0 + n * S::kRowKeys, n * S::kRowKeys, vkey, kt.end);
-      x.k[n] = load16<T, MX, ONCE>(row_at(a.c.k, a.c.kst, r, kvh, EB) + koff);
-      x.v[n] = load16<T, MX, ONCE>(row_at(a.c.v, a.c.vst, r, kvh, EB) + voff);
+      const int at = n * S::kRowKeys;
+      x.k[n] = load16<T, MX, ONCE>(pools.k + offset_at<PAGE16>(r.k, at, vkey) + koff);
+      x.v[n] = load16<T, MX, ONCE>(pools.v + offset_at<PAGE16>(r.v, at, vkey) + voff);
       if constexpr (MX) {
-        x.kcode[n] = row_at(a.c.ks, a.c.ksst, r, kvh, 1)[kcoff];
-        x.vcode[n] = row_at(a.c.vs, a.c.vsst, r, kvh, 1)[vcoff];
+        x.kcode[n] = (pools.ks + offset_at<PAGE16>(r.ks, at, vkey))[kcoff];
+        x.vcode[n] = (pools.vs + offset_at<PAGE16>(r.vs, at, vkey))[vcoff];
       }
     }
     x.there = static_cast<unsigned>(__ballot(pages >= 0 && pages < a.c.num_pages && lane < KT && k0 + lane < kt.end));
@@ -751,16 +779,17 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
   const unsigned voff = ((PAGE16 ? wkey * static_cast<unsigned>(a.c.vst[2]) : 0) + pd) * EB;
   const unsigned kcoff = (PAGE16 ? wkey * static_cast<unsigned>(a.c.ksst[2]) : 0) + pd / 32;
   const unsigned vcoff = (PAGE16 ? wkey * static_cast<unsigned>(a.c.vsst[2]) : 0) + pd / 32;
+  const HeadPools pools = head_pools<T, MX>(a.c, kvh);
   const auto load_tile = [&](int i, int pages) {
+    const RowOffsets<MX> r = row_offsets<T, MX, PAGE16>(a.c, pages, tile_start(i) + lane % KT, kt.end);
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
       const int at = n * PASS + wave * KPW;
-      const RowPlace r = row_place<PAGE16>(a.c, pages, tile_start(i) + at, at, wkey, kt.end);
-      kreg[n] = load16<T, MX, false>(row_at(a.c.k, a.c.kst, r, kvh, EB) + koff);
-      vreg[n] = load16<T, MX, false>(row_at(a.c.v, a.c.vst, r, kvh, EB) + voff);
+      kreg[n] = load16<T, MX, false>(pools.k + offset_at<PAGE16>(r.k, at, wkey) + koff);
+      vreg[n] = load16<T, MX, false>(pools.v + offset_at<PAGE16>(r.v, at, wkey) + voff);
       if constexpr (MX) {
-        kcode[n] = row_at(a.c.ks, a.c.ksst, r, kvh, 1)[kcoff];
-        vcode[n] = row_at(a.c.vs, a.c.vsst, r, kvh, 1)[vcoff];
+        kcode[n] = (pools.ks + offset_at<PAGE16>(r.ks, at, wkey))[kcoff];
+        vcode[n] = (pools.vs + offset_at<PAGE16>(r.vs, at, wkey))[vcoff];
       }
     }
   };

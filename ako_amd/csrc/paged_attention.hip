@@ -201,13 +201,6 @@ template <> struct Mfma<float> {
   }
 };
 
-// Orders LDS accesses of one wavefront's lanes to each other's data. The LDS
-// serves a wavefront in order; only the compiler has to be held.
-__device__ __forceinline__ void wave_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
-
 __device__ __forceinline__ float max_over_groups(float v) {  // over the lanes l % 16
   v = __builtin_fmaxf(v, __shfl_xor(v, 16));
   return __builtin_fmaxf(v, __shfl_xor(v, 32));
@@ -234,6 +227,13 @@ __device__ __forceinline__ unsigned odd_values(u32x4 w, unsigned code) {
   return odd;
 }
 
+// Orders LDS accesses of one wavefront's lanes to each other's data. The LDS
+// serves a wavefront in order; only the compiler has to be held.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // Infinities and NaN among values that not every row sees: a weight of 0 would
 // not cancel them. They are taken out of V (zeros in their places), and for
 // each of the head's elements two words of `masks` (DP of them, then DP more) tell which of a
@@ -244,33 +244,26 @@ template <typename T, bool MX, int DP, int KPW, int LOADS>
 __device__ __forceinline__ void take_out_odd(u32x4 (&v)[LOADS], const unsigned (&code)[LOADS], unsigned* masks, int lane) {
   constexpr int C = MX ? 16 : 16 / static_cast<int>(sizeof(T)), LANES = DP / C;
   const int part = lane % LANES;
+  for (int i = lane; i < 2 * DP; i += kWave) masks[i] = 0;
+  wave_fence();
 #pragma unroll
-  for (int e = 0; e < C; ++e) {
-    __builtin_amdgcn_sched_barrier(0);  // rare: element by element, to cost the loop around it no registers
-    unsigned plus = 0, minus = 0;
+  for (int n = 0; n < LOADS; ++n)
 #pragma unroll
-    for (int n = 0; n < LOADS; ++n) {
+    for (int e = 0; e < C; ++e) {
+      __builtin_amdgcn_sched_barrier(0);  // rare: element by element, to cost the loop around it no registers
       constexpr int kBits = 128 / C, kPerWord = 32 / kBits;  // of an element of v[n]
       const unsigned word = v[n][e / kPerWord], shift = e % kPerWord * kBits;
       float f;
       if constexpr (MX) f = to_f32(FromE4m3<T>::lo(word >> shift, e8m0_scale(code[n]))[0]);
       else if constexpr (sizeof(T) == 4) f = __builtin_bit_cast(float, word);
       else f = to_f32(__builtin_bit_cast(T, static_cast<unsigned short>(word >> shift)));
-      const bool odd = !(__builtin_fabsf(f) < __builtin_inff());
-      const uint64_t up = __ballot(odd && !(f < 0.0f)), down = __ballot(odd && !(f > 0.0f));
-#pragma unroll
-      for (int w = 0; w < KPW; ++w) {
-        plus |= static_cast<unsigned>(up >> (w * LANES + part) & 1) << (n * KPW + w);
-        minus |= static_cast<unsigned>(down >> (w * LANES + part) & 1) << (n * KPW + w);
-      }
+      if (__builtin_fabsf(f) < __builtin_inff()) continue;
+      const unsigned bit = 1u << (n * KPW + lane / LANES);
+      if (!(f < 0.0f)) atomicOr(&masks[part * C + e], bit);
+      if (!(f > 0.0f)) atomicOr(&masks[DP + part * C + e], bit);
       const unsigned all = kBits == 32 ? ~0u : ((1u << (kBits % 32)) - 1) << shift;
-      v[n][e / kPerWord] = odd ? word & ~all : word;
+      v[n][e / kPerWord] = word & ~all;
     }
-    if (lane < LANES) {
-      masks[part * C + e] = plus;
-      masks[DP + part * C + e] = minus;
-    }
-  }
 }
 
 // Adds to elements e .. e + 3 the infinities that a row sees.

@@ -52,8 +52,9 @@ struct AttnDev {
   int window, sinks;
   int item0;        // first work item of the launch
   int max_parts;    // 1: key ranges are not split
-  int min_tiles;    // least key tiles of a part
+  int min_tiles;    // ranges of up to so many key tiles are not cut
   float per_item;   // 1 / work items wanted for each key head
+  float per_few;    // 1 / items of a launch that is not worth cutting further, for each key head
   float scale_log2;       // |scale| * log2(e), above 0: exponentials are of base 2
   unsigned q_sign;        // sign bits to flip in a word of q (scale < 0)
   FastDiv by_kv_heads, by_group;
@@ -93,8 +94,9 @@ struct Item {
 
 // Work item `item` of one key head. Items are laid out on the device, from the
 // lengths that are only known there: with T the key tiles of all row tiles,
-// a range of n tiles is cut into n / L parts, L = max(min_tiles, T * per_item). That
-// makes at most 1 / per_item items more than there are row tiles, which the host
+// a range of n > min_tiles tiles is cut into n / L parts, L = max(min_tiles, T * per_item),
+// or less than min_tiles as long as there are few items (per_few): then the time
+// is that of one item, and not of the bytes. That makes at most 1 / per_item items more than there are row tiles, which the host
 // launches; long sequences do not hold up a step of short ones, and where all
 // are long the items are 1 / per_item, a number of whole rounds of the chip
 // (one item more would cost another round). What lies behind the last packed sequence counts as one more, padding. Sequences are
@@ -133,12 +135,13 @@ __device__ __forceinline__ bool find_item(const AttnDev& a, int item, Item& t) {
       total += static_cast<float>(more.row_tiles) * static_cast<float>(more.tiles);
     }
     // Rounded up past the float sum's own error, so that the items stay in bound.
-    len = max(a.min_tiles, static_cast<int>(__builtin_fminf(wave_sum(total) * a.per_item * 1.0001f, 1e9f)) + 1);
+    total = __builtin_fminf(wave_sum(total) * 1.0001f, 1e9f);
+    len = max(static_cast<int>(total * a.per_item) + 1, min(a.min_tiles, max(2, static_cast<int>(total * a.per_few) + 1)));
   }
   int before = 0, slots_before = 0;
   for (int base = 0; base < n; base += kWave) {
     if (base > 0) s = look(base + lane);
-    const int parts = min(a.max_parts, max(1, s.tiles / len));
+    const int parts = s.tiles > a.min_tiles ? min(a.max_parts, max(1, s.tiles / len)) : 1;
     const int items = s.row_tiles * parts, slots = parts > 1 ? items : 0;
     int upto = items, slots_upto = slots;
 #pragma unroll
@@ -204,6 +207,11 @@ template <> struct Mfma<float> {
 __device__ __forceinline__ float max_over_groups(float v) {  // over the lanes l % 16
   v = __builtin_fmaxf(v, __shfl_xor(v, 16));
   return __builtin_fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float max_of_halves(float v) {  // over the lanes l % 32
+  const unsigned x = __builtin_bit_cast(unsigned, v);
+  const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return __builtin_fmaxf(__builtin_bit_cast(float, static_cast<unsigned>(r[0])), __builtin_bit_cast(float, static_cast<unsigned>(r[1])));
 }
 __device__ __forceinline__ float sum_over_groups(float v) {
   v += __shfl_xor(v, 16);
@@ -680,6 +688,13 @@ __device__ __forceinline__ f32x16 mfma32(const Eight<_Float16>& a, const Eight<_
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
+// Packets of a row of V here: half a wavefront's transposing read takes 64 bytes of
+// four keys' rows, which lie on different banks when packets are exchanged in fours.
+template <int ROW_BYTES>
+__device__ __forceinline__ int lds_packet_v(int key, int p) {
+  return key * ROW_BYTES + ((p ^ (ROW_BYTES >= 256 ? (key & 3) << 2 : (key >> 1 & 1) << 2)) << 4);
+}
+
 // Four keys' (from `key` on) 16 elements (from d on) transposed by 16 lanes: a lane
 // gives the address of 8 bytes and receives its column; then the same 8 keys on.
 template <typename T, int ROW_BYTES>
@@ -689,7 +704,7 @@ __device__ __forceinline__ Eight<T> read_v(const unsigned char* v, int d, int ke
 #pragma unroll
   for (int n = 0; n < 2; ++n)
     x[n] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (__attribute__((address_space(3))) s16x4*)(const_cast<unsigned char*>(v) + lds_packet<ROW_BYTES>(k + 8 * n, at / 8) + at % 8 * 2)));
+        (__attribute__((address_space(3))) s16x4*)(const_cast<unsigned char*>(v) + lds_packet_v<ROW_BYTES>(k + 8 * n, at / 8) + at % 8 * 2)));
   Eight<T> r;
   r.p[0].raw = u32x4{x[0][0], x[0][1], x[1][0], x[1][1]};
   return r;
@@ -779,11 +794,13 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
     for (int n = 0; n < NP; ++n) {
       const int at = n * PASS + wave * KPW;
       kreg[n] = load16<T, MX, false>(pools.k + offset_at<PAGE16>(r.k, at, wkey) + koff);
+      if constexpr (MX) kcode[n] = (pools.ks + offset_at<PAGE16>(r.ks, at, wkey))[kcoff];
+    }
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+      const int at = n * PASS + wave * KPW;
       vreg[n] = load16<T, MX, false>(pools.v + offset_at<PAGE16>(r.v, at, wkey) + voff);
-      if constexpr (MX) {
-        kcode[n] = (pools.ks + offset_at<PAGE16>(r.ks, at, wkey))[kcoff];
-        vcode[n] = (pools.vs + offset_at<PAGE16>(r.vs, at, wkey))[vcoff];
-      }
+      if constexpr (MX) vcode[n] = (pools.vs + offset_at<PAGE16>(r.vs, at, wkey))[vcoff];
     }
   };
   // A tile that some row of the workgroup does not see whole.
@@ -824,7 +841,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
         if (a.head_dim != DP && !part_in) k[c] = zero_eight<T>();
         const int p = part * (C / 8) + c;
         *reinterpret_cast<u32x4*>(lds[buf][0] + lds_packet_k<ROW>(j, p)) = k[c].p[0].raw;
-        *reinterpret_cast<u32x4*>(lds[buf][1] + lds_packet<ROW>(j, p)) = v[c].p[0].raw;
+        *reinterpret_cast<u32x4*>(lds[buf][1] + lds_packet_v<ROW>(j, p)) = v[c].p[0].raw;
       }
     }
 
@@ -881,7 +898,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
       for (int b = 0; b < KB; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = __builtin_fmaxf(top, s[b][r]);
-      const float mn = __builtin_fmaxf(m, __builtin_fmaxf(top, __shfl_xor(top, 32)));
+      const float mn = __builtin_fmaxf(m, max_of_halves(top));
       const float base = mn == -__builtin_inff() ? 0.0f : mn;
       if (__ballot(mn != m)) {
         const float keep = __builtin_amdgcn_exp2f((m - base) * a.scale_log2);
@@ -1033,6 +1050,7 @@ struct Plan {
   int rows;           // of a row tile
   int64_t row_tiles;  // for one key head, at most
   int64_t items;      // work items wanted for one key head beyond one for each row tile
+  int64_t few;        // items for one key head up to which ranges are cut below min_keys (0: not)
   int max_parts, min_keys;
   int64_t slots;      // row tiles of parts, of all key heads, at most
 };
@@ -1048,14 +1066,16 @@ Plan plan(const PagedAttentionArgs& a) {
   p.row_tiles = a.c.cu ? a.c.tokens * group / p.rows + a.c.n_seqs + 1 : a.c.n_seqs * ceil_div(rows, p.rows);
   const int forced_items = g_paged_tuning.items, forced_keys = g_paged_tuning.min_keys;
   p.items = ceil_div(forced_items > 0 ? forced_items : p.chunk ? 512 : 1024, a.c.kv_heads);
-  p.min_keys = forced_keys > 0 ? forced_keys : 256;
+  p.min_keys = forced_keys > 0 ? forced_keys : p.chunk && !a.c.cu ? 1024 : 256;
   // No more than without a window: the workspace is asked for without knowing it.
   const int64_t capacity = a.c.table_width * a.c.page_size;
   const int64_t keys = a.window > 0 ? std::min(capacity, std::min(a.window, capacity) + std::min(a.sinks, capacity)) : capacity;
-  p.max_parts = static_cast<int>(std::min<int64_t>(kMaxParts, keys / p.min_keys));
-  if (p.max_parts <= 1) {
+  p.few = p.chunk ? 0 : ceil_div(256, a.c.kv_heads);
+  p.max_parts = static_cast<int>(std::min<int64_t>(kMaxParts, keys / (p.chunk ? p.min_keys : std::min(p.min_keys, 64))));
+  if (p.max_parts <= 1 || keys <= p.min_keys) {
     p.max_parts = 1;
     p.items = 0;
+    p.few = 0;
   } else {
     p.items = std::min(p.items, p.row_tiles * p.max_parts);
     p.slots = p.items * a.c.kv_heads;  // a range that is cut has at most length / L parts
@@ -1091,6 +1111,7 @@ hipError_t run(const PagedAttentionArgs& a, hipStream_t stream) {
   d.max_parts = p.max_parts;
   const int tile = p.chunk ? (DP <= 128 ? 64 : 32) : sizeof(T) == 4 ? 16 : 32;
   d.min_tiles = std::max(1, p.min_keys / tile);
+  d.per_few = p.few > 0 ? 1.0f / static_cast<float>(p.few) : 1.0f;
   d.per_item = p.items > 0 ? 1.0f / static_cast<float>(p.items) : 0.0f;
   // Not 0: times it a masked score, -inf, has to stay that.
   d.scale_log2 = std::max(std::fabs(a.scale) * 1.44269504088896340736f, std::numeric_limits<float>::min());

@@ -8,7 +8,8 @@ dispatcher (``backend="ako"``) or the unfused eager references
 steps and per step), wall clock around a synchronised region, plus the
 generated tokens so the two backends can be compared. Prefill is the median of
 20 passes after 3 untimed ones; decode the median of 3 full 128-step runs. Each backend is also
-run with every decode step replayed from a HIP graph (``GraphedGreedy``),
+run with every decode step replayed from a HIP graph (``GraphedGreedy``; ``--cache
+paged`` or ``paged-mx8`` decodes on a paged cache, in the model's type or 8 bits),
 which removes the per-launch host cost that dominates batch-1 decoding.
 
     python -m ako_amd.models.bench_decoder [--steps 128] [--prompt 512] [--backend ako]
@@ -99,7 +100,8 @@ def graphed_step_breakdown(model, prompt: torch.Tensor, steps: int = 32) -> dict
 
 def run_config5(backend: str, *, prompt_len: int = 512, decode_steps: int = 128, repeats: int = 3,
                 device: str = "cuda", seed: int = 0, graphed: bool = True, prefill_warmup: int = 3,
-                prefill_repeats: int = 20, breakdown: bool = False, fused_qkv: bool = True) -> dict[str, Any]:
+                prefill_repeats: int = 20, breakdown: bool = False, fused_qkv: bool = True,
+                cache: str = "static") -> dict[str, Any]:
     cfg = config5()
     cfg.max_seq_len = prompt_len + decode_steps
     cfg.fused_qkv = fused_qkv
@@ -135,7 +137,9 @@ def run_config5(backend: str, *, prompt_len: int = 512, decode_steps: int = 128,
         graphed_ms, graphed_tokens = [], None
         if graphed:
             for _ in range(repeats):
-                runner = GraphedGreedy(model, prompt, decode_steps)
+                paged = None if cache == "static" else model.stack.new_paged_cache(
+                    prompt_len + decode_steps, quantized=cache == "paged-mx8")
+                runner = GraphedGreedy(model, prompt, decode_steps, cache=paged)
                 graphed_tokens, t_g = _timed(runner.run)
                 graphed_ms.append(t_g)
                 del runner
@@ -153,6 +157,7 @@ def run_config5(backend: str, *, prompt_len: int = 512, decode_steps: int = 128,
         }
     return {
         "backend": backend,
+        **({"graphed_cache": cache} if cache != "static" else {}),
         "prefill_ms": round(prefill, 3),
         "prefill_samples": len(prefill_ms),
         "decode_ms": round(dec, 3),
@@ -201,13 +206,17 @@ def main(argv: list[str] | None = None) -> int:
                     help="run one backend only (e.g. under a profiler) instead of comparing both")
     ap.add_argument("--separate-qkv", action="store_true",
                     help="three q/k/v projections (the reference's layout) instead of one fused GEMM")
+    ap.add_argument("--cache", choices=("static", "paged", "paged-mx8"), default="static",
+                    help="the cache of the graph-replayed steps (paged: with --backend ako)")
     args = ap.parse_args(argv)
+    if args.cache != "static" and args.backend != "ako":
+        ap.error("--cache paged needs --backend ako")
     if not torch.cuda.is_available():
         print("configs[4] needs a GPU", file=sys.stderr)
         return 1
     if args.backend:
         out = run_config5(args.backend, prompt_len=args.prompt, decode_steps=args.steps, repeats=args.repeats,
-                          fused_qkv=not args.separate_qkv)
+                          fused_qkv=not args.separate_qkv, cache=args.cache)
         out.pop("tokens")
     else:
         out = compare(args.prompt, args.steps, args.repeats, fused_qkv=not args.separate_qkv)

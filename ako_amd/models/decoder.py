@@ -16,7 +16,9 @@ or head, ``decoder.py:261-266``): ``CausalLM`` adds a token embedding, the
 LM head and a greedy decode loop. ``KVCache`` can be preallocated to a
 maximum length (``max_len``); appending then writes into the slab instead
 of re-concatenating the whole cache on every step as ``torch.cat`` does
-(``decoder.py:84-93``); the returned views are the same.
+(``decoder.py:84-93``); the returned views are the same. ``PagedKVCache`` keeps
+keys and values in pages, in the model's type or in 8 bits; a step on it
+rotates, stores and attends through ``rope_qk_paged`` and ``paged_attention``.
 """
 
 from __future__ import annotations
@@ -28,6 +30,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+from ako_amd.ops.paged import new_pages, paged_attention, paged_read, rope_qk_paged
 from ako_amd.ops.rmsnorm import rmsnorm, rmsnorm_residual
 from ako_amd.ops.rmsnorm_ref import rmsnorm_ref
 from ako_amd.ops.rope import rope, rope_qk, rope_qk_cache
@@ -224,6 +227,64 @@ class StaticKVCache:
         return self.k[layer_idx][:, :, :end], self.v[layer_idx][:, :, :end], None, start == 0
 
 
+class PagedKVCache:
+    """Key/value cache in pages, for prompts in one piece or in chunks and for decoding.
+
+    Each layer has a pool of pages, ``(pages, kv_heads, page_size, head_dim)``, in
+    ``dtype`` or, with ``torch.float8_e4m3fn``, in 8 bits with one power-of-two
+    scale per 32 elements; all layers share the block table. ``window`` and
+    ``sinks`` limit what a token attends to: the last ``window`` positions and the
+    first ``sinks``. Lengths live on the device (``seq_lens``), so a step has static
+    shapes and can be captured and replayed; ``host_len`` mirrors them.
+    """
+
+    def __init__(self, n_layers: int, batch: int, kv_heads: int, head_dim: int, max_len: int, *,
+                 dtype: torch.dtype, device: torch.device | str, page_size: int = 64,
+                 window: int | None = None, sinks: int = 0) -> None:
+        width = -(-max_len // page_size)
+        self.n_layers = n_layers
+        self.max_len = max_len
+        self.window = window
+        self.sinks = sinks
+        self.pools = [new_pages(batch * width, kv_heads, page_size, head_dim, dtype, device=device)
+                      for _ in range(n_layers)]
+        self.block_table = torch.arange(batch * width, dtype=torch.int32, device=device).view(batch, width)
+        self.seq_lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.host_len = 0
+
+    @property
+    def length(self) -> int:
+        return self.host_len
+
+    def begin_step(self, tokens: int) -> None:
+        """Make room for ``tokens`` more positions of every sequence; refused on
+        the host when they pass ``max_len``."""
+        if self.host_len + tokens > self.max_len:
+            raise ValueError(f"KV cache overflow: {self.host_len + tokens} > max_len {self.max_len}")
+        self.seq_lens.add_(tokens)
+        self.host_len += tokens
+
+    def rewind(self, tokens: int) -> None:
+        """Forget the last ``tokens`` positions."""
+        if not 0 <= tokens <= self.host_len:
+            raise ValueError(f"cannot rewind {tokens} of {self.host_len} positions")
+        self.seq_lens.sub_(tokens)
+        self.host_len -= tokens
+
+    def attend(self, layer_idx: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
+               sin: torch.Tensor, style: str) -> torch.Tensor:
+        """Rotate q and k, store k and v at the step's positions, and attend over all that is stored."""
+        kp, vp, ks, vs = self.pools[layer_idx]
+        where = (kp, vp, self.block_table, self.seq_lens)
+        q = rope_qk_paged(q, k, v, cos, sin, *where, style, k_scales=ks, v_scales=vs)
+        return paged_attention(q, *where, k_scales=ks, v_scales=vs, window=self.window, sinks=self.sinks)
+
+    def read(self, layer_idx: int, dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """This layer's filled keys and values as dense ``(batch, length, kv_heads, head_dim)`` tensors."""
+        kp, vp, ks, vs = self.pools[layer_idx]
+        return paged_read(kp, vp, self.block_table, self.seq_lens, self.host_len, dtype, k_scales=ks, v_scales=vs)
+
+
 def _norm(backend: Backend, x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor,
           eps: float, override: KernelOverride | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Residual add + RMSNorm, returning ``(normed, residual)``."""
@@ -332,6 +393,10 @@ class Attention(nn.Module):
         batch, seq_len, _ = x.shape
         cfg = self.config
         q, k, v = self.project_qkv(x)
+        if isinstance(kv_cache, PagedKVCache):
+            # cos/sin are the full tables; positions are read on the device.
+            attn = kv_cache.attend(layer_idx, q, k, v, cos, sin, cfg.rope_style)
+            return self.o_proj(attn.reshape(batch, seq_len, cfg.hidden_dim))
         if (isinstance(kv_cache, StaticKVCache) and seq_len == 1
                 and _fused_cache_rope(self.backend, self.kernel_override)):
             # cos/sin are the full tables here; the position is read on the device.
@@ -458,9 +523,15 @@ class DecoderStack(nn.Module):
         cos, sin = self._rope_tables
         return cos[offset:end], sin[offset:end]
 
-    def forward(self, x: torch.Tensor, *, kv_cache: KVCache | StaticKVCache | None = None) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, *,
+                kv_cache: KVCache | StaticKVCache | PagedKVCache | None = None) -> torch.Tensor:
         static_step = isinstance(kv_cache, StaticKVCache) and x.shape[1] == 1
-        if static_step:
+        if isinstance(kv_cache, PagedKVCache):
+            if self.backend != "ako":
+                raise ValueError("a paged cache needs backend='ako'")
+            cos, sin = self.rope_tables(max(kv_cache.max_len, self.config.max_seq_len), device=x.device)
+            kv_cache.begin_step(x.shape[1])
+        elif static_step:
             full = self.rope_tables(self.config.max_seq_len, device=x.device)
             if _fused_cache_rope(self.backend, self.kernel_override):
                 cos, sin = full  # the fused cache RoPE picks row pos itself
@@ -486,6 +557,14 @@ class DecoderStack(nn.Module):
         p = next(self.parameters())
         return StaticKVCache(self.config.n_layers, batch, self.config.n_kv_heads, self.config.head_dim,
                              max_len, dtype=p.dtype, device=p.device)
+
+    def new_paged_cache(self, max_len: int, *, batch: int = 1, page_size: int = 64, quantized: bool = False,
+                        window: int | None = None, sinks: int = 0) -> PagedKVCache:
+        """A paged cache in the model's type, or with ``quantized`` in 8 bits."""
+        p = next(self.parameters())
+        return PagedKVCache(self.config.n_layers, batch, self.config.n_kv_heads, self.config.head_dim, max_len,
+                            dtype=torch.float8_e4m3fn if quantized else p.dtype, device=p.device,
+                            page_size=page_size, window=window, sinks=sinks)
 
     def new_kv_cache(self, max_len: int | None = None) -> KVCache:
         return KVCache(n_layers=self.config.n_layers, max_len=max_len)
@@ -531,8 +610,8 @@ class CausalLM(nn.Module):
 class GraphedGreedy:
     """Greedy decoding with every decode step replayed from one HIP graph.
 
-    The prompt is prefilled eagerly into a ``StaticKVCache``; one eager decode
-    step then runs on a side stream (kernel selection and allocator warmup
+    The prompt is prefilled eagerly into a ``StaticKVCache`` (or into the
+    ``PagedKVCache`` that is given); one eager decode step then runs on a side stream (kernel selection and allocator warmup
     happen there, and its cache slot is rewritten by the first real step),
     and the next step is captured. Each replay reads the token in ``ids``,
     writes the next one back into ``ids`` and into ``history``, and advances
@@ -540,7 +619,8 @@ class GraphedGreedy:
     beyond the replay call.
     """
 
-    def __init__(self, model: "CausalLM", prompt: torch.Tensor, steps: int) -> None:
+    def __init__(self, model: "CausalLM", prompt: torch.Tensor, steps: int, *,
+                 cache: PagedKVCache | None = None) -> None:
         if prompt.shape[0] != 1:
             raise ValueError("graphed decoding is written for batch 1")
         self.model = model
@@ -549,7 +629,11 @@ class GraphedGreedy:
         max_len = self.prompt_len + steps
         if model.config.max_seq_len < max_len:
             raise ValueError(f"max_seq_len {model.config.max_seq_len} < prompt + steps {max_len}")
-        self.cache = model.stack.new_static_cache(max_len)
+        if cache is not None and (cache.host_len or cache.max_len < max_len):
+            raise ValueError(f"graphed decoding needs an empty cache of {max_len} positions")
+        self.cache = model.stack.new_static_cache(max_len) if cache is None else cache
+        #: Device-side count of the positions held.
+        self.position = self.cache.pos if cache is None else cache.seq_lens
         self.ids = model.logits_last(prompt, self.cache).argmax(-1, keepdim=True)
         self.history = torch.zeros(steps, dtype=torch.long, device=prompt.device)
         self.history[:1] = self.ids.view(1)
@@ -563,7 +647,7 @@ class GraphedGreedy:
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
             self._step()
-            self.cache.pos.sub_(1)  # undo the warmup step: position and token
+            self.position.sub_(1)  # undo the warmup step: position and token
             self.cache.host_len -= 1
             self.ids.copy_(first)
         torch.cuda.current_stream().wait_stream(side)
@@ -577,7 +661,7 @@ class GraphedGreedy:
     def _step(self) -> None:
         logits = self.model.logits_last(self.ids, self.cache)
         torch.argmax(logits, -1, keepdim=True, out=self.ids)
-        torch.sub(self.cache.pos, self.base, out=self.slot)
+        torch.sub(self.position, self.base, out=self.slot)
         self.history.index_copy_(0, self.slot, self.ids.view(1))
 
     @torch.no_grad()

@@ -21,6 +21,7 @@ from __future__ import annotations
 import torch
 
 from ako_amd.ops._registry import hip_disabled
+from ako_amd.ops.paged_hip import paged_attention_hip, paged_read_hip, rope_qk_paged_hip
 from ako_amd.ops.paged_ref import new_pages, paged_attention_ref, paged_read_ref, rope_qk_paged_ref
 
 
@@ -52,8 +53,6 @@ def rope_qk_paged(
     """
     args = (q, k, v, cos, sin, k_pages, v_pages, block_table, seq_lens, style)
     if q.is_cuda and not hip_disabled():
-        from ako_amd.ops.paged_hip import rope_qk_paged_hip
-
         return rope_qk_paged_hip(*args, k_scales, v_scales, cu_seqlens)
     return rope_qk_paged_ref(*args, k_scales=k_scales, v_scales=v_scales, cu_seqlens=cu_seqlens)
 
@@ -79,8 +78,6 @@ def paged_read(
     that are padding or have no page are zero.
     """
     if k_pages.is_cuda and not hip_disabled():
-        from ako_amd.ops.paged_hip import paged_read_hip
-
         return paged_read_hip(k_pages, v_pages, block_table, seq_lens, rows, dtype, k_scales, v_scales, cu_seqlens)
     return paged_read_ref(k_pages, v_pages, block_table, seq_lens, rows, dtype, k_scales=k_scales,
                           v_scales=v_scales, cu_seqlens=cu_seqlens)
@@ -108,12 +105,11 @@ def paged_attention(
     unless given. Rows that see nothing (padding) are zero, and what a row does
     not see has no influence on it, whatever is stored there.
     """
-    kw = {"k_scales": k_scales, "v_scales": v_scales, "cu_seqlens": cu_seqlens}
     if q.is_cuda and not hip_disabled():
-        from ako_amd.ops.paged_hip import paged_attention_hip
-
-        return paged_attention_hip(q, k_pages, v_pages, block_table, seq_lens, scale, window, sinks, **kw)
-    return paged_attention_ref(q, k_pages, v_pages, block_table, seq_lens, scale=scale, window=window, sinks=sinks, **kw)
+        return paged_attention_hip(q, k_pages, v_pages, block_table, seq_lens, scale, window, sinks,
+                                   k_scales, v_scales, cu_seqlens)
+    return paged_attention_ref(q, k_pages, v_pages, block_table, seq_lens, k_scales=k_scales, v_scales=v_scales,
+                               cu_seqlens=cu_seqlens, scale=scale, window=window, sinks=sinks)
 
 
 __all__ = ["new_pages", "paged_attention", "paged_read", "rope_qk_paged"]

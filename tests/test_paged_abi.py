@@ -137,6 +137,14 @@ def test_write_refusals() -> None:
     assert write(cache(dtype=E4M3, k_scales=KP)) == INVALID and write(cache(dtype=E4M3, k_scales=VS)) == INVALID
 
 
+def test_tuning_keys() -> None:
+    lib = _native.load()
+    for key in (1, 2):
+        assert lib.ako_set_tuning(3, key, 0) == OK and lib.ako_set_tuning(3, key, -1) == INVALID
+        assert lib.ako_set_tuning(3, key, 65537) == INVALID
+    assert lib.ako_set_tuning(3, 3, 0) == INVALID and lib.ako_set_tuning(3, 0, 0) == INVALID
+
+
 def test_read_refusals() -> None:
     assert read(cache(), k=None) == INVALID
     for kw in (dict(k=KP), dict(k=OUT), dict(v=LENS), dict(v=TABLE)):

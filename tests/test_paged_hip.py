@@ -134,6 +134,49 @@ def test_long_contexts_are_split_and_joined() -> None:
             check(s, f"{dtype} {held} {news} window", window=2500, sinks=7)
 
 
+@pytest.fixture
+def tuned():
+    from ako_amd import _native
+
+    def set_keys(items: int, keys: int) -> None:
+        _native.set_tuning(3, 1, items)
+        _native.set_tuning(3, 2, keys)
+
+    yield set_keys
+    set_keys(0, 0)
+
+
+@pytest.mark.parametrize("items,keys", [(1, 1), (64, 64), (4096, 64), (65536, 1), (16, 65536)])
+def test_however_the_keys_are_cut(tuned, items: int, keys: int) -> None:
+    tuned(items, keys)
+    for dtype, mx in ((torch.bfloat16, False), (torch.float16, True), (torch.float32, False)):
+        for held, news, packed in (([900, 40, 1, 333], [1] * 4, False), ([700, 1000], [50, 50], False),
+                                   ([600, 40, 1, 333, 0], [200, 1, 1, 90, 0], True)):
+            s = step(held, news, heads=8, kv_heads=2, dtype=dtype, mx=mx, packed=packed, pad_rows=3 * packed, device=DEV)
+            check(s, f"{dtype} {held} {news}")
+            check(s, f"{dtype} {held} {news} window", window=100, sinks=40)
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_many_sequences(packed: bool) -> None:
+    """More sequences than a wavefront has lanes, empty ones among them."""
+    for dtype in DTYPES:
+        held = [(7 * i * i) % 300 if i % 9 else 0 for i in range(150)]
+        held[70] = 2000
+        news = [min(n, 1 + i % 5) for i, n in enumerate(held)] if packed else [3] * 150
+        s = step(held, news, heads=4, kv_heads=2, dtype=dtype, packed=packed, pad_rows=70 * packed, device=DEV)
+        check(s, str(dtype))
+        if packed:  # and a few long ones: the many-row kernel
+            s = step(held[60:140], [min(n, 40 * (i % 3)) for i, n in enumerate(held[60:140])], heads=4, kv_heads=2, dtype=dtype,
+                     packed=True, device=DEV)
+            check(s, f"{dtype} chunks")
+        cos, sin = tables(2048, 64, DEV)
+        before = [t.clone() for t in (s.k_pages, s.v_pages)]
+        out = ako.rope_qk_paged(s.q, s.k, s.v, cos, sin, *s.where, **s.kw)
+        if packed:
+            check_write(s, out, cos, sin, "neox", before)
+
+
 def test_a_wide_table_is_read_only_as_far_as_needed() -> None:
     s = step([50, 3], [1, 1], width=1 << 16, dtype=torch.float16, device=DEV)
     check(s)

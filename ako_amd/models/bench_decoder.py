@@ -101,7 +101,7 @@ def graphed_step_breakdown(model, prompt: torch.Tensor, steps: int = 32) -> dict
 def run_config5(backend: str, *, prompt_len: int = 512, decode_steps: int = 128, repeats: int = 3,
                 device: str = "cuda", seed: int = 0, graphed: bool = True, prefill_warmup: int = 3,
                 prefill_repeats: int = 20, breakdown: bool = False, fused_qkv: bool = True,
-                cache: str = "static") -> dict[str, Any]:
+                graph_cache: str = "static") -> dict[str, Any]:
     cfg = config5()
     cfg.max_seq_len = prompt_len + decode_steps
     cfg.fused_qkv = fused_qkv
@@ -137,8 +137,8 @@ def run_config5(backend: str, *, prompt_len: int = 512, decode_steps: int = 128,
         graphed_ms, graphed_tokens = [], None
         if graphed:
             for _ in range(repeats):
-                paged = None if cache == "static" else model.stack.new_paged_cache(
-                    prompt_len + decode_steps, quantized=cache == "paged-mx8")
+                paged = None if graph_cache == "static" else model.stack.new_paged_cache(
+                    prompt_len + decode_steps, quantized=graph_cache == "paged-mx8")
                 runner = GraphedGreedy(model, prompt, decode_steps, cache=paged)
                 graphed_tokens, t_g = _timed(runner.run)
                 graphed_ms.append(t_g)
@@ -157,7 +157,7 @@ def run_config5(backend: str, *, prompt_len: int = 512, decode_steps: int = 128,
         }
     return {
         "backend": backend,
-        **({"graphed_cache": cache} if cache != "static" else {}),
+        **({"graphed_cache": graph_cache} if graph_cache != "static" else {}),
         "prefill_ms": round(prefill, 3),
         "prefill_samples": len(prefill_ms),
         "decode_ms": round(dec, 3),
@@ -216,7 +216,7 @@ def main(argv: list[str] | None = None) -> int:
         return 1
     if args.backend:
         out = run_config5(args.backend, prompt_len=args.prompt, decode_steps=args.steps, repeats=args.repeats,
-                          fused_qkv=not args.separate_qkv, cache=args.cache)
+                          fused_qkv=not args.separate_qkv, graph_cache=args.cache)
         out.pop("tokens")
     else:
         out = compare(args.prompt, args.steps, args.repeats, fused_qkv=not args.separate_qkv)

@@ -99,3 +99,29 @@ def test_graph_replays_match_eager_steps(quantized: bool) -> None:
         assert torch.equal(runner.run(), eager)
         with pytest.raises(ValueError, match="empty cache"):
             GraphedGreedy(model, prompt, 30, cache=new())
+
+
+def test_the_benchmark_decodes_on_the_cache_it_is_asked_for(monkeypatch) -> None:
+    """``run_config5`` on a CPU stub of the graph runner: which cache each choice hands to it."""
+    from ako_amd.models import bench_decoder
+
+    seen = []
+
+    class Runner:
+        def __init__(self, model, prompt, steps, *, cache=None):
+            seen.append(cache)
+            self.steps = steps
+
+        def run(self):
+            return torch.zeros(1, self.steps, dtype=torch.long)
+
+    monkeypatch.setattr(bench_decoder, "GraphedGreedy", Runner)
+    monkeypatch.setattr(bench_decoder, "config5", lambda: ModelConfig(**{**CFG.__dict__}))
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: None)
+    for choice, dtype in (("static", None), ("paged", torch.float16), ("paged-mx8", torch.float8_e4m3fn)):
+        seen.clear()
+        out = bench_decoder.run_config5("ako", prompt_len=5, decode_steps=3, repeats=1, device="cpu", prefill_warmup=0,
+                                        prefill_repeats=1, graph_cache=choice)
+        assert (seen[0] is None) == (choice == "static") and ("graphed_cache" in out) == (choice != "static")
+        if dtype is not None:
+            assert seen[0].pools[0][0].dtype == dtype and seen[0].max_len == 8

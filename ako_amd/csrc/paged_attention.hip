@@ -37,6 +37,13 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 PagedTuning g_paged_tuning;
 
+// The maximum of a row that sees keys but only scores of -infinity: 0 / 0, as its
+// softmax says, where a row that sees nothing (its maximum -infinity) is zero.
+constexpr float kAllInf = -std::numeric_limits<float>::max();
+__device__ __forceinline__ float inverse_total(float m, float l) {
+  return l != 0.0f ? 1.0f / l : m == -__builtin_inff() ? 0.0f : __builtin_nanf("");
+}
+
 struct AttnDev {
   PagedDev c;
   const void* q;
@@ -135,8 +142,10 @@ __device__ __forceinline__ bool find_item(const AttnDev& a, int item, Item& t) {
       total += static_cast<float>(more.row_tiles) * static_cast<float>(more.tiles);
     }
     // Rounded up past the float sum's own error, so that the items stay in bound.
-    total = __builtin_fminf(wave_sum(total) * 1.0001f, 1e9f);
-    len = max(static_cast<int>(total * a.per_item) + 1, min(a.min_tiles, max(2, static_cast<int>(total * a.per_few) + 1)));
+    // 1e9 tiles are more than any range has.
+    total = wave_sum(total) * 1.0001f;
+    const auto share = [&](float per) { return static_cast<int>(__builtin_fminf(total * per, 1e9f)) + 1; };
+    len = max(share(a.per_item), min(a.min_tiles, max(2, share(a.per_few))));
   }
   int before = 0, slots_before = 0;
   for (int base = 0; base < n; base += kWave) {
@@ -505,6 +514,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 && !MX ? 3 : DP
   };
 
   Loaded loaded[AHEAD];
+  unsigned any = 0;  // nonzero where the row sees a key
   int pages = 0;  // of the next tile to load
   const auto work = [&](Loaded& x, int i) {
     const int k0 = tile_start(i);
@@ -513,6 +523,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 && !MX ? 3 : DP
     const bool whole = here == (KT == 32 ? ~0u : 0xffffu) && k0 + KT - 1 <= first_pos &&
                        (a.window <= 0 || k0 > last_pos - a.window || k0 + KT <= a.sinks);
     const unsigned seen = whole ? ~0u : static_cast<unsigned>(keys_seen(here, k0, lo, hi, a.sinks));
+    any |= seen;
 
     // K and V into LDS; rows of V that are not there as zeros.
     wave_fence();
@@ -635,6 +646,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 && !MX ? 3 : DP
   // Join the wavefronts: o as rows of DP floats in the wavefront's own LDS, 16-byte
   // packets exchanged by the row's number against bank conflicts.
   l = sum_over_groups(l);
+  if (any && m == -__builtin_inff()) m = kAllInf;
   if (g == 0) lds_ml[wave][col] = float2{m, l};
   float* const mine = reinterpret_cast<float*>(vt);
 #pragma unroll
@@ -663,7 +675,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 && !MX ? 3 : DP
       if (d == 0) a.part_ml[slot_row] = float2{M, L};
       if (L != 0.0f) *reinterpret_cast<f32x4*>(a.part_o + int64_t(slot_row) * a.head_dim + d) = x;
     } else {
-      const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+      const float inv = inverse_total(M, L);
       Pack<T, 4> y;
 #pragma unroll
       for (int e = 0; e < 4; ++e) y.e[e] = from_f32<T>(x[e] * inv);
@@ -848,6 +860,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
   };
 
   uint64_t here = 0;
+  bool any = false;  // the row sees a key
   int pg = 0;
   if (begin < end) {
     pg = look_up(begin);
@@ -883,7 +896,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
           x.p[0].raw = *reinterpret_cast<const u32x4*>(kl + lds_packet_k<ROW>(32 * b + col, 2 * d + h));
           s[b] = mfma32(x, q[d], s[b]);
         }
-      uint64_t seen = 0;
+      uint64_t seen = ~uint64_t(0);
       if (edge) {
         seen = keys_seen(here, k0, lo, hi, a.sinks);
 #pragma unroll
@@ -893,6 +906,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
           for (int r = 0; r < 16; ++r) s[b][r] = bits >> (8 * (r / 4) + r % 4) & 1 ? s[b][r] : -__builtin_inff();
         }
       }
+      any |= seen != 0;
       float top = -__builtin_inff();
 #pragma unroll
       for (int b = 0; b < KB; ++b)
@@ -951,11 +965,12 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
 
   if (!row_live) return;
   l += __shfl_xor(l, 32);
+  m = any && m == -__builtin_inff() ? kAllInf : m * a.scale_log2;
   const int64_t at = int64_t(t.token0 + my_token) * a.q_heads + my_head;
   const int slot_row = ((t.slot + t.part) * a.kv_heads + kvh) * R + 32 * wave + col;
   if (a.max_parts > 1 && t.part == 0 && h == 0) a.row_parts[at] = int2{slot_row, t.parts};
   if (t.parts > 1) {
-    if (h == 0) a.part_ml[slot_row] = float2{m * a.scale_log2, l};
+    if (h == 0) a.part_ml[slot_row] = float2{m, l};
     if (l != 0.0f) {
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
@@ -969,7 +984,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
     }
     return;
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const float inv = inverse_total(m, l);
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -1028,7 +1043,7 @@ __global__ __launch_bounds__(256) void attn_join(const float* __restrict__ part_
   for (int k = LANES; k < kWave; k *= 2)
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] += __shfl_xor(x[e], k);
-  const float inv = some ? 1.0f / L : 0.0f;
+  const float inv = some ? 1.0f / L : inverse_total(M, 0.0f);
   if (lane < LANES && d < head_dim) {
     Pack<T, 4> y;
 #pragma unroll

@@ -241,6 +241,29 @@ def test_values_that_a_row_does_not_see_do_not_reach_it(mx: bool, news: int) -> 
             assert not torch.isfinite(out[:, first:]).all()
 
 
+@pytest.mark.parametrize("news", [1, 40])
+def test_scores_of_minus_infinity(tuned, news: int) -> None:
+    """Rows that see keys but nothing above -infinity are 0 / 0; one finite score is enough for a sum."""
+    for dtype in DTYPES:
+        for keys in (0, 64):
+            tuned(0, keys)
+            s = step([720, 90], [news, news], heads=8, kv_heads=2, page=16, dtype=dtype, device=DEV)
+            s.k_pages[..., 0] = 1.0
+            s.q[:, ::2, :, 0] = -math.inf
+            want, bound = attention64(s)
+            out = attend(s)
+            assert out[:, ::2].isnan().all()
+            assert_within(out, want, bound, f"{dtype} {keys}")
+            s = step([720, 90], [news, news], heads=8, kv_heads=2, page=16, dtype=dtype, device=DEV)
+            s.q[..., 0] = 1.0
+            first = s.table[0, :37].long()
+            s.table[0, :37] = -1
+            want, bound = attention64(s)
+            s.table[0, :37] = first.int()
+            s.k_pages[first, ..., 0] = -math.inf  # a weight of 0, as if the keys were not there
+            assert_within(attend(s), want, bound, f"{dtype} {keys} some")
+
+
 @pytest.mark.parametrize("layout", ["heads", "tokens", "pair", "odd"])
 def test_layouts(layout: str) -> None:
     for dtype, mx in ((torch.float16, False), (torch.bfloat16, True), (torch.float32, False), (torch.bfloat16, False)):

@@ -197,6 +197,11 @@ int ako_set_tuning(int op, int key, int value) {
       if (value > 65536) return fail(AKO_ERR_INVALID_ARGUMENT, "paged attention tuning values are at most 65536");
       if (key == 1) { ako::g_paged_tuning.items = value; return AKO_OK; }
       if (key == 2) { ako::g_paged_tuning.min_keys = value; return AKO_OK; }
+      if (key == 3) {
+        if (value > 2) return fail(AKO_ERR_INVALID_ARGUMENT, "paged attention kernel must be 0, 1 or 2, got %d", value);
+        ako::g_paged_tuning.kernel = value;
+        return AKO_OK;
+      }
       break;
     default:
       break;

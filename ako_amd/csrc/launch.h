@@ -78,8 +78,9 @@ struct SwigluTuning {
   TuningKey xcd_chunk{0};        // key 2: consecutive workgroups per XCD run (1 = block order; 0 = runs of 4 for launches of 2048-65535 workgroups)
 };
 struct PagedTuning {
-  TuningKey items{0};     // key 1: work items wanted beyond one for each row tile (0 = by kernel)
-  TuningKey min_keys{0};  // key 2: least keys of a part of a split key range (0 = 256)
+  TuningKey items{0};     // key 1: work items wanted beyond one for each row tile (0 = 1024; attn_chunk 512)
+  TuningKey min_keys{0};  // key 2: least keys of a part of a split key range (0 = 256; attn_chunk 1024 where sequences bring equally many rows)
+  TuningKey kernel{0};    // key 3: 1 attn_rows, 2 attn_chunk in 16-bit types (0 = by size)
 };
 extern PagedTuning g_paged_tuning;
 extern RmsTuning g_rms_tuning;

@@ -59,7 +59,8 @@ struct AttnDev {
   int window, sinks;
   int item0;        // first work item of the launch
   int max_parts;    // 1: key ranges are not split
-  int min_tiles;    // ranges of up to so many key tiles are not cut
+  int min_tiles;    // ranges of up to so many key tiles are not cut, and parts are at least so long,
+  int few_tiles;    // or so long, where a launch has few items
   float per_item;   // 1 / work items wanted for each key head
   float per_few;    // 1 / items of a launch that is not worth cutting further, for each key head
   float scale_log2;       // |scale| * log2(e), above 0: exponentials are of base 2
@@ -102,12 +103,12 @@ struct Item {
 // Work item `item` of one key head. Items are laid out on the device, from the
 // lengths that are only known there: with T the key tiles of all row tiles,
 // a range of n > min_tiles tiles is cut into n / L parts, L = max(min_tiles, T * per_item),
-// or less than min_tiles as long as there are few items (per_few): then the time
-// is that of one item, and not of the bytes. That makes at most 1 / per_item items more than there are row tiles, which the host
-// launches; long sequences do not hold up a step of short ones, and where all
+// or as little as few_tiles as long as that makes few items (T * per_few): then the
+// time is that of one item, and not of the bytes. That makes at most 1 / per_item
+// items more than there are row tiles, which the host launches; long sequences do not hold up a step of short ones, and where all
 // are long the items are 1 / per_item, a number of whole rounds of the chip
-// (one item more would cost another round). What lies behind the last packed sequence counts as one more, padding. Sequences are
-// looked at 64 at a time, one per lane.
+// (one item more would cost another round). What lies behind the last packed
+// sequence counts as one more, padding. Sequences are looked at 64 at a time, one per lane.
 template <int R, int KT>
 __device__ __forceinline__ bool find_item(const AttnDev& a, int item, Item& t) {
   const PagedDev& p = a.c;
@@ -145,7 +146,7 @@ __device__ __forceinline__ bool find_item(const AttnDev& a, int item, Item& t) {
     // 1e9 tiles are more than any range has.
     total = wave_sum(total) * 1.0001f;
     const auto share = [&](float per) { return static_cast<int>(__builtin_fminf(total * per, 1e9f)) + 1; };
-    len = max(share(a.per_item), min(a.min_tiles, max(2, share(a.per_few))));
+    len = max(share(a.per_item), min(a.min_tiles, max(a.few_tiles, share(a.per_few))));
   }
   int before = 0, slots_before = 0;
   for (int base = 0; base < n; base += kWave) {
@@ -1065,8 +1066,9 @@ struct Plan {
   int rows;           // of a row tile
   int64_t row_tiles;  // for one key head, at most
   int64_t items;      // work items wanted for one key head beyond one for each row tile
-  int64_t few;        // items for one key head up to which ranges are cut below min_keys (0: not)
+  int64_t few;        // items for one key head up to which ranges are cut below min_keys
   int max_parts, min_keys;
+  int few_keys;       // of a part, where there are few
   int64_t slots;      // row tiles of parts, of all key heads, at most
 };
 
@@ -1075,22 +1077,40 @@ Plan plan(const PagedAttentionArgs& a) {
   Plan p{};
   // Rows that share a key head, per sequence (on average in a packed step).
   const int64_t rows = a.c.n_seqs > 0 ? ceil_div(a.c.tokens * group, a.c.n_seqs) : 1;
-  p.chunk = a.dtype != kF32 && rows > 16;
-  p.once = a.dtype != kF32 || rows <= 16;
-  p.rows = p.chunk ? kChunkRows : 16;
-  p.row_tiles = a.c.cu ? a.c.tokens * group / p.rows + a.c.n_seqs + 1 : a.c.n_seqs * ceil_div(rows, p.rows);
-  const int forced_items = g_paged_tuning.items, forced_keys = g_paged_tuning.min_keys;
-  p.items = ceil_div(forced_items > 0 ? forced_items : p.chunk ? 512 : 1024, a.c.kv_heads);
-  p.min_keys = forced_keys > 0 ? forced_keys : p.chunk && !a.c.cu ? 1024 : 256;
-  // No more than without a window: the workspace is asked for without knowing it.
+  // 128 rows share each key tile's way through LDS, 16 do not, but make eight times the
+  // workgroups and walk their tiles four at a time. So small launches go to the
+  // latter; by the capacity, as the lengths are only known on the device. Measured,
+  // heads of 128 in bf16, attn_rows / attn_chunk, by 16-row tiles of all heads times keys:
+  // 2^15 (a prompt of 128, 32 heads) 7.5 / 11.4 us, 2^17 (of 256) 9.4 / 15.1,
+  // 160 K (16 x 640 keys, 32 rows) 19.5 / 23.4, 2^18 (16384 keys, 32 rows) 36 / 28,
+  // 2^19 (a prompt of 512) 25.4 / 22.1, 2^21 (16384 keys, 256 rows) 81 / 43.
+  // Up to 16 rows attn_chunk has nothing to share: 8 x 16384 keys 84 / 97.
   const int64_t capacity = a.c.table_width * a.c.page_size;
+  const auto row_tiles = [&](int64_t r) { return a.c.cu ? a.c.tokens * group / r + a.c.n_seqs + 1 : a.c.n_seqs * ceil_div(rows, r); };
+  constexpr int64_t kSmall = 3 << 16;
+  p.chunk = a.dtype != kF32 && rows > 16 && row_tiles(16) * a.c.kv_heads > kSmall / std::max<int64_t>(1, capacity);
+  if (g_paged_tuning.kernel > 0) p.chunk = a.dtype != kF32 && g_paged_tuning.kernel == 2;
+  p.once = rows <= 16;
+  p.rows = p.chunk ? kChunkRows : 16;
+  p.row_tiles = row_tiles(p.rows);
+  const int forced_items = g_paged_tuning.items, forced_keys = g_paged_tuning.min_keys;
+  // Two rounds of the two workgroups that a CU holds; attn_chunk's sums of 128 rows
+  // are eight times as much to write and join, so one. attn_rows with 512 / 1024 / 2048:
+  // 16 x 32768 keys in bf16 347 / 331 / 331 us.
+  p.items = ceil_div(forced_items > 0 ? forced_items : p.chunk ? 512 : 1024, a.c.kv_heads);
+  // Cutting costs the second kernel, some 4 us. attn_chunk, cut from 256 / from 1024 keys: a prompt
+  // of 512 24.8 / 22.0 us, but a ragged packed step, whose longest sequence is the time, 40.7 / 57.9.
+  p.min_keys = forced_keys > 0 ? forced_keys : p.chunk && !a.c.cu ? 1024 : 256;
+  // Few items: one token at 640 keys, 32 heads, in parts of 256 / 64 14.1 / 10.1 us; attn_chunk, 32
+  // rows at 2048 keys, 32 heads, in parts of 1024 / 256 60 / 20.6.
+  p.few_keys = std::min(p.min_keys, p.chunk ? 256 : 64);
+  // No more than without a window: the workspace is asked for without knowing it.
   const int64_t keys = a.window > 0 ? std::min(capacity, std::min(a.window, capacity) + std::min(a.sinks, capacity)) : capacity;
-  p.few = p.chunk ? 0 : ceil_div(256, a.c.kv_heads);
-  p.max_parts = static_cast<int>(std::min<int64_t>(kMaxParts, keys / (p.chunk ? p.min_keys : std::min(p.min_keys, 64))));
+  p.few = ceil_div(256, a.c.kv_heads);
+  p.max_parts = static_cast<int>(std::min<int64_t>(kMaxParts, keys / p.few_keys));
   if (p.max_parts <= 1 || keys <= p.min_keys) {
     p.max_parts = 1;
     p.items = 0;
-    p.few = 0;
   } else {
     p.items = std::min(p.items, p.row_tiles * p.max_parts);
     p.slots = p.items * a.c.kv_heads;  // a range that is cut has at most length / L parts
@@ -1126,7 +1146,8 @@ hipError_t run(const PagedAttentionArgs& a, hipStream_t stream) {
   d.max_parts = p.max_parts;
   const int tile = p.chunk ? (DP <= 128 ? 64 : 32) : sizeof(T) == 4 ? 16 : 32;
   d.min_tiles = std::max(1, p.min_keys / tile);
-  d.per_few = p.few > 0 ? 1.0f / static_cast<float>(p.few) : 1.0f;
+  d.few_tiles = std::max(1, p.few_keys / tile);
+  d.per_few = 1.0f / static_cast<float>(p.few);
   d.per_item = p.items > 0 ? 1.0f / static_cast<float>(p.items) : 0.0f;
   // Not 0: times it a masked score, -inf, has to stay that.
   d.scale_log2 = std::max(std::fabs(a.scale) * 1.44269504088896340736f, std::numeric_limits<float>::min());
@@ -1153,7 +1174,7 @@ hipError_t run(const PagedAttentionArgs& a, hipStream_t stream) {
       if (p.once) {
         if (page16) AKO_LAUNCH((attn_rows<T, MX, DP, kWaves, true, true>), grid, block, 0, stream, d);
         else AKO_LAUNCH((attn_rows<T, MX, DP, kWaves, false, true>), grid, block, 0, stream, d);
-      } else if constexpr (sizeof(T) == 4) {
+      } else {
         if (page16) AKO_LAUNCH((attn_rows<T, MX, DP, kWaves, true, false>), grid, block, 0, stream, d);
         else AKO_LAUNCH((attn_rows<T, MX, DP, kWaves, false, false>), grid, block, 0, stream, d);
       }

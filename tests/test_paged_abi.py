@@ -142,7 +142,8 @@ def test_tuning_keys() -> None:
     for key in (1, 2):
         assert lib.ako_set_tuning(3, key, 0) == OK and lib.ako_set_tuning(3, key, -1) == INVALID
         assert lib.ako_set_tuning(3, key, 65537) == INVALID
-    assert lib.ako_set_tuning(3, 3, 0) == INVALID and lib.ako_set_tuning(3, 0, 0) == INVALID
+    assert lib.ako_set_tuning(3, 3, 2) == OK and lib.ako_set_tuning(3, 3, 0) == OK and lib.ako_set_tuning(3, 3, 3) == INVALID
+    assert lib.ako_set_tuning(3, 4, 0) == INVALID and lib.ako_set_tuning(3, 0, 0) == INVALID
 
 
 def test_read_refusals() -> None:
@@ -155,8 +156,16 @@ def test_read_refusals() -> None:
 @given(dtype=st.sampled_from([F32, F16, BF16]), mx=st.booleans(), heads=st.sampled_from([1, 2, 4, 8]), group=st.sampled_from([1, 2, 5, 8]),
        d=st.sampled_from([16, 64, 128, 256]), page=st.integers(1, 300), width=st.integers(0, 400), n=st.integers(1, 70),
        new=st.integers(1, 300), packed=st.booleans(), window=st.one_of(st.just(0), st.integers(1, 100000), st.just(2**40)),
-       sinks=st.one_of(st.integers(0, 3000), st.just(2**40)))
-def test_the_workspace_does_for_every_window(dtype, mx, heads, group, d, page, width, n, new, packed, window, sinks) -> None:
+       sinks=st.one_of(st.integers(0, 3000), st.just(2**40)), kernel=st.integers(0, 2))
+def test_the_workspace_does_for_every_window(dtype, mx, heads, group, d, page, width, n, new, packed, window, sinks, kernel) -> None:
+    _native.set_tuning(3, 3, kernel)
+    try:
+        workspace_does(dtype, mx, heads, group, d, page, width, n, new, packed, window, sinks)
+    finally:
+        _native.set_tuning(3, 3, 0)
+
+
+def workspace_does(dtype, mx, heads, group, d, page, width, n, new, packed, window, sinks) -> None:
     c = cache(dtype=E4M3 if mx else dtype, kv_heads=heads, d=d, page=page, width=width, n=n, tokens=n * new,
               cu=CU if packed else None, pages=4)
     need = _native.load().ako_paged_attention_workspace(ctypes.addressof(c), heads * group, dtype)

@@ -20,13 +20,33 @@ DTYPES = [torch.float32, torch.float16, torch.bfloat16]
 HEAD_DIMS = [16, 32, 48, 64, 80, 96, 112, 128, 160, 192, 256]
 
 
+def set_kernel(n: int) -> None:
+    from ako_amd import _native
+
+    _native.set_tuning(3, 3, n)
+
+
+@pytest.fixture(params=["by size", "chunk"])
+def kernel(request):
+    """As the sizes choose, which for small cases is 16 rows per workgroup, and with 128."""
+    set_kernel(2 if request.param == "chunk" else 0)
+    yield
+    set_kernel(0)
+
+
 def attend(s, **opts):
     return ako.paged_attention(s.q, *s.where, **opts, **s.kw)
 
 
 def check(s, what="", **opts) -> None:
+    """Against 64 bits, with the kernel that the sizes choose and with that of long chunks."""
     want, bound = attention64(s, **opts)
     assert_within(attend(s, **opts), want, bound, what)
+    set_kernel(2)
+    try:
+        assert_within(attend(s, **opts), want, bound, what + ", chunk")
+    finally:
+        set_kernel(0)
 
 
 # ------------------------------------------------------------------------ write, read --
@@ -184,6 +204,7 @@ def test_a_wide_table_is_read_only_as_far_as_needed() -> None:
     check(s)
 
 
+@pytest.mark.usefixtures("kernel")
 @pytest.mark.parametrize("news", [1, 40])
 def test_padding_and_short_sequences(news: int) -> None:
     for dtype in DTYPES:
@@ -196,6 +217,7 @@ def test_padding_and_short_sequences(news: int) -> None:
         assert not attend(e).any()
 
 
+@pytest.mark.usefixtures("kernel")
 @pytest.mark.parametrize("news", [1, 33])
 def test_lengths_and_tables_that_make_no_sense(news: int) -> None:
     """Device-side indexes cannot be checked on the host: whatever they hold, nothing outside the
@@ -219,6 +241,7 @@ def test_lengths_and_tables_that_make_no_sense(news: int) -> None:
     torch.cuda.synchronize()
 
 
+@pytest.mark.usefixtures("kernel")
 @pytest.mark.parametrize("news", [1, 5, 40, 129])
 @pytest.mark.parametrize("mx", [False, True])
 def test_values_that_a_row_does_not_see_do_not_reach_it(mx: bool, news: int) -> None:
@@ -241,6 +264,7 @@ def test_values_that_a_row_does_not_see_do_not_reach_it(mx: bool, news: int) -> 
             assert not torch.isfinite(out[:, first:]).all()
 
 
+@pytest.mark.usefixtures("kernel")
 @pytest.mark.parametrize("news", [1, 40])
 def test_scores_of_minus_infinity(tuned, news: int) -> None:
     """Rows that see keys but nothing above -infinity are 0 / 0; one finite score is enough for a sum."""
@@ -402,6 +426,7 @@ def test_sequences_that_share_pages() -> None:
     check(s)
 
 
+@pytest.mark.usefixtures("kernel")
 def test_results_do_not_change_from_run_to_run() -> None:
     s = step([3000, 900, 5], [7, 7, 7], heads=8, kv_heads=2, dtype=torch.bfloat16, device=DEV)
     first = attend(s)

@@ -828,6 +828,9 @@ int attention_common(const char* fn, const ako_paged_t* cache, int64_t q_heads, 
   *empty = *empty || q_heads == 0;
   a->q_heads = q_heads;
   a->dtype = dtype;
+  a->tuned_items = ako::g_paged_tuning.items;
+  a->tuned_min_keys = ako::g_paged_tuning.min_keys;
+  a->tuned_kernel = ako::g_paged_tuning.kernel;
   return AKO_OK;
 }
 

@@ -212,6 +212,8 @@ struct PagedAttentionArgs {
   float scale;
   int dtype;
   void* workspace;  // paged_attention_workspace bytes
+  // The tuning keys, read once for the call: the workspace is sized and used by the same values.
+  int tuned_items, tuned_min_keys, tuned_kernel;
 };
 int64_t paged_attention_workspace(const PagedAttentionArgs& a);
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t stream);

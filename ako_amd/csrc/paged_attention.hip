@@ -377,6 +377,13 @@ __device__ __forceinline__ u32x4 load16(const uint8_t* p) {
 // piece of LDS, so that no barrier stands in the loop; the loads of a later tile
 // are issued as soon as those registers are free, and are in flight while this
 // tile is worked on. The wavefronts' results are joined in LDS at the end.
+//
+// Bound by HBM once the ranges are long: 2.1 GB of e4m3 pages in 342 us, 6.1 TB/s, 538 MB
+// of bf16 under a window in 90 us, 6.0 TB/s (a large copy reaches 6.67). Whole rows of K through
+// LDS rather than the operand's 16 bytes of 16 rows per load, and non-temporal
+// loads, took the first from 5.6 TB/s. The 8-bit tiles are half as large, so
+// two of them are in flight. Short ranges are latency: 10 us at 640 keys, of
+// which 4 are the join's.
 template <typename T, bool MX, int DP>
 struct RowsShape {
   static constexpr int kBlocks = sizeof(T) == 4 ? 1 : 2;    // 16-key blocks per tile
@@ -687,11 +694,16 @@ __global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 && !MX ? 3 : DP
 
 // ---- many rows per workgroup ---------------------------------------------------------
 // Chunks of a prompt in half types: 32 rows per wavefront, which share each key
-// tile through LDS. Bound by the matrix cores and, about as much, by the
-// exponentials beside them: two workgroups fit on a CU, so that one's
-// exponentials run under the other's products. A tile's loads are issued a whole
-// tile ahead, into registers, and go to the other half of LDS after the
-// products of the tile before.
+// tile through LDS. A tile's loads are issued a whole tile ahead, into registers,
+// and go to the other half of LDS after the products of the tile before.
+//
+// 2048 tokens at the end of 32768 keys, 32 heads of 128 in groups of 4 (1.07 TFLOP
+// in bf16): 1216 us, 876 TFLOP/s (1196 to 1268 us over the cards tried), where a
+// large library product reaches 1255. Counters: matrix cores busy 34% of the cycles, VALU 23%, LDS
+// 35%, 98% of the loads from L2. So neither is the bound, but the chain of
+// product, maximum, exponentials, product within a wavefront (2.1 us per tile of 64
+// keys alone on a CU), and what fills it is other wavefronts: two workgroups
+// on a CU, eight wavefronts, at 256 registers each. 64 rows per workgroup: 2142 us.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ f32x16 mfma32(const Eight<__bf16>& a, const Eight<__bf16>& b, f32x16 c) {
@@ -1089,18 +1101,17 @@ Plan plan(const PagedAttentionArgs& a) {
   const auto row_tiles = [&](int64_t r) { return a.c.cu ? a.c.tokens * group / r + a.c.n_seqs + 1 : a.c.n_seqs * ceil_div(rows, r); };
   constexpr int64_t kSmall = 3 << 16;
   p.chunk = a.dtype != kF32 && rows > 16 && row_tiles(16) * a.c.kv_heads > kSmall / std::max<int64_t>(1, capacity);
-  if (g_paged_tuning.kernel > 0) p.chunk = a.dtype != kF32 && g_paged_tuning.kernel == 2;
+  if (a.tuned_kernel > 0) p.chunk = a.dtype != kF32 && a.tuned_kernel == 2;
   p.once = rows <= 16;
   p.rows = p.chunk ? kChunkRows : 16;
   p.row_tiles = row_tiles(p.rows);
-  const int forced_items = g_paged_tuning.items, forced_keys = g_paged_tuning.min_keys;
   // Two rounds of the two workgroups that a CU holds; attn_chunk's sums of 128 rows
   // are eight times as much to write and join, so one. attn_rows with 512 / 1024 / 2048:
   // 16 x 32768 keys in bf16 347 / 331 / 331 us.
-  p.items = ceil_div(forced_items > 0 ? forced_items : p.chunk ? 512 : 1024, a.c.kv_heads);
+  p.items = ceil_div(a.tuned_items > 0 ? a.tuned_items : p.chunk ? 512 : 1024, a.c.kv_heads);
   // Cutting costs the second kernel, some 4 us. attn_chunk, cut from 256 / from 1024 keys: a prompt
   // of 512 24.8 / 22.0 us, but a ragged packed step, whose longest sequence is the time, 40.7 / 57.9.
-  p.min_keys = forced_keys > 0 ? forced_keys : p.chunk && !a.c.cu ? 1024 : 256;
+  p.min_keys = a.tuned_min_keys > 0 ? a.tuned_min_keys : p.chunk && !a.c.cu ? 1024 : 256;
   // Few items: one token at 640 keys, 32 heads, in parts of 256 / 64 14.1 / 10.1 us; attn_chunk, 32
   // rows at 2048 keys, 32 heads, in parts of 1024 / 256 60 / 20.6.
   p.few_keys = std::min(p.min_keys, p.chunk ? 256 : 64);

@@ -5,8 +5,12 @@
 // model's type or as e4m3 with a power-of-two scale per 32 elements (paged.h).
 // paged_read: the same rows of both caches as dense tensors.
 //
-// Both move every byte once. A workgroup stays inside one token, so that the token's sequence, position and page are found once per
-// wavefront and not per lane.
+// Both move every byte once. A workgroup stays inside one token, so that the
+// token's sequence, position and page are found once per wavefront and not per
+// lane. Bound by HBM on long prompts: 4 x 2048 tokens into e4m3 pages, 186 MB, in
+// 37.5 us, 4.9 TB/s (a copy of that size reaches 6.5); 69 MB of such pages and
+// what comes of them in 13.7, 5.0 TB/s. One step's 1.6 MB is launch latency: 2.8 us
+// replayed from a graph.
 
 #include <algorithm>
 

@@ -297,7 +297,7 @@ int64_t ako_paged_attention_workspace(const ako_paged_t* cache, int64_t q_heads,
  * Launch-shape override for tuning sweeps and tests (no counterpart in the
  * reference, whose Triton autotuner explored num_warps itself); production
  * callers leave it alone. op: 0 = rmsnorm and rmsnorm_residual, 1 = rope,
- * 2 = swiglu. key/value pairs are documented in the kernel sources; value 0
+ * 2 = swiglu, 3 = paged attention. key/value pairs are documented in the kernel sources; value 0
  * restores the built-in heuristic. Process-wide. Each key is an atomic int,
  * so the call is safe from any host thread: a launch that runs concurrently
  * sees each key's value from before or after the call (a launch concurrent

@@ -103,7 +103,8 @@ def paged_attention(
     position ``p`` sees the positions ``j <= p``; with ``window``, of those only
     ``j > p - window`` and the first ``sinks``. ``scale`` is ``head_dim ** -0.5``
     unless given. Rows that see nothing (padding) are zero, and what a row does
-    not see has no influence on it, whatever is stored there.
+    not see has no influence on it, whatever is stored there. A row that sees keys, but
+    whose scores are all -infinity, is NaN, as their softmax is.
     """
     if q.is_cuda and not hip_disabled():
         return paged_attention_hip(q, k_pages, v_pages, block_table, seq_lens, scale, window, sinks,

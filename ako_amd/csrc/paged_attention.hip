@@ -834,6 +834,8 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
     return here != (KT == 64 ? ~uint64_t(0) : (uint64_t(1) << (KT % 64)) - 1) || k0 + KT - 1 > first ||
            (a.window > 0 && k0 <= last - a.window && k0 + KT > a.sinks);
   };
+  // A tile into LDS; returns whether it is an edge for some wavefront, and infinities
+  // and NaN were therefore taken out of V for all of them.
   const auto store_tile = [&](int i, int buf, uint64_t here) {
     const bool edge = is_edge(i, here, first_all, last_all);
     unsigned odd = 0;
@@ -869,18 +871,19 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
         *reinterpret_cast<u32x4*>(lds[buf][1] + lds_packet_v<ROW>(j, p)) = v[c].p[0].raw;
       }
     }
-
+    return edge;
   };
 
   uint64_t here = 0;
-  bool any = false;  // the row sees a key
+  bool taken_out = false;  // of the tile in LDS
+  bool any = false;        // the row sees a key
   int pg = 0;
   if (begin < end) {
     pg = look_up(begin);
     here = present(pg, begin);
     load_tile(begin, pg);
     if (begin + 1 < end) pg = look_up(begin + 1);
-    store_tile(begin, 0, here);
+    taken_out = store_tile(begin, 0, here);
   }
   __syncthreads();
   for (int i = begin; i < end; ++i) {
@@ -951,7 +954,8 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)
           o[d] = mfma32(read_v<T, ROW>(vl, 32 * d + 16 * (lane / 16 % 2), 16 * j + 4 * h, lane), p[j], o[d]);
-      if (edge) {
+      // Also by a wavefront whose own rows see the whole tile.
+      if (taken_out) {
 #pragma nounroll
         for (int w = 0; w < WAVES; ++w) {
           if (__builtin_expect(!__builtin_amdgcn_readfirstlane(lds_odd[buf][w]), 1)) continue;
@@ -971,7 +975,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
         }
       }
     }
-    if (i + 1 < end) store_tile(i + 1, buf ^ 1, next);
+    if (i + 1 < end) taken_out = store_tile(i + 1, buf ^ 1, next);
     here = next;
     __syncthreads();
   }

@@ -1,0 +1,86 @@
+"""Infinities and NaN among stored values, and scale codes at the end of their range: they reach
+every row that sees them, as the signed infinity or NaN, and no other row, whichever wavefront or
+workgroup a row lies in."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import ako_amd as ako
+from tests._paged import E4M3, Step, attention64, step
+
+gpu = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a GPU")]
+DEVICES = ["cpu", pytest.param("cuda", marks=gpu)]
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def results(s: Step, **opts):
+    """The result with the kernel that the sizes choose and, on a GPU, with each by name."""
+    yield "by size", ako.paged_attention(s.q, *s.where, **opts, **s.kw)
+    if s.q.is_cuda:
+        from ako_amd import _native
+
+        for n, name in ((1, "rows"), (2, "chunk")):
+            _native.set_tuning(3, 3, n)
+            try:
+                yield name, ako.paged_attention(s.q, *s.where, **opts, **s.kw)
+            finally:
+                _native.set_tuning(3, 3, 0)
+
+
+def sees(s: Step, i: int, j: int, window=None, sinks=0) -> list[int]:
+    """The rows of q that see key ``j`` of sequence ``i``."""
+    first, n, m = sum(s.news[:i]), s.held[i], s.news[i]
+    return [first + a for a in range(m)
+            if j <= n - m + a and (window is None or j > n - m + a - window or j < sinks)]
+
+
+def assert_same(got: torch.Tensor, want: torch.Tensor, bound: torch.Tensor, what: str) -> None:
+    """NaN where NaN is wanted, the signed infinity where that is, and everything else within ``bound``."""
+    got, want = got.double(), want.double()
+    finite = want.isfinite()
+    assert torch.equal(got.isnan(), want.isnan()), f"{what}: NaN in other places"
+    assert torch.equal(got[want.isinf()], want[want.isinf()]), f"{what}: other infinities"
+    off = (got - want).abs()[finite] / bound[finite]
+    assert bool((off <= 1).all()), f"{what}: off by up to {float(off.max()):.2f} bounds"
+
+
+def put(s: Step, wanted: torch.Tensor, i: int, j: int, kv_head: int, e: int, value: float, **opts) -> None:
+    """Stores ``value`` as element ``e`` of key ``j``'s row of V, and in ``wanted`` for the rows that see it."""
+    page, kv_heads = s.v_pages.shape[2], s.v_pages.shape[1]
+    group = s.q.shape[-2] // kv_heads
+    s.v_pages[s.table[i, j // page], kv_head, j % page, e] = value
+    at = wanted.flatten(0, -3)
+    heads = slice(kv_head * group, (kv_head + 1) * group)
+    rows = sees(s, i, j, **opts)
+    at[rows, heads, e] += value  # two at one place: their sum, as in the formula
+
+
+CASES = [  # held, new rows, packed, query heads of 2 key heads
+    ([129], [129], False, 2), ([512], [512], False, 2), ([200, 166], [129, 129], False, 8),
+    ([75, 230, 1, 150], [75, 193, 1, 120], True, 8),
+]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("opts", [{}, {"window": 100, "sinks": 3}, {"window": 200}], ids=["causal", "sinks", "window"])
+@pytest.mark.parametrize("case", range(len(CASES)))
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_values_that_are_not_finite_reach_every_row_that_sees_them(dtype, case: int, opts, device: str) -> None:
+    held, news, packed, heads = CASES[case]
+    for head_dim in (64, 256) if case == 0 else (64,):
+        s = step(held, news, heads=heads, head_dim=head_dim, dtype=dtype, packed=packed, device=device, seed=case)
+        want, bound = attention64(s, **opts)
+        for i, n in enumerate(held):
+            for e, (j, value) in enumerate(((0, math.nan), (10, math.inf), (37, -math.inf), (63, math.nan), (64, math.inf),
+                                            (100, -math.inf), (127, math.inf), (128, math.nan), (n - 1, math.inf))):
+                if j < n:
+                    put(s, want, i, j, e % 2, 7 * e, value, **opts)
+            if n > 20:  # two at one element: NaN where a row sees both
+                put(s, want, i, 15, 0, 5, math.inf, **opts)
+                put(s, want, i, 20, 0, 5, -math.inf, **opts)
+        for name, out in results(s, **opts):
+            assert_same(out, want, bound, f"{name}, heads of {head_dim}")

@@ -97,7 +97,7 @@ __device__ __forceinline__ int page_of(const PagedDev& p, int s, int pos, int& s
 }
 
 // ---- e4m3 rows with a power-of-two scale per 32 elements -----------------------
-// An E8M0 code c stands for 2^(c - 127). A block's code is the smallest under
+// An E8M0 code c stands for 2^(c - 127), 255 for NaN. A block's code is the smallest under
 // which no finite element passes e4m3's largest value, 448 = 1.75 * 2^8; so
 // nothing is clipped, and every element at or above 2^-6 of its scale is off
 // by at most half a step of e4m3, 2^-4 of itself. Codes below 1 are not used:

@@ -12,7 +12,7 @@ positions of sequence ``i``. Packed rows behind the last sequence, and rows whos
 position would be negative, are padding.
 
 Pages are of the rows' type, or ``torch.float8_e4m3fn`` with one E8M0 code
-(``uint8`` c, standing for 2^(c-127)) per 32 elements of a row.
+(``uint8`` c, standing for 2^(c-127), 255 for NaN) per 32 elements of a row.
 """
 
 from __future__ import annotations
@@ -163,8 +163,8 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 
 def dequantize_rows(q: torch.Tensor, codes: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    """What e4m3 rows with scale codes stand for, in ``dtype``."""
-    scale = torch.ldexp(torch.ones((), device=q.device), codes.int() - 127)
+    """What e4m3 rows with scale codes stand for, in ``dtype``; code 255 is E8M0's NaN."""
+    scale = torch.ldexp(torch.ones((), device=q.device), codes.int() - 127).masked_fill_(codes == 255, math.nan)
     return (q.float() * scale.repeat_interleave(SCALE_BLOCK, -1)[..., : q.shape[-1]]).to(dtype)
 
 

@@ -224,7 +224,7 @@ int ako_swiglu_fwd(const void* gate, const void* up, void* y,
  * outside the tensors.
  *
  * page_dtype is the rows' own dtype, or AKO_DTYPE_E4M3: one byte per element
- * and, for each 32 elements of a row, an E8M0 scale code c (2^(c-127)) in
+ * and, for each 32 elements of a row, an E8M0 scale code c (2^(c-127); 255 is NaN) in
  * k_scales / v_scales [num_pages, kv_heads, page_size, ceil(head_dim/32)],
  * last dimension contiguous. A block is written with the smallest code >= 1
  * under which none of its finite elements passes 448, elements rounded to

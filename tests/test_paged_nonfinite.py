@@ -84,3 +84,24 @@ def test_values_that_are_not_finite_reach_every_row_that_sees_them(dtype, case: 
                 put(s, want, i, 20, 0, 5, -math.inf, **opts)
         for name, out in results(s, **opts):
             assert_same(out, want, bound, f"{name}, heads of {head_dim}")
+
+
+# ------------------------------------------------------------------- scale codes --
+def element(byte: int, code: int) -> float:
+    """What an e4m3 byte under an E8M0 code stands for: 255 is the format's NaN."""
+    x = float(torch.tensor([byte], dtype=torch.uint8).view(E4M3).double())
+    return math.nan if code == 255 else x * 2.0 ** (code - 127)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_every_byte_under_every_code_reads_as_the_format_says(dtype, device: str) -> None:
+    pages = torch.arange(256, dtype=torch.uint8).repeat(256, 1, 1, 1).contiguous().to(device).view(E4M3)
+    codes = torch.arange(256, dtype=torch.uint8).view(256, 1, 1, 1).repeat(1, 1, 1, 8).to(device)
+    table = torch.arange(256, dtype=torch.int32, device=device).view(256, 1)
+    lens = torch.ones(256, dtype=torch.int32, device=device)
+    k, v = ako.paged_read(pages, pages, table, lens, 1, dtype, k_scales=codes, v_scales=codes)
+    want = torch.tensor([[element(b, c) for b in range(256)] for c in range(256)], dtype=torch.float64)
+    want = want.float().to(dtype)  # exact in 32 bits but for what is infinite there: one rounding
+    for got in (k.cpu().view(256, 256), v.cpu().view(256, 256)):
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(7, 8, 9), want.nan_to_num(7, 8, 9))

@@ -108,6 +108,7 @@ __device__ __forceinline__ unsigned e8m0_code(float amax) {
   const int e = static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u);
   return static_cast<unsigned>(max(e, -126) + 127);
 }
+constexpr unsigned kUnitCode = 127;
 __device__ __forceinline__ float e8m0_scale(unsigned code) { return __builtin_bit_cast(float, code << 23); }
 __device__ __forceinline__ float e8m0_inverse(unsigned code) { return __builtin_bit_cast(float, (254u - code) << 23); }
 

@@ -231,7 +231,8 @@ __device__ __forceinline__ float sum_over_groups(float v) {
 // Nonzero where a word of values holds an infinity or NaN (or might, once
 // multiplied by its scale): their exponents are all ones, and one more in the exponent's
 // last place then carries into the sign's, which was masked out. e4m3 has only NaN,
-// all ones below the sign; in fp16 scales from 2^8 on can take it past the end.
+// all ones below the sign; scales from 2^8 on in fp16, from 2^120 on in the other types,
+// can take it past the end, and under code 255 everything is NaN, zeros too.
 template <typename T, bool MX>
 __device__ __forceinline__ unsigned odd_values(u32x4 w, unsigned code) {
   constexpr unsigned kMask = MX ? 0x7f7f7f7fu : sizeof(T) == 4 ? 0x7f800000u : __is_same(T, __bf16) ? 0x7f807f80u : 0x7c007c00u;
@@ -241,7 +242,7 @@ __device__ __forceinline__ unsigned odd_values(u32x4 w, unsigned code) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) odd |= (w[i] & kMask) + kOne;
   odd &= kSign;
-  if constexpr (MX && __is_same(T, _Float16)) odd |= code >= 127 + 8;
+  if constexpr (MX) odd |= code >= (__is_same(T, _Float16) ? 127 + 8 : 127 + 120);
   return odd;
 }
 
@@ -259,13 +260,13 @@ __device__ __forceinline__ void wave_fence() {
 // then adds the infinities of those keys that it does see (add_odd).
 // Bit n * KPW + w is the key of load n that is w-th among the KPW of the wavefront.
 template <typename T, bool MX, int DP, int KPW, int LOADS>
-__device__ __forceinline__ void take_out_odd(u32x4 (&v)[LOADS], const unsigned (&code)[LOADS], unsigned* masks, int lane) {
+__device__ __forceinline__ void take_out_odd(u32x4 (&v)[LOADS], unsigned (&code)[LOADS], unsigned* masks, int lane) {
   constexpr int C = MX ? 16 : 16 / static_cast<int>(sizeof(T)), LANES = DP / C;
   const int part = lane % LANES;
   for (int i = lane; i < 2 * DP; i += kWave) masks[i] = 0;
   wave_fence();
 #pragma unroll
-  for (int n = 0; n < LOADS; ++n)
+  for (int n = 0; n < LOADS; ++n) {
 #pragma unroll
     for (int e = 0; e < C; ++e) {
       __builtin_amdgcn_sched_barrier(0);  // rare: element by element, to cost the loop around it no registers
@@ -282,6 +283,8 @@ __device__ __forceinline__ void take_out_odd(u32x4 (&v)[LOADS], const unsigned (
       const unsigned all = kBits == 32 ? ~0u : ((1u << (kBits % 32)) - 1) << shift;
       v[n][e / kPerWord] = word & ~all;
     }
+    if (MX && code[n] == 255) code[n] = kUnitCode;
+  }
 }
 
 // Adds to elements e .. e + 3 the infinities that a row sees.
@@ -539,7 +542,10 @@ __global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 && !MX ? 3 : DP
     if (!whole) {
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
-        if (!(here >> (n * S::kRowKeys + vkey) & 1)) x.v[n] = u32x4{0, 0, 0, 0};
+        if (!(here >> (n * S::kRowKeys + vkey) & 1)) {
+          x.v[n] = u32x4{0, 0, 0, 0};
+          x.vcode[n] = kUnitCode;
+        }
         odd |= odd_values<T, MX>(x.v[n], MX ? x.vcode[n] : 0);
       }
       odd = __ballot(odd != 0) != 0;
@@ -842,7 +848,10 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
     if (edge) {
 #pragma unroll
       for (int n = 0; n < NP; ++n) {
-        if (!(here >> (n * PASS + key0) & 1)) vreg[n] = u32x4{0, 0, 0, 0};
+        if (!(here >> (n * PASS + key0) & 1)) {
+          vreg[n] = u32x4{0, 0, 0, 0};
+          vcode[n] = kUnitCode;
+        }
         odd |= odd_values<T, MX>(vreg[n], MX ? vcode[n] : 0);
       }
       odd = __ballot(odd != 0) != 0;

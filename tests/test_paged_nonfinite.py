@@ -105,3 +105,59 @@ def test_every_byte_under_every_code_reads_as_the_format_says(dtype, device: str
     want = want.float().to(dtype)  # exact in 32 bits but for what is infinite there: one rounding
     for got in (k.cpu().view(256, 256), v.cpu().view(256, 256)):
         assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(7, 8, 9), want.nan_to_num(7, 8, 9))
+
+
+def swap_out_page_0(s: Step) -> None:
+    """Moves what page 0 holds to a page that no sequence has: absent pages are often read as the first."""
+    free = min(set(range(1, s.k_pages.shape[0])) - set(s.table.flatten().tolist()))
+    for t in (s.k_pages.view(torch.uint8), s.v_pages.view(torch.uint8), s.k_scales, s.v_scales):
+        t[free] = t[0]
+    s.table[s.table == 0] = free
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("code", [0, 134, 135, 246, 247, 254, 255])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_codes_of_what_a_row_does_not_see_do_not_matter(dtype, code: int, device: str) -> None:
+    """Slots and pages that no sequence has, and keys outside every row's window, under any code."""
+    for held, news, packed in (([170, 90], [1, 1], False), ([170, 140], [129, 129], False), ([170, 33, 140], [150, 1, 64], True)):
+        for head_dim, page in ((64, 16), (48, 7)):
+            s = step(held, news, heads=8, head_dim=head_dim, page=page, dtype=dtype, mx=True, packed=packed, device=device)
+            swap_out_page_0(s)
+            s.table[0, 12 // page] = -1  # a page that is not there
+            opts = {"window": 160, "sinks": 2} if held[0] - news[0] > 160 else {}
+            want, bound = attention64(s, **opts)
+            live = torch.zeros(s.k_pages.shape[0], page, dtype=torch.bool)
+            for i, n in enumerate(held):
+                for j in range(n):
+                    if s.table[i, j // page] >= 0 and sees(s, i, j, **opts):
+                        live[s.table[i, j // page], j % page] = True
+            dead = ~live[:, None, :, None].to(device)
+            for byte in (0x00, 0x01, 0x7E, 0xFE):
+                for pages, codes in ((s.k_pages, s.k_scales), (s.v_pages, s.v_scales)):
+                    pages.view(torch.uint8).masked_fill_(dead, byte)
+                    codes.masked_fill_(dead, code)
+                for name, out in results(s, **opts):
+                    assert_same(out, want, bound, f"{name}, {held}, heads of {head_dim}, byte {byte:#x}")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype,code", [(dtype, code) for dtype in DTYPES
+                                        for code in ((135, 247, 255) if dtype == torch.float16 else (247, 254, 255))])
+def test_codes_past_the_types_range_reach_the_rows_that_see_their_keys(dtype, code: int, device: str) -> None:
+    """448 and -448 in one block of a key's values, under a code that makes them infinite in the rows' type.
+    A scale that keeps every weight far above 0, times which an infinity would be NaN."""
+    heads, kv_heads, page = 4, 2, 16
+    for j in (3, 70, 127):
+        s = step([150], [150], heads=heads, kv_heads=kv_heads, dtype=dtype, mx=True, device=device, seed=j)
+        at = s.table[0, j // page], 0, j % page
+        s.v_pages.view(torch.uint8)[at] = 0
+        want, bound = attention64(s, scale=0.01)
+        for e, byte in ((32, 0x7E), (40, 0xFE)):
+            s.v_pages.view(torch.uint8)[(*at, e)] = byte
+            want[0, j:, : heads // kv_heads, e] = math.copysign(math.inf, element(byte, 127))
+        s.v_scales[(*at, 1)] = code
+        if code == 255:
+            want[0, j:, : heads // kv_heads, 32:] = math.nan
+        for name, out in results(s, scale=0.01):
+            assert_same(out, want, bound, f"{name}, key {j}")

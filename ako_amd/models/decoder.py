@@ -530,8 +530,14 @@ class DecoderStack(nn.Module):
             if self.backend != "ako":
                 raise ValueError("a paged cache needs backend='ako'")
             cos, sin = self.rope_tables(max(kv_cache.max_len, self.config.max_seq_len), device=x.device)
-            kv_cache.begin_step(x.shape[1])
-        elif static_step:
+            tokens = x.shape[1]
+            kv_cache.begin_step(tokens)
+            try:
+                return self._run_layers(x, cos, sin, kv_cache)
+            except BaseException:
+                kv_cache.rewind(tokens)  # what a step that failed has stored lies past the length again
+                raise
+        if static_step:
             full = self.rope_tables(self.config.max_seq_len, device=x.device)
             if _fused_cache_rope(self.backend, self.kernel_override):
                 cos, sin = full  # the fused cache RoPE picks row pos itself
@@ -541,16 +547,21 @@ class DecoderStack(nn.Module):
         else:
             offset = kv_cache.length if kv_cache is not None else 0
             cos, sin = self.rope_tables(x.shape[1], offset=offset, device=x.device)
-        residual: torch.Tensor | None = None
-        for layer in self.layers:
-            x, residual = layer(x, residual, cos, sin, kv_cache=kv_cache)
-        x, _ = _norm(self.backend, x, residual, self.final_norm_weight, self.config.eps,
-                     self.kernel_override)
+        x = self._run_layers(x, cos, sin, kv_cache)
         if isinstance(kv_cache, StaticKVCache):
             if static_step:
                 kv_cache.end_step(1)
             else:
                 kv_cache.set_length(kv_cache.host_len + x.shape[1])
+        return x
+
+    def _run_layers(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                    kv_cache: KVCache | StaticKVCache | PagedKVCache | None) -> torch.Tensor:
+        residual: torch.Tensor | None = None
+        for layer in self.layers:
+            x, residual = layer(x, residual, cos, sin, kv_cache=kv_cache)
+        x, _ = _norm(self.backend, x, residual, self.final_norm_weight, self.config.eps,
+                     self.kernel_override)
         return x
 
     def new_static_cache(self, max_len: int, *, batch: int = 1) -> StaticKVCache:

@@ -667,6 +667,8 @@ class GraphedGreedy:
         with torch.cuda.graph(self.graph):
             self._step()
         self.cache.host_len -= 1  # capture ran no step on the device
+        #: The tables that the graph reads: the stack replaces its own by longer ones when it needs them.
+        self.rope_tables = model.stack._rope_tables
         self._ran = False
 
     def _step(self) -> None:

@@ -640,8 +640,8 @@ class GraphedGreedy:
         max_len = self.prompt_len + steps
         if model.config.max_seq_len < max_len:
             raise ValueError(f"max_seq_len {model.config.max_seq_len} < prompt + steps {max_len}")
-        if cache is not None and (cache.host_len or cache.max_len < max_len):
-            raise ValueError(f"graphed decoding needs an empty cache of {max_len} positions")
+        if cache is not None and (cache.host_len or cache.max_len < max_len or cache.block_table.shape[0] != 1):
+            raise ValueError(f"graphed decoding needs an empty cache of {max_len} positions and one sequence")
         self.cache = model.stack.new_static_cache(max_len) if cache is None else cache
         #: Device-side count of the positions held.
         self.position = self.cache.pos if cache is None else cache.seq_lens

@@ -89,3 +89,11 @@ def test_a_replay_after_longer_tables_were_built(paged: bool) -> None:
         taken = [torch.full((32, 8), float("nan"), device="cuda") for _ in range(64)]  # what was freed is used again
         assert torch.equal(runner.run(), want)
     del taken
+
+
+def test_graphed_decoding_refuses_a_cache_of_several_sequences() -> None:
+    model = build_lm(ModelConfig(**SIZES), dtype=torch.float32, seed=5)
+    cache = model.stack.new_paged_cache(20, batch=2)
+    with torch.no_grad(), pytest.raises(ValueError, match="empty cache of 15 positions and one sequence"):
+        GraphedGreedy(model, torch.zeros(1, 9, dtype=torch.long), 6, cache=cache)
+    assert cache.length == 0 and not cache.seq_lens.any()

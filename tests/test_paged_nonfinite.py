@@ -161,3 +161,32 @@ def test_codes_past_the_types_range_reach_the_rows_that_see_their_keys(dtype, co
             want[0, j:, : heads // kv_heads, 32:] = math.nan
         for name, out in results(s, scale=0.01):
             assert_same(out, want, bound, f"{name}, key {j}")
+
+
+# -------------------------------------------------------------------------- write --
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("mx", [False, True])
+@pytest.mark.parametrize("style", ["neox", "interleaved"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_q_and_other_slots_of_a_write_of_values_that_are_not_finite(dtype, style: str, mx: bool, device: str) -> None:
+    """A rotation by nothing: q comes back as it was, whatever k and v hold beside it, and slots that the step
+    does not write keep their bytes."""
+    for head_dim in (64, 80):
+        s = step([70, 9], [5, 5], dtype=dtype, mx=mx, head_dim=head_dim, device=device)
+        top = torch.finfo(dtype).max
+        for x in (s.k, s.v):
+            x[0, 0], x[0, 1, 0, 3], x[0, 2, 1, 40], x[1, 3, 0, 5], x[1, 4] = 0.0, math.inf, math.nan, -math.inf, top
+        s.q[0, 1], s.q[1, 2, 0] = torch.finfo(dtype).tiny, top
+        cos = torch.ones(70, head_dim // 2, device=device)
+        bits = {1: torch.uint8, 2: torch.int16, 4: torch.int32}
+        raw = lambda t: t.view(bits[t.element_size()])  # noqa: E731
+        pools = [t for t in (s.k_pages, s.v_pages, s.k_scales, s.v_scales) if t is not None]
+        before = [raw(t).clone() for t in pools]
+        out = ako.rope_qk_paged(s.q, s.k, s.v, cos, torch.zeros_like(cos), *s.where, style, **s.kw)
+        assert torch.equal(out, s.q)
+        page = s.k_pages.shape[2]
+        kept = torch.ones(s.k_pages.shape[0], 1, page, 1, dtype=torch.bool, device=device)
+        for i, n in enumerate(s.held):
+            for p in range(n - 5, n):
+                kept[s.table[i, p // page], :, p % page] = False
+        assert all(torch.equal(raw(t)[kept.expand(t.shape)], was[kept.expand(t.shape)]) for t, was in zip(pools, before))

@@ -108,7 +108,8 @@ struct Item {
 // items more than there are row tiles, which the host launches; long sequences do not hold up a step of short ones, and where all
 // are long the items are 1 / per_item, a number of whole rounds of the chip
 // (one item more would cost another round). What lies behind the last packed
-// sequence counts as one more, padding. Sequences are looked at 64 at a time, one per lane.
+// sequence counts as one more, padding. Sequences are looked at 64 at a time, one per lane,
+// by every workgroup: at 64 keys and 8 key heads 64 sequences take 7.4 us, 256 30, 1024 168.
 template <int R, int KT>
 __device__ __forceinline__ bool find_item(const AttnDev& a, int item, Item& t) {
   const PagedDev& p = a.c;
@@ -381,11 +382,12 @@ __device__ __forceinline__ u32x4 load16(const uint8_t* p) {
 // are issued as soon as those registers are free, and are in flight while this
 // tile is worked on. The wavefronts' results are joined in LDS at the end.
 //
-// Bound by HBM once the ranges are long: 2.1 GB of e4m3 pages in 342 us, 6.1 TB/s, 538 MB
-// of bf16 under a window in 90 us, 6.0 TB/s (a large copy reaches 6.67). Whole rows of K through
+// Bound by HBM once the ranges are long: 2.1 GB of e4m3 pages in 341 us, 6.2 TB/s, 538 MB
+// of fp16 under a window in 90 us, 6.0 TB/s (a large copy reaches 6.67); what is
+// fetched is within 1.5% of the keys and values seen. Whole rows of K through
 // LDS rather than the operand's 16 bytes of 16 rows per load, and non-temporal
 // loads, took the first from 5.6 TB/s. The 8-bit tiles are half as large, so
-// two of them are in flight. Short ranges are latency: 10 us at 640 keys, of
+// two of them are in flight. Short ranges are latency: 11 us at 640 keys, of
 // which 4 are the join's.
 template <typename T, bool MX, int DP>
 struct RowsShape {
@@ -704,9 +706,9 @@ __global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 && !MX ? 3 : DP
 // and go to the other half of LDS after the products of the tile before.
 //
 // 2048 tokens at the end of 32768 keys, 32 heads of 128 in groups of 4 (1.07 TFLOP
-// in bf16): 1216 us, 876 TFLOP/s (1196 to 1268 us over the cards tried), where a
-// large library product reaches 1255. Counters: matrix cores busy 34% of the cycles, VALU 23%, LDS
-// 35%, 98% of the loads from L2. So neither is the bound, but the chain of
+// in bf16): 1270 us, 839 TFLOP/s (1230 us in one run of five), where a
+// large library product reaches 1255. Counters: matrix cores busy 36% of the cycles, LDS
+// 27% without a bank conflict, 97% of the loads from L2. So neither is the bound, but the chain of
 // product, maximum, exponentials, product within a wavefront (2.1 us per tile of 64
 // keys alone on a CU), and what fills it is other wavefronts: two workgroups
 // on a CU, eight wavefronts, at 256 registers each. 64 rows per workgroup: 2142 us.
@@ -1084,7 +1086,10 @@ constexpr int kWaves = 4;
 constexpr int kChunkRows = 32 * kWaves;
 
 // How a call is cut up: known from what the host knows of it, so that the
-// workspace can be sized before the call.
+// workspace can be sized before the call. The lengths are on the device, so these rules go
+// by the table's width, and sequences much shorter than it pay for that: a prompt of 128
+// 7.4 us in a table of 128 positions, 13.0 in one of 8192; one token at 128 keys, 32 heads,
+// 6.3 and 8.0. Times here are of calls replayed from a graph.
 struct Plan {
   bool chunk;         // attn_chunk's row tiles, else attn_rows'
   bool once;          // attn_rows reads (nearly) every key in one workgroup only
@@ -1123,10 +1128,11 @@ Plan plan(const PagedAttentionArgs& a) {
   // 16 x 32768 keys in bf16 347 / 331 / 331 us.
   p.items = ceil_div(a.tuned_items > 0 ? a.tuned_items : p.chunk ? 512 : 1024, a.c.kv_heads);
   // Cutting costs the second kernel, some 4 us. attn_chunk, cut from 256 / from 1024 keys: a prompt
-  // of 512 24.8 / 22.0 us, but a ragged packed step, whose longest sequence is the time, 40.7 / 57.9.
+  // of 512 24.6 / 22.0 us, but a ragged packed step, whose longest sequence is the time, 40.7 / 57.9.
+  // A packed step may also be that one prompt, and then takes 28.3.
   p.min_keys = a.tuned_min_keys > 0 ? a.tuned_min_keys : p.chunk && !a.c.cu ? 1024 : 256;
   // Few items: one token at 640 keys, 32 heads, in parts of 256 / 64 14.1 / 10.1 us; attn_chunk, 32
-  // rows at 2048 keys, 32 heads, in parts of 1024 / 256 60 / 20.6.
+  // rows at 2048 keys, 32 heads, in parts of 1024 / 256 60 / 20.4 (such a launch goes to attn_rows: 17.5).
   p.few_keys = std::min(p.min_keys, p.chunk ? 256 : 64);
   // No more than without a window: the workspace is asked for without knowing it.
   const int64_t keys = a.window > 0 ? std::min(capacity, std::min(a.window, capacity) + std::min(a.sinks, capacity)) : capacity;

@@ -8,9 +8,9 @@
 // Both move every byte once. A workgroup stays inside one token, so that the
 // token's sequence, position and page are found once per wavefront and not per
 // lane. Bound by HBM on long prompts: 4 x 2048 tokens into e4m3 pages, 186 MB, in
-// 37.5 us, 4.9 TB/s (a copy of that size reaches 6.5); 69 MB of such pages and
-// what comes of them in 13.7, 5.0 TB/s. One step's 1.6 MB is launch latency: 2.8 us
-// replayed from a graph.
+// 37.6 us, 4.9 TB/s (a copy of that size reaches 6.5); 69 MB of such pages and
+// what comes of them in 14.9, 4.6 TB/s, calls one after the other. One step's 1.6 MB is
+// launch latency: 2.8 us replayed from a graph.
 
 #include <algorithm>
 
@@ -79,8 +79,8 @@ __device__ __forceinline__ void put(const PagedDev& c, bool is_v, int page, int 
 // 64 bytes of the tables for each packet of 16. kPair lanes (neox) hold packet j
 // of both halves of a head, which share those 64 bytes and are each other's
 // partners; it takes halves of whole blocks for e4m3 pages (head sizes of
-// 64, 128, ...): 8192 tokens of 32 + 8 heads of 128 in bfloat16 to e4m3 pages, 185
-// MB, 45 us with kOwn lanes and 36 us (5.1 TB/s) so. kOwn lanes hold one packet and read its partner too: the other
+// 64, 128, ...): 8192 tokens of 32 + 8 heads of 128 in bfloat16 to e4m3 pages took
+// 1.25 times as long with kOwn lanes. kOwn lanes hold one packet and read its partner too: the other
 // sizes, and interleaved pairs, whose packets are complete in themselves.
 enum WriteLayout { kOwnNeox, kPairNeox, kInterleaved };
 
@@ -180,9 +180,9 @@ struct ReadDev {
 
 // A lane moves eight elements: its store is 16 bytes of a half type, and a
 // wavefront's stores are one run. Sixteen elements of e4m3 a lane, in one load
-// and two stores 32 bytes apart, took 18.8 us where this takes 14.4 (16 sequences of
-// up to 4096 positions, 8 heads of 128, e4m3 to bfloat16, 69 MB: 4.8 TB/s; 16.1 without the
-// non-temporal hint).
+// and two stores 32 bytes apart, took 1.3 times as long, and stores without the
+// non-temporal hint 1.1 times (16 sequences of up to 4096 positions, 8 heads of 128, e4m3
+// to bfloat16, 69 MB).
 template <typename T, bool MX>
 __global__ __launch_bounds__(256) void paged_read(ReadDev a) {
   const int nth = fast_div(blockIdx.x, a.by_blocks), token = a.token0 + nth;

@@ -84,8 +84,8 @@ inline RegShape sum_order(int64_t nvec, bool one_packet) {
 // than one packet (plain rows of 10240-16384, 279-500 rows: 10-25% behind 8 of
 // four). Against the order's own shape, fp16, cold and graph-replayed:
 // residual 512 x 4096 5.8 -> 4.6 us, 2048 x 4096 15.2 -> 12.6, 4096 x 4096 29.5 ->
-// 25.2, 1024 x 8192 15.2 -> 12.8; plain 4096 x 3072 11.9 -> 10.2, 4096 x 4096
-// 14.6 -> 12.8, 1024 x 16384 15.0 -> 13.4.
+// 25.2, 1024 x 8192 15.2 -> 12.8; plain 4096 x 4096 14.6 -> 12.8, 1024 x 16384
+// 15.0 -> 13.4.
 //
 // Wavefronts that fit, from sweeps of every shape over 13 widths x 24 row
 // counts (bf16, cold, MI355X). A CU holds 32, 24 at eight packets per lane, but

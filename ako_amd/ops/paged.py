@@ -104,7 +104,9 @@ def paged_attention(
     ``j > p - window`` and the first ``sinks``. ``scale`` is ``head_dim ** -0.5``
     unless given. Rows that see nothing (padding) are zero, and what a row does
     not see has no influence on it, whatever is stored there. A row that sees keys, but
-    whose scores are all -infinity, is NaN, as their softmax is.
+    whose scores are all -infinity, is NaN, as their softmax is; an infinity or NaN among
+    the values that it sees makes its element of them that infinity or NaN (NaN also
+    where an infinity's weight vanishes).
     """
     if q.is_cuda and not hip_disabled():
         return paged_attention_hip(q, k_pages, v_pages, block_table, seq_lens, scale, window, sinks,

@@ -278,8 +278,11 @@ int ako_paged_read_fwd(const ako_paged_t* cache, void* k_out, void* v_out, int d
  * sees the positions j <= p with (window == 0, or j > p - window, or
  * j < sinks), except those whose page is not there:
  *   out = to_dtype( sum_j softmax_j(scale * q.k_j) v_j ),
- * zero where a row sees nothing (padding). Positions a row does not see have
- * no influence on it, whatever they hold. out is [tokens, q_heads, head_dim],
+ * zero where a row sees nothing (padding), NaN where all it sees scores
+ * -infinity. Positions a row does not see have no influence on it, whatever
+ * they and their scale codes hold. An infinity or NaN among the values that a
+ * row sees makes the row's element of it that infinity or NaN (an infinity
+ * whose weight vanishes may give NaN). out is [tokens, q_heads, head_dim],
  * dense; q's strides are sequence, token, head. e4m3 pages are read as values
  * of dtype. workspace holds ako_paged_attention_workspace bytes of device
  * memory, 16-byte aligned, that nothing else uses until the work on `stream`
@@ -314,8 +317,8 @@ int ako_set_tuning(int op, int key, int value);
  * then the kernel's own start-to-end time, the figure a kernel trace reports,
  * without the marker packets that an hipEventRecord on each side would queue
  * around it. The events are the caller's (hipEventCreate, timing enabled);
- * an entry point that makes several launches (inputs past 2^31 work-items)
- * times its first. Arming replaces a pair that no launch has taken. Do
+ * an entry point that makes several launches (inputs past 2^31 work-items,
+ * attention that joins split key ranges) times its first. Arming replaces a pair that no launch has taken. Do
  * not arm a pair while the thread captures a stream into a graph: the next
  * launch takes it whether or not it is captured.
  * start and stop both NULL disarms: the return value is then 1 when a pair

@@ -213,7 +213,7 @@ def rope_qk_paged_ref(q, k, v, cos, sin, k_pages, v_pages, block_table, seq_lens
     refuse("rope_qk_paged", cache_error(k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, cu_seqlens)
            or write_error(q, k, v, cos, sin, k_pages, block_table, style, cu_seqlens))
     num_pages, kv_heads, page_size, head_dim = k_pages.shape
-    q2, k2, v2 = (x.reshape(-1, x.shape[-2], head_dim) for x in (q, k, v))
+    q2, k2, v2 = (x.flatten(0, -3) for x in (q, k, v))
     s, pos = row_places(q2.shape[0], seq_lens, cu_seqlens)
     page, slot = row_slots(s, pos, block_table, page_size, num_pages)
     page = torch.where(pos < cos.shape[0], page, -1)
@@ -274,7 +274,7 @@ def paged_attention_ref(q, k_pages, v_pages, block_table, seq_lens, *, k_scales=
     refuse("paged_attention", attention_error(q, k_pages, scale, window, sinks))
     num_pages, kv_heads, page_size, head_dim = k_pages.shape
     heads = q.shape[-2]
-    q2 = q.reshape(-1, heads, head_dim)
+    q2 = q.flatten(0, -3)
     out = torch.zeros_like(q2, memory_format=torch.contiguous_format)
     s, pos = row_places(q2.shape[0], seq_lens, cu_seqlens)
     for i in range(block_table.shape[0]):

@@ -43,6 +43,9 @@ constexpr float kAllInf = -std::numeric_limits<float>::max();
 __device__ __forceinline__ float inverse_total(float m, float l) {
   return l != 0.0f ? 1.0f / l : m == -__builtin_inff() ? 0.0f : __builtin_nanf("");
 }
+// Whether a part of a row's keys has sums: those under scores of -infinity alone
+// are 0, but 0 * NaN where a value is not finite.
+__device__ __forceinline__ bool holds_sums(float m, float l) { return l != 0.0f || m != -__builtin_inff(); }
 
 struct AttnDev {
   PagedDev c;
@@ -681,7 +684,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 && !MX ? 3 : DP
       const float keep = __builtin_amdgcn_exp2f(lds_ml[w][row].x - base);
       L += lds_ml[w][row].y * keep;
       const f32x4 y = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds[w][1]) + row * DP + (((d / 4) ^ row) << 2));
-      if (lds_ml[w][row].y != 0.0f) x += y * keep;  // a wavefront without keys holds nothing
+      x += y * keep;  // zeros of a wavefront without keys; 0 * NaN where its scores were all -infinity
     }
     const int token = fast_div(t.row0 + row, a.by_group);
     const int64_t at = int64_t(t.token0 + token) * a.q_heads + kvh * a.group + (t.row0 + row - token * a.group);
@@ -689,7 +692,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 && !MX ? 3 : DP
     if (a.max_parts > 1 && t.part == 0 && d == 0) a.row_parts[at] = int2{slot_row, t.parts};
     if (t.parts > 1) {
       if (d == 0) a.part_ml[slot_row] = float2{M, L};
-      if (L != 0.0f) *reinterpret_cast<f32x4*>(a.part_o + int64_t(slot_row) * a.head_dim + d) = x;
+      if (holds_sums(M, L)) *reinterpret_cast<f32x4*>(a.part_o + int64_t(slot_row) * a.head_dim + d) = x;
     } else {
       const float inv = inverse_total(M, L);
       Pack<T, 4> y;
@@ -706,7 +709,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 && !MX ? 3 : DP
 // and go to the other half of LDS after the products of the tile before.
 //
 // 2048 tokens at the end of 32768 keys, 32 heads of 128 in groups of 4 (1.07 TFLOP
-// in bf16): 1270 us, 839 TFLOP/s (1230 us in one run of five), where a
+// in bf16): 1270 us, 839 TFLOP/s (1230 to 1270 us over the runs), where a
 // large library product reaches 1255. Counters: matrix cores busy 36% of the cycles, LDS
 // 27% without a bank conflict, 97% of the loads from L2. So neither is the bound, but the chain of
 // product, maximum, exponentials, product within a wavefront (2.1 us per tile of 64
@@ -999,7 +1002,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
   if (a.max_parts > 1 && t.part == 0 && h == 0) a.row_parts[at] = int2{slot_row, t.parts};
   if (t.parts > 1) {
     if (h == 0) a.part_ml[slot_row] = float2{m, l};
-    if (l != 0.0f) {
+    if (holds_sums(m, l)) {
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -1031,7 +1034,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? 2 : 1) void attn_chunk(At
 // latency: LANES lanes hold a part's row, the groups of lanes take every
 // (64 / LANES)-th part and eight of them at a time, and are added up at the end; an
 // order that depends on nothing but the number of parts. A part without keys
-// has l = 0 and is not read further.
+// has no sums and is not read further.
 constexpr int kMaxParts = kWave;
 
 template <typename T, int LANES>
@@ -1051,7 +1054,7 @@ __global__ __launch_bounds__(256) void attn_join(const float* __restrict__ part_
 #pragma unroll
   for (int k = 1; k < kWave; k *= 2) M = __builtin_fmaxf(M, __shfl_xor(M, k));
   const float w = __builtin_amdgcn_exp2f(ml.x - (M == -__builtin_inff() ? 0.0f : M));
-  const uint64_t some = __ballot(ml.y != 0.0f);
+  const uint64_t some = __ballot(holds_sums(ml.x, ml.y));
   const float L = wave_sum(ml.y != 0.0f ? ml.y * w : 0.0f);
   const int d = lane % LANES * 4;
   f32x4 x = {0, 0, 0, 0};
@@ -1071,7 +1074,7 @@ __global__ __launch_bounds__(256) void attn_join(const float* __restrict__ part_
   for (int k = LANES; k < kWave; k *= 2)
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] += __shfl_xor(x[e], k);
-  const float inv = some ? 1.0f / L : inverse_total(M, 0.0f);
+  const float inv = inverse_total(M, L);
   if (lane < LANES && d < head_dim) {
     Pack<T, 4> y;
 #pragma unroll

@@ -190,3 +190,33 @@ def test_q_and_other_slots_of_a_write_of_values_that_are_not_finite(dtype, style
             for p in range(n - 5, n):
                 kept[s.table[i, p // page], :, p % page] = False
         assert all(torch.equal(raw(t)[kept.expand(t.shape)], was[kept.expand(t.shape)]) for t, was in zip(pools, before))
+
+
+# ------------------------------------------------------------------ weights of zero --
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("keys", [0, 64])
+@pytest.mark.parametrize("news", [1, 40])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_nan_under_a_score_of_minus_infinity_is_not_lost(dtype, news: int, keys: int, device: str) -> None:
+    """0 times NaN is NaN in the formula, also where a wavefront or a part of the keys sees nothing but scores
+    of -infinity: the last key alone in its tile, and stretches of whole tiles."""
+    from ako_amd import _native
+
+    for held, first, last in ((33, 32, 33), (65, 64, 65), (97, 96, 97), (129, 128, 129), (300, 64, 128), (700, 0, 600),
+                              (700, 576, 700)):
+        if held < news:
+            continue
+        s = step([held], [news], heads=4, page=16, dtype=dtype, device=device, seed=held)
+        s.q[..., 0] = 1.0
+        for j in range(first, last):
+            s.k_pages[s.table[0, j // 16], :, j % 16, 0] = -math.inf
+        for j, e in ((first, 3), (last - 1, 50)):
+            s.v_pages[s.table[0, j // 16], :, j % 16, e] = math.nan
+        want, bound = attention64(s)
+        assert bool(want.isnan().any())
+        _native.set_tuning(3, 2, keys)
+        try:
+            for name, out in results(s):
+                assert_same(out, want, bound, f"{name}, {held} keys, {first} to {last}")
+        finally:
+            _native.set_tuning(3, 2, 0)

@@ -112,7 +112,7 @@ struct Item {
 // are long the items are 1 / per_item, a number of whole rounds of the chip
 // (one item more would cost another round). What lies behind the last packed
 // sequence counts as one more, padding. Sequences are looked at 64 at a time, one per lane,
-// by every workgroup: at 64 keys and 8 key heads 64 sequences take 7.4 us, 256 30, 1024 168.
+// by every workgroup: at 64 keys and 8 key heads 64 sequences take 7.1 us, 256 29, 1024 165.
 template <int R, int KT>
 __device__ __forceinline__ bool find_item(const AttnDev& a, int item, Item& t) {
   const PagedDev& p = a.c;
@@ -709,7 +709,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 && !MX ? 3 : DP
 // and go to the other half of LDS after the products of the tile before.
 //
 // 2048 tokens at the end of 32768 keys, 32 heads of 128 in groups of 4 (1.07 TFLOP
-// in bf16): 1270 us, 839 TFLOP/s (1230 to 1270 us over the runs), where a
+// in bf16): 1251 us, 851 TFLOP/s (1230 to 1272 us over ten runs), where a
 // large library product reaches 1255. Counters: matrix cores busy 36% of the cycles, LDS
 // 27% without a bank conflict, 97% of the loads from L2. So neither is the bound, but the chain of
 // product, maximum, exponentials, product within a wavefront (2.1 us per tile of 64
@@ -1091,8 +1091,8 @@ constexpr int kChunkRows = 32 * kWaves;
 // How a call is cut up: known from what the host knows of it, so that the
 // workspace can be sized before the call. The lengths are on the device, so these rules go
 // by the table's width, and sequences much shorter than it pay for that: a prompt of 128
-// 7.4 us in a table of 128 positions, 13.0 in one of 8192; one token at 128 keys, 32 heads,
-// 6.3 and 8.0. Times here are of calls replayed from a graph.
+// 6.9 us in a table of 128 positions, 13.1 in one of 8192; one token at 128 keys, 32 heads,
+// 6.0 and 7.7. Times here are of calls replayed from a graph.
 struct Plan {
   bool chunk;         // attn_chunk's row tiles, else attn_rows'
   bool once;          // attn_rows reads (nearly) every key in one workgroup only
@@ -1131,11 +1131,11 @@ Plan plan(const PagedAttentionArgs& a) {
   // 16 x 32768 keys in bf16 347 / 331 / 331 us.
   p.items = ceil_div(a.tuned_items > 0 ? a.tuned_items : p.chunk ? 512 : 1024, a.c.kv_heads);
   // Cutting costs the second kernel, some 4 us. attn_chunk, cut from 256 / from 1024 keys: a prompt
-  // of 512 24.6 / 22.0 us, but a ragged packed step, whose longest sequence is the time, 40.7 / 57.9.
+  // of 512 24.6 / 22.1 us, but a ragged packed step, whose longest sequence is the time, 40.7 / 57.9.
   // A packed step may also be that one prompt, and then takes 28.3.
   p.min_keys = a.tuned_min_keys > 0 ? a.tuned_min_keys : p.chunk && !a.c.cu ? 1024 : 256;
-  // Few items: one token at 640 keys, 32 heads, in parts of 256 / 64 14.1 / 10.1 us; attn_chunk, 32
-  // rows at 2048 keys, 32 heads, in parts of 1024 / 256 60 / 20.4 (such a launch goes to attn_rows: 17.5).
+  // Few items: one token at 640 keys, 32 heads, in parts of 256 / 64 14.1 / 9.7 us; attn_chunk, 32
+  // rows at 2048 keys, 32 heads, in parts of 1024 / 256 60 / 20.4 (such a launch goes to attn_rows: 17.2).
   p.few_keys = std::min(p.min_keys, p.chunk ? 256 : 64);
   // No more than without a window: the workspace is asked for without knowing it.
   const int64_t keys = a.window > 0 ? std::min(capacity, std::min(a.window, capacity) + std::min(a.sinks, capacity)) : capacity;

@@ -8,8 +8,8 @@
 // Both move every byte once. A workgroup stays inside one token, so that the
 // token's sequence, position and page are found once per wavefront and not per
 // lane. Bound by HBM on long prompts: 4 x 2048 tokens into e4m3 pages, 186 MB, in
-// 37.6 us, 4.9 TB/s (a copy of that size reaches 6.5); 69 MB of such pages and
-// what comes of them in 14.9, 4.6 TB/s, calls one after the other. One step's 1.6 MB is
+// 37.5 us, 5.0 TB/s (a copy of that size reaches 6.5); 69 MB of such pages and
+// what comes of them in 15.0, 4.6 TB/s, calls one after the other. One step's 1.6 MB is
 // launch latency: 2.8 us replayed from a graph.
 
 #include <algorithm>

@@ -90,6 +90,16 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         _int,
         [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _ptr, _ptr, _ptr, _i64, _i64, _int, _int, _int, _ptr],
     ),
+    "ako_rmsnorm_rope_qk_fwd": (
+        _int,
+        [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _ptr, _ptr, _i64, _f32,
+         _int, _int, _int, _int, _ptr],
+    ),
+    "ako_rmsnorm_rope_qk_paged_fwd": (
+        _int,
+        [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _ptr, _ptr, _ptr, _i64, _i64, _f32,
+         _int, _int, _int, _int, _ptr],
+    ),
     "ako_paged_read_fwd": (_int, [_ptr, _ptr, _ptr, _int, _ptr]),
     "ako_paged_attention_fwd": (
         _int, [_ptr, _ptr, _ptr, _ptr, _i64, _f32, _i64, _i64, _ptr, _i64, _int, _ptr],

@@ -713,11 +713,29 @@ bool rows_apart(const Span& sa, const Span& sb, int64_t n0, int64_t n1, int64_t 
 }  // namespace
 }  // extern "C++"
 
-int ako_rope_qk_paged_fwd(const void* q, const void* k, const void* v, const void* cos_table, const void* sin_table,
-                          void* q_out, const ako_paged_t* cache, int64_t q_heads, const int64_t* q_strides,
-                          const int64_t* k_strides, const int64_t* v_strides, int64_t table_rows,
-                          int64_t table_row_stride, int dtype, int table_dtype, int style, void* stream) {
-  const char* fn = "ako_rope_qk_paged_fwd";
+extern "C++" {
+namespace {
+
+// RMSNorm weights of a call's heads; no weights: no norm.
+struct HeadNorm {
+  const void* qw = nullptr;
+  const void* kw = nullptr;
+  float eps = 0.0f;
+  int w_dtype = 0;
+};
+
+int norm_args(const char* fn, const HeadNorm& w, int dtype) {
+  if (w.w_dtype != dtype && w.w_dtype != AKO_DTYPE_F32)
+    return fail(AKO_ERR_UNSUPPORTED, "%s: weight dtype %s with input dtype %s (weight must match or be f32)", fn,
+                dtype_name(w.w_dtype), dtype_name(dtype));
+  if (!(w.eps >= 0.0f)) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: eps must be >= 0", fn);
+  return AKO_OK;
+}
+
+int paged_write(const char* fn, const HeadNorm* norm, const void* q, const void* k, const void* v, const void* cos_table,
+                const void* sin_table, void* q_out, const ako_paged_t* cache, int64_t q_heads, const int64_t* q_strides,
+                const int64_t* k_strides, const int64_t* v_strides, int64_t table_rows, int64_t table_row_stride, int dtype,
+                int table_dtype, int style, void* stream) {
   ako::PagedWriteArgs a{};
   bool empty = false;
   if (const int rc = paged_common(fn, cache, q_heads, dtype, &a.c, &empty)) return rc;
@@ -725,6 +743,8 @@ int ako_rope_qk_paged_fwd(const void* q, const void* k, const void* v, const voi
   if (style != AKO_ROPE_NEOX && style != AKO_ROPE_INTERLEAVED)
     return fail(AKO_ERR_UNSUPPORTED, "%s: unknown RoPE style %d", fn, style);
   if (table_rows < 0) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: negative size", fn);
+  if (norm)
+    if (const int rc = norm_args(fn, *norm, dtype)) return rc;
   if (empty) return AKO_OK;
   const int64_t d = cache->head_dim, kvh = cache->kv_heads, n = cache->num_pages, ps = cache->page_size;
   const int64_t per = cache->cu_seqlens ? cache->tokens : cache->tokens / cache->n_seqs;
@@ -739,8 +759,18 @@ int ako_rope_qk_paged_fwd(const void* q, const void* k, const void* v, const voi
       return fail(AKO_ERR_INVALID_ARGUMENT, "%s: negative stride", fn);
   const int eb = ako::dtype_bytes(dtype), tb = ako::dtype_bytes(table_dtype);
   const PagedSpans held(cache, dtype);
-  Span in[5];
+  Span in[7];
   int n_in = 0;
+  if (norm) {
+    if (!norm->qw || !norm->kw) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: null weight", fn);
+    const int wb = ako::dtype_bytes(norm->w_dtype);
+    in[n_in++] = span_2d(norm->qw, 1, d, d, wb);
+    in[n_in++] = span_2d(norm->kw, 1, d, d, wb);
+    a.qw = norm->qw;
+    a.kw = norm->kw;
+    a.eps = norm->eps;
+    a.w_dtype = norm->w_dtype;
+  }
   if (q_heads > 0) in[n_in++] = span_4d(q, seqs, per, q_heads, d, q_strides, eb);
   in[n_in++] = span_4d(k, seqs, per, kvh, d, k_strides, eb);
   in[n_in++] = span_4d(v, seqs, per, kvh, d, v_strides, eb);
@@ -794,6 +824,105 @@ int ako_rope_qk_paged_fwd(const void* q, const void* k, const void* v, const voi
   a.table_dtype = table_dtype;
   a.neox = style == AKO_ROPE_NEOX;
   return hip_status(ako::launch_paged_write(a, static_cast<hipStream_t>(stream)), fn);
+}
+
+}  // namespace
+}  // extern "C++"
+
+int ako_rope_qk_paged_fwd(const void* q, const void* k, const void* v, const void* cos_table, const void* sin_table,
+                          void* q_out, const ako_paged_t* cache, int64_t q_heads, const int64_t* q_strides,
+                          const int64_t* k_strides, const int64_t* v_strides, int64_t table_rows,
+                          int64_t table_row_stride, int dtype, int table_dtype, int style, void* stream) {
+  return paged_write("ako_rope_qk_paged_fwd", nullptr, q, k, v, cos_table, sin_table, q_out, cache, q_heads, q_strides,
+                     k_strides, v_strides, table_rows, table_row_stride, dtype, table_dtype, style, stream);
+}
+
+int ako_rmsnorm_rope_qk_paged_fwd(const void* q, const void* k, const void* v, const void* q_weight, const void* k_weight,
+                                  const void* cos_table, const void* sin_table, void* q_out, const ako_paged_t* cache,
+                                  int64_t q_heads, const int64_t* q_strides, const int64_t* k_strides,
+                                  const int64_t* v_strides, int64_t table_rows, int64_t table_row_stride, float eps,
+                                  int dtype, int w_dtype, int table_dtype, int style, void* stream) {
+  const HeadNorm norm{q_weight, k_weight, eps, w_dtype};
+  return paged_write("ako_rmsnorm_rope_qk_paged_fwd", &norm, q, k, v, cos_table, sin_table, q_out, cache, q_heads, q_strides,
+                     k_strides, v_strides, table_rows, table_row_stride, dtype, table_dtype, style, stream);
+}
+
+int ako_rmsnorm_rope_qk_fwd(const void* q, const void* k, const void* q_weight, const void* k_weight,
+                            const void* cos_table, const void* sin_table, void* q_out, void* k_out, int64_t batch,
+                            int64_t seq, int64_t q_heads, int64_t k_heads, int64_t head_dim, const int64_t* q_strides,
+                            const int64_t* k_strides, int64_t table_row_stride, float eps, int dtype, int w_dtype,
+                            int table_dtype, int style, void* stream) {
+  const char* fn = "ako_rmsnorm_rope_qk_fwd";
+  if (!valid_dtype(dtype) || !valid_dtype(table_dtype))
+    return fail(AKO_ERR_UNSUPPORTED, "%s: unknown dtype code (x %d, table %d)", fn, dtype, table_dtype);
+  if (style != AKO_ROPE_NEOX && style != AKO_ROPE_INTERLEAVED)
+    return fail(AKO_ERR_UNSUPPORTED, "%s: unknown RoPE style %d", fn, style);
+  const HeadNorm norm{q_weight, k_weight, eps, w_dtype};
+  if (const int rc = norm_args(fn, norm, dtype)) return rc;
+  if (batch < 0 || seq < 0 || q_heads < 0 || k_heads < 0) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: negative size", fn);
+  if (head_dim < 2 || head_dim > 512 || head_dim % 2)
+    return fail(AKO_ERR_UNSUPPORTED, "%s: head_dim must be even and 2 to 512, got %lld", fn, (long long)head_dim);
+  if (batch == 0 || seq == 0 || (q_heads == 0 && k_heads == 0)) return AKO_OK;
+  constexpr int64_t kMaxHeads = int64_t(1) << 23;  // of q or of k: a token's lanes stay below 2^30
+  if (batch > kMaxInt / seq || q_heads > kMaxHeads || k_heads > kMaxHeads)
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: batch*seq must stay below 2^31, the heads at most 2^23", fn);
+  if ((q_heads > 0 && (!q || !q_out || !q_weight || !q_strides)) || (k_heads > 0 && (!k || !k_out || !k_weight || !k_strides)) ||
+      !cos_table || !sin_table)
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: null pointer argument", fn);
+  if (table_row_stride < 0 || (seq > 1 && table_row_stride < head_dim / 2))
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: table row stride %lld < head_dim/2", fn, (long long)table_row_stride);
+  for (int i = 0; i < 3; ++i)
+    if ((q_heads > 0 && q_strides[i] < 0) || (k_heads > 0 && k_strides[i] < 0))
+      return fail(AKO_ERR_INVALID_ARGUMENT, "%s: negative stride", fn);
+  const int eb = ako::dtype_bytes(dtype), tb = ako::dtype_bytes(table_dtype), wb = ako::dtype_bytes(w_dtype);
+  const __int128 row = static_cast<__int128>(batch) * seq * head_dim * eb;
+  Span in[6], out[2];
+  int n_in = 0, n_out = 0;
+  in[n_in++] = span_2d(cos_table, seq, head_dim / 2, table_row_stride, tb);
+  in[n_in++] = span_2d(sin_table, seq, head_dim / 2, table_row_stride, tb);
+  if (q_heads > 0) {
+    in[n_in++] = span_4d(q, batch, seq, q_heads, head_dim, q_strides, eb);
+    in[n_in++] = span_2d(q_weight, 1, head_dim, head_dim, wb);
+    out[n_out++] = span_bytes(q_out, row * q_heads);
+  }
+  if (k_heads > 0) {
+    in[n_in++] = span_4d(k, batch, seq, k_heads, head_dim, k_strides, eb);
+    in[n_in++] = span_2d(k_weight, 1, head_dim, head_dim, wb);
+    out[n_out++] = span_bytes(k_out, row * k_heads);
+  }
+  bool ok = true, apart = n_out < 2 || !overlap(out[0], out[1]);
+  for (int i = 0; i < n_in; ++i) ok = ok && in[i].ok;
+  for (int o = 0; o < n_out; ++o) {
+    ok = ok && out[o].ok;
+    for (int i = 0; i < n_in; ++i) apart = apart && !overlap(out[o], in[i]);
+  }
+  if (!ok) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: sizes and strides overflow the address space", fn);
+  if (!apart) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: an output overlaps another buffer", fn);
+  ako::NormRopeArgs a{};
+  a.q = q;
+  a.k = k;
+  a.qw = q_weight;
+  a.kw = k_weight;
+  a.cos = cos_table;
+  a.sin = sin_table;
+  a.q_out = q_out;
+  a.k_out = k_out;
+  for (int i = 0; i < 3; ++i) {
+    a.qs[i] = q_heads > 0 ? q_strides[i] : 0;
+    a.ks[i] = k_heads > 0 ? k_strides[i] : 0;
+  }
+  a.batch = batch;
+  a.seq = seq;
+  a.q_heads = q_heads;
+  a.k_heads = k_heads;
+  a.head_dim = head_dim;
+  a.st = table_row_stride;
+  a.eps = eps;
+  a.dtype = dtype;
+  a.w_dtype = w_dtype;
+  a.table_dtype = table_dtype;
+  a.neox = style == AKO_ROPE_NEOX;
+  return hip_status(ako::launch_norm_rope(a, static_cast<hipStream_t>(stream)), fn);
 }
 
 int ako_paged_read_fwd(const ako_paged_t* cache, void* k_out, void* v_out, int dtype, void* stream) {

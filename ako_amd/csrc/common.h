@@ -150,6 +150,17 @@ __device__ __forceinline__ float lane_group_sum(float v) {
 
 __device__ __forceinline__ float wave_sum(float v) { return lane_group_sum<kWave>(v); }
 
+// The same over each aligned group of 2^log2 lanes, log2 the same in all lanes.
+__device__ __forceinline__ float lane_group_sum(float v, int log2) {
+  if (log2 > 0) v += dpp_mov<0xB1>(v);
+  if (log2 > 1) v += dpp_mov<0x4E>(v);
+  if (log2 > 2) v += dpp_mov<0x141>(v);
+  if (log2 > 3) v += dpp_mov<0x140>(v);
+  if (log2 > 4) v += __shfl_xor(v, 16);
+  if (log2 > 5) v += __shfl_xor(v, 32);
+  return v;
+}
+
 // ---- workgroup order over the XCDs ------------------------------------------
 // Workgroups are dispatched round-robin over the 8 XCDs (workgroup b runs on
 // XCD b % 8). block_order hands each XCD runs of `chunk` consecutive blocks:

@@ -153,6 +153,25 @@ struct RopeArgs {
 };
 hipError_t launch_rope(const RopeArgs& a, hipStream_t stream);
 
+// RMSNorm of every head of q and k, and RoPE; outputs dense.
+struct NormRopeArgs {
+  const void* q;
+  const void* k;
+  const void* qw;
+  const void* kw;
+  const void* cos;
+  const void* sin;
+  void* q_out;
+  void* k_out;
+  int64_t qs[3], ks[3];  // batch, token, head
+  int64_t batch, seq, q_heads, k_heads, head_dim;
+  int64_t st;  // table row stride, elements
+  float eps;
+  int dtype, w_dtype, table_dtype;
+  bool neox;
+};
+hipError_t launch_norm_rope(const NormRopeArgs& a, hipStream_t stream);
+
 struct SwigluArgs {
   const void* g;
   const void* u;
@@ -192,6 +211,10 @@ struct PagedWriteArgs {
   int64_t st, table_rows, q_heads;
   int dtype, table_dtype;
   bool neox;
+  const void* qw;  // weights of the heads' norms, or null: no norm
+  const void* kw;
+  float eps;
+  int w_dtype;
 };
 hipError_t launch_paged_write(const PagedWriteArgs& a, hipStream_t stream);
 

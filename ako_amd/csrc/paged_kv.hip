@@ -3,6 +3,8 @@
 // paged_write: RoPE of a step's q and k at the positions that the device-side
 // lengths give, q to its output, k and v into their sequences' pages, in the
 // model's type or as e4m3 with a power-of-two scale per 32 elements (paged.h).
+// With weights, every head of q and k goes through its RMSNorm first, in 32 bits and
+// without a rounding between the two (qk_norm.hip has the formulas).
 // paged_read: the same rows of both caches as dense tensors.
 //
 // Both move every byte once. A workgroup stays inside one token, so that the
@@ -43,6 +45,10 @@ struct WriteDev {
   int lanes;                      // lanes of a token: heads of q, k and v times per_head
   FastDiv by_blocks, by_head;     // workgroups per token, lanes per head
   int blocks, per_head, token0;
+  const void* qw;                 // NORM: weights of T's type, or (w_f32) of float
+  const void* kw;
+  int w_f32, head_log2;           // 2^head_log2 lanes per head
+  float eps, inv_dim;
 };
 
 // Eight values of a row of the key or value pages; for e4m3 also their block's
@@ -81,10 +87,11 @@ __device__ __forceinline__ void put(const PagedDev& c, bool is_v, int page, int 
 // partners; it takes halves of whole blocks for e4m3 pages (head sizes of
 // 64, 128, ...): 8192 tokens of 32 + 8 heads of 128 in bfloat16 to e4m3 pages took
 // 1.25 times as long with kOwn lanes. kOwn lanes hold one packet and read its partner too: the other
-// sizes, and interleaved pairs, whose packets are complete in themselves.
+// sizes, and interleaved pairs, whose packets are complete in themselves. NORM: a head's
+// lanes are rounded up to a power of two, and its sum of squares is taken over that group.
 enum WriteLayout { kOwnNeox, kPairNeox, kInterleaved };
 
-template <typename T, typename TT, bool MX, WriteLayout LAYOUT>
+template <typename T, typename TT, bool MX, WriteLayout LAYOUT, bool NORM>
 __global__ __launch_bounds__(256) void paged_write(WriteDev a) {
   constexpr bool PAIR = LAYOUT == kPairNeox;
   const int nth = fast_div(blockIdx.x, a.by_blocks), token = a.token0 + nth;
@@ -110,6 +117,35 @@ __global__ __launch_bounds__(256) void paged_write(WriteDev a) {
     if (LAYOUT == kOwnNeox && !is_v) other = load_eight<T>(x + (upper ? e0 - half : e0 + half));
   }
 
+  // NORM: the factors of the lane's own elements and of their partners.
+  [[maybe_unused]] float f[8], f2[8];
+  if constexpr (NORM) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float o = to_f32(own[i]), p = to_f32(other[i]);
+      ss = __builtin_fmaf(o, o, ss);
+      if (PAIR) ss = __builtin_fmaf(p, p, ss);
+    }
+    const auto weights = [&](int e, float (&w)[8]) {
+      const void* const base = is_q ? a.qw : a.kw;
+      if (a.w_f32) load_f32<float, 8>(static_cast<const float*>(base) + e, w);
+      else load_f32<T, 8>(static_cast<const T*>(base) + e, w);
+    };
+    if (live && !is_v) {
+      weights(e0, f);
+      if (LAYOUT != kInterleaved) weights(PAIR ? e0 + half : upper ? e0 - half : e0 + half, f2);
+    }
+    ss = rsqrtf(lane_group_sum(ss, a.head_log2) * a.inv_dim + a.eps);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      f[i] = to_f32(own[i]) * ss * f[i];
+      f2[i] = to_f32(other[i]) * ss * f2[i];
+    }
+  }
+  const auto value = [&](int i) { return NORM ? f[i] : to_f32(own[i]); };
+  const auto partner = [&](int i) { return NORM ? f2[i] : to_f32(other[i]); };
+
   const TokenPlace at = token_place(a.c, token);
   int slot = 0, page = -1;
   const bool known = at.seq >= 0 && at.pos >= 0 && at.pos < a.c.capacity && at.pos < a.table_rows;
@@ -124,7 +160,7 @@ __global__ __launch_bounds__(256) void paged_write(WriteDev a) {
       load_f32<TT, 8>(static_cast<const TT*>(a.sin) + row, n);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float o = to_f32(own[i]), p = to_f32(other[i]);
+        const float o = value(i), p = partner(i);
         r[i] = upper ? p * n[i] + o * c[i] : o * c[i] - p * n[i];
         r2[i] = o * n[i] + p * c[i];
       }
@@ -135,7 +171,7 @@ __global__ __launch_bounds__(256) void paged_write(WriteDev a) {
       load_f32<TT, 4>(static_cast<const TT*>(a.sin) + row, n);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float o = to_f32(own[2 * i]), p = to_f32(own[2 * i + 1]);
+        const float o = value(2 * i), p = value(2 * i + 1);
         r[2 * i] = o * c[i] - p * n[i];
         r[2 * i + 1] = o * n[i] + p * c[i];
       }
@@ -230,7 +266,7 @@ hipError_t by_tokens(int64_t tokens, int64_t blocks, Launch launch) {
   return hipSuccess;
 }
 
-template <typename T, typename TT, bool MX>
+template <typename T, typename TT, bool MX, bool NORM>
 hipError_t run_write(const PagedWriteArgs& a, hipStream_t stream) {
   WriteDev d{};
   d.c = paged_dev(a.c);
@@ -253,6 +289,15 @@ hipError_t run_write(const PagedWriteArgs& a, hipStream_t stream) {
   const bool pair = a.neox && (!MX || d.head_dim % 64 == 0);
   d.per_head = d.head_dim / (pair ? 16 : 8);
   if (MX) d.per_head = static_cast<int>(ceil_div(d.per_head, 4) * 4);
+  if (NORM) {
+    while ((1 << d.head_log2) < d.per_head) ++d.head_log2;
+    d.per_head = 1 << d.head_log2;
+    d.qw = a.qw;
+    d.kw = a.kw;
+    d.w_f32 = a.w_dtype == kF32;
+    d.eps = a.eps;
+    d.inv_dim = 1.0f / static_cast<float>(d.head_dim);
+  }
   d.lanes = (d.q_heads + 2 * d.kv_heads) * d.per_head;
   const int block = block_size(d.lanes);
   d.blocks = static_cast<int>(ceil_div(d.lanes, block));
@@ -260,18 +305,19 @@ hipError_t run_write(const PagedWriteArgs& a, hipStream_t stream) {
   d.by_head = make_fastdiv(d.per_head);
   return by_tokens(a.c.tokens, d.blocks, [&](int token0, dim3 grid) {
     d.token0 = token0;
-    if (pair) AKO_LAUNCH((paged_write<T, TT, MX, kPairNeox>), grid, dim3(block), 0, stream, d);
-    else if (!a.neox) AKO_LAUNCH((paged_write<T, TT, MX, kInterleaved>), grid, dim3(block), 0, stream, d);
-    else if constexpr (MX) AKO_LAUNCH((paged_write<T, TT, MX, kOwnNeox>), grid, dim3(block), 0, stream, d);
+    if (pair) AKO_LAUNCH((paged_write<T, TT, MX, kPairNeox, NORM>), grid, dim3(block), 0, stream, d);
+    else if (!a.neox) AKO_LAUNCH((paged_write<T, TT, MX, kInterleaved, NORM>), grid, dim3(block), 0, stream, d);
+    else if constexpr (MX) AKO_LAUNCH((paged_write<T, TT, MX, kOwnNeox, NORM>), grid, dim3(block), 0, stream, d);
   });
 }
 
 template <typename T, bool MX>
 hipError_t write_tables(const PagedWriteArgs& a, hipStream_t stream) {
+  const bool norm = a.qw != nullptr;
   switch (a.table_dtype) {
-    case kF32: return run_write<T, float, MX>(a, stream);
-    case kF16: return run_write<T, _Float16, MX>(a, stream);
-    case kBF16: return run_write<T, __bf16, MX>(a, stream);
+    case kF32: return norm ? run_write<T, float, MX, true>(a, stream) : run_write<T, float, MX, false>(a, stream);
+    case kF16: return norm ? run_write<T, _Float16, MX, true>(a, stream) : run_write<T, _Float16, MX, false>(a, stream);
+    case kBF16: return norm ? run_write<T, __bf16, MX, true>(a, stream) : run_write<T, __bf16, MX, false>(a, stream);
     default: return hipErrorInvalidValue;
   }
 }

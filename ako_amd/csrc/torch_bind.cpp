@@ -276,6 +276,65 @@ std::pair<at::Tensor, at::Tensor> rope_qk(const at::Tensor& q, const at::Tensor&
   return {q_out, k_out};
 }
 
+// ---------------------------------------------------- RMSNorm of heads, with RoPE --
+// The checks and messages of ako_amd/ops/qk_norm.py (weights_error, _check), in the same order.
+// A number as Python prints it.
+std::string number(double v) { return std::string(py::str(py::float_(v))); }
+
+struct HeadWeights {
+  at::Tensor q, k;
+  int dtype;
+};
+
+HeadWeights head_weights(const std::string& pre, const at::Tensor& qw, const at::Tensor& kw, double eps, int64_t head_dim,
+                         const at::Tensor& x) {
+  const at::Tensor* ws[2] = {&qw, &kw};
+  for (int i = 0; i < 2; ++i) {
+    const char* name = i ? "k_weight" : "q_weight";
+    if (ws[i]->dim() != 1 || ws[i]->size(0) != head_dim)
+      value_error(pre + "Expected " + name + " of shape (" + std::to_string(head_dim) + ",), got " + shape_str(ws[i]->sizes()));
+    if (ws[i]->device() != x.device()) value_error(pre + name + " must be on the device of q");
+  }
+  if (!(eps >= 0)) value_error(pre + "eps must be at least 0, got " + number(eps));
+  const bool same = qw.scalar_type() == x.scalar_type() && kw.scalar_type() == x.scalar_type();
+  HeadWeights w{same ? qw : qw.to(at::kFloat), same ? kw : kw.to(at::kFloat), 0};
+  w.q = w.q.contiguous();
+  w.k = w.k.contiguous();
+  w.dtype = dtype_code_or(w.q.scalar_type());
+  return w;
+}
+
+std::pair<at::Tensor, at::Tensor> rmsnorm_rope_qk(const at::Tensor& q, const at::Tensor& k, const at::Tensor& q_weight,
+                                                  const at::Tensor& k_weight, const at::Tensor& cos, const at::Tensor& sin,
+                                                  double eps, const std::string& style) {
+  const char* fn = "rmsnorm_rope_qk_hip";
+  const std::string pre = std::string(fn) + ": ";
+  const int index = gpu_index(q, fn);
+  const int sc = style_code(style);
+  validate_rope(q, cos, sin);
+  validate_rope(k, cos, sin);
+  if (q.size(0) != k.size(0) || q.size(1) != k.size(1) || q.size(3) != k.size(3) || q.scalar_type() != k.scalar_type() ||
+      !on(k, index))
+    value_error(pre + "q " + shape_str(q.sizes()) + " " + dtype_str(q.scalar_type()) + " and k " + shape_str(k.sizes()) + " " +
+                dtype_str(k.scalar_type()) + " must match but for their heads");
+  const int dt = dtype_code_or(q.scalar_type());
+  if (dt < 0) value_error(pre + "q must be float32/float16/bfloat16, got " + dtype_str(q.scalar_type()));
+  const int64_t head_dim = q.size(3);
+  if (head_dim < 2 || head_dim > 512) value_error(pre + "head_dim must be 2 to 512, got " + std::to_string(head_dim));
+  const HeadWeights w = head_weights(pre, q_weight, k_weight, eps, head_dim, q);
+  if (!on(cos, index) || !on(sin, index)) value_error(pre + "tables must be on the device of q");
+  const at::Tensor qv = head_view(q), kv = head_view(k);
+  const Tables t = tables(cos, sin, index);
+  at::Tensor qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), k.options());
+  check(on_device(index, [&](hipStream_t s) {
+          return ako_rmsnorm_rope_qk_fwd(qv.data_ptr(), kv.data_ptr(), w.q.data_ptr(), w.k.data_ptr(), t.cos.data_ptr(),
+                                         t.sin.data_ptr(), qo.data_ptr(), ko.data_ptr(), q.size(0), q.size(1), q.size(2),
+                                         k.size(2), head_dim, qv.strides().data(), kv.strides().data(), t.stride,
+                                         static_cast<float>(eps), dt, w.dtype, t.dtype, sc, s);
+        }), fn);
+  return {qo, ko};
+}
+
 at::Tensor rope_qk_cache(const at::Tensor& q, const at::Tensor& k, const c10::optional<at::Tensor>& v,
                          const at::Tensor& cos, const at::Tensor& sin, const at::Tensor& pos,
                          const at::Tensor& k_cache, const c10::optional<at::Tensor>& v_cache,
@@ -471,7 +530,8 @@ struct RowStrides {
 at::Tensor rope_qk_paged(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cos,
                          const at::Tensor& sin, const at::Tensor& k_pages, const at::Tensor& v_pages,
                          const at::Tensor& block_table, const at::Tensor& seq_lens, const std::string& style,
-                         const OptTensor& k_scales, const OptTensor& v_scales, const OptTensor& cu_seqlens) {
+                         const OptTensor& k_scales, const OptTensor& v_scales, const OptTensor& cu_seqlens,
+                         const OptTensor& q_weight, const OptTensor& k_weight, double eps) {
   const char* fn = "rope_qk_paged_hip";
   const int index = gpu_index(q, fn);
   const PagedArg p{k_pages, v_pages, block_table, seq_lens, get(k_scales), get(v_scales), get(cu_seqlens),
@@ -494,12 +554,22 @@ at::Tensor rope_qk_paged(const at::Tensor& q, const at::Tensor& k, const at::Ten
     p.refuse("tables must be (positions, " + std::to_string(k_pages.size(3) / 2) + "), got " + shape_str(cos.sizes()) +
              " and " + shape_str(sin.sizes()));
   if (cos.device() != q.device() || sin.device() != q.device()) p.refuse("tables must be on the device of the pages");
+  const at::Tensor *qw = get(q_weight), *kw = get(k_weight);
+  if ((qw == nullptr) != (kw == nullptr)) p.refuse("q_weight and k_weight must both be given or both be None");
+  HeadWeights w{};
+  if (qw) w = head_weights(p.pre, *qw, *kw, eps, k_pages.size(3), q);
   const at::Tensor qv = head_view(q), kv = head_view(k), vv = head_view(v);
   const Tables t = tables(cos, sin, index);
   at::Tensor out = at::empty(q.sizes(), q.options());
   const ako_paged_t c = p.c(row_count(q));
   const RowStrides qs(qv), ks(kv), vs(vv);
   check(on_device(index, [&](hipStream_t s) {
+          if (qw)
+            return ako_rmsnorm_rope_qk_paged_fwd(qv.data_ptr(), kv.data_ptr(), vv.data_ptr(), w.q.data_ptr(),
+                                                 w.k.data_ptr(), t.cos.data_ptr(), t.sin.data_ptr(), out.data_ptr(), &c,
+                                                 q.size(-2), qs.s, ks.s, vs.s, t.cos.size(0), t.stride,
+                                                 static_cast<float>(eps), dtype_code_or(q.scalar_type()), w.dtype, t.dtype,
+                                                 style_code(style), s);
           return ako_rope_qk_paged_fwd(qv.data_ptr(), kv.data_ptr(), vv.data_ptr(), t.cos.data_ptr(), t.sin.data_ptr(),
                                        out.data_ptr(), &c, q.size(-2), qs.s, ks.s, vs.s, t.cos.size(0), t.stride,
                                        dtype_code_or(q.scalar_type()), t.dtype, style_code(style), s);
@@ -592,7 +662,10 @@ PYBIND11_MODULE(_ako_torch, m) {
   m.def("swiglu", &swiglu, py::arg("gate"), py::arg("up"));
   m.def("rope_qk_paged", &rope_qk_paged, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("cos"), py::arg("sin"),
         py::arg("k_pages"), py::arg("v_pages"), py::arg("block_table"), py::arg("seq_lens"), py::arg("style"),
-        py::arg("k_scales"), py::arg("v_scales"), py::arg("cu_seqlens"));
+        py::arg("k_scales"), py::arg("v_scales"), py::arg("cu_seqlens"), py::arg("q_weight") = py::none(),
+        py::arg("k_weight") = py::none(), py::arg("eps") = 1e-6);
+  m.def("rmsnorm_rope_qk", &rmsnorm_rope_qk, py::arg("q"), py::arg("k"), py::arg("q_weight"), py::arg("k_weight"),
+        py::arg("cos"), py::arg("sin"), py::arg("eps") = 1e-6, py::arg("style") = "neox");
   m.def("paged_read", &paged_read, py::arg("k_pages"), py::arg("v_pages"), py::arg("block_table"), py::arg("seq_lens"),
         py::arg("rows"), py::arg("dtype"), py::arg("k_scales"), py::arg("v_scales"), py::arg("cu_seqlens"));
   m.def("paged_attention", &paged_attention, py::arg("q"), py::arg("k_pages"), py::arg("v_pages"),

@@ -40,9 +40,15 @@ def rope_qk_paged(
     k_scales: torch.Tensor | None = None,
     v_scales: torch.Tensor | None = None,
     cu_seqlens: torch.Tensor | None = None,
+    q_weight: torch.Tensor | None = None,
+    k_weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
 ) -> torch.Tensor:
     """RoPE of a step's q and k at their positions, with the rotated keys and the
     values stored in their sequences' pages; returns the rotated q.
+
+    With ``q_weight`` and ``k_weight``, ``(head_dim,)`` each, every head of q and k goes
+    through its RMSNorm first, as in ``rmsnorm_rope_qk``.
 
     ``cos``/``sin`` hold the rows of positions 0, 1, .... With e4m3 pages
     (``k_scales``, ``v_scales``) keys and values are quantised as they are
@@ -53,8 +59,9 @@ def rope_qk_paged(
     """
     args = (q, k, v, cos, sin, k_pages, v_pages, block_table, seq_lens, style)
     if q.is_cuda and not hip_disabled():
-        return rope_qk_paged_hip(*args, k_scales, v_scales, cu_seqlens)
-    return rope_qk_paged_ref(*args, k_scales=k_scales, v_scales=v_scales, cu_seqlens=cu_seqlens)
+        return rope_qk_paged_hip(*args, k_scales, v_scales, cu_seqlens, q_weight, k_weight, eps)
+    return rope_qk_paged_ref(*args, k_scales=k_scales, v_scales=v_scales, cu_seqlens=cu_seqlens, q_weight=q_weight,
+                             k_weight=k_weight, eps=eps)
 
 
 def paged_read(

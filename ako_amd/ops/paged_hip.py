@@ -15,6 +15,7 @@ import torch
 from ako_amd import _native
 from ako_amd.ops import paged_ref as ref
 from ako_amd.ops._hip_common import DT, call, gpu_index, lib, raw_stream
+from ako_amd.ops.qk_norm import kernel_weights
 from ako_amd.ops.rope_hip import _head_view, _table, _table_stride
 
 _I64x3 = ctypes.c_int64 * 3
@@ -42,30 +43,36 @@ def _tokens(x: torch.Tensor) -> int:
 
 
 def rope_qk_paged_hip(q, k, v, cos, sin, k_pages, v_pages, block_table, seq_lens, style="neox",
-                      k_scales=None, v_scales=None, cu_seqlens=None) -> torch.Tensor:
-    """Rotated q out, rotated k and v into their pages, in one launch."""
+                      k_scales=None, v_scales=None, cu_seqlens=None, q_weight=None, k_weight=None, eps=1e-6) -> torch.Tensor:
+    """Rotated (with weights, normed and rotated) q out, k and v into their pages, in one launch."""
     fast = _native.torch_binding()
-    if fast is not None:
-        return fast.rope_qk_paged(q, k, v, cos, sin, k_pages, v_pages, block_table, seq_lens, style,
-                                  k_scales, v_scales, cu_seqlens)
-    return rope_qk_paged_hip_ctypes(q, k, v, cos, sin, k_pages, v_pages, block_table, seq_lens, style,
-                                    k_scales, v_scales, cu_seqlens)
+    run = rope_qk_paged_hip_ctypes if fast is None else fast.rope_qk_paged
+    return run(q, k, v, cos, sin, k_pages, v_pages, block_table, seq_lens, style, k_scales, v_scales, cu_seqlens,
+               q_weight, k_weight, eps)
 
 
 def rope_qk_paged_hip_ctypes(q, k, v, cos, sin, k_pages, v_pages, block_table, seq_lens, style="neox",
-                             k_scales=None, v_scales=None, cu_seqlens=None) -> torch.Tensor:
+                             k_scales=None, v_scales=None, cu_seqlens=None, q_weight=None, k_weight=None,
+                             eps=1e-6) -> torch.Tensor:
     fn = "rope_qk_paged_hip"
     index = gpu_index(q, fn)
     ref.refuse(fn, ref.cache_error(k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, cu_seqlens)
-               or ref.write_error(q, k, v, cos, sin, k_pages, block_table, style, cu_seqlens))
+               or ref.write_error(q, k, v, cos, sin, k_pages, block_table, style, cu_seqlens)
+               or ref.norm_error(q_weight, k_weight, eps, k_pages))
     qv, kv, vv = _head_view(q), _head_view(k), _head_view(v)
     c, s, st = _table_stride(_table(cos, index), _table(sin, index))
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     cache = _cache(k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, cu_seqlens, _tokens(q))
-    status = call(index, lib().ako_rope_qk_paged_fwd, qv.data_ptr(), kv.data_ptr(), vv.data_ptr(), c.data_ptr(),
-                  s.data_ptr(), out.data_ptr(), ctypes.addressof(cache), q.shape[-2], _row_strides(qv),
-                  _row_strides(kv), _row_strides(vv), c.shape[0], st, DT[q.dtype], DT[c.dtype],
-                  _native.ROPE_STYLE_CODES[style], raw_stream(index))
+    step = (c.data_ptr(), s.data_ptr(), out.data_ptr(), ctypes.addressof(cache), q.shape[-2], _row_strides(qv),
+            _row_strides(kv), _row_strides(vv), c.shape[0], st)
+    types = (DT[c.dtype], _native.ROPE_STYLE_CODES[style], raw_stream(index))
+    rows = (qv.data_ptr(), kv.data_ptr(), vv.data_ptr())
+    if q_weight is None:
+        status = call(index, lib().ako_rope_qk_paged_fwd, *rows, *step, DT[q.dtype], *types)
+    else:
+        qw, kw = kernel_weights(q_weight, k_weight, q.dtype)
+        status = call(index, lib().ako_rmsnorm_rope_qk_paged_fwd, *rows, qw.data_ptr(), kw.data_ptr(), *step, eps,
+                      DT[q.dtype], DT[qw.dtype], *types)
     if status:
         _native.check(status, fn)
     return out

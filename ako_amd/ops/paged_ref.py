@@ -21,6 +21,7 @@ import math
 
 import torch
 
+from ako_amd.ops.qk_norm import norm_rope_rows, weights_error
 from ako_amd.ops.rope_ref import ROPE_STYLES, rope_ref
 
 ROW_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
@@ -140,6 +141,12 @@ def write_error(q, k, v, cos, sin, k_pages, block_table, style, cu_seqlens) -> s
     return None
 
 
+def norm_error(q_weight, k_weight, eps, k_pages) -> str | None:
+    if (q_weight is None) != (k_weight is None):
+        return "q_weight and k_weight must both be given or both be None"
+    return None if q_weight is None else weights_error(q_weight, k_weight, eps, k_pages.shape[3], k_pages)
+
+
 def refuse(fn_name: str, *errors: str | None) -> None:
     for e in errors:
         if e:
@@ -209,9 +216,11 @@ def _rows(pages, codes, page, slot, dtype) -> torch.Tensor:
 
 
 def rope_qk_paged_ref(q, k, v, cos, sin, k_pages, v_pages, block_table, seq_lens, style="neox", *,
-                      k_scales=None, v_scales=None, cu_seqlens=None) -> torch.Tensor:
+                      k_scales=None, v_scales=None, cu_seqlens=None, q_weight=None, k_weight=None,
+                      eps=1e-6) -> torch.Tensor:
     refuse("rope_qk_paged", cache_error(k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, cu_seqlens)
-           or write_error(q, k, v, cos, sin, k_pages, block_table, style, cu_seqlens))
+           or write_error(q, k, v, cos, sin, k_pages, block_table, style, cu_seqlens)
+           or norm_error(q_weight, k_weight, eps, k_pages))
     num_pages, kv_heads, page_size, head_dim = k_pages.shape
     q2, k2, v2 = (x.flatten(0, -3) for x in (q, k, v))
     s, pos = row_places(q2.shape[0], seq_lens, cu_seqlens)
@@ -222,11 +231,14 @@ def rope_qk_paged_ref(q, k, v, cos, sin, k_pages, v_pages, block_table, seq_lens
     out = torch.full_like(q2, float("nan")).masked_fill(pos.lt(0)[:, None, None], 0.0)
     if bool(at.any()):
         c, n, page, slot = cos[row[at]], sin[row[at]], page[at], slot[at]
-        out[at] = rope_ref(q2[at][None], c, n, style)[0]
-        # One rounding to 8 bits: the rotated keys are not rounded to the rows' type first.
-        kr = rope_ref((k2[at] if k_scales is None else k2[at].float())[None], c, n, style)[0]
+        # One rounding, also to 8 bits: rotated rows are not rounded to the rows' type first.
+        if q_weight is None:
+            qr, kr = (rope_ref(x[at].float()[None], c, n, style)[0] for x in (q2, k2))
+        else:
+            qr, kr = (norm_rope_rows(x[at][None], w, c, n, eps, style)[0] for x, w in ((q2, q_weight), (k2, k_weight)))
+        out[at] = qr.to(q.dtype)
         if k_scales is None:
-            k_pages[page, :, slot], v_pages[page, :, slot] = kr, v2[at]
+            k_pages[page, :, slot], v_pages[page, :, slot] = kr.to(k.dtype), v2[at]
         else:
             for pages, codes, x in ((k_pages, k_scales, kr), (v_pages, v_scales, v2[at])):
                 b, e = quantize_rows(x)

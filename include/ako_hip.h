@@ -192,6 +192,24 @@ int ako_rope_qk_cache_fwd(const void* q, const void* k, const void* v,
                           int dtype, int table_dtype, int style, void* stream);
 
 /*
+ * RMSNorm of every head of q and k with a weight per element, and RoPE, in one
+ * pass: for each head x of q (w = q_weight) and of k (w = k_weight)
+ *   y = (x * rsqrt(sum(x^2) / head_dim + eps)) * w      (fp32)
+ * and y's pairs rotated as by ako_rope_fwd, the result rounded once. The
+ * reference has no such pass; it is rmsnorm_ref (ako/ops/rmsnorm_ref.py:8-24) over
+ * heads, then rope_ref (ako/ops/rope_ref.py:73-107), without the rounding between.
+ * q and k are [batch, seq, heads, head_dim] with strides as in ako_rope_fwd (either
+ * may have no heads), the outputs dense. head_dim is even, at most 512. The weights
+ * are of dtype or AKO_DTYPE_F32.
+ */
+int ako_rmsnorm_rope_qk_fwd(const void* q, const void* k, const void* q_weight, const void* k_weight,
+                            const void* cos_table, const void* sin_table, void* q_out, void* k_out,
+                            int64_t batch, int64_t seq, int64_t q_heads, int64_t k_heads,
+                            int64_t head_dim, const int64_t* q_strides, const int64_t* k_strides,
+                            int64_t table_row_stride, float eps, int dtype, int w_dtype,
+                            int table_dtype, int style, void* stream);
+
+/*
  * SwiGLU activation: y = to_dtype( silu(gate) * up ), silu(g) = g / (1 + e^-g),
  * over [rows, n] with row strides in elements.
  * Replaces swiglu_triton + _swiglu_kernel_impl
@@ -264,6 +282,20 @@ int ako_rope_qk_paged_fwd(const void* q, const void* k, const void* v,
                           const int64_t* q_strides, const int64_t* k_strides,
                           const int64_t* v_strides, int64_t table_rows, int64_t table_row_stride,
                           int dtype, int table_dtype, int style, void* stream);
+
+/*
+ * The same with every head of q and k through its RMSNorm first, as in
+ * ako_rmsnorm_rope_qk_fwd: nothing is rounded between the norm and the rotation, nor
+ * between those and an e4m3 page. Values are stored as they are.
+ */
+int ako_rmsnorm_rope_qk_paged_fwd(const void* q, const void* k, const void* v,
+                                  const void* q_weight, const void* k_weight,
+                                  const void* cos_table, const void* sin_table, void* q_out,
+                                  const ako_paged_t* cache, int64_t q_heads,
+                                  const int64_t* q_strides, const int64_t* k_strides,
+                                  const int64_t* v_strides, int64_t table_rows,
+                                  int64_t table_row_stride, float eps, int dtype, int w_dtype,
+                                  int table_dtype, int style, void* stream);
 
 /*
  * The keys and values stored at the rows' positions, as dense [tokens,

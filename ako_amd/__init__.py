@@ -16,6 +16,7 @@ from ako_amd.ops.paged import new_pages, paged_attention, paged_read, rope_qk_pa
 from ako_amd.ops.qk_norm import rmsnorm_rope_qk
 from ako_amd.ops.rmsnorm import rmsnorm, rmsnorm_residual
 from ako_amd.ops.rope import build_rope_tables, rope, rope_qk, rope_qk_cache
+from ako_amd.ops.sample import sample
 from ako_amd.ops.swiglu import swiglu
 
 __all__ = [
@@ -31,5 +32,6 @@ __all__ = [
     "rope_qk",
     "rope_qk_cache",
     "rope_qk_paged",
+    "sample",
     "swiglu",
 ]

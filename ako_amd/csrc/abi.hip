@@ -1011,4 +1011,53 @@ int64_t ako_paged_attention_workspace(const ako_paged_t* cache, int64_t q_heads,
   return empty ? 0 : ako::paged_attention_workspace(a);
 }
 
+// --------------------------------------------------------------- sampling --
+int ako_sample_fwd(const void* logits, const float* uniform, const float* temperature, float temperature_all,
+                   const int32_t* top_k, int32_t top_k_all, const float* top_p, float top_p_all, const float* min_p,
+                   float min_p_all, int64_t* out, int64_t rows, int64_t vocab, int64_t row_stride, int dtype, void* stream) {
+  const char* fn = "ako_sample_fwd";
+  if (!valid_dtype(dtype)) return fail(AKO_ERR_UNSUPPORTED, "%s: unknown dtype code %d", fn, dtype);
+  if (rows < 0) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: negative size", fn);
+  constexpr int64_t kMaxVocab = int64_t(1) << 22;
+  if (vocab < 1 || vocab > kMaxVocab)
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: vocab must be 1 to %lld, got %lld", fn, (long long)kMaxVocab, (long long)vocab);
+  if (!temperature && !(temperature_all >= 0.0f))
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: temperature must be >= 0", fn);
+  if (!top_k && top_k_all < 0) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: top_k must be >= 0", fn);
+  if ((!top_p && !(top_p_all >= 0.0f && top_p_all <= 1.0f)) || (!min_p && !(min_p_all >= 0.0f && min_p_all <= 1.0f)))
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: top_p and min_p must be 0 to 1", fn);
+  if (rows == 0) return AKO_OK;
+  if (!logits || !uniform || !out) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: null pointer argument", fn);
+  if (row_stride < 0) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: negative row stride", fn);
+  const Span in = span_2d(logits, rows, vocab, row_stride, ako::dtype_bytes(dtype));
+  const Span o = span_2d(out, 1, rows, rows, 8);
+  const void* const per_row[5] = {uniform, temperature, top_k, top_p, min_p};
+  bool ok = in.ok && o.ok, apart = !overlap(o, in);
+  for (const void* p : per_row) {
+    if (!p) continue;
+    const Span s = span_2d(p, 1, rows, rows, 4);
+    ok = ok && s.ok;
+    apart = apart && !overlap(o, s);
+  }
+  if (!ok) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: sizes and strides overflow the address space", fn);
+  if (!apart) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: out overlaps an input", fn);
+  ako::SampleArgs a{};
+  a.x = logits;
+  a.rows = rows;
+  a.vocab = vocab;
+  a.stride = row_stride;
+  a.u = uniform;
+  a.temperatures = temperature;
+  a.top_ks = top_k;
+  a.top_ps = top_p;
+  a.min_ps = min_p;
+  a.temperature = temperature_all;
+  a.top_k = top_k_all;
+  a.top_p = top_p_all;
+  a.min_p = min_p_all;
+  a.out = out;
+  a.dtype = dtype;
+  return hip_status(ako::launch_sample(a, static_cast<hipStream_t>(stream)), fn);
+}
+
 }  // extern "C"

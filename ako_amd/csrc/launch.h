@@ -241,4 +241,20 @@ struct PagedAttentionArgs {
 int64_t paged_attention_workspace(const PagedAttentionArgs& a);
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t stream);
 
+// A token for each row of logits from a given uniform number.
+struct SampleArgs {
+  const void* x;
+  int64_t rows, vocab, stride;
+  const float* u;
+  const float* temperatures;  // one for each row, or null: the one for all
+  const int* top_ks;
+  const float* top_ps;
+  const float* min_ps;
+  float temperature, top_p, min_p;
+  int top_k;
+  int64_t* out;
+  int dtype;
+};
+hipError_t launch_sample(const SampleArgs& a, hipStream_t stream);
+
 }  // namespace ako

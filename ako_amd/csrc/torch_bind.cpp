@@ -14,6 +14,7 @@
 #include <ATen/hip/HIPContext.h>
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 #include <utility>
@@ -635,6 +636,62 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const
   return out;
 }
 
+// ----------------------------------------------------------------- sampling --
+// The checks and messages of ako_amd/ops/sample.py (sample_error), in the same order. A setting is a
+// number for all rows or a tensor of one for each.
+struct Setting {
+  const at::Tensor* rows = nullptr;
+  at::Tensor held;
+  double all = 0;
+
+  Setting(const std::string& pre, const char* name, const py::object& v, const at::Tensor& x, at::ScalarType type) {
+    if (THPVariable_Check(v.ptr())) {
+      held = THPVariable_Unpack(v.ptr());
+      rows = &held;
+      if (held.dim() != 1 || held.size(0) != x.size(0) || held.scalar_type() != type || !held.is_contiguous() ||
+          held.device() != x.device())
+        value_error(pre + name + " must be a number or a contiguous " + dtype_str(type) + " tensor of shape (" +
+                    std::to_string(x.size(0)) + ",) on the device of the logits");
+    } else {
+      all = v.cast<double>();
+    }
+  }
+  template <typename T>
+  const T* ptr() const { return rows ? static_cast<const T*>(rows->data_ptr()) : nullptr; }
+};
+
+at::Tensor sample(const at::Tensor& logits, const at::Tensor& uniform, const py::object& temperature, const py::object& top_k,
+                  const py::object& top_p, const py::object& min_p) {
+  const char* fn = "sample_hip";
+  const std::string pre = std::string(fn) + ": ";
+  const int index = gpu_index(logits, fn);
+  if (logits.dim() != 2) value_error(pre + "logits must be (rows, vocab), got " + shape_str(logits.sizes()));
+  const int dt = dtype_code_or(logits.scalar_type());
+  if (dt < 0) value_error(pre + "logits must be float32/float16/bfloat16, got " + dtype_str(logits.scalar_type()));
+  const int64_t rows = logits.size(0), vocab = logits.size(1);
+  if (vocab < 1 || vocab > 4194304) value_error(pre + "vocab must be 1 to 4194304, got " + std::to_string(vocab));
+  if (uniform.dim() != 1 || uniform.size(0) != rows || uniform.scalar_type() != at::kFloat || !uniform.is_contiguous() ||
+      uniform.device() != logits.device())
+    value_error(pre + "uniform must be a contiguous torch.float32 tensor of shape (" + std::to_string(rows) +
+                ",) on the device of the logits");
+  const Setting t(pre, "temperature", temperature, logits, at::kFloat), k(pre, "top_k", top_k, logits, at::kInt),
+      p(pre, "top_p", top_p, logits, at::kFloat), m(pre, "min_p", min_p, logits, at::kFloat);
+  if (!t.rows && !(t.all >= 0)) value_error(pre + "temperature must be at least 0, got " + number(t.all));
+  if (!k.rows && !(k.all >= 0 && k.all == std::floor(k.all) && std::isfinite(k.all)))
+    value_error(pre + "top_k must be a whole number, at least 0, got " + std::string(py::str(top_k)));
+  if (!p.rows && !(p.all >= 0 && p.all <= 1)) value_error(pre + "top_p must be 0 to 1, got " + number(p.all));
+  if (!m.rows && !(m.all >= 0 && m.all <= 1)) value_error(pre + "min_p must be 0 to 1, got " + number(m.all));
+  const at::Tensor x = logits.stride(1) == 1 || vocab == 1 ? logits : logits.contiguous();
+  at::Tensor out = at::empty({rows}, logits.options().dtype(at::kLong));
+  check(on_device(index, [&](hipStream_t s) {
+          return ako_sample_fwd(x.data_ptr(), static_cast<const float*>(uniform.data_ptr()), t.ptr<float>(),
+                                static_cast<float>(t.all), k.ptr<int32_t>(), static_cast<int32_t>(std::min(k.all, 2147483647.0)),
+                                p.ptr<float>(), static_cast<float>(p.all), m.ptr<float>(), static_cast<float>(m.all),
+                                static_cast<int64_t*>(out.data_ptr()), rows, vocab, rows > 1 ? x.stride(0) : vocab, dt, s);
+        }), fn);
+  return out;
+}
+
 // The stream this binding launches on, for tests: torch's current stream.
 int64_t current_stream(int64_t index) {
   return reinterpret_cast<int64_t>(at::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(index)).stream());
@@ -671,6 +728,8 @@ PYBIND11_MODULE(_ako_torch, m) {
   m.def("paged_attention", &paged_attention, py::arg("q"), py::arg("k_pages"), py::arg("v_pages"),
         py::arg("block_table"), py::arg("seq_lens"), py::arg("scale"), py::arg("window"), py::arg("sinks"),
         py::arg("k_scales"), py::arg("v_scales"), py::arg("cu_seqlens"));
+  m.def("sample", &sample, py::arg("logits"), py::arg("uniform"), py::arg("temperature") = 1.0, py::arg("top_k") = 0,
+        py::arg("top_p") = 1.0, py::arg("min_p") = 0.0);
   m.def("current_stream", &current_stream);
   m.def("row_walk", &row_walk, py::arg("t"));
 }

@@ -329,6 +329,29 @@ int ako_paged_attention_fwd(const void* q, const int64_t* q_strides, void* out,
 int64_t ako_paged_attention_workspace(const ako_paged_t* cache, int64_t q_heads, int dtype);
 
 /*
+ * A token for each of `rows` rows of `vocab` logits (1 to 2^22), from one uniform number each.
+ * With w_i = e^((x_i - max x) / temperature), in descending order of the logits (of
+ * equal ones the lowest index first) the first top_k tokens stay (0 or less: all), of
+ * those the shortest run from the front that weighs at least top_p of them all
+ * (1 or more: all; at least one), and of those the ones with w_i >= min_p (0 or less: all). out is
+ * the first token, by index, at which the sum of the weights of what stays, so far, passes
+ * uniform times their whole sum; for numbers from 1 on the last that weighs anything.
+ * temperature 0 or less, or NaN, takes the largest logit's first token. Tokens of -infinity
+ * or NaN are never drawn; where there are no others out is -1. Among several +infinities only
+ * those are drawn, alike. Weights are sums of whole numbers, 2^-46 of the largest at 131072
+ * tokens and finer below: the token does not depend on how the work was divided.
+ * temperature, top_k, top_p and min_p hold one value for each row, or are NULL and the
+ * value behind them holds for all rows (temperature_all >= 0 and not NaN, the others' in
+ * [0, 1], top_k_all >= 0). row_stride: elements between rows. The reference has no
+ * counterpart (its decoder returns hidden states, ako/models/decoder.py:261-266).
+ */
+int ako_sample_fwd(const void* logits, const float* uniform, const float* temperature,
+                   float temperature_all, const int32_t* top_k, int32_t top_k_all,
+                   const float* top_p, float top_p_all, const float* min_p, float min_p_all,
+                   int64_t* out, int64_t rows, int64_t vocab, int64_t row_stride, int dtype,
+                   void* stream);
+
+/*
  * Launch-shape override for tuning sweeps and tests (no counterpart in the
  * reference, whose Triton autotuner explored num_warps itself); production
  * callers leave it alone. op: 0 = rmsnorm and rmsnorm_residual, 1 = rope,

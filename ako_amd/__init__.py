@@ -12,7 +12,7 @@ So are the operations on a paged cache: ``rope_qk_paged``, ``paged_read`` and
 
 __version__ = "0.1.0"
 
-from ako_amd.ops.paged import new_pages, paged_attention, paged_read, rope_qk_paged
+from ako_amd.ops.paged import new_pages, paged_attention, paged_means, paged_read, paged_select, rope_qk_paged
 from ako_amd.ops.qk_norm import rmsnorm_rope_qk
 from ako_amd.ops.rmsnorm import rmsnorm, rmsnorm_residual
 from ako_amd.ops.rope import build_rope_tables, rope, rope_qk, rope_qk_cache
@@ -24,7 +24,9 @@ __all__ = [
     "build_rope_tables",
     "new_pages",
     "paged_attention",
+    "paged_means",
     "paged_read",
+    "paged_select",
     "rmsnorm",
     "rmsnorm_residual",
     "rmsnorm_rope_qk",

@@ -1011,6 +1011,141 @@ int64_t ako_paged_attention_workspace(const ako_paged_t* cache, int64_t q_heads,
   return empty ? 0 : ako::paged_attention_workspace(a);
 }
 
+// ------------------------------------------------- blocks of a paged cache --
+extern "C++" {
+namespace {
+
+// What a call on means has of a cache: the keys alone, or no pages at all.
+ako_paged_t keys_only(const ako_paged_t& c) {
+  ako_paged_t k = c;
+  k.v_pages = c.k_pages;
+  k.v_scales = c.k_scales;
+  for (int i = 0; i < 3; ++i) {
+    k.v_strides[i] = c.k_strides[i];
+    k.v_scale_strides[i] = c.k_scale_strides[i];
+  }
+  return k;
+}
+ako_paged_t no_pages(const ako_paged_t& c, const void* means, int dtype) {
+  ako_paged_t k = c;
+  k.k_pages = const_cast<void*>(means);  // not read
+  k.k_scales = nullptr;
+  for (int i = 0; i < 3; ++i) k.k_strides[i] = 0;
+  k.page_dtype = dtype;
+  return keys_only(k);
+}
+
+Span means_span(const ako_paged_t& c, const float* means, const int64_t* st) {
+  const int64_t st3[3] = {st[0], st[1], 0};
+  return span_4d(means, c.num_pages, c.kv_heads, 1, c.head_dim, st3, 4);
+}
+
+int select_common(const char* fn, const ako_paged_t& cache, int64_t q_heads, int64_t count, int dtype,
+                  ako::PagedSelectArgs* a, bool* empty) {
+  if (const int rc = paged_common(fn, &cache, q_heads, dtype, &a->c, empty)) return rc;
+  if (q_heads % cache.kv_heads)
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: %lld query heads are no multiple of %lld", fn, (long long)q_heads,
+                (long long)cache.kv_heads);
+  if (count < 1 || count > kMaxInt / 2) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: count must be 1 to 2^30", fn);
+  // Of a launch's workgroups, 16 rows by 512 blocks each: work-items stay below 2^32.
+  if (cache.table_width > (int64_t(1) << 28) / cache.kv_heads)
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: more than 2^28 blocks and key heads", fn);
+  a->q_heads = q_heads;
+  a->count = count;
+  a->dtype = dtype;
+  return AKO_OK;
+}
+
+}  // namespace
+}  // extern "C++"
+
+int ako_paged_means_fwd(const ako_paged_t* cache, float* means, const int64_t* means_strides, int dtype, void* stream) {
+  const char* fn = "ako_paged_means_fwd";
+  if (!cache) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: null cache", fn);
+  const ako_paged_t c = keys_only(*cache);
+  if (c.page_dtype == AKO_DTYPE_E4M3) dtype = AKO_DTYPE_F32;
+  ako::PagedMeansArgs a{};
+  bool empty = false;
+  if (const int rc = paged_common(fn, &c, 0, dtype, &a.c, &empty)) return rc;
+  if (empty || c.num_pages == 0) return AKO_OK;
+  if (!means || !means_strides) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: null pointer argument", fn);
+  if (means_strides[0] < 0 || means_strides[1] < 0) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: negative stride", fn);
+  const int64_t st3[3] = {means_strides[0], means_strides[1], 0};
+  if (!distinct_rows(c.num_pages, c.kv_heads, 1, c.head_dim, st3))
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: rows of the means overlap", fn);
+  const Span m = means_span(c, means, means_strides);
+  const PagedSpans held(&c, dtype);
+  if (!m.ok || !held.ok) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: sizes and strides overflow the address space", fn);
+  if (held.meets(m)) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: the means overlap another buffer", fn);
+  a.means = means;
+  a.ms[0] = means_strides[0];
+  a.ms[1] = means_strides[1];
+  a.dtype = dtype;
+  return hip_status(ako::launch_paged_means(a, static_cast<hipStream_t>(stream)), fn);
+}
+
+int ako_paged_select_fwd(const ako_paged_t* cache, const void* q, const int64_t* q_strides, int64_t q_heads,
+                         const float* means, const int64_t* means_strides, int32_t* blocks, int64_t count, int64_t first,
+                         int64_t last, void* workspace, int64_t workspace_bytes, int dtype, void* stream) {
+  const char* fn = "ako_paged_select_fwd";
+  if (!cache) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: null cache", fn);
+  ako::PagedSelectArgs a{};
+  bool empty = false;
+  const ako_paged_t c = no_pages(*cache, means, dtype);
+  if (c.num_pages > 0 && c.tokens > 0 && !means) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: null means", fn);
+  if (const int rc = select_common(fn, c, q_heads, count, dtype, &a, &empty)) return rc;
+  if (first < 0 || last < 1 || first > count || last > count - first)
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: first must be >= 0, last >= 1 and count >= first + last", fn);
+  if (empty) return AKO_OK;
+  if ((q_heads > 0 && !q) || !q_strides || !blocks || !means_strides)
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: null pointer argument", fn);
+  if (q_strides[0] < 0 || q_strides[1] < 0 || q_strides[2] < 0 || means_strides[0] < 0 || means_strides[1] < 0)
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: negative stride", fn);
+  const int64_t need = ako::paged_select_workspace(a);
+  if (workspace_bytes < need || (need > 0 && (!workspace || !aligned(workspace, 16))))
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: needs a 16-byte aligned workspace of %lld bytes, got %lld", fn,
+                (long long)need, (long long)workspace_bytes);
+  const int64_t per = c.cu_seqlens ? c.tokens : c.tokens / c.n_seqs;
+  const __int128 out_bytes = static_cast<__int128>(c.tokens) * c.kv_heads * count * 4;
+  const Span o = span_bytes(blocks, out_bytes), w = span_bytes(workspace, need);
+  Span in[2];
+  int n_in = 0;
+  if (q_heads > 0)
+    in[n_in++] = span_4d(q, c.cu_seqlens ? 1 : c.n_seqs, per, q_heads, c.head_dim, q_strides, ako::dtype_bytes(dtype));
+  if (c.num_pages > 0) in[n_in++] = means_span(c, means, means_strides);
+  const PagedSpans held(&c, dtype);
+  bool ok = o.ok && w.ok && held.ok, apart = !overlap(o, w) && !held.meets_index(o) && !held.meets_index(w);
+  for (int i = 0; i < n_in; ++i) {
+    ok = ok && in[i].ok;
+    apart = apart && !overlap(o, in[i]) && !overlap(w, in[i]);
+  }
+  if (!ok) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: sizes and strides overflow the address space", fn);
+  if (!apart) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: blocks or the workspace overlap another buffer", fn);
+  a.q = q;
+  a.means = means;
+  for (int i = 0; i < 3; ++i) a.qs[i] = q_strides[i];
+  a.ms[0] = means_strides[0];
+  a.ms[1] = means_strides[1];
+  a.first = first;
+  a.last = last;
+  a.out = blocks;
+  a.workspace = workspace;
+  return hip_status(ako::launch_paged_select(a, static_cast<hipStream_t>(stream)), fn);
+}
+
+int64_t ako_paged_select_workspace(const ako_paged_t* cache, int64_t q_heads, int64_t count, int dtype) {
+  const char* fn = "ako_paged_select_workspace";
+  ako::PagedSelectArgs a{};
+  bool empty = false;
+  if (!cache) {
+    fail(AKO_ERR_INVALID_ARGUMENT, "%s: null cache", fn);
+    return -1;
+  }
+  const ako_paged_t c = no_pages(*cache, cache, dtype);
+  if (select_common(fn, c, q_heads, count, dtype, &a, &empty)) return -1;
+  return empty ? 0 : ako::paged_select_workspace(a);
+}
+
 // --------------------------------------------------------------- sampling --
 int ako_sample_fwd(const void* logits, const float* uniform, const float* temperature, float temperature_all,
                    const int32_t* top_k, int32_t top_k_all, const float* top_p, float top_p_all, const float* min_p,

@@ -241,6 +241,27 @@ struct PagedAttentionArgs {
 int64_t paged_attention_workspace(const PagedAttentionArgs& a);
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t stream);
 
+struct PagedMeansArgs {
+  PagedArgs c;  // keys only
+  float* means;
+  int64_t ms[2];  // page, head
+  int dtype;
+};
+hipError_t launch_paged_means(const PagedMeansArgs& a, hipStream_t stream);
+
+struct PagedSelectArgs {
+  PagedArgs c;  // no pages: their number and sizes, and the step
+  const void* q;
+  const float* means;
+  int64_t qs[3], ms[2];  // batch, token, head; page, head
+  int64_t q_heads, count, first, last;
+  int* out;
+  void* workspace;  // paged_select_workspace bytes
+  int dtype;
+};
+int64_t paged_select_workspace(const PagedSelectArgs& a);
+hipError_t launch_paged_select(const PagedSelectArgs& a, hipStream_t stream);
+
 // A token for each row of logits from a given uniform number.
 struct SampleArgs {
   const void* x;

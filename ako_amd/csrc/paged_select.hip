@@ -1,0 +1,456 @@
+// Choosing the blocks of a paged cache that a token attends to, on gfx950.
+//
+// A block is a page. paged_means: the mean of the keys of every page that a step's
+// rows have filled, per key head, in 32 bits. select_scores and select_blocks: for each token row
+// and key head, of the blocks up to the token's own, the first and last few, and then those
+// whose mean key has the largest product with the sum of the queries that share the
+// key head, which is `group` times the mean score of the block's keys over those
+// heads. Of equal scores the lowest block comes first.
+//
+// Scores are formed in 64 bits, on the matrix cores: which of two blocks is the k-th
+// hangs on the last bits of their scores, and so it is the same for every order of the
+// sums, every batch and every division of the work up to errors of 2^-50 or so.
+
+#include <algorithm>
+#include <limits>
+
+#include "paged.h"
+
+namespace ako {
+
+// As token_place, for a token of each lane's own.
+__device__ __forceinline__ TokenPlace lane_place(const PagedDev& p, int token) {
+  if (p.cu == nullptr) return token_place(p, token);
+  int lo = 0, hi = p.n_seqs + 1;  // the last i with cu[i] <= token lies in [lo, hi)
+  while (hi - lo > 1) {
+    const int mid = lo + (hi - lo) / 2;
+    if (p.cu[mid] <= token) lo = mid;
+    else hi = mid;
+  }
+  if (lo >= p.n_seqs) return TokenPlace{-1, -1};
+  const int first = p.cu[lo], end = p.cu[lo + 1];
+  if (token < first || token >= end) return TokenPlace{-1, -1};
+  return TokenPlace{lo, max(p.lens[lo], 0) - (end - token)};
+}
+
+// ---- means of filled pages ---------------------------------------------------------
+struct MeansDev {
+  PagedDev c;
+  float* means;
+  int64_t ms[2];  // page, head strides
+  int kv_heads, head_dim, lanes, rows;  // lanes across a row, rows of a wavefront's load
+  int token0;
+  FastDiv by_kv_heads, by_lanes;
+};
+
+constexpr int kMeanTokens = 16;  // token rows of a workgroup
+
+template <typename T, bool MX>
+__global__ __launch_bounds__(256) void paged_means(MeansDev a) {
+  __shared__ float part[4][kWave][9];  // 9: lanes' rows on different banks
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int tile = fast_div(blockIdx.x, a.by_kv_heads), head = blockIdx.x - tile * a.kv_heads;
+  const int token = a.token0 + tile * kMeanTokens + lane;
+  // Which of the rows fill a page: lane i holds row i's page.
+  int page = -1;
+  if (lane < kMeanTokens && token < a.c.tokens) {
+    const TokenPlace at = lane_place(a.c, token);
+    if (at.seq >= 0 && at.pos >= 0 && at.pos < a.c.capacity) {
+      int slot;
+      page = page_of(a.c, at.seq, at.pos, slot);
+      if (slot != a.c.page_size - 1) page = -1;
+    }
+  }
+  uint64_t todo = __ballot(page >= 0);
+  const int row = fast_div(lane, a.by_lanes), e0 = (lane - row * a.lanes) * 8;
+  for (int nth = 0; todo != 0; todo &= todo - 1, ++nth) {
+    if (nth % 4 != wave) continue;
+    const int at = __builtin_amdgcn_readlane(page, __builtin_ctzll(todo));
+    float sum[8] = {};
+    constexpr int U = 8;  // loads in flight
+    for (int s0 = 0; s0 < a.c.page_size; s0 += U * a.rows) {
+      Eight<float> x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int s = s0 + u * a.rows + row;
+        x[u] = zero_eight<float>();
+        if (row >= a.rows || s >= a.c.page_size) continue;
+        const int64_t k = at * a.c.kst[0] + head * a.c.kst[1] + s * a.c.kst[2] + e0;
+        if constexpr (MX) {
+          const unsigned code = a.c.ks[at * a.c.ksst[0] + head * a.c.ksst[1] + s * a.c.ksst[2] + e0 / 32];
+          x[u] = from_e4m3<float>(load_bytes8(static_cast<const uint8_t*>(a.c.k) + k), e8m0_scale(code));
+        } else {
+          const Eight<T> y = load_eight<T>(static_cast<const T*>(a.c.k) + k);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[u][i] = to_f32(y[i]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] += x[u][i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) part[wave][lane][i] = sum[i];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (lane < a.lanes) {
+      for (int r = 1; r < a.rows; ++r)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] += part[wave][lane + r * a.lanes][i];
+      Eight<float> y;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = sum[i] / static_cast<float>(a.c.page_size);
+      store_eight<float>(a.means + at * a.ms[0] + head * a.ms[1] + lane * 8, y);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// ---- scores ---------------------------------------------------------------------------
+struct SelectDev {
+  PagedDev c;
+  const void* q;
+  const float* means;
+  int64_t qs[3], ms[2];  // q: batch, token, head; means: page, head
+  double* scores;        // [rows of the slice, kv_heads, width]; NaN: no such page
+  int* out;
+  int kv_heads, group, head_dim;
+  int count, first, last, width;
+  int token0, end;       // the slice's rows
+  int tile, chunk;       // rows of a tile, blocks of a workgroup
+  FastDiv by_kv_heads, by_tiles;
+};
+
+// The blocks that a token at `pos` may attend to are 0 .. blocks - 1.
+__device__ __forceinline__ int blocks_of(const SelectDev& a, int pos) {
+  return pos < 0 ? 0 : min(static_cast<int>(fast_div(pos, a.c.by_page)) + 1, a.width);
+}
+__device__ __forceinline__ int page_at(const SelectDev& a, int seq, int block) {
+  const int page = a.c.table[seq * a.c.table_stride + block];
+  return page >= 0 && page < a.c.num_pages ? page : -1;
+}
+
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+
+// Up to 16 token rows by 16 blocks per wavefront and step. The matrix instruction takes four elements of
+// the inner dimension from the four groups of 16 lanes; which four is only a name, so group g
+// holds the g-th quarter of a row and loads it in 16-byte packets. The rows' sums of
+// queries stay in registers. Rows of a tile that belong to different sequences are
+// done one sequence after the other.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void select_scores(SelectDev a) {
+  constexpr int Q = DP / 4;  // elements of a row in a lane
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, col = lane % 16, g = lane / 16;
+  const int head = blockIdx.x - fast_div(blockIdx.x, a.by_kv_heads) * a.kv_heads;
+  const unsigned nth = fast_div(blockIdx.x, a.by_kv_heads);
+  const int chunk = fast_div(nth, a.by_tiles);
+  const int tile = nth - chunk * ((a.end - a.token0 + a.tile - 1) / a.tile);
+  const int row0 = a.token0 + tile * a.tile, token = row0 + col;
+  const bool live = col < a.tile && token < a.end;
+  TokenPlace at{-1, -1};
+  if (live) at = lane_place(a.c, token);
+  const int blocks = at.seq < 0 ? 0 : blocks_of(a, at.pos);
+  // Rows with no more blocks than are asked for are not scored.
+  unsigned todo = static_cast<unsigned>(__ballot(blocks > a.count && blocks > chunk * a.chunk)) & 0xffffu;
+  if (todo == 0) return;
+
+  double q[Q];
+#pragma unroll
+  for (int i = 0; i < Q; ++i) q[i] = 0.0;
+  if (todo >> col & 1) {
+    const int b = a.c.cu ? 0 : at.seq, s = token - b * a.c.seq;
+    const T* x = static_cast<const T*>(a.q) + b * a.qs[0] + s * a.qs[1] + int64_t(head) * a.group * a.qs[2] + g * Q;
+    for (int h = 0; h < a.group; ++h, x += a.qs[2]) {
+#pragma unroll
+      for (int i = 0; i < Q; i += 4) {
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (g * Q + i < a.head_dim) load_f32<T, 4>(x + i, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q[i + j] += static_cast<double>(v[j]);
+      }
+    }
+  }
+
+  while (todo != 0) {
+    const int from = __builtin_ctz(todo), seq = __builtin_amdgcn_readlane(at.seq, from);
+    const unsigned rows = static_cast<unsigned>(__ballot(at.seq == seq && (todo >> col & 1))) & 0xffffu;
+    todo &= ~rows;
+    // Positions ascend, so the sequence's last row has the most blocks.
+    const int most = __builtin_amdgcn_readlane(blocks, 31 - __builtin_clz(rows));
+    for (int b0 = chunk * a.chunk + wave * 16; b0 < min(most, (chunk + 1) * a.chunk); b0 += 4 * 16) {
+      const int block = b0 + col, page = block < most ? page_at(a, seq, block) : -1;
+      const float* m = a.means + max(page, 0) * a.ms[0] + head * a.ms[1] + g * Q;
+      float k[Q];
+#pragma unroll
+      for (int i = 0; i < Q; i += 4) {
+        Pack<float, 4> p;
+        p.raw = u32x4{0, 0, 0, 0};
+        if (page >= 0 && g * Q + i < a.head_dim) p = load_pack<float, 4>(m + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) k[i + j] = p.e[j];
+      }
+      f64x4 s = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < Q; ++i) s = __builtin_amdgcn_mfma_f64_16x16x4f64(q[i], static_cast<double>(k[i]), s, 0, 0, 0);
+      if (block < most) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {  // a lane holds column `col` of the rows 4 v + g
+          const int r = 4 * v + g;
+          if (!(rows >> r & 1)) continue;
+          const double x = page < 0 ? __builtin_nan("") : s[v] != s[v] ? -__builtin_inf() : s[v];
+          a.scores[(int64_t(row0 + r - a.token0) * a.kv_heads + head) * a.width + block] = x;
+        }
+      }
+    }
+  }
+}
+
+// ---- the choice ---------------------------------------------------------------------
+// Doubles as whole numbers in the same order.
+__device__ __forceinline__ int64_t order_of(double x) {
+  const int64_t b = __builtin_bit_cast(int64_t, x + 0.0);
+  return b ^ (b >> 63 & 0x7fffffffffffffffll);
+}
+__device__ __forceinline__ double of_order(int64_t k) {
+  return __builtin_bit_cast(double, k ^ (k >> 63 & 0x7fffffffffffffffll));
+}
+
+// A wavefront per row and key head. The score that parts the `want` largest from the rest is
+// found by halving the interval between the least and the greatest, first of values, then of
+// their bits, until as many lie above as are wanted or one value is left, whose lowest blocks
+// are then taken. N: scores in a lane's registers, 0 where they are too many and are read
+// again for every step.
+template <int N>
+__global__ __launch_bounds__(256) void select_blocks(SelectDev a) {
+  const int lane = threadIdx.x % kWave;
+  const int64_t item = int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  if (item >= int64_t(a.end - a.token0) * a.kv_heads) return;
+  const int row = fast_div(static_cast<unsigned>(item), a.by_kv_heads);
+  const TokenPlace at = token_place(a.c, a.token0 + row);
+  const int blocks = at.seq < 0 ? 0 : blocks_of(a, at.pos);
+  int* const out = a.out + (int64_t(a.token0) * a.kv_heads + item) * a.count;
+  const double* const scores = a.scores + item * a.width;
+  const bool all = blocks <= a.count;
+  // Always taken: below `low` and from `high` on, the token's own block being the last.
+  const int own = blocks > 0 ? static_cast<int>(fast_div(at.pos, a.c.by_page)) : 0;
+  const int low = min(a.first, blocks), high = max(low, min(blocks, max(0, own - a.last + 1)));
+  const auto there = [&](int b) { return page_at(a, at.seq, b) >= 0; };
+
+  double cut = -__builtin_inf();  // scores above it are taken, and of those equal to it the first `equal`
+  int equal = std::numeric_limits<int>::max();
+  constexpr int R = N > 0 ? N : 1;
+  double mine[R];
+  // f(score) of this lane's scores between the blocks that are always taken; those of absent pages are NaN.
+  const auto each = [&](auto f) {
+    if constexpr (N > 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) f(mine[i]);
+    } else {
+      for (int b = low + lane; b < high; b += kWave) f(scores[b]);
+    }
+  };
+  if (!all) {
+    if constexpr (N > 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int b = low + i * kWave + lane;
+        mine[i] = b < high ? scores[b] : __builtin_nan("");
+      }
+    }
+    double least = __builtin_inf(), most = -__builtin_inf();
+    int held = 0;
+    each([&](double x) {
+      least = fmin(least, x);
+      most = fmax(most, x);
+      held += x == x;
+    });
+    int always = 0;
+    for (int b = lane; b < low; b += kWave) always += there(b);
+    for (int b = high + lane; b < blocks; b += kWave) always += there(b);
+#pragma unroll
+    for (int k = 1; k < kWave; k *= 2) {
+      least = fmin(least, __shfl_xor(least, k));
+      most = fmax(most, __shfl_xor(most, k));
+      held += __shfl_xor(held, k);
+      always += __shfl_xor(always, k);
+    }
+    const int want = max(0, a.count - always);
+    if (want == 0) {
+      cut = __builtin_inf();
+      equal = 0;
+    } else if (held > want) {
+      // At least `want` scores are at or above lo, fewer above hi.
+      int64_t lo = order_of(least), hi = order_of(most) + 1;
+      for (int step = 0; static_cast<uint64_t>(hi) - static_cast<uint64_t>(lo) > 1; ++step) {
+        int64_t mid = (lo & hi) + ((lo ^ hi) >> 1);  // their mean, without overflow
+        if (step < 32) {
+          const double x = 0.5 * of_order(lo) + 0.5 * of_order(hi);
+          const int64_t k = order_of(x);
+          if (x == x && k > lo && k < hi) mid = k;
+        }
+        const double bar = of_order(mid);
+        int above = 0;
+        each([&](double x) {
+          if constexpr (N > 0) above += __popcll(__ballot(x >= bar));
+          else above += x >= bar;
+        });
+        if constexpr (N == 0) {
+#pragma unroll
+          for (int k = 1; k < kWave; k *= 2) above += __shfl_xor(above, k);
+        }
+        if (above >= want) lo = mid;
+        else hi = mid;
+        if (above == want) break;
+      }
+      cut = of_order(lo);
+      int above = 0;
+      each([&](double x) { above += x > cut; });
+#pragma unroll
+      for (int k = 1; k < kWave; k *= 2) above += __shfl_xor(above, k);
+      equal = want - above;
+    }
+  }
+
+  int written = 0, equals = 0;
+  for (int b0 = 0; b0 < blocks; b0 += kWave) {
+    const int b = b0 + lane;
+    bool take = false, same = false;
+    if (b < blocks) {
+      if (all || b < low || b >= high) {
+        take = there(b);
+      } else {
+        const double x = scores[b];
+        take = x > cut;
+        same = x == cut;
+      }
+    }
+    const uint64_t ties = __ballot(same), below = (uint64_t(1) << lane) - 1;
+    if (same) take = equals + __popcll(ties & below) < equal;
+    equals = min(equals + static_cast<int>(__popcll(ties)), std::numeric_limits<int>::max() / 2);
+    const uint64_t taken = __ballot(take);
+    const int to = written + __popcll(taken & below);
+    if (take && to < a.count) out[to] = b;
+    written += __popcll(taken);
+  }
+  for (int i = min(written, a.count) + lane; i < a.count; i += kWave) out[i] = -1;
+}
+
+// Workgroups of a launch, at most, for a call of many rows: work-items stay below 2^32.
+constexpr int64_t kSlice = int64_t(1) << 22;
+
+hipError_t launch_paged_means(const PagedMeansArgs& a, hipStream_t stream) {
+  MeansDev d{};
+  d.c = paged_dev(a.c);
+  d.means = a.means;
+  d.ms[0] = a.ms[0];
+  d.ms[1] = a.ms[1];
+  d.kv_heads = static_cast<int>(a.c.kv_heads);
+  d.head_dim = static_cast<int>(a.c.head_dim);
+  d.lanes = d.head_dim / 8;
+  d.rows = kWave / d.lanes;
+  d.by_kv_heads = make_fastdiv(d.kv_heads);
+  d.by_lanes = make_fastdiv(d.lanes);
+  const int64_t slice = std::max<int64_t>(1, kSlice / a.c.kv_heads) * kMeanTokens;
+  for (int64_t t = 0; t < a.c.tokens; t += slice) {
+    d.token0 = static_cast<int>(t);
+    const dim3 grid(static_cast<unsigned>(ceil_div(std::min(slice, a.c.tokens - t), kMeanTokens) * a.c.kv_heads)), block(256);
+    if (a.c.mx) {
+      AKO_LAUNCH((paged_means<float, true>), grid, block, 0, stream, d);
+    } else {
+      switch (a.dtype) {
+        case kF32: AKO_LAUNCH((paged_means<float, false>), grid, block, 0, stream, d); break;
+        case kF16: AKO_LAUNCH((paged_means<_Float16, false>), grid, block, 0, stream, d); break;
+        case kBF16: AKO_LAUNCH((paged_means<__bf16, false>), grid, block, 0, stream, d); break;
+        default: return hipErrorInvalidValue;
+      }
+    }
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return err;
+  }
+  return hipSuccess;
+}
+
+namespace {
+
+constexpr int kTileRows = 16;
+
+// Token rows whose scores are held at a time: 64 MiB of them, so that they stay in the last level cache.
+int64_t slice_rows(const PagedSelectArgs& a) {
+  const int64_t row = a.c.kv_heads * a.c.table_width * static_cast<int64_t>(sizeof(double));
+  const int64_t rows = std::max<int64_t>(1, (int64_t(1) << 26) / std::max<int64_t>(1, row) / kTileRows) * kTileRows;
+  return std::min(rows, a.c.tokens);
+}
+
+template <typename T>
+void launch_scores(const SelectDev& d, dim3 grid, hipStream_t stream) {
+  const dim3 block(256);
+  if (d.head_dim <= 64) AKO_LAUNCH((select_scores<T, 64>), grid, block, 0, stream, d);
+  else if (d.head_dim <= 128) AKO_LAUNCH((select_scores<T, 128>), grid, block, 0, stream, d);
+  else AKO_LAUNCH((select_scores<T, 256>), grid, block, 0, stream, d);
+}
+
+}  // namespace
+
+int64_t paged_select_workspace(const PagedSelectArgs& a) {
+  if (a.c.table_width <= a.count) return 0;  // every block is taken
+  return slice_rows(a) * a.c.kv_heads * a.c.table_width * static_cast<int64_t>(sizeof(double));
+}
+
+hipError_t launch_paged_select(const PagedSelectArgs& a, hipStream_t stream) {
+  SelectDev d{};
+  d.c = paged_dev(a.c);
+  d.q = a.q;
+  d.means = a.means;
+  for (int i = 0; i < 3; ++i) d.qs[i] = a.qs[i];
+  d.ms[0] = a.ms[0];
+  d.ms[1] = a.ms[1];
+  d.scores = static_cast<double*>(a.workspace);
+  d.out = a.out;
+  d.kv_heads = static_cast<int>(a.c.kv_heads);
+  d.group = static_cast<int>(a.q_heads / a.c.kv_heads);
+  d.head_dim = static_cast<int>(a.c.head_dim);
+  d.count = static_cast<int>(a.count);
+  d.first = static_cast<int>(std::min<int64_t>(a.first, a.count));
+  d.last = static_cast<int>(a.last);
+  d.width = a.c.num_pages > 0 ? static_cast<int>(a.c.table_width) : 0;
+  d.by_kv_heads = make_fastdiv(d.kv_heads);
+  // As many rows to a tile as a sequence has on average: rows of one sequence share its blocks' means.
+  const int64_t per_seq = ceil_div(a.c.tokens, std::max<int64_t>(1, a.c.n_seqs));
+  d.tile = 1;
+  while (d.tile < kTileRows && d.tile < per_seq) d.tile *= 2;
+  const bool scored = d.width > a.count;
+  const int64_t slice = scored ? slice_rows(a) : std::max<int64_t>(1, 4 * kSlice / a.c.kv_heads);
+  for (int64_t t = 0; t < a.c.tokens; t += slice) {
+    d.token0 = static_cast<int>(t);
+    d.end = static_cast<int>(std::min(t + slice, a.c.tokens));
+    const int64_t rows = d.end - d.token0, items = rows * a.c.kv_heads;
+    if (scored) {
+      const int64_t tiles = ceil_div(rows, d.tile), sets = ceil_div(d.width, 64);
+      // A workgroup's four wavefronts take 16 blocks each at a time; several times, where there are many.
+      const int64_t times = std::min<int64_t>(8, std::max<int64_t>(1, tiles * a.c.kv_heads * sets / 2048));
+      d.chunk = static_cast<int>(64 * times);
+      d.by_tiles = make_fastdiv(static_cast<unsigned>(tiles));
+      const dim3 grid(static_cast<unsigned>(tiles * a.c.kv_heads * ceil_div(d.width, d.chunk)));
+      switch (a.dtype) {
+        case kF32: launch_scores<float>(d, grid, stream); break;
+        case kF16: launch_scores<_Float16>(d, grid, stream); break;
+        case kBF16: launch_scores<__bf16>(d, grid, stream); break;
+        default: return hipErrorInvalidValue;
+      }
+      const hipError_t err = hipGetLastError();
+      if (err != hipSuccess) return err;
+    }
+    const dim3 grid(static_cast<unsigned>(ceil_div(items, 4))), block(256);
+    if (d.width <= 4 * kWave) AKO_LAUNCH((select_blocks<4>), grid, block, 0, stream, d);
+    else if (d.width <= 16 * kWave) AKO_LAUNCH((select_blocks<16>), grid, block, 0, stream, d);
+    else if (d.width <= 64 * kWave) AKO_LAUNCH((select_blocks<64>), grid, block, 0, stream, d);
+    else AKO_LAUNCH((select_blocks<0>), grid, block, 0, stream, d);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return err;
+  }
+  return hipSuccess;
+}
+
+}  // namespace ako

@@ -469,7 +469,7 @@ struct PagedArg {
     if (t && t->device() != k.device()) refuse(std::string(name) + " must be on the device of the pages");
   }
 
-  void check_rows(const char* name, const at::Tensor& x, int64_t heads) const {
+  void check_rows(const char* name, const at::Tensor& x, int64_t heads, bool any_type = false) const {
     if (x.dim() != (cu ? 3 : 4))
       refuse(std::string(name) + " must be (batch, seq, heads, head_dim), or (tokens, heads, head_dim) with cu_seqlens, got " +
              shape_str(x.sizes()));
@@ -479,7 +479,7 @@ struct PagedArg {
       refuse(std::string(name) + " has " + std::to_string(x.size(0)) + " sequences, the block table " + std::to_string(n()));
     if (dtype_code_or(x.scalar_type()) < 0)
       refuse(std::string(name) + " must be float32/float16/bfloat16, got " + dtype_str(x.scalar_type()));
-    if (!mx() && x.scalar_type() != k.scalar_type())
+    if (!mx() && x.scalar_type() != k.scalar_type() && !any_type)
       refuse(std::string(name) + " is " + dtype_str(x.scalar_type()) + ", the pages " + dtype_str(k.scalar_type()));
     if (x.device() != k.device()) refuse(std::string(name) + " must be on the device of the pages");
   }
@@ -600,6 +600,69 @@ std::pair<at::Tensor, at::Tensor> paged_read(const at::Tensor& k_pages, const at
           return ako_paged_read_fwd(&c, k.data_ptr(), v.data_ptr(), dtype_code_or(to), s);
         }), fn);
   return {k, v};
+}
+
+at::Tensor paged_means(const at::Tensor& k_pages, const at::Tensor& k_means, const at::Tensor& block_table,
+                       const at::Tensor& seq_lens, int64_t rows, const OptTensor& k_scales, const OptTensor& cu_seqlens) {
+  const char* fn = "paged_means_hip";
+  const int index = gpu_index(k_pages, fn);
+  const PagedArg p{k_pages, k_pages, block_table, seq_lens, get(k_scales), get(k_scales), get(cu_seqlens),
+                   std::string(fn) + ": "};
+  p.check_cache();
+  const int64_t want[3] = {k_pages.size(0), k_pages.size(1), k_pages.size(3)};
+  if (!k_means.sizes().equals(at::IntArrayRef(want, 3)) || k_means.scalar_type() != at::kFloat)
+    p.refuse("k_means must be a float32 tensor of shape " + shape_str(at::IntArrayRef(want, 3)) + ", got " +
+             shape_str(k_means.sizes()) + " " + dtype_str(k_means.scalar_type()));
+  if (k_means.stride(2) != 1) p.refuse("k_means must be contiguous in the last dimension");
+  p.same_device("k_means", &k_means);
+  if (rows < 0) p.refuse("rows must be at least 0, got " + std::to_string(rows));
+  const ako_paged_t c = p.c(p.cu ? rows : p.n() * rows);
+  check(on_device(index, [&](hipStream_t s) {
+          return ako_paged_means_fwd(&c, static_cast<float*>(k_means.data_ptr()), k_means.strides().data(),
+                                     std::max(0, dtype_code_or(k_pages.scalar_type())), s);
+        }), fn);
+  return k_means;
+}
+
+at::Tensor paged_select(const at::Tensor& q, const at::Tensor& k_means, const at::Tensor& block_table,
+                        const at::Tensor& seq_lens, int64_t page_size, int64_t count, int64_t first, int64_t last,
+                        const OptTensor& cu_seqlens) {
+  const char* fn = "paged_select_hip";
+  const std::string pre = std::string(fn) + ": ";
+  const int index = gpu_index(q, fn);
+  if (k_means.dim() != 3 || k_means.scalar_type() != at::kFloat)
+    value_error(pre + "k_means must be a float32 tensor (pages, kv_heads, head_dim), got " + shape_str(k_means.sizes()) + " " +
+                dtype_str(k_means.scalar_type()));
+  if (page_size < 1 || page_size > kMaxPositions)
+    value_error(pre + "page_size must be 1 to " + std::to_string(kMaxPositions) + ", got " + std::to_string(page_size));
+  // The means as if they were pages whose rows are all alike, for the checks of a cache.
+  const at::Tensor pages = k_means.unsqueeze(2).expand({-1, -1, page_size, -1});
+  const PagedArg p{pages, pages, block_table, seq_lens, nullptr, nullptr, get(cu_seqlens), pre};
+  p.check_cache();
+  p.check_rows("q", q, -1, true);
+  const int64_t heads = q.size(-2), kv_heads = k_means.size(1);
+  if (heads % kv_heads)
+    p.refuse(std::to_string(heads) + " query heads are no multiple of " + std::to_string(kv_heads) + " key heads");
+  if (first < 0 || last < 1 || count < first + last)
+    p.refuse("first must be at least 0, last at least 1 and count at least their sum, got " + std::to_string(first) + ", " +
+             std::to_string(last) + " and " + std::to_string(count));
+  const at::Tensor qv = head_view(q);
+  std::vector<int64_t> shape(q.sizes().begin(), q.sizes().end());
+  shape[shape.size() - 2] = kv_heads;
+  shape.back() = count;
+  at::Tensor out = at::empty(shape, q.options().dtype(at::kInt));
+  ako_paged_t c = p.c(row_count(q));
+  const int dt = c.page_dtype = dtype_code_or(q.scalar_type());
+  const int64_t need = ako_paged_select_workspace(&c, heads, count, dt);
+  at::Tensor space;
+  if (need > 0) space = at::empty({need}, q.options().dtype(at::kByte));
+  const RowStrides qs(qv);
+  check(on_device(index, [&](hipStream_t s) {
+          return ako_paged_select_fwd(&c, qv.data_ptr(), qs.s, heads, static_cast<const float*>(k_means.data_ptr()),
+                                      k_means.strides().data(), static_cast<int32_t*>(out.data_ptr()), count, first, last,
+                                      need > 0 ? space.data_ptr() : nullptr, need > 0 ? need : 0, dt, s);
+        }), fn);
+  return out;
 }
 
 at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
@@ -725,6 +788,10 @@ PYBIND11_MODULE(_ako_torch, m) {
         py::arg("cos"), py::arg("sin"), py::arg("eps") = 1e-6, py::arg("style") = "neox");
   m.def("paged_read", &paged_read, py::arg("k_pages"), py::arg("v_pages"), py::arg("block_table"), py::arg("seq_lens"),
         py::arg("rows"), py::arg("dtype"), py::arg("k_scales"), py::arg("v_scales"), py::arg("cu_seqlens"));
+  m.def("paged_means", &paged_means, py::arg("k_pages"), py::arg("k_means"), py::arg("block_table"), py::arg("seq_lens"),
+        py::arg("rows"), py::arg("k_scales"), py::arg("cu_seqlens"));
+  m.def("paged_select", &paged_select, py::arg("q"), py::arg("k_means"), py::arg("block_table"), py::arg("seq_lens"),
+        py::arg("page_size"), py::arg("count"), py::arg("first"), py::arg("last"), py::arg("cu_seqlens"));
   m.def("paged_attention", &paged_attention, py::arg("q"), py::arg("k_pages"), py::arg("v_pages"),
         py::arg("block_table"), py::arg("seq_lens"), py::arg("scale"), py::arg("window"), py::arg("sinks"),
         py::arg("k_scales"), py::arg("v_scales"), py::arg("cu_seqlens"));

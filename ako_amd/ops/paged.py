@@ -21,8 +21,12 @@ from __future__ import annotations
 import torch
 
 from ako_amd.ops._registry import hip_disabled
-from ako_amd.ops.paged_hip import paged_attention_hip, paged_read_hip, rope_qk_paged_hip
-from ako_amd.ops.paged_ref import new_pages, paged_attention_ref, paged_read_ref, rope_qk_paged_ref
+from ako_amd.ops.paged_hip import (
+    paged_attention_hip, paged_means_hip, paged_read_hip, paged_select_hip, rope_qk_paged_hip,
+)
+from ako_amd.ops.paged_ref import (
+    new_pages, paged_attention_ref, paged_means_ref, paged_read_ref, paged_select_ref, rope_qk_paged_ref,
+)
 
 
 def rope_qk_paged(
@@ -90,6 +94,53 @@ def paged_read(
                           v_scales=v_scales, cu_seqlens=cu_seqlens)
 
 
+def paged_means(
+    k_pages: torch.Tensor,
+    k_means: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    rows: int,
+    *,
+    k_scales: torch.Tensor | None = None,
+    cu_seqlens: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """The means of the keys of every page that a step's rows have filled, into ``k_means
+    (pages, kv_heads, head_dim)``, float32, which is returned.
+
+    To be called after the step's write; ``rows`` is as in ``paged_read``. Pages that the step has not
+    filled keep what stands there. ``paged_select`` reads the means of a sequence's full pages.
+    """
+    if k_pages.is_cuda and not hip_disabled():
+        return paged_means_hip(k_pages, k_means, block_table, seq_lens, rows, k_scales, cu_seqlens)
+    return paged_means_ref(k_pages, k_means, block_table, seq_lens, rows, k_scales=k_scales, cu_seqlens=cu_seqlens)
+
+
+def paged_select(
+    q: torch.Tensor,
+    k_means: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    page_size: int,
+    count: int,
+    *,
+    cu_seqlens: torch.Tensor | None = None,
+    first: int = 1,
+    last: int = 1,
+) -> torch.Tensor:
+    """The blocks (pages of a sequence, numbered from 0) that each row of q attends to, for each
+    key head: int32 ``(..., kv_heads, count)``, ascending, -1 behind the last.
+
+    A row may take the blocks up to its own. If they are more than ``count``, it takes the ``first``
+    first and the ``last`` last of them, and of the others those whose mean key has the largest product with
+    the sum of the queries that share the key head; of equal ones the lowest. Scores are formed in
+    64 bits, so the choice does not depend on how the work was divided. Blocks without a
+    page are not taken; padding rows take none.
+    """
+    if q.is_cuda and not hip_disabled():
+        return paged_select_hip(q, k_means, block_table, seq_lens, page_size, count, first, last, cu_seqlens)
+    return paged_select_ref(q, k_means, block_table, seq_lens, page_size, count, cu_seqlens=cu_seqlens, first=first, last=last)
+
+
 def paged_attention(
     q: torch.Tensor,
     k_pages: torch.Tensor,
@@ -122,4 +173,4 @@ def paged_attention(
                                cu_seqlens=cu_seqlens, scale=scale, window=window, sinks=sinks)
 
 
-__all__ = ["new_pages", "paged_attention", "paged_read", "rope_qk_paged"]
+__all__ = ["new_pages", "paged_attention", "paged_means", "paged_read", "paged_select", "rope_qk_paged"]

@@ -105,6 +105,54 @@ def paged_read_hip_ctypes(k_pages, v_pages, block_table, seq_lens, rows, dtype=N
     return k, v
 
 
+def paged_means_hip(k_pages, k_means, block_table, seq_lens, rows, k_scales=None, cu_seqlens=None) -> torch.Tensor:
+    """Means of the pages that the step's rows fill, in one launch."""
+    fast = _native.torch_binding()
+    run = paged_means_hip_ctypes if fast is None else fast.paged_means
+    return run(k_pages, k_means, block_table, seq_lens, rows, k_scales, cu_seqlens)
+
+
+def paged_means_hip_ctypes(k_pages, k_means, block_table, seq_lens, rows, k_scales=None, cu_seqlens=None) -> torch.Tensor:
+    fn = "paged_means_hip"
+    index = gpu_index(k_pages, fn)
+    ref.refuse(fn, ref.cache_error(k_pages, k_pages, k_scales, k_scales, block_table, seq_lens, cu_seqlens)
+               or ref.means_error(k_means, k_pages) or ref.count_error(rows))
+    tokens = rows if cu_seqlens is not None else block_table.shape[0] * rows
+    cache = _cache(k_pages, k_pages, k_scales, k_scales, block_table, seq_lens, cu_seqlens, tokens)
+    status = call(index, lib().ako_paged_means_fwd, ctypes.addressof(cache), k_means.data_ptr(),
+                  _I64x3(*k_means.stride()[:2], 0), DT.get(k_pages.dtype, 0), raw_stream(index))
+    if status:
+        _native.check(status, fn)
+    return k_means
+
+
+def paged_select_hip(q, k_means, block_table, seq_lens, page_size, count, first=1, last=1, cu_seqlens=None) -> torch.Tensor:
+    """The blocks that each row and key head attends to."""
+    fast = _native.torch_binding()
+    run = paged_select_hip_ctypes if fast is None else fast.paged_select
+    return run(q, k_means, block_table, seq_lens, page_size, count, first, last, cu_seqlens)
+
+
+def paged_select_hip_ctypes(q, k_means, block_table, seq_lens, page_size, count, first=1, last=1, cu_seqlens=None) -> torch.Tensor:
+    fn = "paged_select_hip"
+    index = gpu_index(q, fn)
+    ref.refuse(fn, ref.select_error(q, k_means, block_table, seq_lens, page_size, count, first, last, cu_seqlens))
+    qv = _head_view(q)
+    out = torch.empty(*q.shape[:-2], k_means.shape[1], count, dtype=torch.int32, device=q.device)
+    pages = ref.blocks_as_pages(k_means, page_size)
+    cache = _cache(pages, pages, None, None, block_table, seq_lens, cu_seqlens, _tokens(q))
+    cache.page_dtype = DT[q.dtype]
+    at, heads, dt = ctypes.addressof(cache), q.shape[-2], DT[q.dtype]
+    need = lib().ako_paged_select_workspace(at, heads, count, dt)
+    space = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
+    status = call(index, lib().ako_paged_select_fwd, at, qv.data_ptr(), _row_strides(qv), heads, k_means.data_ptr(),
+                  _I64x3(*k_means.stride()[:2], 0), out.data_ptr(), count, first, last,
+                  space.data_ptr() if space is not None else None, max(need, 0), dt, raw_stream(index))
+    if status:
+        _native.check(status, fn)
+    return out
+
+
 def paged_attention_hip(q, k_pages, v_pages, block_table, seq_lens, scale=None, window=None, sinks=0,
                         k_scales=None, v_scales=None, cu_seqlens=None) -> torch.Tensor:
     """Attention of a step's rows over their sequences' pages."""

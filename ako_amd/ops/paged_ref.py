@@ -96,8 +96,9 @@ def cache_error(k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, cu_
     return None
 
 
-def rows_error(name, x, heads, k_pages, block_table, cu_seqlens) -> str | None:
-    """The first thing wrong with a step's rows ``x``, or ``None``; ``heads`` -1 takes any number."""
+def rows_error(name, x, heads, k_pages, block_table, cu_seqlens, *, any_type: bool = False) -> str | None:
+    """The first thing wrong with a step's rows ``x``, or ``None``; ``heads`` -1 takes any number,
+    ``any_type`` rows of another type than the pages'."""
     head_dim = k_pages.shape[3]
     if x.dim() != (4 if cu_seqlens is None else 3):
         return (f"{name} must be (batch, seq, heads, head_dim), or (tokens, heads, head_dim) with cu_seqlens, "
@@ -108,7 +109,7 @@ def rows_error(name, x, heads, k_pages, block_table, cu_seqlens) -> str | None:
         return f"{name} has {x.shape[0]} sequences, the block table {block_table.shape[0]}"
     if x.dtype not in ROW_DTYPES:
         return f"{name} must be float32/float16/bfloat16, got {x.dtype}"
-    if k_pages.dtype not in (x.dtype, E4M3):
+    if k_pages.dtype not in (x.dtype, E4M3) and not any_type:
         return f"{name} is {x.dtype}, the pages {k_pages.dtype}"
     if not _on(x, k_pages):
         return f"{name} must be on the device of the pages"
@@ -145,6 +146,39 @@ def norm_error(q_weight, k_weight, eps, k_pages) -> str | None:
     if (q_weight is None) != (k_weight is None):
         return "q_weight and k_weight must both be given or both be None"
     return None if q_weight is None else weights_error(q_weight, k_weight, eps, k_pages.shape[3], k_pages)
+
+
+def means_error(k_means, k_pages) -> str | None:
+    want = (k_pages.shape[0], k_pages.shape[1], k_pages.shape[3])
+    if tuple(k_means.shape) != want or k_means.dtype != torch.float32:
+        return f"k_means must be a float32 tensor of shape {want}, got {tuple(k_means.shape)} {k_means.dtype}"
+    if k_means.stride(2) != 1:
+        return "k_means must be contiguous in the last dimension"
+    if not _on(k_means, k_pages):
+        return "k_means must be on the device of the pages"
+    return None
+
+
+def blocks_as_pages(k_means: torch.Tensor, page_size: int) -> torch.Tensor:
+    """Means as if they were pages whose rows are all alike, for the checks of a cache."""
+    return k_means.unsqueeze(2).expand(-1, -1, page_size, -1)
+
+
+def select_error(q, k_means, block_table, seq_lens, page_size, count, first, last, cu_seqlens) -> str | None:
+    if k_means.dim() != 3 or k_means.dtype != torch.float32:
+        return f"k_means must be a float32 tensor (pages, kv_heads, head_dim), got {tuple(k_means.shape)} {k_means.dtype}"
+    if not 1 <= page_size <= MAX_POSITIONS:
+        return f"page_size must be 1 to {MAX_POSITIONS}, got {page_size}"
+    pages = blocks_as_pages(k_means, page_size)
+    wrong = (cache_error(pages, pages, None, None, block_table, seq_lens, cu_seqlens)
+             or rows_error("q", q, -1, pages, block_table, cu_seqlens, any_type=True))
+    if wrong:
+        return wrong
+    if q.shape[-2] % k_means.shape[1]:
+        return f"{q.shape[-2]} query heads are no multiple of {k_means.shape[1]} key heads"
+    if first < 0 or last < 1 or count < first + last:
+        return f"first must be at least 0, last at least 1 and count at least their sum, got {first}, {last} and {count}"
+    return None
 
 
 def refuse(fn_name: str, *errors: str | None) -> None:
@@ -275,6 +309,57 @@ def read_error(k_pages, rows, dtype) -> str | None:
     if dtype is not None and k_pages.dtype not in (dtype, E4M3):
         return f"dtype is {dtype}, the pages {k_pages.dtype}"
     return None
+
+
+def paged_means_ref(k_pages, k_means, block_table, seq_lens, rows, *, k_scales=None, cu_seqlens=None) -> torch.Tensor:
+    refuse("paged_means", cache_error(k_pages, k_pages, k_scales, k_scales, block_table, seq_lens, cu_seqlens)
+           or means_error(k_means, k_pages) or count_error(rows))
+    num_pages, _, page_size, _ = k_pages.shape
+    tokens = rows if cu_seqlens is not None else block_table.shape[0] * rows
+    s, pos = row_places(tokens, seq_lens, cu_seqlens)
+    page, slot = row_slots(s, pos, block_table, page_size, num_pages)
+    full = page[(page >= 0) & (slot == page_size - 1)]
+    x = _bytes(k_pages)[full].view(k_pages.dtype)
+    x = x.float() if k_scales is None else dequantize_rows(x, k_scales[full], torch.float32)
+    k_means[full] = x.sum(2) / page_size
+    return k_means
+
+
+def count_error(rows) -> str | None:
+    return f"rows must be at least 0, got {rows}" if rows < 0 else None
+
+
+def paged_select_ref(q, k_means, block_table, seq_lens, page_size, count, *, cu_seqlens=None, first=1, last=1) -> torch.Tensor:
+    """Scores in 64 bits; of equal ones the lowest block."""
+    refuse("paged_select", select_error(q, k_means, block_table, seq_lens, page_size, count, first, last, cu_seqlens))
+    num_pages, kv_heads, head_dim = k_means.shape
+    n, width = block_table.shape
+    width = width if num_pages else 0
+    q2 = q.flatten(0, -3)
+    tokens = q2.shape[0]
+    out = torch.full((tokens, kv_heads, count), -1, dtype=torch.int32, device=q.device)
+    s, pos = row_places(tokens, seq_lens, cu_seqlens)
+    if tokens and width and n:
+        sums = q2.double().unflatten(1, (kv_heads, -1)).sum(2)
+        block = torch.arange(width, device=q.device)
+        for i in range(n):
+            rows = torch.nonzero((s == i) & (pos >= 0)).flatten()
+            if not rows.numel():
+                continue
+            page = block_table[i].long()
+            there = (page >= 0) & (page < num_pages)
+            mean = k_means[page.where(there, 0)].double().permute(1, 2, 0).contiguous()
+            score = torch.matmul(sums[rows].transpose(0, 1).contiguous(), mean).transpose(0, 1).nan_to_num(-math.inf, math.inf, -math.inf)
+            own = (pos[rows] // page_size)[:, None, None]
+            seen = (block <= own) & there
+            always = (block < first) | (block > own - last)
+            # 0: always taken, 1: by score, 2: not there; then by score, then by number.
+            order = torch.sort(score, dim=-1, descending=True, stable=True).indices
+            rank = torch.where(seen, torch.where(always, 0, 1), 2).expand_as(score)
+            order = order.gather(-1, torch.sort(rank.gather(-1, order), dim=-1, stable=True).indices)[..., :count]
+            order = torch.where(rank.gather(-1, order) < 2, order, width).sort(-1).values
+            out[rows, :, : order.shape[-1]] = torch.where(order < width, order, -1).int()
+    return out.view(*q.shape[:-2], kv_heads, count)
 
 
 def paged_attention_ref(q, k_pages, v_pages, block_table, seq_lens, *, k_scales=None, v_scales=None,

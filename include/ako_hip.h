@@ -329,6 +329,39 @@ int ako_paged_attention_fwd(const void* q, const int64_t* q_strides, void* out,
 int64_t ako_paged_attention_workspace(const ako_paged_t* cache, int64_t q_heads, int dtype);
 
 /*
+ * The mean of the keys of every page that the step's rows fill: for a row at the last
+ * slot of its page, means[page][head] = sum over the page's slots of the keys as stored / page_size
+ * (fp32; e4m3 keys times their scales). means is [num_pages, kv_heads, head_dim] floats,
+ * means_strides those of page and head; no other page's means are touched. The cache's
+ * v_pages, v_scales and their strides are not used; the pages are of dtype, or e4m3
+ * (dtype is then not used).
+ */
+int ako_paged_means_fwd(const ako_paged_t* cache, float* means, const int64_t* means_strides,
+                        int dtype, void* stream);
+
+/*
+ * For each row and key head the blocks (pages) to attend to, into
+ * blocks[row][head][0 .. count-1], ascending, -1 behind the last. A row at position p may take
+ * the blocks 0 .. p / page_size whose page is there; all of them, if they are no more
+ * than count, else count of them: the first `first`, the last `last` up to its own,
+ * and of the others those with the largest scores
+ *   sum over the heads h that read key head `head` of q[row][h] . means[page][head],
+ * of equal ones the lowest blocks (64-bit sums; NaN counts as -infinity). first >= 0,
+ * last >= 1, count >= first + last. Rows that are padding get -1 only. Of the cache, the pages, scales and their
+ * strides are not used and page_dtype is dtype, that of q. workspace
+ * holds ako_paged_select_workspace bytes, 16-byte aligned, that nothing else uses until the
+ * work on `stream` is done.
+ */
+int ako_paged_select_fwd(const ako_paged_t* cache, const void* q, const int64_t* q_strides,
+                         int64_t q_heads, const float* means, const int64_t* means_strides,
+                         int32_t* blocks, int64_t count, int64_t first, int64_t last,
+                         void* workspace, int64_t workspace_bytes, int dtype, void* stream);
+
+/* Bytes of workspace for such a call (0: none); -1 for arguments it refuses. */
+int64_t ako_paged_select_workspace(const ako_paged_t* cache, int64_t q_heads, int64_t count,
+                                   int dtype);
+
+/*
  * A token for each of `rows` rows of `vocab` logits (1 to 2^22), from one uniform number each.
  * With w_i = e^((x_i - max x) / temperature), in descending order of the logits (of
  * equal ones the lowest index first) the first top_k tokens stay (0 or less: all), of

@@ -30,7 +30,7 @@ INCLUDE = REPO_DIR / "include"
 LIB_DIR = PACKAGE_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libako_hip.so"
 OBJ_DIR = LIB_DIR / "_build"
-SOURCES = ("abi.hip", "paged_attention.hip", "paged_kv.hip", "paged_select.hip", "qk_norm.hip", "rmsnorm.hip",
+SOURCES = ("abi.hip", "paged_attention.hip", "paged_blocks.hip", "paged_kv.hip", "paged_select.hip", "qk_norm.hip", "rmsnorm.hip",
            "rope.hip", "sample.hip", "swiglu.hip")
 ARCH = "gfx950"
 

@@ -105,6 +105,10 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         _int, [_ptr, _ptr, _ptr, _ptr, _i64, _f32, _i64, _i64, _ptr, _i64, _int, _ptr],
     ),
     "ako_paged_attention_workspace": (_i64, [_ptr, _i64, _int]),
+    "ako_paged_attention_blocks_fwd": (
+        _int, [_ptr, _ptr, _ptr, _ptr, _i64, _f32, _ptr, _i64, _ptr, _i64, _int, _ptr],
+    ),
+    "ako_paged_attention_blocks_workspace": (_i64, [_ptr, _i64, _i64, _int]),
     "ako_paged_means_fwd": (_int, [_ptr, _ptr, _ptr, _int, _ptr]),
     "ako_paged_select_fwd": (
         _int, [_ptr, _ptr, _ptr, _i64, _ptr, _ptr, _ptr, _i64, _i64, _i64, _ptr, _i64, _int, _ptr],

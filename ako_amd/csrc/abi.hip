@@ -966,10 +966,13 @@ int attention_common(const char* fn, const ako_paged_t* cache, int64_t q_heads, 
 }  // namespace
 }  // extern "C++"
 
-int ako_paged_attention_fwd(const void* q, const int64_t* q_strides, void* out, const ako_paged_t* cache, int64_t q_heads,
-                            float scale, int64_t window, int64_t sinks, void* workspace, int64_t workspace_bytes, int dtype,
-                            void* stream) {
-  const char* fn = "ako_paged_attention_fwd";
+extern "C++" {
+namespace {
+
+// `blocks`: those listed for each row and key head, `count` of them; 0: all.
+int attend(const char* fn, const void* q, const int64_t* q_strides, void* out, const ako_paged_t* cache, int64_t q_heads,
+           float scale, int64_t window, int64_t sinks, const int32_t* blocks, int64_t count, void* workspace,
+           int64_t workspace_bytes, int dtype, void* stream) {
   ako::PagedAttentionArgs a{};
   bool empty = false;
   if (const int rc = attention_common(fn, cache, q_heads, dtype, &a, &empty)) return rc;
@@ -979,8 +982,11 @@ int ako_paged_attention_fwd(const void* q, const int64_t* q_strides, void* out, 
   if (!q || !out || !q_strides) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: null pointer argument", fn);
   if (q_strides[0] < 0 || q_strides[1] < 0 || q_strides[2] < 0)
     return fail(AKO_ERR_INVALID_ARGUMENT, "%s: negative stride", fn);
+  if (count > 0 && !blocks) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: null blocks", fn);
   a.window = window;
   a.sinks = sinks;
+  a.blocks = blocks;
+  a.block_count = count;
   const int64_t need = ako::paged_attention_workspace(a);
   if (workspace_bytes < need || (need > 0 && (!workspace || !aligned(workspace, 16))))
     return fail(AKO_ERR_INVALID_ARGUMENT, "%s: needs a 16-byte aligned workspace of %lld bytes, got %lld", fn,
@@ -990,11 +996,12 @@ int ako_paged_attention_fwd(const void* q, const int64_t* q_strides, void* out, 
   const Span qi = span_4d(q, cache->cu_seqlens ? 1 : cache->n_seqs, per, q_heads, d, q_strides, ako::dtype_bytes(dtype));
   const Span o = span_2d(out, 1, cache->tokens * q_heads * d, 0, ako::dtype_bytes(dtype));
   const Span w = span_bytes(workspace, need);
+  const Span b = span_bytes(blocks, static_cast<__int128>(cache->tokens) * cache->kv_heads * count * 4);
   const PagedSpans held(cache, dtype);
-  if (!qi.ok || !o.ok || !w.ok || !held.ok)
+  if (!qi.ok || !o.ok || !w.ok || !b.ok || !held.ok)
     return fail(AKO_ERR_INVALID_ARGUMENT, "%s: sizes and strides overflow the address space", fn);
-  if (overlap(o, qi) || held.meets(o)) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: out overlaps an input", fn);
-  if (overlap(w, qi) || overlap(w, o) || held.meets(w))
+  if (overlap(o, qi) || held.meets(o) || (count > 0 && overlap(o, b))) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: out overlaps an input", fn);
+  if (overlap(w, qi) || overlap(w, o) || held.meets(w) || (count > 0 && overlap(w, b)))
     return fail(AKO_ERR_INVALID_ARGUMENT, "%s: the workspace overlaps another buffer", fn);
   a.q = q;
   a.out = out;
@@ -1002,6 +1009,37 @@ int ako_paged_attention_fwd(const void* q, const int64_t* q_strides, void* out, 
   a.scale = scale;
   a.workspace = workspace;
   return hip_status(ako::launch_paged_attention(a, static_cast<hipStream_t>(stream)), fn);
+}
+
+}  // namespace
+}  // extern "C++"
+
+int ako_paged_attention_fwd(const void* q, const int64_t* q_strides, void* out, const ako_paged_t* cache, int64_t q_heads,
+                            float scale, int64_t window, int64_t sinks, void* workspace, int64_t workspace_bytes, int dtype,
+                            void* stream) {
+  return attend("ako_paged_attention_fwd", q, q_strides, out, cache, q_heads, scale, window, sinks, nullptr, 0, workspace,
+                workspace_bytes, dtype, stream);
+}
+
+int ako_paged_attention_blocks_fwd(const void* q, const int64_t* q_strides, void* out, const ako_paged_t* cache,
+                                   int64_t q_heads, float scale, const int32_t* blocks, int64_t count, void* workspace,
+                                   int64_t workspace_bytes, int dtype, void* stream) {
+  const char* fn = "ako_paged_attention_blocks_fwd";
+  if (count < 1 || count > kMaxInt / 2) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: count must be 1 to 2^30", fn);
+  return attend(fn, q, q_strides, out, cache, q_heads, scale, 0, 0, blocks, count, workspace, workspace_bytes, dtype, stream);
+}
+
+int64_t ako_paged_attention_blocks_workspace(const ako_paged_t* cache, int64_t q_heads, int64_t count, int dtype) {
+  const char* fn = "ako_paged_attention_blocks_workspace";
+  ako::PagedAttentionArgs a{};
+  bool empty = false;
+  if (count < 1 || count > kMaxInt / 2) {
+    fail(AKO_ERR_INVALID_ARGUMENT, "%s: count must be 1 to 2^30", fn);
+    return -1;
+  }
+  if (attention_common(fn, cache, q_heads, dtype, &a, &empty)) return -1;
+  a.block_count = count;
+  return empty ? 0 : ako::paged_attention_workspace(a);
 }
 
 int64_t ako_paged_attention_workspace(const ako_paged_t* cache, int64_t q_heads, int dtype) {

@@ -235,11 +235,17 @@ struct PagedAttentionArgs {
   float scale;
   int dtype;
   void* workspace;  // paged_attention_workspace bytes
+  // Listed blocks only: [tokens, kv_heads, block_count]; 0: all.
+  const int* blocks;
+  int64_t block_count;
   // The tuning keys, read once for the call: the workspace is sized and used by the same values.
   int tuned_items, tuned_min_keys, tuned_kernel;
 };
 int64_t paged_attention_workspace(const PagedAttentionArgs& a);
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t stream);
+// The same for calls with listed blocks.
+int64_t paged_blocks_workspace(const PagedAttentionArgs& a);
+hipError_t launch_paged_blocks(const PagedAttentionArgs& a, hipStream_t stream);
 
 struct PagedMeansArgs {
   PagedArgs c;  // keys only

@@ -668,7 +668,7 @@ at::Tensor paged_select(const at::Tensor& q, const at::Tensor& k_means, const at
 at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
                            const at::Tensor& block_table, const at::Tensor& seq_lens, const c10::optional<double>& scale_in,
                            const c10::optional<int64_t>& window, int64_t sinks, const OptTensor& k_scales,
-                           const OptTensor& v_scales, const OptTensor& cu_seqlens) {
+                           const OptTensor& v_scales, const OptTensor& cu_seqlens, const OptTensor& blocks_in) {
   const char* fn = "paged_attention_hip";
   const int index = gpu_index(q, fn);
   const PagedArg p{k_pages, v_pages, block_table, seq_lens, get(k_scales), get(v_scales), get(cu_seqlens),
@@ -683,15 +683,32 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const
   if ((window.has_value() && *window < 1) || sinks < 0)
     p.refuse("window must be at least 1 (or None) and sinks at least 0, got " +
              (window.has_value() ? std::to_string(*window) : std::string("None")) + " and " + std::to_string(sinks));
+  at::Tensor blocks;
+  if (const at::Tensor* b = get(blocks_in)) {
+    if (window.has_value() || sinks != 0) p.refuse("blocks leave no room for a window or sinks");
+    std::vector<int64_t> want(q.sizes().begin(), q.sizes().end() - 1);
+    want.back() = k_pages.size(1);
+    if (b->dim() != q.dim() || !b->sizes().slice(0, q.dim() - 1).equals(want) || b->scalar_type() != at::kInt || b->size(-1) < 1)
+      p.refuse("blocks must be an int32 tensor of shape " + shape_str(want) + " and at least one number for each, got " +
+               shape_str(b->sizes()) + " " + dtype_str(b->scalar_type()));
+    p.same_device("blocks", b);
+    blocks = b->contiguous();
+  }
   const at::Tensor qv = head_view(q);
   at::Tensor out = at::empty(q.sizes(), q.options());
   const ako_paged_t c = p.c(row_count(q));
   const int dt = dtype_code_or(q.scalar_type());
-  const int64_t need = ako_paged_attention_workspace(&c, heads, dt);
+  const int64_t count = blocks.defined() ? blocks.size(-1) : 0;
+  const int64_t need = count > 0 ? ako_paged_attention_blocks_workspace(&c, heads, count, dt)
+                                 : ako_paged_attention_workspace(&c, heads, dt);
   at::Tensor space;
   if (need > 0) space = at::empty({need}, q.options().dtype(at::kByte));
   const RowStrides qs(qv);
   check(on_device(index, [&](hipStream_t s) {
+          if (count > 0)
+            return ako_paged_attention_blocks_fwd(qv.data_ptr(), qs.s, out.data_ptr(), &c, heads, static_cast<float>(scale),
+                                                  static_cast<const int32_t*>(blocks.data_ptr()), count,
+                                                  need > 0 ? space.data_ptr() : nullptr, need > 0 ? need : 0, dt, s);
           return ako_paged_attention_fwd(qv.data_ptr(), qs.s, out.data_ptr(), &c, heads, static_cast<float>(scale),
                                          window.value_or(0), sinks, need > 0 ? space.data_ptr() : nullptr,
                                          need > 0 ? need : 0, dt, s);
@@ -794,7 +811,7 @@ PYBIND11_MODULE(_ako_torch, m) {
         py::arg("page_size"), py::arg("count"), py::arg("first"), py::arg("last"), py::arg("cu_seqlens"));
   m.def("paged_attention", &paged_attention, py::arg("q"), py::arg("k_pages"), py::arg("v_pages"),
         py::arg("block_table"), py::arg("seq_lens"), py::arg("scale"), py::arg("window"), py::arg("sinks"),
-        py::arg("k_scales"), py::arg("v_scales"), py::arg("cu_seqlens"));
+        py::arg("k_scales"), py::arg("v_scales"), py::arg("cu_seqlens"), py::arg("blocks") = py::none());
   m.def("sample", &sample, py::arg("logits"), py::arg("uniform"), py::arg("temperature") = 1.0, py::arg("top_k") = 0,
         py::arg("top_p") = 1.0, py::arg("min_p") = 0.0);
   m.def("current_stream", &current_stream);

@@ -154,12 +154,16 @@ def paged_attention(
     scale: float | None = None,
     window: int | None = None,
     sinks: int = 0,
+    blocks: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """Attention of a step's tokens over what their sequences hold.
 
     Head ``h`` of q reads head ``h // (heads // kv_heads)`` of the cache. A row at
     position ``p`` sees the positions ``j <= p``; with ``window``, of those only
-    ``j > p - window`` and the first ``sinks``. ``scale`` is ``head_dim ** -0.5``
+    ``j > p - window`` and the first ``sinks``. With ``blocks``, int32 ``(..., kv_heads, count)`` as
+    ``paged_select`` gives it, a row sees of the positions ``j <= p`` those whose block ``j // page_size`` is
+    listed for its token and key head: a set, in any order; a number below 0 or past the table
+    names nothing. ``scale`` is ``head_dim ** -0.5``
     unless given. Rows that see nothing (padding) are zero, and what a row does
     not see has no influence on it, whatever is stored there. A row that sees keys, but
     whose scores are all -infinity, is NaN, as their softmax is; an infinity or NaN among
@@ -168,9 +172,9 @@ def paged_attention(
     """
     if q.is_cuda and not hip_disabled():
         return paged_attention_hip(q, k_pages, v_pages, block_table, seq_lens, scale, window, sinks,
-                                   k_scales, v_scales, cu_seqlens)
+                                   k_scales, v_scales, cu_seqlens, blocks)
     return paged_attention_ref(q, k_pages, v_pages, block_table, seq_lens, k_scales=k_scales, v_scales=v_scales,
-                               cu_seqlens=cu_seqlens, scale=scale, window=window, sinks=sinks)
+                               cu_seqlens=cu_seqlens, scale=scale, window=window, sinks=sinks, blocks=blocks)
 
 
 __all__ = ["new_pages", "paged_attention", "paged_means", "paged_read", "paged_select", "rope_qk_paged"]

@@ -154,33 +154,38 @@ def paged_select_hip_ctypes(q, k_means, block_table, seq_lens, page_size, count,
 
 
 def paged_attention_hip(q, k_pages, v_pages, block_table, seq_lens, scale=None, window=None, sinks=0,
-                        k_scales=None, v_scales=None, cu_seqlens=None) -> torch.Tensor:
-    """Attention of a step's rows over their sequences' pages."""
+                        k_scales=None, v_scales=None, cu_seqlens=None, blocks=None) -> torch.Tensor:
+    """Attention of a step's rows over their sequences' pages, or the listed ones of them."""
     fast = _native.torch_binding()
-    if fast is not None:
-        return fast.paged_attention(q, k_pages, v_pages, block_table, seq_lens, scale, window, sinks,
-                                    k_scales, v_scales, cu_seqlens)
-    return paged_attention_hip_ctypes(q, k_pages, v_pages, block_table, seq_lens, scale, window, sinks,
-                                      k_scales, v_scales, cu_seqlens)
+    run = paged_attention_hip_ctypes if fast is None else fast.paged_attention
+    return run(q, k_pages, v_pages, block_table, seq_lens, scale, window, sinks, k_scales, v_scales, cu_seqlens, blocks)
 
 
 def paged_attention_hip_ctypes(q, k_pages, v_pages, block_table, seq_lens, scale=None, window=None, sinks=0,
-                               k_scales=None, v_scales=None, cu_seqlens=None) -> torch.Tensor:
+                               k_scales=None, v_scales=None, cu_seqlens=None, blocks=None) -> torch.Tensor:
     fn = "paged_attention_hip"
     index = gpu_index(q, fn)
     ref.refuse(fn, ref.cache_error(k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, cu_seqlens)
                or ref.rows_error("q", q, -1, k_pages, block_table, cu_seqlens))
     scale = k_pages.shape[3] ** -0.5 if scale is None else scale
-    ref.refuse(fn, ref.attention_error(q, k_pages, scale, window, sinks))
+    ref.refuse(fn, ref.attention_error(q, k_pages, scale, window, sinks)
+               or ref.blocks_error(q, k_pages, blocks, window, sinks))
     qv = _head_view(q)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     cache = _cache(k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, cu_seqlens, _tokens(q))
     at, heads, dt = ctypes.addressof(cache), q.shape[-2], DT[q.dtype]
-    need = lib().ako_paged_attention_workspace(at, heads, dt)
+    if blocks is None:
+        need = lib().ako_paged_attention_workspace(at, heads, dt)
+    else:
+        blocks = blocks.contiguous()
+        need = lib().ako_paged_attention_blocks_workspace(at, heads, blocks.shape[-1], dt)
     space = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
-    status = call(index, lib().ako_paged_attention_fwd, qv.data_ptr(), _row_strides(qv), out.data_ptr(), at, heads,
-                  scale, window or 0, sinks, space.data_ptr() if space is not None else None, max(need, 0), dt,
-                  raw_stream(index))
+    work = (space.data_ptr() if space is not None else None, max(need, 0), dt, raw_stream(index))
+    step = (qv.data_ptr(), _row_strides(qv), out.data_ptr(), at, heads, scale)
+    if blocks is None:
+        status = call(index, lib().ako_paged_attention_fwd, *step, window or 0, sinks, *work)
+    else:
+        status = call(index, lib().ako_paged_attention_blocks_fwd, *step, blocks.data_ptr(), blocks.shape[-1], *work)
     if status:
         _native.check(status, fn)
     return out

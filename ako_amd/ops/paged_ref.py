@@ -126,6 +126,19 @@ def attention_error(q, k_pages, scale, window, sinks) -> str | None:
     return None
 
 
+def blocks_error(q, k_pages, blocks, window, sinks) -> str | None:
+    if blocks is None:
+        return None
+    if window is not None or sinks:
+        return "blocks leave no room for a window or sinks"
+    want = (*q.shape[:-2], k_pages.shape[1])
+    if blocks.dim() != len(want) + 1 or tuple(blocks.shape[:-1]) != want or blocks.dtype != torch.int32 or blocks.shape[-1] < 1:
+        return f"blocks must be an int32 tensor of shape {want} and at least one number for each, got {tuple(blocks.shape)} {blocks.dtype}"
+    if not _on(blocks, k_pages):
+        return "blocks must be on the device of the pages"
+    return None
+
+
 def write_error(q, k, v, cos, sin, k_pages, block_table, style, cu_seqlens) -> str | None:
     if style not in ROPE_STYLES:
         return f"Unknown RoPE style '{style}', expected one of {ROPE_STYLES}"
@@ -363,12 +376,12 @@ def paged_select_ref(q, k_means, block_table, seq_lens, page_size, count, *, cu_
 
 
 def paged_attention_ref(q, k_pages, v_pages, block_table, seq_lens, *, k_scales=None, v_scales=None,
-                        cu_seqlens=None, scale=None, window=None, sinks=0) -> torch.Tensor:
+                        cu_seqlens=None, scale=None, window=None, sinks=0, blocks=None) -> torch.Tensor:
     """Sequence by sequence, in 32 bits (64 for 64-bit arithmetic checks is the tests' own)."""
     refuse("paged_attention", cache_error(k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, cu_seqlens)
            or rows_error("q", q, -1, k_pages, block_table, cu_seqlens))
     scale = k_pages.shape[3] ** -0.5 if scale is None else scale
-    refuse("paged_attention", attention_error(q, k_pages, scale, window, sinks))
+    refuse("paged_attention", attention_error(q, k_pages, scale, window, sinks) or blocks_error(q, k_pages, blocks, window, sinks))
     num_pages, kv_heads, page_size, head_dim = k_pages.shape
     heads = q.shape[-2]
     q2 = q.flatten(0, -3)
@@ -381,19 +394,28 @@ def paged_attention_ref(q, k_pages, v_pages, block_table, seq_lens, *, k_scales=
         key = torch.arange(min(int(pos[rows].max()) + 1, block_table.shape[1] * page_size), device=q.device)
         page, slot = row_slots(torch.full_like(key, i), key, block_table, page_size, num_pages)
         key, page, slot = key[page >= 0], page[page >= 0], slot[page >= 0]
+        if not key.numel():
+            continue
         kk = _rows(k_pages, k_scales, page, slot, q.dtype).float().repeat_interleave(heads // kv_heads, 1)
         vv = _rows(v_pages, v_scales, page, slot, q.dtype).float().repeat_interleave(heads // kv_heads, 1)
         at = pos[rows][:, None]
         seen = key <= at
         if window is not None:
             seen &= (key > at - window) | (key < sinks)
+        seen = seen[None]
+        if blocks is not None:  # a set of blocks for each key head
+            width = block_table.shape[1]
+            listed = blocks.flatten(0, -3)[rows].transpose(0, 1).long()
+            taken = torch.zeros(*listed.shape[:2], width + 1, dtype=torch.bool, device=q.device)
+            taken.scatter_(-1, listed.where((listed >= 0) & (listed < width), width), True)
+            seen = seen & taken[..., key // page_size]
+        seen = seen.expand(kv_heads, -1, -1).repeat_interleave(heads // kv_heads, 0)
         score = torch.einsum("thd,jhd->htj", q2[rows].float(), kk) * scale
         score = score.masked_fill(~seen, float("-inf"))
-        some = seen.any(-1)
-        p = torch.softmax(score[:, some], -1)
+        p = torch.softmax(score, -1)
         if bool(vv.isfinite().all()):
-            o = torch.einsum("htj,jhd->thd", p, vv)
+            o = torch.einsum("htj,jhd->thd", p.masked_fill(~seen, 0.0), vv)
         else:  # a value that a row does not see must not reach it, not even as 0 * inf
-            o = torch.where(seen[some][None, :, :, None], p[..., None] * vv.transpose(0, 1)[:, None], 0.0).sum(2).transpose(0, 1)
-        out[rows[some]] = o.to(q.dtype)
+            o = torch.where(seen[..., None], p[..., None] * vv.transpose(0, 1)[:, None], 0.0).sum(2).transpose(0, 1)
+        out[rows] = o.masked_fill(~seen.any(-1).T[..., None], 0.0).to(q.dtype)
     return out.view(q.shape)

@@ -329,6 +329,22 @@ int ako_paged_attention_fwd(const void* q, const int64_t* q_strides, void* out,
 int64_t ako_paged_attention_workspace(const ako_paged_t* cache, int64_t q_heads, int dtype);
 
 /*
+ * The same over listed blocks only: a row at position p of key head `head` sees the
+ * positions j <= p whose block j / page_size is among blocks[row][head][0 .. count-1], int32,
+ * dense (as ako_paged_select_fwd writes it). The list is a set: in any order, and a block that
+ * stands there twice counts once; numbers below 0 or past the table name nothing. A row with
+ * no such position is zero.
+ */
+int ako_paged_attention_blocks_fwd(const void* q, const int64_t* q_strides, void* out,
+                                   const ako_paged_t* cache, int64_t q_heads, float scale,
+                                   const int32_t* blocks, int64_t count, void* workspace,
+                                   int64_t workspace_bytes, int dtype, void* stream);
+
+/* Bytes of workspace for such a call (0: none); -1 for arguments it refuses. */
+int64_t ako_paged_attention_blocks_workspace(const ako_paged_t* cache, int64_t q_heads,
+                                             int64_t count, int dtype);
+
+/*
  * The mean of the keys of every page that the step's rows fill: for a row at the last
  * slot of its page, means[page][head] = sum over the page's slots of the keys as stored / page_size
  * (fp32; e4m3 keys times their scales). means is [num_pages, kv_heads, head_dim] floats,

@@ -567,7 +567,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 && !MX ? 3 : DP
   const unsigned kcoff = (PAGE16 ? vkey * static_cast<unsigned>(a.c.ksst[2]) : 0) + pd / 32;
   const unsigned vcoff = (PAGE16 ? vkey * static_cast<unsigned>(a.c.vsst[2]) : 0) + pd / 32;
   const HeadPools pools = head_pools<T, MX>(a.c, kvh);
-  const auto load = [&](Loaded& x, int i, int pages) {
+  const auto load = [&](Loaded& x, int i, int pages) __attribute__((always_inline)) {
     const int k0 = BLOCKS ? i * KT : tile_start(i);
     // Pages laid end to end: a place's slot is a position's.
     const RowOffsets<MX> r = row_offsets<T, MX, PAGE16>(a.c, pages, k0 + lane % KT, BLOCKS ? listed : kt.end);
@@ -601,7 +601,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 && !MX ? 3 : DP
   Loaded loaded[AHEAD];
   unsigned any = 0;  // nonzero where the row sees a key
   int pages = 0;  // of the next tile to load
-  const auto work = [&](Loaded& x, int i) {
+  const auto work = [&](Loaded& x, int i) __attribute__((always_inline)) {
     const unsigned here = x.there;
     // Whether every live row sees every key of the tile, and the keys that this lane's row sees.
     constexpr unsigned kAll = KT == 32 ? ~0u : 0xffffu;
@@ -733,7 +733,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 && !MX ? 3 : DP
   };
 
   // Key tiles first, first + STEP, ... below `end`.
-  const auto walk = [&](int first, int step) {
+  const auto walk = [&](int first, int step) __attribute__((always_inline)) {
 #pragma unroll
     for (int n = 0; n < AHEAD; ++n)
       if (first + n * step < end) {

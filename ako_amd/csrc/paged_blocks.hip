@@ -20,7 +20,10 @@ Plan plan(const PagedAttentionArgs& a) {
   const int64_t rows = a.c.n_seqs > 0 ? ceil_div(a.c.tokens * group, a.c.n_seqs) : 1;
   p.row_tiles = a.c.cu ? a.c.tokens * group / 16 + a.c.n_seqs + 1 : a.c.n_seqs * ceil_div(rows, 16);
   p.once = rows <= 16;
-  const int64_t items = a.tuned_items > 0 ? a.tuned_items : 1024, least = a.tuned_min_keys > 0 ? a.tuned_min_keys : 128;
+  // Two workgroups to a CU, in one round, as each finds its blocks anew: 16 tokens of 4096 keys, 8 key heads, in 8
+  // bits, 256 / 512 / 1024 workgroups 51.7 / 40.5 / 47.2 us. Parts of 128 keys, a tile for each
+  // wavefront: one token of 1024 keys in parts of 64 / 128 / 256 12.2 / 12.0 / 13.6.
+  const int64_t items = a.tuned_items > 0 ? a.tuned_items : 512, least = a.tuned_min_keys > 0 ? a.tuned_min_keys : 128;
   const int64_t keys = std::min(a.c.table_width, a.block_count) * a.c.page_size;
   const int64_t parts = std::min(items / std::max<int64_t>(1, p.row_tiles * a.c.kv_heads), keys / least);
   p.parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMaxParts, parts)));

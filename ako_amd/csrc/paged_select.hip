@@ -39,21 +39,23 @@ struct MeansDev {
   float* means;
   int64_t ms[2];  // page, head strides
   int kv_heads, head_dim, lanes, rows;  // lanes across a row, rows of a wavefront's load
-  int token0;
+  int token0, tile;                     // token rows of a workgroup
   FastDiv by_kv_heads, by_lanes;
 };
 
-constexpr int kMeanTokens = 16;  // token rows of a workgroup
-
+// A workgroup looks at `tile` token rows for those at the last slot of their page, and takes
+// their pages one after the other: each wavefront a quarter of the slots, a kilobyte per load and
+// eight loads in flight, added up in the order of the slots' residues and then of
+// the wavefronts. Bound by HBM where pages are many.
 template <typename T, bool MX>
 __global__ __launch_bounds__(256) void paged_means(MeansDev a) {
   __shared__ float part[4][kWave][9];  // 9: lanes' rows on different banks
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int tile = fast_div(blockIdx.x, a.by_kv_heads), head = blockIdx.x - tile * a.kv_heads;
-  const int token = a.token0 + tile * kMeanTokens + lane;
+  const int token = a.token0 + tile * a.tile + lane;
   // Which of the rows fill a page: lane i holds row i's page.
   int page = -1;
-  if (lane < kMeanTokens && token < a.c.tokens) {
+  if (lane < a.tile && token < a.c.tokens) {
     const TokenPlace at = lane_place(a.c, token);
     if (at.seq >= 0 && at.pos >= 0 && at.pos < a.c.capacity) {
       int slot;
@@ -61,18 +63,16 @@ __global__ __launch_bounds__(256) void paged_means(MeansDev a) {
       if (slot != a.c.page_size - 1) page = -1;
     }
   }
-  uint64_t todo = __ballot(page >= 0);
   const int row = fast_div(lane, a.by_lanes), e0 = (lane - row * a.lanes) * 8;
-  for (int nth = 0; todo != 0; todo &= todo - 1, ++nth) {
-    if (nth % 4 != wave) continue;
+  for (uint64_t todo = __ballot(page >= 0); todo != 0; todo &= todo - 1) {  // the same in every wavefront
     const int at = __builtin_amdgcn_readlane(page, __builtin_ctzll(todo));
     float sum[8] = {};
     constexpr int U = 8;  // loads in flight
-    for (int s0 = 0; s0 < a.c.page_size; s0 += U * a.rows) {
+    for (int s0 = wave * a.rows; s0 < a.c.page_size; s0 += U * 4 * a.rows) {
       Eight<float> x[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int s = s0 + u * a.rows + row;
+        const int s = s0 + u * 4 * a.rows + row;
         x[u] = zero_eight<float>();
         if (row >= a.rows || s >= a.c.page_size) continue;
         const int64_t k = at * a.c.kst[0] + head * a.c.kst[1] + s * a.c.kst[2] + e0;
@@ -92,19 +92,14 @@ __global__ __launch_bounds__(256) void paged_means(MeansDev a) {
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) part[wave][lane][i] = sum[i];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    if (lane < a.lanes) {
-      for (int r = 1; r < a.rows; ++r)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum[i] += part[wave][lane + r * a.lanes][i];
-      Eight<float> y;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = sum[i] / static_cast<float>(a.c.page_size);
-      store_eight<float>(a.means + at * a.ms[0] + head * a.ms[1] + lane * 8, y);
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.head_dim; e += 4 * kWave) {
+      float total = 0.0f;
+      for (int w = 0; w < 4; ++w)
+        for (int r = 0; r < a.rows; ++r) total += part[w][r * a.lanes + e / 8][e % 8];
+      a.means[at * a.ms[0] + head * a.ms[1] + e] = total / static_cast<float>(a.c.page_size);
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    __syncthreads();
   }
 }
 
@@ -123,6 +118,8 @@ struct SelectDev {
   FastDiv by_kv_heads, by_tiles;
 };
 
+constexpr int kTileRows = 16;  // token rows of a tile, at most
+
 // The blocks that a token at `pos` may attend to are 0 .. blocks - 1.
 __device__ __forceinline__ int blocks_of(const SelectDev& a, int pos) {
   return pos < 0 ? 0 : min(static_cast<int>(fast_div(pos, a.c.by_page)) + 1, a.width);
@@ -132,6 +129,7 @@ __device__ __forceinline__ int page_at(const SelectDev& a, int seq, int block) {
   return page >= 0 && page < a.c.num_pages ? page : -1;
 }
 
+typedef double f64x2 __attribute__((ext_vector_type(2)));
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
 // Up to 16 token rows by 16 blocks per wavefront and step. The matrix instruction takes four elements of
@@ -217,21 +215,14 @@ __device__ __forceinline__ double of_order(int64_t k) {
   return __builtin_bit_cast(double, k ^ (k >> 63 & 0x7fffffffffffffffll));
 }
 
-// A wavefront per row and key head. The score that parts the `want` largest from the rest is
+// The choice for one row and key head, by one wavefront. The score that parts the `want` largest from the rest is
 // found by halving the interval between the least and the greatest, first of values, then of
 // their bits, until as many lie above as are wanted or one value is left, whose lowest blocks
 // are then taken. N: scores in a lane's registers, 0 where they are too many and are read
-// again for every step.
-template <int N>
-__global__ __launch_bounds__(256) void select_blocks(SelectDev a) {
+// again for every step. score(b): that of block b, NaN where its page is absent.
+template <int N, typename Score>
+__device__ __forceinline__ void choose(const SelectDev& a, const TokenPlace& at, int blocks, int* out, Score score) {
   const int lane = threadIdx.x % kWave;
-  const int64_t item = int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  if (item >= int64_t(a.end - a.token0) * a.kv_heads) return;
-  const int row = fast_div(static_cast<unsigned>(item), a.by_kv_heads);
-  const TokenPlace at = token_place(a.c, a.token0 + row);
-  const int blocks = at.seq < 0 ? 0 : blocks_of(a, at.pos);
-  int* const out = a.out + (int64_t(a.token0) * a.kv_heads + item) * a.count;
-  const double* const scores = a.scores + item * a.width;
   const bool all = blocks <= a.count;
   // Always taken: below `low` and from `high` on, the token's own block being the last.
   const int own = blocks > 0 ? static_cast<int>(fast_div(at.pos, a.c.by_page)) : 0;
@@ -248,7 +239,7 @@ __global__ __launch_bounds__(256) void select_blocks(SelectDev a) {
 #pragma unroll
       for (int i = 0; i < N; ++i) f(mine[i]);
     } else {
-      for (int b = low + lane; b < high; b += kWave) f(scores[b]);
+      for (int b = low + lane; b < high; b += kWave) f(score(b));
     }
   };
   if (!all) {
@@ -256,7 +247,7 @@ __global__ __launch_bounds__(256) void select_blocks(SelectDev a) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int b = low + i * kWave + lane;
-        mine[i] = b < high ? scores[b] : __builtin_nan("");
+        mine[i] = b < high ? score(b) : __builtin_nan("");
       }
     }
     double least = __builtin_inf(), most = -__builtin_inf();
@@ -321,7 +312,7 @@ __global__ __launch_bounds__(256) void select_blocks(SelectDev a) {
       if (all || b < low || b >= high) {
         take = there(b);
       } else {
-        const double x = scores[b];
+        const double x = score(b);
         take = x > cut;
         same = x == cut;
       }
@@ -335,6 +326,117 @@ __global__ __launch_bounds__(256) void select_blocks(SelectDev a) {
     written += __popcll(taken);
   }
   for (int i = min(written, a.count) + lane; i < a.count; i += kWave) out[i] = -1;
+}
+
+// A wavefront per row and key head, from the scores that select_scores has left.
+template <int N>
+__global__ __launch_bounds__(256) void select_blocks(SelectDev a) {
+  const int64_t item = int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  if (item >= int64_t(a.end - a.token0) * a.kv_heads) return;
+  const int row = fast_div(static_cast<unsigned>(item), a.by_kv_heads);
+  const TokenPlace at = token_place(a.c, a.token0 + row);
+  const double* const scores = a.scores + item * a.width;
+  choose<N>(a, at, at.seq < 0 ? 0 : blocks_of(a, at.pos), a.out + (int64_t(a.token0) * a.kv_heads + item) * a.count,
+            [&](int b) { return scores[b]; });
+}
+
+// Both in one, where a tile's scores fit in LDS: as many rows and blocks as SCORES allows. The
+// rows' sums of queries are formed once for the workgroup and lie in LDS too, pairs of them
+// exchanged by the row's number so that 16 rows' lie on different banks. A wavefront's means for the
+// next 16 blocks are loaded while it works on these, and their pages one step before.
+template <typename T, int DP, int SCORES>
+__global__ __launch_bounds__(512, DP <= 128 ? 4 : 2) void select_tile(SelectDev a) {
+  constexpr int Q = DP / 4, WAVES = 8;
+  __shared__ double scores[SCORES];
+  __shared__ __align__(16) double sums[kTileRows * DP];
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), col = lane % 16, g = lane / 16;
+  const unsigned tile = fast_div(blockIdx.x, a.by_kv_heads);
+  const int head = blockIdx.x - tile * a.kv_heads;
+  const int row0 = a.token0 + tile * a.tile, token = row0 + col;
+  TokenPlace at{-1, -1};
+  if (col < a.tile && token < a.end) at = lane_place(a.c, token);
+  const int blocks = at.seq < 0 ? 0 : blocks_of(a, at.pos);
+  // Rows with no more blocks than are asked for are not scored.
+  unsigned todo = static_cast<unsigned>(__ballot(blocks > a.count)) & 0xffffu;
+
+  if (todo != 0) {
+    for (int i = threadIdx.x; i < a.tile * (DP / 4); i += WAVES * kWave) {
+      const int r = i / (DP / 4), e = i % (DP / 4) * 4;
+      double sum[4] = {0.0, 0.0, 0.0, 0.0};
+      const int seq = __shfl(at.seq, r);  // rows' places stand in the first lanes of every wavefront
+      if ((todo >> r & 1) && e < a.head_dim) {
+        const int b = a.c.cu ? 0 : seq, s = row0 + r - b * a.c.seq;
+        const T* x = static_cast<const T*>(a.q) + b * a.qs[0] + s * a.qs[1] + int64_t(head) * a.group * a.qs[2] + e;
+        for (int h = 0; h < a.group; ++h, x += a.qs[2]) {
+          float v[4];
+          load_f32<T, 4>(x, v);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sum[j] += static_cast<double>(v[j]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j += 2) *reinterpret_cast<f64x2*>(sums + r * DP + ((e + j) / 2 ^ r) * 2) = f64x2{sum[j], sum[j + 1]};
+    }
+    __syncthreads();
+
+    while (todo != 0) {
+      const int from = __builtin_ctz(todo), seq = __builtin_amdgcn_readlane(at.seq, from);
+      const unsigned rows = static_cast<unsigned>(__ballot(at.seq == seq && (todo >> col & 1))) & 0xffffu;
+      todo &= ~rows;
+      // Positions ascend, so the sequence's last row has the most blocks.
+      const int most = __builtin_amdgcn_readlane(blocks, 31 - __builtin_clz(rows));
+      const auto page_of_tile = [&](int b0) { return b0 + col < most ? page_at(a, seq, b0 + col) : -1; };
+      Pack<float, 4> next[Q / 4];
+      const auto load = [&](int page) {
+        const float* m = a.means + max(page, 0) * a.ms[0] + head * a.ms[1] + g * Q;
+#pragma unroll
+        for (int i = 0; i < Q / 4; ++i) {
+          next[i].raw = u32x4{0, 0, 0, 0};
+          if (page >= 0 && g * Q + 4 * i < a.head_dim) next[i] = load_pack<float, 4>(m + 4 * i);
+        }
+      };
+      int page = page_of_tile(wave * 16), ahead = page_of_tile((wave + WAVES) * 16);
+      load(page);
+      for (int b0 = wave * 16; b0 < most; b0 += WAVES * 16) {
+        Pack<float, 4> k[Q / 4];
+#pragma unroll
+        for (int i = 0; i < Q / 4; ++i) k[i] = next[i];
+        const bool there = page >= 0;
+        page = ahead;
+        load(page);
+        ahead = page_of_tile(b0 + 2 * WAVES * 16);
+        f64x4 s = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < Q; i += 2) {
+          f64x2 x = {0.0, 0.0};
+          if (col < a.tile) x = *reinterpret_cast<const f64x2*>(sums + col * DP + ((g * Q + i) / 2 ^ col) * 2);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            s = __builtin_amdgcn_mfma_f64_16x16x4f64(x[j], static_cast<double>(k[(i + j) / 4].e[(i + j) % 4]), s, 0, 0, 0);
+        }
+        const int block = b0 + col;
+        if (block < most) {
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {  // a lane holds column `col` of the rows 4 v + g
+            const int r = 4 * v + g;
+            if (rows >> r & 1) scores[r * a.width + block] = !there ? __builtin_nan("") : s[v] != s[v] ? -__builtin_inf() : s[v];
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+
+  for (int r = wave; r < a.tile; r += WAVES) {
+    if (row0 + r >= a.end) break;
+    const TokenPlace mine{__builtin_amdgcn_readlane(at.seq, r), __builtin_amdgcn_readlane(at.pos, r)};
+    const int n = __builtin_amdgcn_readlane(blocks, r);
+    int* const out = a.out + (int64_t(row0 + r) * a.kv_heads + head) * a.count;
+    const auto score = [&](int b) { return scores[r * a.width + b]; };
+    if (n <= 4 * kWave) choose<4>(a, mine, n, out, score);
+    else if (n <= 16 * kWave) choose<16>(a, mine, n, out, score);
+    else choose<0>(a, mine, n, out, score);
+  }
 }
 
 // Workgroups of a launch, at most, for a call of many rows: work-items stay below 2^32.
@@ -352,10 +454,13 @@ hipError_t launch_paged_means(const PagedMeansArgs& a, hipStream_t stream) {
   d.rows = kWave / d.lanes;
   d.by_kv_heads = make_fastdiv(d.kv_heads);
   d.by_lanes = make_fastdiv(d.lanes);
-  const int64_t slice = std::max<int64_t>(1, kSlice / a.c.kv_heads) * kMeanTokens;
+  // A page's worth of a sequence's rows fills one page; single rows of many sequences may each fill theirs, all at once.
+  const int64_t per_seq = ceil_div(a.c.tokens, std::max<int64_t>(1, a.c.n_seqs));
+  d.tile = static_cast<int>(std::min<int64_t>(kWave, std::max<int64_t>(4, std::min(per_seq, a.c.page_size))));
+  const int64_t slice = std::max<int64_t>(1, kSlice / a.c.kv_heads) * d.tile;
   for (int64_t t = 0; t < a.c.tokens; t += slice) {
     d.token0 = static_cast<int>(t);
-    const dim3 grid(static_cast<unsigned>(ceil_div(std::min(slice, a.c.tokens - t), kMeanTokens) * a.c.kv_heads)), block(256);
+    const dim3 grid(static_cast<unsigned>(ceil_div(std::min(slice, a.c.tokens - t), d.tile) * a.c.kv_heads)), block(256);
     if (a.c.mx) {
       AKO_LAUNCH((paged_means<float, true>), grid, block, 0, stream, d);
     } else {
@@ -374,13 +479,37 @@ hipError_t launch_paged_means(const PagedMeansArgs& a, hipStream_t stream) {
 
 namespace {
 
-constexpr int kTileRows = 16;
+// Token rows of a tile: as many as a sequence has on average, since rows of one sequence share its blocks' means.
+int tile_rows(const PagedSelectArgs& a) {
+  const int64_t per_seq = ceil_div(a.c.tokens, std::max<int64_t>(1, a.c.n_seqs));
+  int tile = 1;
+  while (tile < kTileRows && tile < per_seq) tile *= 2;
+  return tile;
+}
+
+// Whether a tile's scores stay in LDS.
+constexpr int kFewScores = 8192, kMostScores = 14336;
+bool in_lds(const PagedSelectArgs& a) { return tile_rows(a) * a.c.table_width <= (a.c.head_dim <= 128 ? kMostScores : kFewScores); }
 
 // Token rows whose scores are held at a time: 64 MiB of them, so that they stay in the last level cache.
 int64_t slice_rows(const PagedSelectArgs& a) {
   const int64_t row = a.c.kv_heads * a.c.table_width * static_cast<int64_t>(sizeof(double));
   const int64_t rows = std::max<int64_t>(1, (int64_t(1) << 26) / std::max<int64_t>(1, row) / kTileRows) * kTileRows;
   return std::min(rows, a.c.tokens);
+}
+
+template <typename T>
+void launch_tile(const SelectDev& d, bool few, dim3 grid, hipStream_t stream) {
+  const dim3 block(512);
+  if (d.head_dim <= 64) {
+    if (few) AKO_LAUNCH((select_tile<T, 64, kFewScores>), grid, block, 0, stream, d);
+    else AKO_LAUNCH((select_tile<T, 64, kMostScores>), grid, block, 0, stream, d);
+  } else if (d.head_dim <= 128) {
+    if (few) AKO_LAUNCH((select_tile<T, 128, kFewScores>), grid, block, 0, stream, d);
+    else AKO_LAUNCH((select_tile<T, 128, kMostScores>), grid, block, 0, stream, d);
+  } else {
+    AKO_LAUNCH((select_tile<T, 256, kFewScores>), grid, block, 0, stream, d);
+  }
 }
 
 template <typename T>
@@ -394,7 +523,7 @@ void launch_scores(const SelectDev& d, dim3 grid, hipStream_t stream) {
 }  // namespace
 
 int64_t paged_select_workspace(const PagedSelectArgs& a) {
-  if (a.c.table_width <= a.count) return 0;  // every block is taken
+  if (a.c.table_width <= a.count || in_lds(a)) return 0;
   return slice_rows(a) * a.c.kv_heads * a.c.table_width * static_cast<int64_t>(sizeof(double));
 }
 
@@ -416,11 +545,26 @@ hipError_t launch_paged_select(const PagedSelectArgs& a, hipStream_t stream) {
   d.last = static_cast<int>(a.last);
   d.width = a.c.num_pages > 0 ? static_cast<int>(a.c.table_width) : 0;
   d.by_kv_heads = make_fastdiv(d.kv_heads);
-  // As many rows to a tile as a sequence has on average: rows of one sequence share its blocks' means.
-  const int64_t per_seq = ceil_div(a.c.tokens, std::max<int64_t>(1, a.c.n_seqs));
-  d.tile = 1;
-  while (d.tile < kTileRows && d.tile < per_seq) d.tile *= 2;
+  d.tile = tile_rows(a);
   const bool scored = d.width > a.count;
+  if (scored && in_lds(a)) {
+    const int64_t rows = std::max<int64_t>(1, 2 * kSlice / a.c.kv_heads) * d.tile;
+    const bool few = d.tile * a.c.table_width <= kFewScores;
+    for (int64_t t = 0; t < a.c.tokens; t += rows) {
+      d.token0 = static_cast<int>(t);
+      d.end = static_cast<int>(std::min(t + rows, a.c.tokens));
+      const dim3 grid(static_cast<unsigned>(ceil_div(d.end - d.token0, d.tile) * a.c.kv_heads));
+      switch (a.dtype) {
+        case kF32: launch_tile<float>(d, few, grid, stream); break;
+        case kF16: launch_tile<_Float16>(d, few, grid, stream); break;
+        case kBF16: launch_tile<__bf16>(d, few, grid, stream); break;
+        default: return hipErrorInvalidValue;
+      }
+      const hipError_t err = hipGetLastError();
+      if (err != hipSuccess) return err;
+    }
+    return hipSuccess;
+  }
   const int64_t slice = scored ? slice_rows(a) : std::max<int64_t>(1, 4 * kSlice / a.c.kv_heads);
   for (int64_t t = 0; t < a.c.tokens; t += slice) {
     d.token0 = static_cast<int>(t);

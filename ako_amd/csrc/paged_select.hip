@@ -134,7 +134,8 @@ typedef double f64x4 __attribute__((ext_vector_type(4)));
 
 // Up to 16 token rows by 16 blocks per wavefront and step. The matrix instruction takes four elements of
 // the inner dimension from the four groups of 16 lanes; which four is only a name, so group g
-// holds the g-th quarter of a row and loads it in 16-byte packets. The rows' sums of
+// holds packet 4 i + g of a row in its i-th 16 bytes, and a load takes 64 bytes in a row of each of 16 means. (With a quarter of the row
+// in each group, a load touched 64 lines, which the L1 did not hold until the eighth: 4 times as long.) The rows' sums of
 // queries stay in registers. Rows of a tile that belong to different sequences are
 // done one sequence after the other.
 template <typename T, int DP>
@@ -159,12 +160,12 @@ __global__ __launch_bounds__(256) void select_scores(SelectDev a) {
   for (int i = 0; i < Q; ++i) q[i] = 0.0;
   if (todo >> col & 1) {
     const int b = a.c.cu ? 0 : at.seq, s = token - b * a.c.seq;
-    const T* x = static_cast<const T*>(a.q) + b * a.qs[0] + s * a.qs[1] + int64_t(head) * a.group * a.qs[2] + g * Q;
+    const T* x = static_cast<const T*>(a.q) + b * a.qs[0] + s * a.qs[1] + int64_t(head) * a.group * a.qs[2] + 4 * g;
     for (int h = 0; h < a.group; ++h, x += a.qs[2]) {
 #pragma unroll
       for (int i = 0; i < Q; i += 4) {
         float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (g * Q + i < a.head_dim) load_f32<T, 4>(x + i, v);
+        if (4 * i + 4 * g < a.head_dim) load_f32<T, 4>(x + 4 * i, v);
 #pragma unroll
         for (int j = 0; j < 4; ++j) q[i + j] += static_cast<double>(v[j]);
       }
@@ -179,13 +180,13 @@ __global__ __launch_bounds__(256) void select_scores(SelectDev a) {
     const int most = __builtin_amdgcn_readlane(blocks, 31 - __builtin_clz(rows));
     for (int b0 = chunk * a.chunk + wave * 16; b0 < min(most, (chunk + 1) * a.chunk); b0 += 4 * 16) {
       const int block = b0 + col, page = block < most ? page_at(a, seq, block) : -1;
-      const float* m = a.means + max(page, 0) * a.ms[0] + head * a.ms[1] + g * Q;
+      const float* m = a.means + max(page, 0) * a.ms[0] + head * a.ms[1] + 4 * g;
       float k[Q];
 #pragma unroll
       for (int i = 0; i < Q; i += 4) {
         Pack<float, 4> p;
         p.raw = u32x4{0, 0, 0, 0};
-        if (page >= 0 && g * Q + i < a.head_dim) p = load_pack<float, 4>(m + i);
+        if (page >= 0 && 4 * i + 4 * g < a.head_dim) p = load_pack<float, 4>(m + 4 * i);
 #pragma unroll
         for (int j = 0; j < 4; ++j) k[i + j] = p.e[j];
       }
@@ -215,11 +216,13 @@ __device__ __forceinline__ double of_order(int64_t k) {
   return __builtin_bit_cast(double, k ^ (k >> 63 & 0x7fffffffffffffffll));
 }
 
-// The choice for one row and key head, by one wavefront. The score that parts the `want` largest from the rest is
-// found by halving the interval between the least and the greatest, first of values, then of
-// their bits, until as many lie above as are wanted or one value is left, whose lowest blocks
-// are then taken. N: scores in a lane's registers, 0 where they are too many and are read
-// again for every step. score(b): that of block b, NaN where its page is absent.
+// The choice for one row and key head, by one wavefront: the score that parts the `want` largest from
+// the rest. First for scores rounded to 32 bits, which keeps their order: the interval between
+// the least and the greatest is halved until as many lie above as are wanted. Where that meets
+// scores that round alike, the interval of the 64-bit scores is halved, first of values,
+// then of their bits, until one value is left, whose lowest blocks are then taken. N: scores
+// in a lane's registers, 0 where they are too many and are read again for every step.
+// score(b): that of block b, NaN where its page is absent.
 template <int N, typename Score>
 __device__ __forceinline__ void choose(const SelectDev& a, const TokenPlace& at, int blocks, int* out, Score score) {
   const int lane = threadIdx.x % kWave;
@@ -229,78 +232,89 @@ __device__ __forceinline__ void choose(const SelectDev& a, const TokenPlace& at,
   const int low = min(a.first, blocks), high = max(low, min(blocks, max(0, own - a.last + 1)));
   const auto there = [&](int b) { return page_at(a, at.seq, b) >= 0; };
 
-  double cut = -__builtin_inf();  // scores above it are taken, and of those equal to it the first `equal`
+  // Scores above `cut` are taken, and of those equal to it the first `equal`; `rough`: 32-bit ones from bar on.
+  double cut = -__builtin_inf();
+  float bar = 0.0f;
+  bool rough = false;
   int equal = std::numeric_limits<int>::max();
+  // The number of this row's scores between the blocks that are always taken for which f holds; those of absent pages are NaN.
   constexpr int R = N > 0 ? N : 1;
-  double mine[R];
-  // f(score) of this lane's scores between the blocks that are always taken; those of absent pages are NaN.
-  const auto each = [&](auto f) {
+  float mine[R];
+  const auto count = [&](auto f) {
+    int n = 0;
     if constexpr (N > 0) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) f(mine[i]);
+      for (int i = 0; i < N; ++i) n += __popcll(__ballot(f(mine[i])));
     } else {
-      for (int b = low + lane; b < high; b += kWave) f(score(b));
+      for (int b0 = low; b0 < high; b0 += kWave) n += __popcll(__ballot(b0 + lane < high && f(static_cast<float>(score(b0 + lane)))));
     }
+    return n;
+  };
+  const auto count64 = [&](auto f) {
+    int n = 0;
+    for (int b0 = low; b0 < high; b0 += kWave) n += __popcll(__ballot(b0 + lane < high && f(score(b0 + lane))));
+    return n;
   };
   if (!all) {
+    float least = __builtin_inff(), most = -__builtin_inff();
+    const auto widen = [&](float x) {  // NaN changes neither
+      least = __builtin_fminf(least, x);
+      most = __builtin_fmaxf(most, x);
+    };
     if constexpr (N > 0) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int b = low + i * kWave + lane;
-        mine[i] = b < high ? score(b) : __builtin_nan("");
+        mine[i] = b < high ? static_cast<float>(score(b)) : __builtin_nanf("");
+        widen(mine[i]);
       }
+    } else {
+      for (int b = low + lane; b < high; b += kWave) widen(static_cast<float>(score(b)));
     }
-    double least = __builtin_inf(), most = -__builtin_inf();
-    int held = 0;
-    each([&](double x) {
-      least = fmin(least, x);
-      most = fmax(most, x);
-      held += x == x;
-    });
-    int always = 0;
-    for (int b = lane; b < low; b += kWave) always += there(b);
-    for (int b = high + lane; b < blocks; b += kWave) always += there(b);
 #pragma unroll
     for (int k = 1; k < kWave; k *= 2) {
-      least = fmin(least, __shfl_xor(least, k));
-      most = fmax(most, __shfl_xor(most, k));
-      held += __shfl_xor(held, k);
-      always += __shfl_xor(always, k);
+      least = __builtin_fminf(least, __shfl_xor(least, k));
+      most = __builtin_fmaxf(most, __shfl_xor(most, k));
     }
+    int always = 0;
+    for (int b0 = 0; b0 < low; b0 += kWave) always += __popcll(__ballot(b0 + lane < low && there(b0 + lane)));
+    for (int b0 = high; b0 < blocks; b0 += kWave) always += __popcll(__ballot(b0 + lane < blocks && there(b0 + lane)));
     const int want = max(0, a.count - always);
     if (want == 0) {
       cut = __builtin_inf();
       equal = 0;
-    } else if (held > want) {
-      // At least `want` scores are at or above lo, fewer above hi.
-      int64_t lo = order_of(least), hi = order_of(most) + 1;
-      for (int step = 0; static_cast<uint64_t>(hi) - static_cast<uint64_t>(lo) > 1; ++step) {
-        int64_t mid = (lo & hi) + ((lo ^ hi) >> 1);  // their mean, without overflow
-        if (step < 32) {
-          const double x = 0.5 * of_order(lo) + 0.5 * of_order(hi);
-          const int64_t k = order_of(x);
-          if (x == x && k > lo && k < hi) mid = k;
-        }
-        const double bar = of_order(mid);
-        int above = 0;
-        each([&](double x) {
-          if constexpr (N > 0) above += __popcll(__ballot(x >= bar));
-          else above += x >= bar;
-        });
-        if constexpr (N == 0) {
-#pragma unroll
-          for (int k = 1; k < kWave; k *= 2) above += __shfl_xor(above, k);
-        }
-        if (above >= want) lo = mid;
-        else hi = mid;
-        if (above == want) break;
+    } else if (count([](float x) { return x == x; }) > want) {
+      // At least `want` scores are at or above lo, fewer from hi on (all of them lie below infinity, or rounded to it).
+      float lo = least, hi = most;
+      while (!rough) {
+        bar = lo + (hi - lo) * 0.5f;
+        if (!(bar > lo && bar <= hi)) break;
+        const int above = count([&](float x) { return x >= bar; });
+        if (above == want) rough = true;
+        else if (above > want) lo = bar;
+        else if (bar == hi) break;
+        else hi = bar;
       }
-      cut = of_order(lo);
-      int above = 0;
-      each([&](double x) { above += x > cut; });
-#pragma unroll
-      for (int k = 1; k < kWave; k *= 2) above += __shfl_xor(above, k);
-      equal = want - above;
+      if (!rough) {
+        int64_t first = order_of(-__builtin_inf()), end = order_of(__builtin_inf()) + 1;
+        for (int step = 0; static_cast<uint64_t>(end) - static_cast<uint64_t>(first) > 1; ++step) {
+          int64_t mid = (first & end) + ((first ^ end) >> 1);  // their mean, without overflow
+          if (step == 0 && lo > -__builtin_inff()) mid = order_of(lo);
+          if (step == 1 && hi < __builtin_inff()) mid = order_of(hi);
+          if (step > 1 && step < 32) {
+            const double x = 0.5 * of_order(first) + 0.5 * of_order(end);
+            if (x == x) mid = order_of(x);
+          }
+          if (mid <= first || mid >= end) mid = (first & end) + ((first ^ end) >> 1);
+          const double at64 = of_order(mid);
+          const int above = count64([&](double x) { return x >= at64; });
+          if (above >= want) first = mid;
+          else end = mid;
+          if (above == want) break;
+        }
+        cut = of_order(first);
+        equal = want - count64([&](double x) { return x > cut; });
+      }
     }
   }
 
@@ -313,8 +327,8 @@ __device__ __forceinline__ void choose(const SelectDev& a, const TokenPlace& at,
         take = there(b);
       } else {
         const double x = score(b);
-        take = x > cut;
-        same = x == cut;
+        take = rough ? static_cast<float>(x) >= bar : x > cut;
+        same = !rough && x == cut;
       }
     }
     const uint64_t ties = __ballot(same), below = (uint64_t(1) << lane) - 1;
@@ -344,11 +358,14 @@ __global__ __launch_bounds__(256) void select_blocks(SelectDev a) {
 // rows' sums of queries are formed once for the workgroup and lie in LDS too, pairs of them
 // exchanged by the row's number so that 16 rows' lie on different banks. A wavefront's means for the
 // next 16 blocks are loaded while it works on these, and their pages one step before.
-template <typename T, int DP, int SCORES>
-__global__ __launch_bounds__(512, DP <= 128 ? 4 : 2) void select_tile(SelectDev a) {
-  constexpr int Q = DP / 4, WAVES = 8;
+//
+// ONE: a single row, whose products leave the matrix cores' other rows empty: each lane adds up
+// its quarter of a block's product by itself.
+template <typename T, int DP, int SCORES, int WAVES, bool ONE>
+__global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? (SCORES > 8192 ? WAVES / 4 : 4) : 2) void select_tile(SelectDev a) {
+  constexpr int Q = DP / 4;
   __shared__ double scores[SCORES];
-  __shared__ __align__(16) double sums[kTileRows * DP];
+  __shared__ __align__(16) double sums[(ONE ? 1 : kTileRows) * DP];
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), col = lane % 16, g = lane / 16;
   const unsigned tile = fast_div(blockIdx.x, a.by_kv_heads);
   const int head = blockIdx.x - tile * a.kv_heads;
@@ -388,13 +405,14 @@ __global__ __launch_bounds__(512, DP <= 128 ? 4 : 2) void select_tile(SelectDev 
       const auto page_of_tile = [&](int b0) { return b0 + col < most ? page_at(a, seq, b0 + col) : -1; };
       Pack<float, 4> next[Q / 4];
       const auto load = [&](int page) {
-        const float* m = a.means + max(page, 0) * a.ms[0] + head * a.ms[1] + g * Q;
+        const float* m = a.means + max(page, 0) * a.ms[0] + head * a.ms[1] + 4 * g;
 #pragma unroll
         for (int i = 0; i < Q / 4; ++i) {
           next[i].raw = u32x4{0, 0, 0, 0};
-          if (page >= 0 && g * Q + 4 * i < a.head_dim) next[i] = load_pack<float, 4>(m + 4 * i);
+          if (page >= 0 && 16 * i + 4 * g < a.head_dim) next[i] = load_pack<float, 4>(m + 16 * i);
         }
       };
+      // Loads return in order: a tile's pages are asked for before the means of the tile before it.
       int page = page_of_tile(wave * 16), ahead = page_of_tile((wave + WAVES) * 16);
       load(page);
       for (int b0 = wave * 16; b0 < most; b0 += WAVES * 16) {
@@ -403,18 +421,29 @@ __global__ __launch_bounds__(512, DP <= 128 ? 4 : 2) void select_tile(SelectDev 
         for (int i = 0; i < Q / 4; ++i) k[i] = next[i];
         const bool there = page >= 0;
         page = ahead;
-        load(page);
         ahead = page_of_tile(b0 + 2 * WAVES * 16);
+        load(page);
+        const int block = b0 + col;
+        if constexpr (ONE) {
+          asm volatile("" ::: "memory");  // the sums stay in LDS: in registers they would take 64 of 128
+          double x[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int i = 0; i < Q; ++i) x[i % 4] = __builtin_fma(sums[i / 4 * 16 + 4 * g + i % 4], static_cast<double>(k[i / 4].e[i % 4]), x[i % 4]);
+          double s = (x[0] + x[1]) + (x[2] + x[3]);
+          s += __shfl_xor(s, 16);
+          s += __shfl_xor(s, 32);
+          if (g == 0 && block < most) scores[block] = !there ? __builtin_nan("") : s != s ? -__builtin_inf() : s;
+          continue;
+        }
         f64x4 s = {0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < Q; i += 2) {
           f64x2 x = {0.0, 0.0};
-          if (col < a.tile) x = *reinterpret_cast<const f64x2*>(sums + col * DP + ((g * Q + i) / 2 ^ col) * 2);
+          if (!ONE && col < a.tile) x = *reinterpret_cast<const f64x2*>(sums + col * DP + (8 * (i / 4) + 2 * g + i % 4 / 2 ^ col) * 2);
 #pragma unroll
           for (int j = 0; j < 2; ++j)
             s = __builtin_amdgcn_mfma_f64_16x16x4f64(x[j], static_cast<double>(k[(i + j) / 4].e[(i + j) % 4]), s, 0, 0, 0);
         }
-        const int block = b0 + col;
         if (block < most) {
 #pragma unroll
           for (int v = 0; v < 4; ++v) {  // a lane holds column `col` of the rows 4 v + g
@@ -434,6 +463,7 @@ __global__ __launch_bounds__(512, DP <= 128 ? 4 : 2) void select_tile(SelectDev 
     int* const out = a.out + (int64_t(row0 + r) * a.kv_heads + head) * a.count;
     const auto score = [&](int b) { return scores[r * a.width + b]; };
     if (n <= 4 * kWave) choose<4>(a, mine, n, out, score);
+    else if (n <= 8 * kWave) choose<8>(a, mine, n, out, score);
     else if (n <= 16 * kWave) choose<16>(a, mine, n, out, score);
     else choose<0>(a, mine, n, out, score);
   }
@@ -489,7 +519,7 @@ int tile_rows(const PagedSelectArgs& a) {
 
 // Whether a tile's scores stay in LDS.
 constexpr int kFewScores = 8192, kMostScores = 14336;
-bool in_lds(const PagedSelectArgs& a) { return tile_rows(a) * a.c.table_width <= (a.c.head_dim <= 128 ? kMostScores : kFewScores); }
+bool in_lds(const PagedSelectArgs& a) { return tile_rows(a) * a.c.table_width <= kMostScores; }
 
 // Token rows whose scores are held at a time: 64 MiB of them, so that they stay in the last level cache.
 int64_t slice_rows(const PagedSelectArgs& a) {
@@ -498,18 +528,23 @@ int64_t slice_rows(const PagedSelectArgs& a) {
   return std::min(rows, a.c.tokens);
 }
 
+template <typename T, int DP>
+void launch_tile_dim(const SelectDev& d, bool few, dim3 grid, hipStream_t stream) {
+  // Few workgroups, each of a whole row: 16 wavefronts to have more of it in flight, where the registers allow.
+  constexpr int kOneWaves = DP <= 128 ? 16 : 8;
+  if (d.tile == 1) {
+    if (few) AKO_LAUNCH((select_tile<T, DP, kFewScores, kOneWaves, true>), grid, dim3(kOneWaves * kWave), 0, stream, d);
+    else AKO_LAUNCH((select_tile<T, DP, kMostScores, kOneWaves, true>), grid, dim3(kOneWaves * kWave), 0, stream, d);
+  } else {
+    if (few) AKO_LAUNCH((select_tile<T, DP, kFewScores, 8, false>), grid, dim3(8 * kWave), 0, stream, d);
+    else AKO_LAUNCH((select_tile<T, DP, kMostScores, 8, false>), grid, dim3(8 * kWave), 0, stream, d);
+  }
+}
 template <typename T>
 void launch_tile(const SelectDev& d, bool few, dim3 grid, hipStream_t stream) {
-  const dim3 block(512);
-  if (d.head_dim <= 64) {
-    if (few) AKO_LAUNCH((select_tile<T, 64, kFewScores>), grid, block, 0, stream, d);
-    else AKO_LAUNCH((select_tile<T, 64, kMostScores>), grid, block, 0, stream, d);
-  } else if (d.head_dim <= 128) {
-    if (few) AKO_LAUNCH((select_tile<T, 128, kFewScores>), grid, block, 0, stream, d);
-    else AKO_LAUNCH((select_tile<T, 128, kMostScores>), grid, block, 0, stream, d);
-  } else {
-    AKO_LAUNCH((select_tile<T, 256, kFewScores>), grid, block, 0, stream, d);
-  }
+  if (d.head_dim <= 64) launch_tile_dim<T, 64>(d, few, grid, stream);
+  else if (d.head_dim <= 128) launch_tile_dim<T, 128>(d, few, grid, stream);
+  else launch_tile_dim<T, 256>(d, few, grid, stream);
 }
 
 template <typename T>
@@ -587,8 +622,8 @@ hipError_t launch_paged_select(const PagedSelectArgs& a, hipStream_t stream) {
       if (err != hipSuccess) return err;
     }
     const dim3 grid(static_cast<unsigned>(ceil_div(items, 4))), block(256);
-    if (d.width <= 4 * kWave) AKO_LAUNCH((select_blocks<4>), grid, block, 0, stream, d);
-    else if (d.width <= 16 * kWave) AKO_LAUNCH((select_blocks<16>), grid, block, 0, stream, d);
+    // Up to 14336 scores a tile these come with select_tile; so a wide table here, or few blocks of which all are taken.
+    if (d.width <= 16 * kWave) AKO_LAUNCH((select_blocks<16>), grid, block, 0, stream, d);
     else if (d.width <= 64 * kWave) AKO_LAUNCH((select_blocks<64>), grid, block, 0, stream, d);
     else AKO_LAUNCH((select_blocks<0>), grid, block, 0, stream, d);
     const hipError_t err = hipGetLastError();

@@ -230,7 +230,11 @@ __device__ __forceinline__ void choose(const SelectDev& a, const TokenPlace& at,
   // Always taken: below `low` and from `high` on, the token's own block being the last.
   const int own = blocks > 0 ? static_cast<int>(fast_div(at.pos, a.c.by_page)) : 0;
   const int low = min(a.first, blocks), high = max(low, min(blocks, max(0, own - a.last + 1)));
-  const auto there = [&](int b) { return page_at(a, at.seq, b) >= 0; };
+  const auto there = [&](int b) {  // scored blocks that are not there are NaN
+    if (all) return page_at(a, at.seq, b) >= 0;
+    const double x = score(b);
+    return x == x;
+  };
 
   // Scores above `cut` are taken, and of those equal to it the first `equal`; `rough`: 32-bit ones from bar on.
   double cut = -__builtin_inf();
@@ -319,25 +323,35 @@ __device__ __forceinline__ void choose(const SelectDev& a, const TokenPlace& at,
   }
 
   int written = 0, equals = 0;
-  for (int b0 = 0; b0 < blocks; b0 += kWave) {
-    const int b = b0 + lane;
-    bool take = false, same = false;
-    if (b < blocks) {
-      if (all || b < low || b >= high) {
-        take = there(b);
-      } else {
-        const double x = score(b);
-        take = rough ? static_cast<float>(x) >= bar : x > cut;
-        same = !rough && x == cut;
-      }
-    }
-    const uint64_t ties = __ballot(same), below = (uint64_t(1) << lane) - 1;
-    if (same) take = equals + __popcll(ties & below) < equal;
-    equals = min(equals + static_cast<int>(__popcll(ties)), std::numeric_limits<int>::max() / 2);
+  const uint64_t below = (uint64_t(1) << lane) - 1;
+  const auto emit = [&](int b, bool take) {
     const uint64_t taken = __ballot(take);
     const int to = written + __popcll(taken & below);
     if (take && to < a.count) out[to] = b;
     written += __popcll(taken);
+  };
+  const auto emit_always = [&](int from, int to) {
+    for (int b0 = from; b0 < to; b0 += kWave) emit(b0 + lane, b0 + lane < to && there(b0 + lane));
+  };
+  if (all) {
+    emit_always(0, blocks);
+  } else {
+    emit_always(0, low);
+    if (N > 0 && rough) {
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        if (low + i * kWave < high) emit(low + i * kWave + lane, mine[i] >= bar);
+    } else {
+      for (int b0 = low; b0 < high; b0 += kWave) {
+        const double x = b0 + lane < high ? score(b0 + lane) : __builtin_nan("");
+        const uint64_t ties = __ballot(!rough && x == cut);
+        bool take = rough ? static_cast<float>(x) >= bar : x > cut;
+        if (!rough && x == cut) take = equals + __popcll(ties & below) < equal;
+        equals = min(equals + static_cast<int>(__popcll(ties)), std::numeric_limits<int>::max() / 2);
+        emit(b0 + lane, take);
+      }
+    }
+    emit_always(high, blocks);
   }
   for (int i = min(written, a.count) + lane; i < a.count; i += kWave) out[i] = -1;
 }
@@ -377,6 +391,31 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? (SCORES > 8192 ? WAVES / 
   unsigned todo = static_cast<unsigned>(__ballot(blocks > a.count)) & 0xffffu;
 
   if (todo != 0) {
+    unsigned rows = 0;   // those of the sequence that is worked on
+    int seq = 0, most = 0;
+    const auto page_of_tile = [&](int b0) { return b0 + col < most ? page_at(a, seq, b0 + col) : -1; };
+    Pack<float, 4> next[Q / 4];
+    const auto load = [&](int page) {
+      const float* m = a.means + max(page, 0) * a.ms[0] + head * a.ms[1] + 4 * g;
+#pragma unroll
+      for (int i = 0; i < Q / 4; ++i) {
+        next[i].raw = u32x4{0, 0, 0, 0};
+        if (page >= 0 && 16 * i + 4 * g < a.head_dim) next[i] = load_pack<float, 4>(m + 16 * i);
+      }
+    };
+    int page = -1, ahead = -1;
+    const auto begin = [&](unsigned left) {
+      const int from = __builtin_ctz(left);
+      seq = __builtin_amdgcn_readlane(at.seq, from);
+      rows = static_cast<unsigned>(__ballot(at.seq == seq && (left >> col & 1))) & 0xffffu;
+      // Positions ascend, so the sequence's last row has the most blocks.
+      most = __builtin_amdgcn_readlane(blocks, 31 - __builtin_clz(rows));
+      // Loads return in order: a tile's pages are asked for before the means of the tile before it.
+      page = page_of_tile(wave * 16);
+      ahead = page_of_tile((wave + WAVES) * 16);
+      load(page);
+    };
+    begin(todo);
     for (int i = threadIdx.x; i < a.tile * (DP / 4); i += WAVES * kWave) {
       const int r = i / (DP / 4), e = i % (DP / 4) * 4;
       double sum[4] = {0.0, 0.0, 0.0, 0.0};
@@ -396,25 +435,7 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? (SCORES > 8192 ? WAVES / 
     }
     __syncthreads();
 
-    while (todo != 0) {
-      const int from = __builtin_ctz(todo), seq = __builtin_amdgcn_readlane(at.seq, from);
-      const unsigned rows = static_cast<unsigned>(__ballot(at.seq == seq && (todo >> col & 1))) & 0xffffu;
-      todo &= ~rows;
-      // Positions ascend, so the sequence's last row has the most blocks.
-      const int most = __builtin_amdgcn_readlane(blocks, 31 - __builtin_clz(rows));
-      const auto page_of_tile = [&](int b0) { return b0 + col < most ? page_at(a, seq, b0 + col) : -1; };
-      Pack<float, 4> next[Q / 4];
-      const auto load = [&](int page) {
-        const float* m = a.means + max(page, 0) * a.ms[0] + head * a.ms[1] + 4 * g;
-#pragma unroll
-        for (int i = 0; i < Q / 4; ++i) {
-          next[i].raw = u32x4{0, 0, 0, 0};
-          if (page >= 0 && 16 * i + 4 * g < a.head_dim) next[i] = load_pack<float, 4>(m + 16 * i);
-        }
-      };
-      // Loads return in order: a tile's pages are asked for before the means of the tile before it.
-      int page = page_of_tile(wave * 16), ahead = page_of_tile((wave + WAVES) * 16);
-      load(page);
+    for (;;) {
       for (int b0 = wave * 16; b0 < most; b0 += WAVES * 16) {
         Pack<float, 4> k[Q / 4];
 #pragma unroll
@@ -452,6 +473,9 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? (SCORES > 8192 ? WAVES / 
           }
         }
       }
+      todo &= ~rows;
+      if (todo == 0) break;
+      begin(todo);
     }
     __syncthreads();
   }

@@ -65,111 +65,163 @@ __device__ __forceinline__ int index_at(uint64_t place) { return static_cast<int
 
 // What a row's threads share.
 struct SampleLds {
-  uint64_t hist[kBins];
+  uint64_t hist[kBins];     // weights by bin of depth, or of place
+  uint64_t regions[kBins];  // weights by part of the row
   uint64_t list[kList];
   unsigned count[kBins];
-  double pow2[128];  // 2^(j / 128)
+  double pow2[128];         // 2^(j / 128)
   uint64_t wave_sum[kWaves];
   float wave_top[kWaves], wave_low[kWaves];
   int wave_at[kWaves];
-  uint64_t lo, hi;   // of the elements of a bin
-  unsigned n;        // elements of a bin
+  uint64_t lo, hi;          // of the elements of a bin
+  unsigned n;               // elements of a bin
   int bin;
-  unsigned bin_count;
   uint64_t before;
 };
 
 // The row's own numbers, the same in all threads.
 struct SampleRow {
-  double per_unit;  // log2(e) / T
-  float top;        // the largest logit
-  float per_bin;    // bins of a unit of logits
-  float dead;       // log2 units below the largest from which on weights are 0
-  int bits;         // S
-  double low;       // log2 units that min_p leaves
+  double top64, per_unit;  // the largest logit, and log2(e) / T
+  float top;
+  float floor;             // elements from here on weigh something; not -infinity
+  float keep;              // elements from here on reach min_p
+  float tail;              // elements below here weigh less than 1 - top_p of all together
+  float per_bin;           // bins of a unit of logits
+  int bits;                // S
+  bool flat;               // all that weigh anything weigh the same
 };
 
-// log2 units that x lies below the row's largest.
-__device__ __forceinline__ double depth(const SampleRow& r, float x) {
-  return x == r.top ? 0.0 : (static_cast<double>(r.top) - static_cast<double>(x)) * r.per_unit;
-}
-// 2^(S - t) rounded to a whole number: 2^(j / 128) from a table times e^(z ln 2) of the
-// rest z, at most 1/256, by its Taylor polynomial of degree 4, off by less than 2^-49.
-__device__ __forceinline__ uint64_t weight_of(const SampleLds& l, const SampleRow& r, double t) {
+// 2^(S - t), t log2 units below the largest, rounded to a whole number: 2^(j / 128) from a table
+// times 2^z of the rest z, at most 1/256, by its Taylor polynomial of degree 4, off by less than 2^-49.
+__device__ __forceinline__ uint64_t weight_of(const SampleLds& l, const SampleRow& r, float x) {
+  if (r.flat) return uint64_t(1) << r.bits;
   constexpr double kRound = 0x1.8p45;  // its last bit is 1/128
-  const double y = static_cast<double>(r.bits) - t, near = y + kRound;
+  constexpr double kLn2 = 0.69314718055994530942;
+  const double y = __builtin_fma(static_cast<double>(x) - r.top64, r.per_unit, static_cast<double>(r.bits));
+  const double near = y + kRound, z = y - (near - kRound);
   const int j = static_cast<int>(__builtin_bit_cast(uint64_t, near));
-  const double z = (y - (near - kRound)) * 0.69314718055994530942;
-  double p = __builtin_fma(z, 1.0 / 24, 1.0 / 6);
-  p = __builtin_fma(z, p, 0.5);
-  p = __builtin_fma(z, p, 1.0);
-  p = __builtin_fma(z, p, 1.0);
-  const double w = __builtin_ldexp(l.pow2[j & 127] * p, j >> 7);
-  return __builtin_bit_cast(uint64_t, w + 0x1p52) & 0xfffffffffffffull;
+  double p = __builtin_fma(z, kLn2 * kLn2 * kLn2 * kLn2 / 24, kLn2 * kLn2 * kLn2 / 6);
+  p = __builtin_fma(z, p, kLn2 * kLn2 / 2);
+  p = __builtin_fma(z, p, kLn2);
+  p = __builtin_fma(z, p, 1.0) * l.pow2[j & 127];  // in [1, 2), or next to it
+  const uint64_t scaled = __builtin_bit_cast(uint64_t, p) + (static_cast<uint64_t>(static_cast<unsigned>(j >> 7) << 20) << 32);
+  return __builtin_bit_cast(uint64_t, __builtin_bit_cast(double, scaled) + 0x1p52) & 0xfffffffffffffull;
 }
-__device__ __forceinline__ bool is_live(const SampleRow& r, float x, double t) { return x > -__builtin_inff() && t < r.dead; }
 __device__ __forceinline__ int bin_of(const SampleRow& r, float x) {
   const float d = x == r.top ? 0.0f : (r.top - x) * r.per_bin;
   return d < static_cast<float>(kBins - 1) ? static_cast<int>(d) : kBins - 1;
 }
 
-// Every element of the row: f(x, index), -infinity behind the end; all threads take part
-// in every call. The packets of kUnroll rounds are loaded before the first is used.
-template <typename T, typename F>
-__device__ __forceinline__ void each_packet(const T* row, int vocab, F f) {
-  constexpr int E = 16 / static_cast<int>(sizeof(T)), kUnroll = 4;
-  for (int base = 0; base < vocab; base += kThreads * E * kUnroll) {
-    Pack<T, E> p[kUnroll];
+// The row in packets of 16 bytes: read again for every pass, kRounds of the workgroup's packets
+// at a time, or (HELD) kept in LDS after the first.
+constexpr int kHeldBytes = 1 << 16;
+template <typename T, bool HELD>
+struct Row {
+  static constexpr int E = 16 / static_cast<int>(sizeof(T)), kRounds = HELD ? 1 : 4;
+  using P = Pack<T, E>;
+  const T* x;
+  int vocab;
+  P* held;  // HELD: packet i in place i
+
+  // -infinity behind the end.
+  __device__ __forceinline__ P packet(int i) const {
+    if (i + E <= vocab) return load_pack<T, E>(x + i);
+    P p;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int i = base + (u * kThreads + static_cast<int>(threadIdx.x)) * E;
-      if (i + E <= vocab) {
-        p[u] = load_pack<T, E>(row + i);
-      } else {
+    for (int e = 0; e < E; ++e) p.e[e] = i + e < vocab ? x[i + e] : from_f32<T>(-__builtin_inff());
+    return p;
+  }
+  // f(packet, index of its first element); all threads take part in every call. FIRST: of the row's first pass.
+  template <bool FIRST = false, typename F>
+  __device__ __forceinline__ void each_packet(F f) {
+    constexpr int kAtOnce = HELD && FIRST ? 4 : kRounds;
+    const int mine = static_cast<int>(threadIdx.x) * E;
+#pragma unroll 1
+    for (int base = 0; base < vocab; base += kThreads * E * kAtOnce) {
+      P p[kAtOnce];
 #pragma unroll
-        for (int e = 0; e < E; ++e) p[u].e[e] = i + e < vocab ? row[i + e] : from_f32<T>(-__builtin_inff());
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int i = base + u * kThreads * E + mine;
+        if (HELD && !FIRST) p[u] = held[i / E];
+        else p[u] = packet(i);
+      }
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int i = base + u * kThreads * E + mine;
+        if (base + u * kThreads * E >= vocab) continue;
+        if (HELD && FIRST) held[i / E] = p[u];
+        f(p[u], i);
+        __builtin_amdgcn_sched_barrier(0);  // one packet's work after the other: side by side they would not fit the registers
       }
     }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int i = base + (u * kThreads + static_cast<int>(threadIdx.x)) * E;
-      if (base + u * kThreads * E < vocab) f(p[u], i);
-    }
   }
-}
-template <typename T, typename F>
-__device__ __forceinline__ void each(const T* row, int vocab, F f) {
-  each_packet(row, vocab, [&](const auto& p, int i) {
+  // f(element, index).
+  template <bool FIRST = false, typename F>
+  __device__ __forceinline__ void each(F f) {
+    each_packet<FIRST>([&](const P& p, int i) {
 #pragma unroll
-    for (int e = 0; e < 16 / static_cast<int>(sizeof(T)); ++e) f(to_f32(p.e[e]), i + e);
-  });
-}
-
-__device__ __forceinline__ void clear_bins(SampleLds& l) {
-  for (int i = threadIdx.x; i < kBins; i += kThreads) {
-    l.hist[i] = 0;
-    l.count[i] = 0;
+      for (int e = 0; e < E; ++e) f(to_f32(p.e[e]), i + e);
+    });
   }
-  __syncthreads();
+  __device__ __forceinline__ float at(int i) const { return to_f32(HELD ? held[i / E].e[i % E] : x[i]); }
+};
+
+__device__ __forceinline__ void add64(uint64_t* to, uint64_t v) {
+  atomicAdd(reinterpret_cast<unsigned long long*>(to), static_cast<unsigned long long>(v));
+}
+__device__ __forceinline__ void min64(uint64_t* to, uint64_t v) {
+  atomicMin(reinterpret_cast<unsigned long long*>(to), static_cast<unsigned long long>(v));
+}
+__device__ __forceinline__ void max64(uint64_t* to, uint64_t v) {
+  atomicMax(reinterpret_cast<unsigned long long*>(to), static_cast<unsigned long long>(v));
 }
 
-__device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int by) {
-  const unsigned lo = __shfl_up(static_cast<unsigned>(v), by), hi = __shfl_up(static_cast<unsigned>(v >> 32), by);
-  return uint64_t(hi) << 32 | lo;
+template <typename W>
+__device__ __forceinline__ void clear(W* bins) {
+  for (int i = threadIdx.x; i < kBins; i += kThreads) bins[i] = 0;
 }
 
-// The bin in which the sum of the histogram from the front passes `target` (l.bin, with l.before
-// the sum before it and l.bin_count its elements; -1 where the total does not pass it); returns the total.
-__device__ __forceinline__ uint64_t find_bin(SampleLds& l, uint64_t target) {
+// DPP moves of 32 or 64 bits; lanes without a source take 0.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned dpp_or_zero(unsigned v) {
+  return __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_or_zero(uint64_t v) {
+  return uint64_t(dpp_or_zero<CTRL, ROWS>(static_cast<unsigned>(v >> 32))) << 32 | dpp_or_zero<CTRL, ROWS>(static_cast<unsigned>(v));
+}
+// The sum of this lane's and all lower lanes' v.
+template <typename W>
+__device__ __forceinline__ W scan_lanes(W v) {
+  v += dpp_or_zero<0x111, 0xF>(v);  // row_shr: 1, 2, 4, 8 inside rows of 16
+  v += dpp_or_zero<0x112, 0xF>(v);
+  v += dpp_or_zero<0x114, 0xF>(v);
+  v += dpp_or_zero<0x118, 0xF>(v);
+  v += dpp_or_zero<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+  v += dpp_or_zero<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+// The sum over the 16 lanes around, in the last of them.
+__device__ __forceinline__ uint64_t sum_row16(uint64_t v) {
+  v += dpp_or_zero<0x111, 0xF>(v);
+  v += dpp_or_zero<0x112, 0xF>(v);
+  v += dpp_or_zero<0x114, 0xF>(v);
+  return v + dpp_or_zero<0x118, 0xF>(v);
+}
+
+__device__ __forceinline__ uint64_t lane64(uint64_t v, int lane) {
+  return uint64_t(static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane))) << 32 |
+         static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
+}
+
+// The bin in which the sum of the bins from the front passes `target` (l.bin, with l.before
+// the sum before it; -1 where the total does not pass it); returns the total. Barriers on both sides.
+template <typename W>
+__device__ __forceinline__ uint64_t find_bin(SampleLds& l, const W* bins, uint64_t target) {
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   __syncthreads();
-  const uint64_t a = l.hist[2 * threadIdx.x], b = l.hist[2 * threadIdx.x + 1];
-  uint64_t upto = a + b;
-#pragma unroll
-  for (int k = 1; k < kWave; k *= 2) {
-    const uint64_t x = shfl_up64(upto, k);
-    if (lane >= k) upto += x;
-  }
+  const W a = bins[2 * threadIdx.x], b = bins[2 * threadIdx.x + 1];
+  const W upto = scan_lanes(static_cast<W>(a + b));
   if (lane == kWave - 1) l.wave_sum[wave] = upto;
   if (threadIdx.x == 0) l.bin = -1;
   __syncthreads();
@@ -180,12 +232,11 @@ __device__ __forceinline__ uint64_t find_bin(SampleLds& l, uint64_t target) {
     if (w < wave) before += s;
     total += s;
   }
-  before += upto - a - b;
+  before += static_cast<W>(upto - a - b);
   if (before <= target && target < before + a + b) {
     const bool second = target >= before + a;
     l.bin = 2 * threadIdx.x + second;
     l.before = before + (second ? a : 0);
-    l.bin_count = l.count[2 * threadIdx.x + second];
   }
   __syncthreads();
   return total;
@@ -193,106 +244,147 @@ __device__ __forceinline__ uint64_t find_bin(SampleLds& l, uint64_t target) {
 
 // The element of the list that covers `target` when the weights are laid end to end in descending
 // order of place; the target lies inside. weight(place): 0 for those that do not count.
-template <typename W>
-__device__ __forceinline__ uint64_t find_in_list(SampleLds& l, int n, uint64_t lo, uint64_t hi, uint64_t target, W weight) {
+template <typename F>
+__device__ __forceinline__ uint64_t find_in_list(SampleLds& l, int n, uint64_t lo, uint64_t hi, uint64_t target, F weight) {
+  const int lane = threadIdx.x % kWave;
+  if (n <= kWave) {  // one element a lane, every wavefront by itself
+    const uint64_t p = lane < n ? l.list[lane] : 0, w = lane < n ? weight(p) : 0;
+    uint64_t before = 0;
+    for (int j = 0; j < n; ++j) before += lane64(p, j) > p ? lane64(w, j) : 0;
+    const uint64_t hit = __ballot(before <= target && target < before + w);
+    return hit != 0 ? lane64(p, __builtin_ctzll(hit)) : lo;
+  }
   while (lo < hi) {
     const int shift = max(0, 64 - __builtin_clzll(hi - lo) - 11);  // at most kBins bins
-    clear_bins(l);
+    clear(l.hist);
+    clear(l.count);
+    __syncthreads();
     for (int i = threadIdx.x; i < n; i += kThreads) {
-      const uint64_t p = l.list[i];
-      const uint64_t w = p >= lo && p <= hi ? weight(p) : 0;
+      const uint64_t p = l.list[i], w = p >= lo && p <= hi ? weight(p) : 0;
       if (w != 0) {
-        atomicAdd(reinterpret_cast<unsigned long long*>(&l.hist[(hi - p) >> shift]), static_cast<unsigned long long>(w));
+        add64(&l.hist[(hi - p) >> shift], w);
         atomicAdd(&l.count[(hi - p) >> shift], 1u);
       }
     }
-    find_bin(l, target);
+    find_bin(l, l.hist, target);
     if (l.bin < 0) return lo;  // not reached: the target lies inside
+    const bool alone = l.count[l.bin] == 1;
     target -= l.before;
     hi -= uint64_t(l.bin) << shift;
     const uint64_t span = (uint64_t(1) << shift) - 1;
     lo = hi - lo > span ? hi - span : lo;
-    if (l.bin_count == 1) {
+    if (alone) {
       for (int i = threadIdx.x; i < n; i += kThreads) {
         const uint64_t p = l.list[i];
         if (p >= lo && p <= hi && weight(p) != 0) l.lo = p;
       }
       __syncthreads();
       lo = hi = l.lo;
-      __syncthreads();
-    } else {
-      __syncthreads();
     }
+    __syncthreads();
   }
   return lo;
 }
 
-// Elements for which take(x, index) holds, into the list as places; l.n counts them all, l.lo and
-// l.hi are the least and greatest.
-template <typename T, typename F>
-__device__ __forceinline__ void collect(SampleLds& l, const T* row, int vocab, F take) {
+// Starts a collection of elements: l.n counts them, l.lo and l.hi are the least and greatest places.
+__device__ __forceinline__ void begin_list(SampleLds& l) {
+  __syncthreads();
   if (threadIdx.x == 0) {
     l.n = 0;
     l.lo = ~uint64_t(0);
     l.hi = 0;
   }
   __syncthreads();
+}
+// Appends this lane's element, if it is one; all lanes take part. What the list has no room for is counted.
+__device__ __forceinline__ void append(SampleLds& l, bool mine, float x, int i) {
+  const uint64_t all = __ballot(mine);
+  if (all == 0) return;
+  const int lane = threadIdx.x % kWave, first = __builtin_ctzll(all);
+  unsigned at = 0;
+  if (lane == first) at = atomicAdd(&l.n, static_cast<unsigned>(__popcll(all)));
+  at = __builtin_amdgcn_readlane(at, first);
+  if (mine) {
+    const uint64_t p = place(x, i);
+    at += __popcll(all & ((uint64_t(1) << lane) - 1));
+    if (at < kList) l.list[at] = p;
+    min64(&l.lo, p);
+    max64(&l.hi, p);
+  }
+}
+
+// u times the total as a whole number below it.
+__device__ __forceinline__ uint64_t drawn(float u, uint64_t total) {
+  const double want = (u > 0.0f ? static_cast<double>(u) : 0.0) * static_cast<double>(total);
+  return want < static_cast<double>(total) ? min(static_cast<uint64_t>(want), total - 1) : total - 1;
+}
+// The last of the weights' units that top_p leaves.
+__device__ __forceinline__ uint64_t last_unit(float top_p, uint64_t total) {
+  const double want = ceil(static_cast<double>(top_p > 0.0f ? top_p : 0.0f) * static_cast<double>(total));
+  return want >= 1.0 ? (want < static_cast<double>(total) ? static_cast<uint64_t>(want) : total) - 1 : 0;
+}
+
+// All that is left to do for a list of up to 64 elements among which are all that may stay, one a
+// lane of one wavefront.
+__device__ __forceinline__ void draw_small(const SampleLds& l, const SampleRow& r, int n, int top_k, float top_p, float u, int64_t* out) {
   const int lane = threadIdx.x % kWave;
-  each(row, vocab, [&](float x, int i) {
-    const bool mine = take(x, i);
-    const uint64_t all = __ballot(mine);
-    if (all == 0) return;
-    const int first = __builtin_ctzll(all);
-    unsigned at = 0;
-    if (lane == first) at = atomicAdd(&l.n, static_cast<unsigned>(__popcll(all)));
-    at = __builtin_amdgcn_readlane(at, first);
-    if (mine) {
-      const uint64_t p = place(x, i);
-      at += __popcll(all & ((uint64_t(1) << lane) - 1));
-      if (at < kList) l.list[at] = p;
-      atomicMin(reinterpret_cast<unsigned long long*>(&l.lo), static_cast<unsigned long long>(p));
-      atomicMax(reinterpret_cast<unsigned long long*>(&l.hi), static_cast<unsigned long long>(p));
-    }
-  });
-  __syncthreads();
+  const uint64_t p = lane < n ? l.list[lane] : 0, w = lane < n ? weight_of(l, r, value_at(p)) : 0;
+  int rank = 0;
+  uint64_t before = 0;
+  for (int j = 0; j < n; ++j) {
+    const bool above = lane64(p, j) > p;
+    rank += above;
+    before += above ? lane64(w, j) : 0;
+  }
+  bool stays = lane < n && rank < top_k;
+  const uint64_t last = __ballot(lane < n && rank == min(top_k, n) - 1);
+  const uint64_t total = lane64(before + w, __builtin_ctzll(last | uint64_t(1) << 63));
+  if (top_p < 1.0f) stays = stays && before <= last_unit(top_p, total);
+  stays = stays && value_at(p) >= r.keep;
+  const uint64_t kept = __ballot(stays);
+  uint64_t sum = 0, upto = 0;
+  for (int j = 0; j < n; ++j) {
+    if (!(kept >> j & 1)) continue;
+    const uint64_t x = lane64(w, j);
+    sum += x;
+    upto += static_cast<unsigned>(lane64(p, j)) > static_cast<unsigned>(p) ? x : 0;  // a lower index
+  }
+  const uint64_t target = drawn(u, sum);
+  if (stays && upto <= target && target < upto + w) *out = index_at(p);
 }
 
-// The sum of the 16 lanes around, in all of them.
-template <int CTRL>
-__device__ __forceinline__ uint64_t dpp_mov64(uint64_t v) {
-  const unsigned lo = __builtin_amdgcn_mov_dpp(static_cast<int>(v), CTRL, 0xF, 0xF, false);
-  const unsigned hi = __builtin_amdgcn_mov_dpp(static_cast<int>(v >> 32), CTRL, 0xF, 0xF, false);
-  return uint64_t(hi) << 32 | lo;
-}
-__device__ __forceinline__ uint64_t sum16(uint64_t v) {
-  v += dpp_mov64<0xB1>(v);
-  v += dpp_mov64<0x4E>(v);
-  v += dpp_mov64<0x141>(v);
-  return v + dpp_mov64<0x140>(v);
-}
-
-template <typename T>
+template <typename T, bool HELD>
 __global__ __launch_bounds__(kThreads) void sample_rows(SampleDev a) {
   __shared__ SampleLds l;
+  __shared__ __align__(16) unsigned char held_row[HELD ? kHeldBytes : 16];
   const int64_t n = blockIdx.x;
-  const T* const row = static_cast<const T*>(a.x) + n * a.stride;
+  Row<T, HELD> row;
+  row.x = static_cast<const T*>(a.x) + n * a.stride;
+  row.vocab = a.vocab;
+  row.held = reinterpret_cast<typename Row<T, HELD>::P*>(held_row);
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const float temperature = a.temperatures ? a.temperatures[n] : a.temperature;
   const int top_k = a.top_ks ? a.top_ks[n] : a.top_k;
-  const float top_p = a.top_ps ? a.top_ps[n] : a.top_p, min_p = a.min_ps ? a.min_ps[n] : a.min_p;
+  const float top_p = a.top_ps ? a.top_ps[n] : a.top_p, min_p = a.min_ps ? a.min_ps[n] : a.min_p, u = a.u[n];
   const bool greedy = !(temperature > 0.0f) || top_k == 1;
   if (threadIdx.x < 128) l.pow2[threadIdx.x] = exp2(threadIdx.x / 128.0);
 
   // The largest logit, the first that has it, and the least that is not ruled out.
   float top = -__builtin_inff(), low = __builtin_inff();
   int at = a.vocab;
-  each(row, a.vocab, [&](float x, int i) {
-    if (x > top) {
-      top = x;
-      at = i;
-    }
-    if (x > -__builtin_inff()) low = __builtin_fminf(low, x);
-  });
+  if (greedy) {
+    row.template each<true>([&](float x, int i) {
+      if (x > top) {
+        top = x;
+        at = i;
+      }
+    });
+  } else {
+    row.template each<true>([&](float x, int) {
+      top = __builtin_fmaxf(top, x);
+      low = __builtin_fminf(low, x > -__builtin_inff() ? x : __builtin_inff());
+    });
+  }
 #pragma unroll
   for (int k = 1; k < kWave; k *= 2) {
     const float x = __shfl_xor(top, k), y = __shfl_xor(low, k);
@@ -306,6 +398,9 @@ __global__ __launch_bounds__(kThreads) void sample_rows(SampleDev a) {
     l.wave_low[wave] = low;
     l.wave_at[wave] = at;
   }
+  clear(l.regions);
+  clear(l.hist);
+  clear(l.count);
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
@@ -321,110 +416,99 @@ __global__ __launch_bounds__(kThreads) void sample_rows(SampleDev a) {
 
   SampleRow r;
   r.top = top;
+  r.top64 = static_cast<double>(top);
   r.per_unit = 1.4426950408889634074 / static_cast<double>(temperature);
   r.bits = a.weight_bits;
-  r.dead = static_cast<float>(r.bits + 1);
-  r.low = min_p > 0.0f ? fmax(0.0, -log2(static_cast<double>(min_p))) : __builtin_inf();
-  const double reach = r.per_unit > 0 ? r.dead / r.per_unit : __builtin_inf();
-  const float span = static_cast<float>(fmin(static_cast<double>(top) - static_cast<double>(low), reach));
+  r.flat = !(top < __builtin_inff()) || !(r.per_unit > 0.0);
+  const auto below_top = [&](double units) {  // the logit so many log2 units down
+    return r.flat ? (top < __builtin_inff() ? -std::numeric_limits<float>::max() : top)
+                  : __builtin_fmaxf(static_cast<float>(r.top64 - units / r.per_unit), -std::numeric_limits<float>::max());
+  };
+  r.floor = below_top(r.bits + 1);
+  // As many tokens weigh less than 2^-t of the largest each as there are: together less than 1 - top_p for this t.
+  r.tail = top_p < 1.0f ? below_top(fmin(64.0, log2(static_cast<double>(a.vocab) / (1.0 - static_cast<double>(fmaxf(top_p, 0.0f)))) + 1.0)) : 0.0f;
+  r.keep = -std::numeric_limits<float>::max();
+  if (min_p >= 1.0f) {
+    r.keep = top;
+  } else if (min_p > 0.0f && !r.flat) {
+    const double from = r.top64 + log(static_cast<double>(min_p)) * static_cast<double>(temperature);
+    r.keep = __builtin_fmaxf(static_cast<float>(from), r.keep);
+    if (static_cast<double>(r.keep) < from) r.keep = from_sort_bits(sort_bits(r.keep) + 1);  // the next one up
+  }
+  const float span = top - __builtin_fmaxf(low, r.floor);
   r.per_bin = span > 0.0f && span < __builtin_inff() ? static_cast<float>(kBins) / span : 0.0f;
 
   uint64_t least = 0;   // the place of the last element that stays
-  bool listed = false;  // whether all that stay are in the list
+  bool listed = false;  // whether all that may stay are in the list
+  bool summed = false;  // whether l.regions holds the sums of all that stay
   int held = 0;
-  const auto in = [&](float x, int i, double& t) {
-    t = depth(r, x);
-    return is_live(r, x, t) && place(x, i) >= least;
-  };
-  const auto mass = [&](uint64_t p) { return p >= least ? weight_of(l, r, depth(r, value_at(p))) : 0; };
+  const auto in = [&](float x, int i) { return x >= r.floor && place(x, i) >= least; };
+  const auto mass = [&](uint64_t p) { return p >= least ? weight_of(l, r, value_at(p)) : 0; };
   const auto one = [&](uint64_t p) { return static_cast<uint64_t>(p >= least); };
 
-  // The element that covers the target, among those of the histogram's bin l.bin.
-  const auto resolve = [&](uint64_t target, bool counts) {
-    const int bin = l.bin;
-    uint64_t lo = 0, hi = ~uint64_t(0);
-    target -= l.before;
+  // The element that covers the target, among those of bin l.bin that the list had no room for: bins of their places.
+  const auto resolve = [&](uint64_t lo, uint64_t hi, uint64_t target, bool counts) {
     for (;;) {
-      collect(l, row, a.vocab, [&](float x, int i) {
-        double t;
-        const uint64_t p = place(x, i);
-        return bin_of(r, x) == bin && p >= lo && p <= hi && in(x, i, t);
-      });
-      lo = l.lo;
-      hi = l.hi;
-      const unsigned found = l.n;
-      __syncthreads();
-      if (found <= kList) {
-        return counts ? find_in_list(l, static_cast<int>(found), lo, hi, target, one)
-                      : find_in_list(l, static_cast<int>(found), lo, hi, target, mass);
-      }
-      // Too many for the list: bins of their places.
       const int shift = max(0, 64 - __builtin_clzll(hi - lo) - 11);
-      clear_bins(l);
-      each(row, a.vocab, [&](float x, int i) {
-        double t;
+      __syncthreads();
+      clear(l.hist);
+      __syncthreads();
+      row.each([&](float x, int i) {
         const uint64_t p = place(x, i);
-        if (p < lo || p > hi || !in(x, i, t)) return;
-        const uint64_t w = counts ? 1 : weight_of(l, r, t);
-        atomicAdd(reinterpret_cast<unsigned long long*>(&l.hist[(hi - p) >> shift]), static_cast<unsigned long long>(w));
+        if (p >= lo && p <= hi && in(x, i)) add64(&l.hist[(hi - p) >> shift], counts ? 1 : weight_of(l, r, x));
       });
-      find_bin(l, target);
-      if (l.bin < 0) return lo;  // not reached
+      find_bin(l, l.hist, target);
+      if (l.bin < 0) return lo;  // not reached: the target lies inside
       target -= l.before;
       hi -= uint64_t(l.bin) << shift;
       const uint64_t width = (uint64_t(1) << shift) - 1;
       lo = hi - lo > width ? hi - width : lo;
+      begin_list(l);
+      row.each([&](float x, int i) {
+        const uint64_t p = place(x, i);
+        append(l, p >= lo && p <= hi && in(x, i), x, i);
+      });
       __syncthreads();
+      lo = l.lo;
+      hi = l.hi;
+      const unsigned found = l.n;
+      if (found <= kList)
+        return counts ? find_in_list(l, static_cast<int>(found), lo, hi, target, one)
+                      : find_in_list(l, static_cast<int>(found), lo, hi, target, mass);
     }
   };
 
   if (top_k > 0) {
-    clear_bins(l);
-    each(row, a.vocab, [&](float x, int i) {
-      double t;
-      if (in(x, i, t)) atomicAdd(reinterpret_cast<unsigned long long*>(&l.hist[bin_of(r, x)]), 1ull);
+    row.each([&](float x, int) {
+      if (x >= r.floor) atomicAdd(&l.count[bin_of(r, x)], 1u);
     });
-    find_bin(l, static_cast<uint64_t>(top_k) - 1);
+    find_bin(l, l.count, static_cast<uint64_t>(top_k) - 1);
     const int bin = l.bin;
     if (bin >= 0) {
-      const uint64_t all = l.before + l.hist[bin];
-      if (all <= kList) {
-        __syncthreads();
-        collect(l, row, a.vocab, [&](float x, int i) {
-          double t;
-          return in(x, i, t) && bin_of(r, x) <= bin;
-        });
-        listed = true;
-        held = static_cast<int>(l.n);
-        const uint64_t lo = l.lo, hi = l.hi;
-        __syncthreads();
-        least = find_in_list(l, held, lo, hi, static_cast<uint64_t>(top_k) - 1, one);
-      } else {
-        least = resolve(static_cast<uint64_t>(top_k) - 1, true);
+      const uint64_t before = l.before;
+      listed = before + l.count[bin] <= kList;
+      begin_list(l);
+      row.each([&](float x, int i) {
+        const int b = bin_of(r, x);
+        append(l, x >= r.floor && (listed ? b <= bin : b == bin), x, i);
+      });
+      __syncthreads();
+      held = static_cast<int>(l.n);
+      const uint64_t lo = l.lo, hi = l.hi;
+      if (listed && held <= kWave) {
+        if (wave == 0) draw_small(l, r, held, top_k, top_p, u, a.out + n);
+        return;
       }
+      const uint64_t target = static_cast<uint64_t>(top_k) - 1 - (listed ? 0 : before);
+      least = held <= kList ? find_in_list(l, held, lo, hi, target, one) : resolve(lo, hi, target, true);
     }
+    __syncthreads();
+    clear(l.hist);
   }
 
   if (top_p < 1.0f) {
-    clear_bins(l);
     if (listed) {
-      for (int i = threadIdx.x; i < held; i += kThreads) {
-        const uint64_t p = l.list[i];
-        if (p >= least)
-          atomicAdd(reinterpret_cast<unsigned long long*>(&l.hist[bin_of(r, value_at(p))]), static_cast<unsigned long long>(mass(p)));
-      }
-    } else {
-      each(row, a.vocab, [&](float x, int i) {
-        double t;
-        if (in(x, i, t))
-          atomicAdd(reinterpret_cast<unsigned long long*>(&l.hist[bin_of(r, x)]), static_cast<unsigned long long>(weight_of(l, r, t)));
-      });
-    }
-    const uint64_t total = find_bin(l, 0);
-    const double want = ceil(static_cast<double>(top_p > 0.0f ? top_p : 0.0f) * static_cast<double>(total));
-    const uint64_t target = want >= 1.0 ? (want < static_cast<double>(total) ? static_cast<uint64_t>(want) : total) - 1 : 0;
-    find_bin(l, target);
-    if (listed) {
+      __syncthreads();
       uint64_t lo = ~uint64_t(0), hi = 0;
       if (threadIdx.x == 0) {
         l.lo = lo;
@@ -432,65 +516,114 @@ __global__ __launch_bounds__(kThreads) void sample_rows(SampleDev a) {
       }
       __syncthreads();
       for (int i = threadIdx.x; i < held; i += kThreads) {
-        lo = min(lo, l.list[i]);
-        hi = max(hi, l.list[i]);
+        const uint64_t p = l.list[i];
+        if (p < least) continue;
+        add64(&l.hist[i % kBins], mass(p));  // for the total only
+        lo = min(lo, p);
+        hi = max(hi, p);
       }
-      atomicMin(reinterpret_cast<unsigned long long*>(&l.lo), static_cast<unsigned long long>(lo));
-      atomicMax(reinterpret_cast<unsigned long long*>(&l.hi), static_cast<unsigned long long>(hi));
-      __syncthreads();
+      if (hi != 0) {
+        min64(&l.lo, lo);
+        max64(&l.hi, hi);
+      }
+      const uint64_t total = find_bin(l, l.hist, 0);
       lo = l.lo;
       hi = l.hi;
       __syncthreads();
-      least = find_in_list(l, held, lo, hi, target, mass);
+      least = find_in_list(l, held, lo, hi, last_unit(top_p, total), mass);
     } else {
-      least = resolve(target, false);
+      __syncthreads();
+      uint64_t rest = 0;
+      row.each([&](float x, int i) {
+        if (!in(x, i)) return;
+        const uint64_t w = weight_of(l, r, x);
+        if (x < r.tail) rest += w;
+        else add64(&l.hist[bin_of(r, x)], w);
+      });
+      if (rest != 0) add64(&l.hist[kBins - 1], rest);  // behind the target in any case
+      const uint64_t total = find_bin(l, l.hist, 0), target = last_unit(top_p, total);
+      find_bin(l, l.hist, target);
+      const int bin = l.bin;
+      const uint64_t before = l.before;
+      // The bin's elements into the list, and those above it, which stay, to their parts of the row.
+      begin_list(l);
+      row.each_packet([&](const auto& p, int i) {
+        uint64_t sum = 0;
+#pragma unroll
+        for (int e = 0; e < 16 / static_cast<int>(sizeof(T)); ++e) {
+          const float x = to_f32(p.e[e]);
+          const int b = bin_of(r, x);
+          const bool live = x >= r.floor;
+          if (live && b < bin && x >= r.keep && place(x, i + e) >= least) sum += weight_of(l, r, x);
+          append(l, live && b == bin && place(x, i + e) >= least, x, i + e);
+        }
+        if (__ballot(sum != 0) == 0) return;
+        sum = sum_row16(sum);  // a part of the row is whole runs of 16 lanes' packets
+        if (lane % 16 == 15 && sum != 0) add64(&l.regions[i >> a.region_log2], sum);
+      });
+      __syncthreads();
+      const int found = static_cast<int>(l.n);
+      const uint64_t lo = l.lo, hi = l.hi;
+      if (found <= kList) {
+        least = find_in_list(l, found, lo, hi, target - before, mass);
+        for (int i = threadIdx.x; i < found; i += kThreads) {
+          const uint64_t p = l.list[i];
+          if (p >= least && value_at(p) >= r.keep) add64(&l.regions[index_at(p) >> a.region_log2], weight_of(l, r, value_at(p)));
+        }
+        summed = true;
+      } else {
+        __syncthreads();
+        clear(l.regions);
+        least = resolve(lo, hi, target - before, false);
+      }
     }
   }
 
   // By index: the part of the row in which the sum passes the number drawn, then the token.
-  const auto stays = [&](float x, int i, double& t) { return in(x, i, t) && t <= r.low; };
-  clear_bins(l);
+  const auto stays = [&](float x, int i) { return in(x, i) && x >= r.keep; };
+  __syncthreads();
   if (listed) {
     for (int i = threadIdx.x; i < held; i += kThreads) {
-      double t;
       const uint64_t p = l.list[i];
-      if (stays(value_at(p), index_at(p), t))
-        atomicAdd(reinterpret_cast<unsigned long long*>(&l.hist[index_at(p) >> a.region_log2]),
-                  static_cast<unsigned long long>(weight_of(l, r, t)));
+      if (stays(value_at(p), index_at(p))) add64(&l.regions[index_at(p) >> a.region_log2], weight_of(l, r, value_at(p)));
     }
-  } else {
-    each_packet(row, a.vocab, [&](const auto& p, int i) {
+  } else if (!summed) {
+    row.each_packet([&](const auto& p, int i) {
       uint64_t sum = 0;
 #pragma unroll
       for (int e = 0; e < 16 / static_cast<int>(sizeof(T)); ++e) {
-        double t;
-        if (stays(to_f32(p.e[e]), i + e, t)) sum += weight_of(l, r, t);
+        const float x = to_f32(p.e[e]);
+        if (stays(x, i + e)) sum += weight_of(l, r, x);
       }
-      sum = sum16(sum);  // a part of the row is whole runs of 16 lanes' packets
-      if (lane % 16 == 0 && sum != 0)
-        atomicAdd(reinterpret_cast<unsigned long long*>(&l.hist[i >> a.region_log2]), static_cast<unsigned long long>(sum));
+      sum = sum_row16(sum);
+      if (lane % 16 == 15 && sum != 0) add64(&l.regions[i >> a.region_log2], sum);
     });
   }
-  const uint64_t total = find_bin(l, 0);
-  const float u = a.u[n];
-  const double want = (u > 0.0f ? static_cast<double>(u) : 0.0) * static_cast<double>(total);
-  const uint64_t target = want < static_cast<double>(total) ? min(static_cast<uint64_t>(want), total - 1) : total - 1;
-  find_bin(l, target);
+  const uint64_t total = find_bin(l, l.regions, 0), target = drawn(u, total);
+  find_bin(l, l.regions, target);
   const int region = max(l.bin, 0) << a.region_log2;
   const uint64_t rest = target - l.before;
-  __syncthreads();
   for (int i = threadIdx.x; i < kBins; i += kThreads) {
     uint64_t w = 0;
     if (i < (1 << a.region_log2) && region + i < a.vocab) {
-      const float x = to_f32(row[region + i]);
-      double t;
-      if (stays(x, region + i, t)) w = weight_of(l, r, t);
+      const float x = row.at(region + i);
+      if (stays(x, region + i)) w = weight_of(l, r, x);
     }
     l.hist[i] = w;
   }
-  find_bin(l, rest);
+  find_bin(l, l.hist, rest);
   if (threadIdx.x == 0) a.out[n] = region + max(l.bin, 0);
 }
+
+namespace {
+
+template <typename T>
+void launch_rows(const SampleDev& d, dim3 grid, hipStream_t stream) {
+  if (d.vocab * sizeof(T) <= kHeldBytes) AKO_LAUNCH((sample_rows<T, true>), grid, dim3(kThreads), 0, stream, d);
+  else AKO_LAUNCH((sample_rows<T, false>), grid, dim3(kThreads), 0, stream, d);
+}
+
+}  // namespace
 
 hipError_t launch_sample(const SampleArgs& a, hipStream_t stream) {
   SampleDev d{};
@@ -512,7 +645,7 @@ hipError_t launch_sample(const SampleArgs& a, hipStream_t stream) {
   d.stride = a.stride;
   constexpr int64_t kRows = int64_t(1) << 21;  // per launch: work-items stay below 2^32
   for (int64_t r = 0; r < a.rows; r += kRows) {
-    const dim3 grid(static_cast<unsigned>(std::min(kRows, a.rows - r))), block(kThreads);
+    const dim3 grid(static_cast<unsigned>(std::min(kRows, a.rows - r)));
     d.x = static_cast<const char*>(a.x) + r * a.stride * dtype_bytes(a.dtype);
     d.u = a.u + r;
     d.temperatures = a.temperatures ? a.temperatures + r : nullptr;
@@ -521,9 +654,9 @@ hipError_t launch_sample(const SampleArgs& a, hipStream_t stream) {
     d.min_ps = a.min_ps ? a.min_ps + r : nullptr;
     d.out = a.out + r;
     switch (a.dtype) {
-      case kF32: AKO_LAUNCH((sample_rows<float>), grid, block, 0, stream, d); break;
-      case kF16: AKO_LAUNCH((sample_rows<_Float16>), grid, block, 0, stream, d); break;
-      case kBF16: AKO_LAUNCH((sample_rows<__bf16>), grid, block, 0, stream, d); break;
+      case kF32: launch_rows<float>(d, grid, stream); break;
+      case kF16: launch_rows<_Float16>(d, grid, stream); break;
+      case kBF16: launch_rows<__bf16>(d, grid, stream); break;
       default: return hipErrorInvalidValue;
     }
     const hipError_t err = hipGetLastError();

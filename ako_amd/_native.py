@@ -116,8 +116,9 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "ako_paged_select_workspace": (_i64, [_ptr, _i64, _i64, _int]),
     "ako_sample_fwd": (
         _int,
-        [_ptr, _ptr, _ptr, _f32, _ptr, ctypes.c_int32, _ptr, _f32, _ptr, _f32, _ptr, _i64, _i64, _i64, _int, _ptr],
+        [_ptr, _ptr, _ptr, _f32, _ptr, ctypes.c_int32, _ptr, _f32, _ptr, _f32, _ptr, _i64, _i64, _i64, _ptr, _i64, _int, _ptr],
     ),
+    "ako_sample_workspace": (_i64, [_i64, _i64]),
     "ako_set_tuning": (_int, [_int, _int, _int]),
     "ako_time_next_launch": (_int, [_ptr, _ptr]),
 }

@@ -1185,13 +1185,23 @@ int64_t ako_paged_select_workspace(const ako_paged_t* cache, int64_t q_heads, in
 }
 
 // --------------------------------------------------------------- sampling --
+static constexpr int64_t kMaxVocab = int64_t(1) << 22;
+
+int64_t ako_sample_workspace(int64_t rows, int64_t vocab) {
+  if (rows < 0 || rows > kMaxInt || vocab < 1 || vocab > kMaxVocab) {
+    fail(AKO_ERR_INVALID_ARGUMENT, "ako_sample_workspace: rows must be 0 to 2^31-1 and vocab 1 to %lld", (long long)kMaxVocab);
+    return -1;
+  }
+  return rows == 0 ? 0 : ako::sample_workspace(rows, vocab);
+}
+
 int ako_sample_fwd(const void* logits, const float* uniform, const float* temperature, float temperature_all,
                    const int32_t* top_k, int32_t top_k_all, const float* top_p, float top_p_all, const float* min_p,
-                   float min_p_all, int64_t* out, int64_t rows, int64_t vocab, int64_t row_stride, int dtype, void* stream) {
+                   float min_p_all, int64_t* out, int64_t rows, int64_t vocab, int64_t row_stride, void* workspace,
+                   int64_t workspace_bytes, int dtype, void* stream) {
   const char* fn = "ako_sample_fwd";
   if (!valid_dtype(dtype)) return fail(AKO_ERR_UNSUPPORTED, "%s: unknown dtype code %d", fn, dtype);
-  if (rows < 0) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: negative size", fn);
-  constexpr int64_t kMaxVocab = int64_t(1) << 22;
+  if (rows < 0 || rows > kMaxInt) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: rows must be 0 to 2^31-1", fn);
   if (vocab < 1 || vocab > kMaxVocab)
     return fail(AKO_ERR_INVALID_ARGUMENT, "%s: vocab must be 1 to %lld, got %lld", fn, (long long)kMaxVocab, (long long)vocab);
   if (!temperature && !(temperature_all >= 0.0f))
@@ -1204,16 +1214,21 @@ int ako_sample_fwd(const void* logits, const float* uniform, const float* temper
   if (row_stride < 0) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: negative row stride", fn);
   const Span in = span_2d(logits, rows, vocab, row_stride, ako::dtype_bytes(dtype));
   const Span o = span_2d(out, 1, rows, rows, 8);
+  const int64_t need = ako::sample_workspace(rows, vocab);
+  if (workspace_bytes < need || (need > 0 && (!workspace || !aligned(workspace, 16))))
+    return fail(AKO_ERR_INVALID_ARGUMENT, "%s: needs a 16-byte aligned workspace of %lld bytes, got %lld", fn,
+                (long long)need, (long long)workspace_bytes);
+  const Span ws = span_bytes(workspace, need);
   const void* const per_row[5] = {uniform, temperature, top_k, top_p, min_p};
-  bool ok = in.ok && o.ok, apart = !overlap(o, in);
+  bool ok = in.ok && o.ok && ws.ok, apart = !overlap(o, in) && !overlap(ws, in) && !overlap(ws, o);
   for (const void* p : per_row) {
     if (!p) continue;
     const Span s = span_2d(p, 1, rows, rows, 4);
     ok = ok && s.ok;
-    apart = apart && !overlap(o, s);
+    apart = apart && !overlap(o, s) && !overlap(ws, s);
   }
   if (!ok) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: sizes and strides overflow the address space", fn);
-  if (!apart) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: out overlaps an input", fn);
+  if (!apart) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: out or the workspace overlaps another buffer", fn);
   ako::SampleArgs a{};
   a.x = logits;
   a.rows = rows;
@@ -1229,6 +1244,7 @@ int ako_sample_fwd(const void* logits, const float* uniform, const float* temper
   a.top_p = top_p_all;
   a.min_p = min_p_all;
   a.out = out;
+  a.workspace = workspace;
   a.dtype = dtype;
   return hip_status(ako::launch_sample(a, static_cast<hipStream_t>(stream)), fn);
 }

@@ -280,8 +280,10 @@ struct SampleArgs {
   float temperature, top_p, min_p;
   int top_k;
   int64_t* out;
+  void* workspace;  // sample_workspace bytes
   int dtype;
 };
+int64_t sample_workspace(int64_t rows, int64_t vocab);
 hipError_t launch_sample(const SampleArgs& a, hipStream_t stream);
 
 }  // namespace ako

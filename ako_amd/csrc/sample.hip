@@ -23,6 +23,7 @@
 // target, bins of their 64-bit numbers, until one element is left.
 
 #include <algorithm>
+#include <cmath>
 #include <limits>
 
 #include "common.h"
@@ -43,6 +44,11 @@ struct SampleDev {
   int top_k;
   int64_t* out;
   int vocab, weight_bits, region_log2;
+  // Rows divided over `parts` workgroups of `chunk` tokens (parts 1: not): each row's share of the workspace.
+  unsigned char* space;
+  int parts, chunk;
+  FastDiv by_parts;
+  double pow2[128];  // 2^(j / 128)
 };
 
 constexpr int kThreads = 1024, kWaves = kThreads / kWave;
@@ -63,16 +69,34 @@ __device__ __forceinline__ uint64_t place(float x, int index) {
 __device__ __forceinline__ float value_at(uint64_t place) { return from_sort_bits(static_cast<unsigned>(place >> 32)); }
 __device__ __forceinline__ int index_at(uint64_t place) { return static_cast<int>(0xffffffffu - static_cast<unsigned>(place)); }
 
+// What the kernels of a divided row leave for the next: what its workgroups found of the largest logit, the
+// histogram of the first stage, the sums of the row's parts, and the elements of the bin.
+struct SampleFound {
+  float top, low;
+  int at;
+};
+constexpr int kMaxParts = 64;
+struct SampleSpace {
+  uint64_t hist[kBins];
+  uint64_t regions[kBins];
+  uint64_t list[kList];
+  SampleFound found[kMaxParts];
+  unsigned n;  // elements of the bin
+  unsigned pad[31];
+};
+__device__ __forceinline__ SampleSpace* space_of(const SampleDev& a, int64_t n) {
+  return reinterpret_cast<SampleSpace*>(a.space) + n;
+}
+
 // What a row's threads share.
 struct SampleLds {
   uint64_t hist[kBins];     // weights by bin of depth, or of place
   uint64_t regions[kBins];  // weights by part of the row
   uint64_t list[kList];
-  unsigned count[kBins];
+  unsigned count[kBins];    // elements by bin of place
   double pow2[128];         // 2^(j / 128)
   uint64_t wave_sum[kWaves];
-  float wave_top[kWaves], wave_low[kWaves];
-  int wave_at[kWaves];
+  SampleFound found[kWaves];
   uint64_t lo, hi;          // of the elements of a bin
   unsigned n;               // elements of a bin
   int bin;
@@ -81,23 +105,24 @@ struct SampleLds {
 
 // The row's own numbers, the same in all threads.
 struct SampleRow {
-  double top64, per_unit;  // the largest logit, and log2(e) / T
+  double top64, per_unit;  // the largest finite logit, and log2(e) / T (0 where all that count weigh the same)
   float top;
   float floor;             // elements from here on weigh something; not -infinity
   float keep;              // elements from here on reach min_p
   float tail;              // elements below here weigh less than 1 - top_p of all together
   float per_bin;           // bins of a unit of logits
-  int bits;                // S
-  bool flat;               // all that weigh anything weigh the same
+  double bits;             // S
 };
 
 // 2^(S - t), t log2 units below the largest, rounded to a whole number: 2^(j / 128) from a table
 // times 2^z of the rest z, at most 1/256, by its Taylor polynomial of degree 4, off by less than 2^-49.
-__device__ __forceinline__ uint64_t weight_of(const SampleLds& l, const SampleRow& r, float x) {
-  if (r.flat) return uint64_t(1) << r.bits;
+// Meaningless below r.floor.
+template <typename Lds>
+__device__ __forceinline__ uint64_t weight_of(const Lds& l, const SampleRow& r, float x) {
   constexpr double kRound = 0x1.8p45;  // its last bit is 1/128
   constexpr double kLn2 = 0.69314718055994530942;
-  const double y = __builtin_fma(static_cast<double>(x) - r.top64, r.per_unit, static_cast<double>(r.bits));
+  const double down = static_cast<double>(__builtin_fminf(x, std::numeric_limits<float>::max())) - r.top64;
+  const double y = __builtin_fma(down, r.per_unit, r.bits);
   const double near = y + kRound, z = y - (near - kRound);
   const int j = static_cast<int>(__builtin_bit_cast(uint64_t, near));
   double p = __builtin_fma(z, kLn2 * kLn2 * kLn2 * kLn2 / 24, kLn2 * kLn2 * kLn2 / 6);
@@ -112,58 +137,84 @@ __device__ __forceinline__ int bin_of(const SampleRow& r, float x) {
   return d < static_cast<float>(kBins - 1) ? static_cast<int>(d) : kBins - 1;
 }
 
-// The row in packets of 16 bytes: read again for every pass, kRounds of the workgroup's packets
-// at a time, or (HELD) kept in LDS after the first.
+// The row in packets of 16 bytes, read again for every pass or (HELD) kept in LDS after the
+// first. What is left behind the last whole packet comes as packets of one element, in a round of its own.
 constexpr int kHeldBytes = 1 << 16;
-template <typename T, bool HELD>
+template <typename T, bool HELD, int THREADS = kThreads>
 struct Row {
-  static constexpr int E = 16 / static_cast<int>(sizeof(T)), kRounds = HELD ? 1 : 4;
+  static constexpr int E = 16 / static_cast<int>(sizeof(T));
   using P = Pack<T, E>;
   const T* x;
-  int vocab;
-  P* held;  // HELD: packet i in place i
+  int whole, rest;  // whole packets, elements behind them
+  P* held;          // HELD: round k's packets from place k * THREADS on
 
+  __device__ __forceinline__ Row(const T* row, int vocab, P* lds) : x(row), whole(vocab / E), rest(vocab % E), held(lds) {}
+  __device__ __forceinline__ int rounds() const { return (whole + THREADS - 1) / THREADS + (rest > 0); }
+  // The index of the first element of this thread's packet; in the round behind the whole packets that of its only one.
+  __device__ __forceinline__ int index(int round) const {
+    const int i = round * THREADS + static_cast<int>(threadIdx.x);
+    if (rest == 0 || round + 1 < rounds()) return i * E;
+    return whole * E + (static_cast<int>(threadIdx.x) < rest ? static_cast<int>(threadIdx.x) : 0);
+  }
   // -infinity behind the end.
-  __device__ __forceinline__ P packet(int i) const {
-    if (i + E <= vocab) return load_pack<T, E>(x + i);
+  __device__ __forceinline__ P packet(int round) const {
     P p;
 #pragma unroll
-    for (int e = 0; e < E; ++e) p.e[e] = i + e < vocab ? x[i + e] : from_f32<T>(-__builtin_inff());
+    for (int e = 0; e < E; ++e) p.e[e] = from_f32<T>(-__builtin_inff());
+    const int i = round * THREADS + static_cast<int>(threadIdx.x);
+    if (rest == 0 || round + 1 < rounds()) {
+      if (i < whole) p = load_pack<T, E>(x + int64_t(i) * E);
+    } else if (static_cast<int>(threadIdx.x) < rest) {
+      p.e[0] = x[whole * E + threadIdx.x];
+    }
     return p;
   }
-  // f(packet, index of its first element); all threads take part in every call. FIRST: of the row's first pass.
-  template <bool FIRST = false, typename F>
-  __device__ __forceinline__ void each_packet(F f) {
-    constexpr int kAtOnce = HELD && FIRST ? 4 : kRounds;
-    const int mine = static_cast<int>(threadIdx.x) * E;
+  // f(packet, index of its first element); all threads take part in every call. The next round's
+  // packet is on its way while this one is worked on.
+  template <typename F>
+  __device__ __forceinline__ void each_packet(F f) const {
+    const int n = rounds();
+    P next;
+    if (!HELD) next = packet(0);
 #pragma unroll 1
-    for (int base = 0; base < vocab; base += kThreads * E * kAtOnce) {
-      P p[kAtOnce];
-#pragma unroll
-      for (int u = 0; u < kAtOnce; ++u) {
-        const int i = base + u * kThreads * E + mine;
-        if (HELD && !FIRST) p[u] = held[i / E];
-        else p[u] = packet(i);
+    for (int k = 0; k < n; ++k) {
+      P p;
+      if (HELD) {
+        p = held[k * THREADS + threadIdx.x];
+      } else {
+        p = next;
+        if (k + 1 < n) next = packet(k + 1);
       }
+      f(p, index(k));
+    }
+  }
+  // The same for the first pass, from memory: four rounds at a time.
+  template <typename F>
+  __device__ __forceinline__ void first_pass(F f) const {
+    const int n = rounds();
+#pragma unroll 1
+    for (int k0 = 0; k0 < n; k0 += 4) {
+      P p[4];
 #pragma unroll
-      for (int u = 0; u < kAtOnce; ++u) {
-        const int i = base + u * kThreads * E + mine;
-        if (base + u * kThreads * E >= vocab) continue;
-        if (HELD && FIRST) held[i / E] = p[u];
-        f(p[u], i);
-        __builtin_amdgcn_sched_barrier(0);  // one packet's work after the other: side by side they would not fit the registers
+      for (int u = 0; u < 4; ++u)
+        if (k0 + u < n) p[u] = packet(k0 + u);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (k0 + u >= n) break;
+        if (HELD) held[(k0 + u) * THREADS + threadIdx.x] = p[u];
+#pragma unroll
+        for (int e = 0; e < E; ++e) f(to_f32(p[u].e[e]), index(k0 + u) + e);
       }
     }
   }
   // f(element, index).
-  template <bool FIRST = false, typename F>
-  __device__ __forceinline__ void each(F f) {
-    each_packet<FIRST>([&](const P& p, int i) {
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    each_packet([&](const P& p, int i) {
 #pragma unroll
       for (int e = 0; e < E; ++e) f(to_f32(p.e[e]), i + e);
     });
   }
-  __device__ __forceinline__ float at(int i) const { return to_f32(HELD ? held[i / E].e[i % E] : x[i]); }
 };
 
 __device__ __forceinline__ void add64(uint64_t* to, uint64_t v) {
@@ -214,33 +265,42 @@ __device__ __forceinline__ uint64_t lane64(uint64_t v, int lane) {
          static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
 }
 
-// The bin in which the sum of the bins from the front passes `target` (l.bin, with l.before
-// the sum before it; -1 where the total does not pass it); returns the total. Barriers on both sides.
+// A histogram's running sums: this thread's two bins, what comes before them, and the total.
 template <typename W>
-__device__ __forceinline__ uint64_t find_bin(SampleLds& l, const W* bins, uint64_t target) {
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  __syncthreads();
-  const W a = bins[2 * threadIdx.x], b = bins[2 * threadIdx.x + 1];
-  const W upto = scan_lanes(static_cast<W>(a + b));
-  if (lane == kWave - 1) l.wave_sum[wave] = upto;
-  if (threadIdx.x == 0) l.bin = -1;
-  __syncthreads();
-  uint64_t before = 0, total = 0;
+struct Bins {
+  uint64_t before, total;
+  W a, b;
+
+  // Barriers before and inside.
+  __device__ __forceinline__ Bins(SampleLds& l, const W* bins) {
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    __syncthreads();
+    a = bins[2 * threadIdx.x];
+    b = bins[2 * threadIdx.x + 1];
+    const W upto = scan_lanes(static_cast<W>(a + b));
+    if (lane == kWave - 1) l.wave_sum[wave] = upto;
+    if (threadIdx.x == 0) l.bin = -1;
+    __syncthreads();
+    before = static_cast<W>(upto - a - b);
+    total = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    const uint64_t s = l.wave_sum[w];
-    if (w < wave) before += s;
-    total += s;
+    for (int w = 0; w < kWaves; ++w) {
+      const uint64_t s = l.wave_sum[w];
+      if (w < wave) before += s;
+      total += s;
+    }
   }
-  before += static_cast<W>(upto - a - b);
-  if (before <= target && target < before + a + b) {
-    const bool second = target >= before + a;
-    l.bin = 2 * threadIdx.x + second;
-    l.before = before + (second ? a : 0);
+  // The bin in which the sum from the front passes `target`: l.bin, with l.before the sum before it; -1 where
+  // the total does not pass it. Once, with a barrier behind.
+  __device__ __forceinline__ void find(SampleLds& l, uint64_t target) const {
+    if (before <= target && target < before + a + b) {
+      const bool second = target >= before + a;
+      l.bin = 2 * threadIdx.x + second;
+      l.before = before + (second ? a : 0);
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  return total;
-}
+};
 
 // The element of the list that covers `target` when the weights are laid end to end in descending
 // order of place; the target lies inside. weight(place): 0 for those that do not count.
@@ -266,7 +326,7 @@ __device__ __forceinline__ uint64_t find_in_list(SampleLds& l, int n, uint64_t l
         atomicAdd(&l.count[(hi - p) >> shift], 1u);
       }
     }
-    find_bin(l, l.hist, target);
+    Bins<uint64_t>(l, l.hist).find(l, target);
     if (l.bin < 0) return lo;  // not reached: the target lies inside
     const bool alone = l.count[l.bin] == 1;
     target -= l.before;
@@ -353,286 +413,503 @@ __device__ __forceinline__ void draw_small(const SampleLds& l, const SampleRow& 
   if (stays && upto <= target && target < upto + w) *out = index_at(p);
 }
 
-template <typename T, bool HELD>
-__global__ __launch_bounds__(kThreads) void sample_rows(SampleDev a) {
-  __shared__ SampleLds l;
-  __shared__ __align__(16) unsigned char held_row[HELD ? kHeldBytes : 16];
-  const int64_t n = blockIdx.x;
-  Row<T, HELD> row;
-  row.x = static_cast<const T*>(a.x) + n * a.stride;
-  row.vocab = a.vocab;
-  row.held = reinterpret_cast<typename Row<T, HELD>::P*>(held_row);
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const float temperature = a.temperatures ? a.temperatures[n] : a.temperature;
-  const int top_k = a.top_ks ? a.top_ks[n] : a.top_k;
-  const float top_p = a.top_ps ? a.top_ps[n] : a.top_p, min_p = a.min_ps ? a.min_ps[n] : a.min_p, u = a.u[n];
-  const bool greedy = !(temperature > 0.0f) || top_k == 1;
-  if (threadIdx.x < 128) l.pow2[threadIdx.x] = exp2(threadIdx.x / 128.0);
+// A row's settings; values that a tensor should not hold count as the nearest that it may.
+struct Settings {
+  float temperature, top_p, min_p;
+  int top_k;
+  bool greedy;
+  __device__ __forceinline__ Settings(const SampleDev& a, int64_t n) {
+    temperature = a.temperatures ? a.temperatures[n] : a.temperature;
+    top_k = a.top_ks ? a.top_ks[n] : a.top_k;
+    top_p = a.top_ps ? a.top_ps[n] : a.top_p;
+    min_p = a.min_ps ? a.min_ps[n] : a.min_p;
+    if (top_k >= a.vocab) top_k = 0;
+    greedy = !(temperature > 0.0f) || top_k == 1;
+  }
+};
 
-  // The largest logit, the first that has it, and the least that is not ruled out.
-  float top = -__builtin_inff(), low = __builtin_inff();
-  int at = a.vocab;
-  if (greedy) {
-    row.template each<true>([&](float x, int i) {
-      if (x > top) {
-        top = x;
-        at = i;
-      }
-    });
-  } else {
-    row.template each<true>([&](float x, int) {
-      top = __builtin_fmaxf(top, x);
-      low = __builtin_fminf(low, x > -__builtin_inff() ? x : __builtin_inff());
-    });
-  }
-#pragma unroll
-  for (int k = 1; k < kWave; k *= 2) {
-    const float x = __shfl_xor(top, k), y = __shfl_xor(low, k);
-    const int i = __shfl_xor(at, k);
-    at = x > top ? i : x == top ? min(at, i) : at;
-    top = __builtin_fmaxf(top, x);
-    low = __builtin_fminf(low, y);
-  }
-  if (lane == 0) {
-    l.wave_top[wave] = top;
-    l.wave_low[wave] = low;
-    l.wave_at[wave] = at;
-  }
-  clear(l.regions);
-  clear(l.hist);
-  clear(l.count);
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    const float x = l.wave_top[w];
-    at = x > top ? l.wave_at[w] : x == top ? min(at, l.wave_at[w]) : at;
-    top = __builtin_fmaxf(top, x);
-    low = __builtin_fminf(low, l.wave_low[w]);
-  }
-  if (greedy || !(top > -__builtin_inff())) {
-    if (threadIdx.x == 0) a.out[n] = top > -__builtin_inff() ? at : -1;
-    return;
-  }
-
+__device__ __forceinline__ SampleRow row_of(const SampleDev& a, const Settings& set, float top, float low) {
+  constexpr float kMost = std::numeric_limits<float>::max();
   SampleRow r;
   r.top = top;
-  r.top64 = static_cast<double>(top);
-  r.per_unit = 1.4426950408889634074 / static_cast<double>(temperature);
+  r.top64 = static_cast<double>(__builtin_fminf(top, kMost));
+  r.per_unit = top < __builtin_inff() ? 1.4426950408889634074 / static_cast<double>(set.temperature) : 0.0;
   r.bits = a.weight_bits;
-  r.flat = !(top < __builtin_inff()) || !(r.per_unit > 0.0);
+  const bool flat = !(r.per_unit > 0.0);
   const auto below_top = [&](double units) {  // the logit so many log2 units down
-    return r.flat ? (top < __builtin_inff() ? -std::numeric_limits<float>::max() : top)
-                  : __builtin_fmaxf(static_cast<float>(r.top64 - units / r.per_unit), -std::numeric_limits<float>::max());
+    return flat ? (top < __builtin_inff() ? -kMost : top) : __builtin_fmaxf(static_cast<float>(r.top64 - units / r.per_unit), -kMost);
   };
   r.floor = below_top(r.bits + 1);
-  // As many tokens weigh less than 2^-t of the largest each as there are: together less than 1 - top_p for this t.
-  r.tail = top_p < 1.0f ? below_top(fmin(64.0, log2(static_cast<double>(a.vocab) / (1.0 - static_cast<double>(fmaxf(top_p, 0.0f)))) + 1.0)) : 0.0f;
-  r.keep = -std::numeric_limits<float>::max();
-  if (min_p >= 1.0f) {
+  // As many tokens weigh less than 2^-t of the largest each as there are: together less than 1 - set.top_p for this t.
+  r.tail = set.top_p < 1.0f ? below_top(fmin(64.0, static_cast<double>(__builtin_log2f(static_cast<float>(a.vocab) / (1.0f - __builtin_fmaxf(set.top_p, 0.0f)))) + 1.01)) : 0.0f;
+  r.keep = -kMost;
+  if (set.min_p >= 1.0f) {
     r.keep = top;
-  } else if (min_p > 0.0f && !r.flat) {
-    const double from = r.top64 + log(static_cast<double>(min_p)) * static_cast<double>(temperature);
+  } else if (set.min_p > 0.0f && !flat) {
+    const double from = r.top64 + log(static_cast<double>(set.min_p)) * static_cast<double>(set.temperature);
     r.keep = __builtin_fmaxf(static_cast<float>(from), r.keep);
     if (static_cast<double>(r.keep) < from) r.keep = from_sort_bits(sort_bits(r.keep) + 1);  // the next one up
   }
   const float span = top - __builtin_fmaxf(low, r.floor);
   r.per_bin = span > 0.0f && span < __builtin_inff() ? static_cast<float>(kBins) / span : 0.0f;
+  return r;
+}
 
-  uint64_t least = 0;   // the place of the last element that stays
-  bool listed = false;  // whether all that may stay are in the list
-  bool summed = false;  // whether l.regions holds the sums of all that stay
-  int held = 0;
-  const auto in = [&](float x, int i) { return x >= r.floor && place(x, i) >= least; };
-  const auto mass = [&](uint64_t p) { return p >= least ? weight_of(l, r, value_at(p)) : 0; };
-  const auto one = [&](uint64_t p) { return static_cast<uint64_t>(p >= least); };
+// ---- a row divided over workgroups ---------------------------------------------------
+// Three passes over the row, each a kernel, before sample_rows does the rest: the largest logit; the
+// histogram of the first stage (top_k's counts, or top_p's weights), or the sums of the row's parts where
+// nothing is left out; the elements of the bin, and the sums of what lies above it. A row whose elements do not fit the list is done anew
+// by sample_rows alone.
+constexpr int kPartThreads = 256;
 
-  // The element that covers the target, among those of bin l.bin that the list had no room for: bins of their places.
-  const auto resolve = [&](uint64_t lo, uint64_t hi, uint64_t target, bool counts) {
-    for (;;) {
-      const int shift = max(0, 64 - __builtin_clzll(hi - lo) - 11);
-      __syncthreads();
-      clear(l.hist);
-      __syncthreads();
-      row.each([&](float x, int i) {
-        const uint64_t p = place(x, i);
-        if (p >= lo && p <= hi && in(x, i)) add64(&l.hist[(hi - p) >> shift], counts ? 1 : weight_of(l, r, x));
-      });
-      find_bin(l, l.hist, target);
-      if (l.bin < 0) return lo;  // not reached: the target lies inside
-      target -= l.before;
-      hi -= uint64_t(l.bin) << shift;
-      const uint64_t width = (uint64_t(1) << shift) - 1;
-      lo = hi - lo > width ? hi - width : lo;
-      begin_list(l);
-      row.each([&](float x, int i) {
-        const uint64_t p = place(x, i);
-        append(l, p >= lo && p <= hi && in(x, i), x, i);
-      });
-      __syncthreads();
-      lo = l.lo;
-      hi = l.hi;
-      const unsigned found = l.n;
-      if (found <= kList)
-        return counts ? find_in_list(l, static_cast<int>(found), lo, hi, target, one)
-                      : find_in_list(l, static_cast<int>(found), lo, hi, target, mass);
-    }
-  };
+template <typename T, int THREADS>
+__device__ __forceinline__ Row<T, false, THREADS> part_of_row(const SampleDev& a, int64_t n, int start) {
+  return Row<T, false, THREADS>(static_cast<const T*>(a.x) + n * a.stride + start, min(a.chunk, a.vocab - start), nullptr);
+}
 
-  if (top_k > 0) {
-    row.each([&](float x, int) {
-      if (x >= r.floor) atomicAdd(&l.count[bin_of(r, x)], 1u);
-    });
-    find_bin(l, l.count, static_cast<uint64_t>(top_k) - 1);
-    const int bin = l.bin;
-    if (bin >= 0) {
-      const uint64_t before = l.before;
-      listed = before + l.count[bin] <= kList;
-      begin_list(l);
-      row.each([&](float x, int i) {
-        const int b = bin_of(r, x);
-        append(l, x >= r.floor && (listed ? b <= bin : b == bin), x, i);
-      });
-      __syncthreads();
-      held = static_cast<int>(l.n);
-      const uint64_t lo = l.lo, hi = l.hi;
-      if (listed && held <= kWave) {
-        if (wave == 0) draw_small(l, r, held, top_k, top_p, u, a.out + n);
-        return;
-      }
-      const uint64_t target = static_cast<uint64_t>(top_k) - 1 - (listed ? 0 : before);
-      least = held <= kList ? find_in_list(l, held, lo, hi, target, one) : resolve(lo, hi, target, true);
-    }
-    __syncthreads();
-    clear(l.hist);
-  }
-
-  if (top_p < 1.0f) {
-    if (listed) {
-      __syncthreads();
-      uint64_t lo = ~uint64_t(0), hi = 0;
-      if (threadIdx.x == 0) {
-        l.lo = lo;
-        l.hi = hi;
-      }
-      __syncthreads();
-      for (int i = threadIdx.x; i < held; i += kThreads) {
-        const uint64_t p = l.list[i];
-        if (p < least) continue;
-        add64(&l.hist[i % kBins], mass(p));  // for the total only
-        lo = min(lo, p);
-        hi = max(hi, p);
-      }
-      if (hi != 0) {
-        min64(&l.lo, lo);
-        max64(&l.hi, hi);
-      }
-      const uint64_t total = find_bin(l, l.hist, 0);
-      lo = l.lo;
-      hi = l.hi;
-      __syncthreads();
-      least = find_in_list(l, held, lo, hi, last_unit(top_p, total), mass);
-    } else {
-      __syncthreads();
-      uint64_t rest = 0;
-      row.each([&](float x, int i) {
-        if (!in(x, i)) return;
-        const uint64_t w = weight_of(l, r, x);
-        if (x < r.tail) rest += w;
-        else add64(&l.hist[bin_of(r, x)], w);
-      });
-      if (rest != 0) add64(&l.hist[kBins - 1], rest);  // behind the target in any case
-      const uint64_t total = find_bin(l, l.hist, 0), target = last_unit(top_p, total);
-      find_bin(l, l.hist, target);
-      const int bin = l.bin;
-      const uint64_t before = l.before;
-      // The bin's elements into the list, and those above it, which stay, to their parts of the row.
-      begin_list(l);
-      row.each_packet([&](const auto& p, int i) {
-        uint64_t sum = 0;
+// The largest logit, the first that has it and the least that is not ruled out, over the lanes of a wavefront.
+__device__ __forceinline__ void join_found(SampleFound& f) {
 #pragma unroll
-        for (int e = 0; e < 16 / static_cast<int>(sizeof(T)); ++e) {
-          const float x = to_f32(p.e[e]);
-          const int b = bin_of(r, x);
-          const bool live = x >= r.floor;
-          if (live && b < bin && x >= r.keep && place(x, i + e) >= least) sum += weight_of(l, r, x);
-          append(l, live && b == bin && place(x, i + e) >= least, x, i + e);
-        }
-        if (__ballot(sum != 0) == 0) return;
-        sum = sum_row16(sum);  // a part of the row is whole runs of 16 lanes' packets
-        if (lane % 16 == 15 && sum != 0) add64(&l.regions[i >> a.region_log2], sum);
-      });
-      __syncthreads();
-      const int found = static_cast<int>(l.n);
-      const uint64_t lo = l.lo, hi = l.hi;
-      if (found <= kList) {
-        least = find_in_list(l, found, lo, hi, target - before, mass);
-        for (int i = threadIdx.x; i < found; i += kThreads) {
-          const uint64_t p = l.list[i];
-          if (p >= least && value_at(p) >= r.keep) add64(&l.regions[index_at(p) >> a.region_log2], weight_of(l, r, value_at(p)));
-        }
-        summed = true;
-      } else {
-        __syncthreads();
-        clear(l.regions);
-        least = resolve(lo, hi, target - before, false);
-      }
-    }
+  for (int k = 1; k < kWave; k *= 2) {
+    const float x = __shfl_xor(f.top, k), y = __shfl_xor(f.low, k);
+    const int i = __shfl_xor(f.at, k);
+    f.at = x > f.top ? i : x == f.top ? min(f.at, i) : f.at;
+    f.top = __builtin_fmaxf(f.top, x);
+    f.low = __builtin_fminf(f.low, y);
   }
+}
+__device__ __forceinline__ SampleFound found_in_row(const SampleDev& a, int64_t n) {
+  const int lane = threadIdx.x % kWave;
+  SampleFound f{-__builtin_inff(), __builtin_inff(), a.vocab};
+  if (lane < a.parts) f = space_of(a, n)->found[lane];
+  join_found(f);
+  return f;
+}
 
-  // By index: the part of the row in which the sum passes the number drawn, then the token.
-  const auto stays = [&](float x, int i) { return in(x, i) && x >= r.keep; };
+template <typename T>
+__global__ __launch_bounds__(kPartThreads) void sample_top(SampleDev a) {
+  __shared__ SampleFound waves[kPartThreads / kWave];
+  const int64_t n = fast_div(blockIdx.x, a.by_parts);
+  const int part = blockIdx.x - static_cast<int>(n) * a.parts, start = part * a.chunk;
+  SampleSpace* const space = space_of(a, n);
+  for (int i = part * kPartThreads + threadIdx.x; i < kBins; i += a.parts * kPartThreads) space->hist[i] = space->regions[i] = 0;
+  if (part == 0 && threadIdx.x == 0) space->n = 0;
+  SampleFound f{-__builtin_inff(), __builtin_inff(), a.vocab};
+  part_of_row<T, kPartThreads>(a, n, start).first_pass([&](float x, int i) {
+    f.at = x > f.top ? start + i : f.at;
+    f.top = __builtin_fmaxf(f.top, x);
+    f.low = __builtin_fminf(f.low, x > -__builtin_inff() ? x : __builtin_inff());
+  });
+  join_found(f);
+  if (threadIdx.x % kWave == 0) waves[threadIdx.x / kWave] = f;
   __syncthreads();
-  if (listed) {
-    for (int i = threadIdx.x; i < held; i += kThreads) {
-      const uint64_t p = l.list[i];
-      if (stays(value_at(p), index_at(p))) add64(&l.regions[index_at(p) >> a.region_log2], weight_of(l, r, value_at(p)));
-    }
-  } else if (!summed) {
+  if (threadIdx.x >= kWave) return;
+  f = SampleFound{-__builtin_inff(), __builtin_inff(), a.vocab};
+  if (threadIdx.x < kPartThreads / kWave) f = waves[threadIdx.x];
+  join_found(f);
+  if (threadIdx.x == 0) space->found[part] = f;
+}
+
+// What a part's threads share.
+struct PartLds {
+  uint64_t hist[kBins];
+  double pow2[128];
+};
+__device__ __forceinline__ void add_to_row(const uint64_t* bins, uint64_t* row) {
+  for (int i = threadIdx.x; i < kBins; i += kPartThreads)
+    if (bins[i] != 0) add64(&row[i], bins[i]);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kPartThreads) void sample_bins(SampleDev a) {
+  __shared__ PartLds l;
+  const int64_t n = fast_div(blockIdx.x, a.by_parts);
+  const int start = (blockIdx.x - static_cast<int>(n) * a.parts) * a.chunk, lane = threadIdx.x % kWave;
+  const Settings set(a, n);
+  const SampleFound f = found_in_row(a, n);
+  if (set.greedy || !(f.top > -__builtin_inff())) return;
+  for (int i = threadIdx.x; i < kBins; i += kPartThreads) l.hist[i] = 0;
+  if (threadIdx.x < 128) l.pow2[threadIdx.x] = a.pow2[threadIdx.x];
+  const SampleRow r = row_of(a, set, f.top, f.low);
+  const auto row = part_of_row<T, kPartThreads>(a, n, start);
+  __syncthreads();
+  if (set.top_k > 0) {
+    row.each([&](float x, int) {
+      if (x >= r.floor) add64(&l.hist[bin_of(r, x)], 1);
+    });
+  } else if (set.top_p < 1.0f) {
+    uint64_t rest = 0;
+    row.each([&](float x, int) {
+      const uint64_t w = weight_of(l, r, x);
+      rest += x >= r.floor && x < r.tail ? w : 0;
+      if (x >= r.floor && !(x < r.tail)) add64(&l.hist[bin_of(r, x)], w);
+    });
+    if (rest != 0) add64(&l.hist[kBins - 1], rest);  // behind the target in any case
+  } else {
     row.each_packet([&](const auto& p, int i) {
       uint64_t sum = 0;
 #pragma unroll
       for (int e = 0; e < 16 / static_cast<int>(sizeof(T)); ++e) {
         const float x = to_f32(p.e[e]);
-        if (stays(x, i + e)) sum += weight_of(l, r, x);
+        const bool mine = x >= r.floor && x >= r.keep;
+        if (__ballot(mine) != 0) sum += mine ? weight_of(l, r, x) : 0;
       }
-      sum = sum_row16(sum);
-      if (lane % 16 == 15 && sum != 0) add64(&l.regions[i >> a.region_log2], sum);
+      if (__ballot(sum != 0) == 0) return;
+      sum = sum_row16(sum);  // a part of the row is whole runs of 16 lanes' packets
+      if (lane % 16 == 15 && sum != 0) add64(&l.hist[(start + i) >> a.region_log2], sum);
     });
   }
-  const uint64_t total = find_bin(l, l.regions, 0), target = drawn(u, total);
-  find_bin(l, l.regions, target);
+  __syncthreads();
+  SampleSpace* const space = space_of(a, n);
+  add_to_row(l.hist, set.top_k > 0 || set.top_p < 1.0f ? space->hist : space->regions);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kPartThreads) void sample_list(SampleDev a) {
+  constexpr int PER = kBins / kPartThreads;
+  __shared__ PartLds l;
+  __shared__ uint64_t wave_sum[kPartThreads / kWave];
+  __shared__ int found_bin;
+  __shared__ uint64_t found_before, found_in;
+  const int64_t n = fast_div(blockIdx.x, a.by_parts);
+  const int start = (blockIdx.x - static_cast<int>(n) * a.parts) * a.chunk;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const Settings set(a, n);
+  const SampleFound f = found_in_row(a, n);
+  const bool counts = set.top_k > 0;
+  if (set.greedy || !(f.top > -__builtin_inff()) || !(counts || set.top_p < 1.0f)) return;
+  if (threadIdx.x < 128) l.pow2[threadIdx.x] = a.pow2[threadIdx.x];
+  const SampleRow r = row_of(a, set, f.top, f.low);
+  SampleSpace* const space = space_of(a, n);
+  // The bin that covers the target, found by every part of the row.
+  uint64_t bins[PER], mine = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    bins[i] = space->hist[threadIdx.x * PER + i];
+    mine += bins[i];
+    l.hist[i * kPartThreads + threadIdx.x] = 0;
+  }
+  const uint64_t upto = scan_lanes(mine);
+  if (lane == kWave - 1) wave_sum[wave] = upto;
+  if (threadIdx.x == 0) found_bin = -1;
+  __syncthreads();
+  uint64_t before = upto - mine, total = 0;
+  for (int w = 0; w < kPartThreads / kWave; ++w) {
+    if (w < wave) before += wave_sum[w];
+    total += wave_sum[w];
+  }
+  const uint64_t target = counts ? static_cast<uint64_t>(set.top_k) - 1 : last_unit(set.top_p, total);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (before <= target && target < before + bins[i]) {
+      found_bin = threadIdx.x * PER + i;
+      found_before = before;
+      found_in = bins[i];
+    }
+    before += bins[i];
+  }
+  __syncthreads();
+  const int bin = found_bin;
+  if (bin < 0 || (counts && found_before + found_in > kList)) return;  // no more than top_k, or too many for the list
+  part_of_row<T, kPartThreads>(a, n, start).each_packet([&](const auto& p, int i) {
+    uint64_t sum = 0;
+#pragma unroll
+    for (int e = 0; e < 16 / static_cast<int>(sizeof(T)); ++e) {
+      const float x = to_f32(p.e[e]);
+      const int b = bin_of(r, x);
+      const bool live = x >= r.floor, take = live && (counts ? b <= bin : b == bin);
+      const uint64_t all = __ballot(take);
+      if (all != 0) {
+        const int first = __builtin_ctzll(all);
+        unsigned at = 0;
+        if (lane == first) at = atomicAdd(&space->n, static_cast<unsigned>(__popcll(all)));
+        at = __builtin_amdgcn_readlane(at, first) + __popcll(all & ((uint64_t(1) << lane) - 1));
+        if (take && at < kList) space->list[at] = place(x, start + i + e);
+      }
+      if (!counts) {
+        const bool stays = live && b < bin && x >= r.keep;
+        if (__ballot(stays) != 0) sum += stays ? weight_of(l, r, x) : 0;
+      }
+    }
+    if (counts || __ballot(sum != 0) == 0) return;
+    sum = sum_row16(sum);
+    if (lane % 16 == 15 && sum != 0) add64(&l.hist[(start + i) >> a.region_log2], sum);
+  });
+  if (counts) return;
+  __syncthreads();
+  add_to_row(l.hist, space->regions);
+}
+
+// SPLIT: the passes of the first stage are done.
+template <typename T, bool HELD, bool SPLIT>
+__global__ __launch_bounds__(kThreads) void sample_rows(SampleDev a) {
+  using R = Row<T, HELD>;
+  __shared__ SampleLds l;
+  __shared__ typename R::P held_row[HELD ? kHeldBytes / 16 + kThreads : 1];  // and the round behind the whole packets
+  const int64_t n = blockIdx.x;
+  const R row(static_cast<const T*>(a.x) + n * a.stride, a.vocab, held_row);
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const Settings set(a, n);
+  const int top_k = set.top_k;
+  const float top_p = set.top_p, u = a.u[n];
+  if (threadIdx.x < 128) l.pow2[threadIdx.x] = a.pow2[threadIdx.x];
+
+  // The largest logit, the first that has it, and the least that is not ruled out.
+  float top = -__builtin_inff(), low = __builtin_inff();
+  int at = a.vocab;
+  [[maybe_unused]] SampleSpace* const space = SPLIT ? space_of(a, n) : nullptr;
+  if constexpr (SPLIT) {
+    const SampleFound f = found_in_row(a, n);
+    top = f.top;
+    low = f.low;
+    at = f.at;
+  } else {
+    row.first_pass([&](float x, int i) {
+      at = x > top ? i : at;
+      top = __builtin_fmaxf(top, x);
+      low = __builtin_fminf(low, x > -__builtin_inff() ? x : __builtin_inff());
+    });
+    SampleFound f{top, low, at};
+    join_found(f);
+    if (lane == 0) l.found[wave] = f;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float x = l.found[w].top;
+      at = x > top ? l.found[w].at : x == top ? min(at, l.found[w].at) : at;
+      top = __builtin_fmaxf(top, x);
+      low = __builtin_fminf(low, l.found[w].low);
+    }
+  }
+  clear(l.regions);
+  clear(l.hist);
+  clear(l.count);
+  __syncthreads();
+  if (set.greedy || !(top > -__builtin_inff())) {
+    if (threadIdx.x == 0) a.out[n] = top > -__builtin_inff() ? at : -1;
+    return;
+  }
+
+  const SampleRow r = row_of(a, set, top, low);
+
+  // The last element that stays, and its value and index.
+  uint64_t least = 0;
+  float least_x = -__builtin_inff();
+  int least_i = 0;
+  bool listed = false;  // whether all that may stay are in the list
+  bool summed = false;  // whether l.regions holds the sums of all that stay
+  int held = 0;         // elements in the list
+  bool ready = SPLIT;   // what the other kernels have left is still to be used
+  const auto in = [&](float x, int i) { return x >= r.floor && (x > least_x || (x == least_x && i <= least_i)); };
+
+  for (int stage = 0; stage < 2; ++stage) {  // top_k, then top_p
+    const bool counts = stage == 0;
+    if (counts ? top_k <= 0 : !(top_p < 1.0f)) continue;
+    const auto weight = [&](uint64_t p) { return p < least ? 0 : counts ? 1 : weight_of(l, r, value_at(p)); };
+    uint64_t target = 0, lo = 0, hi = ~uint64_t(0);
+    if (listed) {
+      __syncthreads();
+      clear(l.hist);
+      __syncthreads();
+      for (int i = threadIdx.x; i < held; i += kThreads) add64(&l.hist[i % kBins], weight(l.list[i]));  // for the total only
+      target = last_unit(top_p, Bins<uint64_t>(l, l.hist).total);
+      lo = l.lo;
+      hi = l.hi;
+      __syncthreads();
+    } else {
+      int bin;
+      if (ready) {
+        for (int i = threadIdx.x; i < kBins; i += kThreads) l.hist[i] = space->hist[i];
+      } else if (counts) {
+        row.each([&](float x, int) {
+          if (x >= r.floor) add64(&l.hist[bin_of(r, x)], 1);
+        });
+      } else {
+        uint64_t rest = 0;
+        row.each([&](float x, int i) {
+          const bool mine = in(x, i);
+          const uint64_t w = weight_of(l, r, x);
+          rest += mine && x < r.tail ? w : 0;
+          if (mine && !(x < r.tail)) add64(&l.hist[bin_of(r, x)], w);
+        });
+        if (rest != 0) add64(&l.hist[kBins - 1], rest);  // behind the target in any case
+      }
+      const Bins<uint64_t> bins(l, l.hist);
+      target = counts ? static_cast<uint64_t>(top_k) - 1 : last_unit(top_p, bins.total);
+      bins.find(l, target);
+      bin = l.bin;
+      if (bin < 0) {  // no more than top_k
+        __syncthreads();
+        clear(l.hist);
+        __syncthreads();
+        ready = false;
+        continue;
+      }
+      const uint64_t before = l.before;
+      if (counts) listed = before + l.hist[bin] <= kList;
+      if (!(counts && listed)) target -= before;
+      // The bin's elements into the list (or all up to it), and those above it, which stay, to their parts of the row.
+      for (bool again = false;; again = true) {
+        begin_list(l);
+        if (ready) {
+          ready = false;
+          held = static_cast<int>(space->n);
+          if (counts ? listed : held <= kList) {
+            for (int i = threadIdx.x; i < held; i += kThreads) {
+              const uint64_t p = l.list[i] = space->list[i];
+              min64(&l.lo, p);
+              max64(&l.hi, p);
+            }
+            if (!counts)
+              for (int i = threadIdx.x; i < kBins; i += kThreads) l.regions[i] = space->regions[i];
+            summed = !counts;
+            __syncthreads();
+            lo = l.lo;
+            hi = l.hi;
+            break;
+          }
+        }
+        row.each_packet([&](const typename R::P& p, int i) {
+          uint64_t sum = 0;
+#pragma unroll
+          for (int e = 0; e < R::E; ++e) {
+            const float x = to_f32(p.e[e]);
+            const int b = bin_of(r, x);
+            const bool live = in(x, i + e);
+            append(l, live && (counts && listed ? b <= bin : b == bin) && (!again || (place(x, i + e) >= lo && place(x, i + e) <= hi)), x, i + e);
+            if (!counts && !again && __ballot(live && b < bin && x >= r.keep) != 0) sum += live && b < bin && x >= r.keep ? weight_of(l, r, x) : 0;
+          }
+          if (counts || again || __ballot(sum != 0) == 0) return;
+          sum = sum_row16(sum);  // a part of the row is whole runs of 16 lanes' packets
+          if (lane % 16 == 15 && sum != 0) add64(&l.regions[i >> a.region_log2], sum);
+        });
+        __syncthreads();
+        held = static_cast<int>(l.n);
+        lo = l.lo;
+        hi = l.hi;
+        if (held <= kList) {
+          summed = !counts && !again;
+          break;
+        }
+        // Too many: bins of their places.
+        const int shift = max(0, 64 - __builtin_clzll(hi - lo) - 11);
+        __syncthreads();
+        clear(l.hist);
+        __syncthreads();
+        row.each([&](float x, int i) {
+          const uint64_t p = place(x, i);
+          if (in(x, i) && p >= lo && p <= hi) add64(&l.hist[(hi - p) >> shift], counts ? 1 : weight_of(l, r, x));
+        });
+        Bins<uint64_t>(l, l.hist).find(l, target);
+        if (l.bin < 0) break;  // not reached: the target lies inside
+        target -= l.before;
+        hi -= uint64_t(l.bin) << shift;
+        const uint64_t width = (uint64_t(1) << shift) - 1;
+        lo = hi - lo > width ? hi - width : lo;
+      }
+      if (counts && listed && held <= kWave) {
+        if (wave == 0) draw_small(l, r, held, top_k, top_p, u, a.out + n);
+        return;
+      }
+    }
+    least = find_in_list(l, min(held, kList), lo, hi, target, weight);
+    least_x = value_at(least);
+    least_i = index_at(least);
+    if (summed) {
+      for (int i = threadIdx.x; i < held; i += kThreads) {
+        const uint64_t p = l.list[i];
+        if (p >= least && value_at(p) >= r.keep) add64(&l.regions[index_at(p) >> a.region_log2], weight_of(l, r, value_at(p)));
+      }
+    }
+    __syncthreads();
+    if (counts) clear(l.hist);
+    __syncthreads();
+  }
+
+  // By index: the part of the row in which the sum passes the number drawn, then the token.
+  const auto stays = [&](float x, int i) { return in(x, i) && x >= r.keep; };
+  if (!summed) {
+    clear(l.regions);
+    __syncthreads();
+    if (SPLIT && ready) {
+      for (int i = threadIdx.x; i < kBins; i += kThreads) l.regions[i] = space->regions[i];
+    } else if (listed) {
+      for (int i = threadIdx.x; i < held; i += kThreads) {
+        const uint64_t p = l.list[i];
+        if (stays(value_at(p), index_at(p))) add64(&l.regions[index_at(p) >> a.region_log2], weight_of(l, r, value_at(p)));
+      }
+    } else {
+      row.each_packet([&](const typename R::P& p, int i) {
+        uint64_t sum = 0;
+#pragma unroll
+        for (int e = 0; e < R::E; ++e) {
+          const float x = to_f32(p.e[e]);
+          const bool mine = stays(x, i + e);
+          if (__ballot(mine) != 0) sum += mine ? weight_of(l, r, x) : 0;
+        }
+        if (__ballot(sum != 0) == 0) return;
+        sum = sum_row16(sum);
+        if (lane % 16 == 15 && sum != 0) add64(&l.regions[i >> a.region_log2], sum);
+      });
+    }
+  }
+  const Bins<uint64_t> parts(l, l.regions);
+  const uint64_t target = drawn(u, parts.total);
+  parts.find(l, target);
   const int region = max(l.bin, 0) << a.region_log2;
   const uint64_t rest = target - l.before;
   for (int i = threadIdx.x; i < kBins; i += kThreads) {
     uint64_t w = 0;
     if (i < (1 << a.region_log2) && region + i < a.vocab) {
-      const float x = row.at(region + i);
+      const float x = to_f32(row.x[region + i]);
       if (stays(x, region + i)) w = weight_of(l, r, x);
     }
     l.hist[i] = w;
   }
-  find_bin(l, l.hist, rest);
+  Bins<uint64_t>(l, l.hist).find(l, rest);
   if (threadIdx.x == 0) a.out[n] = region + max(l.bin, 0);
 }
 
 namespace {
 
+// Workgroups of a row, and tokens of each: 4096 tokens or more, as many as fill the chip with a few rows. Rows that one
+// workgroup keeps in LDS, and many of them, are not divided.
+struct Parts {
+  int parts, chunk;
+};
+Parts parts_of(int64_t rows, int64_t vocab) {
+  constexpr int64_t kStep = 2048;  // a multiple of the regions
+  if (vocab <= 8192 || rows > 1024) return Parts{1, static_cast<int>(vocab)};
+  const int64_t most = std::min<int64_t>(kMaxParts, std::max<int64_t>(1, 2048 / rows));
+  const int64_t chunk = std::max<int64_t>(4096, ceil_div(ceil_div(vocab, most), kStep) * kStep);
+  return Parts{static_cast<int>(ceil_div(vocab, chunk)), static_cast<int>(chunk)};
+}
+
 template <typename T>
-void launch_rows(const SampleDev& d, dim3 grid, hipStream_t stream) {
-  if (d.vocab * sizeof(T) <= kHeldBytes) AKO_LAUNCH((sample_rows<T, true>), grid, dim3(kThreads), 0, stream, d);
-  else AKO_LAUNCH((sample_rows<T, false>), grid, dim3(kThreads), 0, stream, d);
+hipError_t launch_rows(const SampleDev& d, int64_t rows, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(rows)), block(kThreads);
+  if (d.parts > 1) {
+    const dim3 parts(static_cast<unsigned>(rows * d.parts)), part_block(kPartThreads);
+    AKO_LAUNCH((sample_top<T>), parts, part_block, 0, stream, d);
+    AKO_LAUNCH((sample_bins<T>), parts, part_block, 0, stream, d);
+    AKO_LAUNCH((sample_list<T>), parts, part_block, 0, stream, d);
+    AKO_LAUNCH((sample_rows<T, false, true>), grid, block, 0, stream, d);
+  } else if (d.vocab * static_cast<int64_t>(sizeof(T)) <= kHeldBytes) {
+    AKO_LAUNCH((sample_rows<T, true, false>), grid, block, 0, stream, d);
+  } else {
+    AKO_LAUNCH((sample_rows<T, false, false>), grid, block, 0, stream, d);
+  }
+  return hipGetLastError();
 }
 
 }  // namespace
 
+int64_t sample_workspace(int64_t rows, int64_t vocab) {
+  return parts_of(rows, vocab).parts > 1 ? rows * static_cast<int64_t>(sizeof(SampleSpace)) : 0;
+}
+
 hipError_t launch_sample(const SampleArgs& a, hipStream_t stream) {
   SampleDev d{};
-  d.x = a.x;
-  d.u = a.u;
-  d.temperatures = a.temperatures;
-  d.top_ks = a.top_ks;
-  d.top_ps = a.top_ps;
-  d.min_ps = a.min_ps;
   d.temperature = a.temperature;
   d.top_k = a.top_k;
   d.top_p = a.top_p;
@@ -642,10 +919,16 @@ hipError_t launch_sample(const SampleArgs& a, hipStream_t stream) {
   while ((int64_t(1) << log2) < a.vocab) ++log2;
   d.weight_bits = std::min(51, 62 - log2);
   d.region_log2 = std::max(7, log2 - 11);  // at most kBins parts, of 16 lanes' packets or more
+  for (int j = 0; j < 128; ++j) d.pow2[j] = std::exp2(j / 128.0);
   d.stride = a.stride;
+  const Parts p = parts_of(a.rows, a.vocab);
+  d.space = static_cast<unsigned char*>(a.workspace);
+  d.parts = p.parts;
+  d.chunk = p.chunk;
+  d.by_parts = make_fastdiv(d.parts);
   constexpr int64_t kRows = int64_t(1) << 21;  // per launch: work-items stay below 2^32
   for (int64_t r = 0; r < a.rows; r += kRows) {
-    const dim3 grid(static_cast<unsigned>(std::min(kRows, a.rows - r)));
+    const int64_t rows = std::min(kRows, a.rows - r);
     d.x = static_cast<const char*>(a.x) + r * a.stride * dtype_bytes(a.dtype);
     d.u = a.u + r;
     d.temperatures = a.temperatures ? a.temperatures + r : nullptr;
@@ -653,13 +936,12 @@ hipError_t launch_sample(const SampleArgs& a, hipStream_t stream) {
     d.top_ps = a.top_ps ? a.top_ps + r : nullptr;
     d.min_ps = a.min_ps ? a.min_ps + r : nullptr;
     d.out = a.out + r;
+    hipError_t err = hipErrorInvalidValue;
     switch (a.dtype) {
-      case kF32: launch_rows<float>(d, grid, stream); break;
-      case kF16: launch_rows<_Float16>(d, grid, stream); break;
-      case kBF16: launch_rows<__bf16>(d, grid, stream); break;
-      default: return hipErrorInvalidValue;
+      case kF32: err = launch_rows<float>(d, rows, stream); break;
+      case kF16: err = launch_rows<_Float16>(d, rows, stream); break;
+      case kBF16: err = launch_rows<__bf16>(d, rows, stream); break;
     }
-    const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
   }
   return hipSuccess;

@@ -762,12 +762,15 @@ at::Tensor sample(const at::Tensor& logits, const at::Tensor& uniform, const py:
   if (!p.rows && !(p.all >= 0 && p.all <= 1)) value_error(pre + "top_p must be 0 to 1, got " + number(p.all));
   if (!m.rows && !(m.all >= 0 && m.all <= 1)) value_error(pre + "min_p must be 0 to 1, got " + number(m.all));
   const at::Tensor x = logits.stride(1) == 1 || vocab == 1 ? logits : logits.contiguous();
-  at::Tensor out = at::empty({rows}, logits.options().dtype(at::kLong));
+  at::Tensor out = at::empty({rows}, logits.options().dtype(at::kLong)), space;
+  const int64_t need = std::max<int64_t>(0, ako_sample_workspace(rows, vocab));
+  if (need > 0) space = at::empty({need}, logits.options().dtype(at::kByte));
   check(on_device(index, [&](hipStream_t s) {
           return ako_sample_fwd(x.data_ptr(), static_cast<const float*>(uniform.data_ptr()), t.ptr<float>(),
                                 static_cast<float>(t.all), k.ptr<int32_t>(), static_cast<int32_t>(std::min(k.all, 2147483647.0)),
                                 p.ptr<float>(), static_cast<float>(p.all), m.ptr<float>(), static_cast<float>(m.all),
-                                static_cast<int64_t*>(out.data_ptr()), rows, vocab, rows > 1 ? x.stride(0) : vocab, dt, s);
+                                static_cast<int64_t*>(out.data_ptr()), rows, vocab, rows > 1 ? x.stride(0) : vocab,
+                                need > 0 ? space.data_ptr() : nullptr, need, dt, s);
         }), fn);
   return out;
 }

@@ -391,14 +391,18 @@ int64_t ako_paged_select_workspace(const ako_paged_t* cache, int64_t q_heads, in
  * tokens and finer below: the token does not depend on how the work was divided.
  * temperature, top_k, top_p and min_p hold one value for each row, or are NULL and the
  * value behind them holds for all rows (temperature_all >= 0 and not NaN, the others' in
- * [0, 1], top_k_all >= 0). row_stride: elements between rows. The reference has no
+ * [0, 1], top_k_all >= 0). row_stride: elements between rows. workspace holds
+ * ako_sample_workspace bytes, 16-byte aligned, that nothing else uses until the work on `stream` is done. The reference has no
  * counterpart (its decoder returns hidden states, ako/models/decoder.py:261-266).
  */
 int ako_sample_fwd(const void* logits, const float* uniform, const float* temperature,
                    float temperature_all, const int32_t* top_k, int32_t top_k_all,
                    const float* top_p, float top_p_all, const float* min_p, float min_p_all,
-                   int64_t* out, int64_t rows, int64_t vocab, int64_t row_stride, int dtype,
-                   void* stream);
+                   int64_t* out, int64_t rows, int64_t vocab, int64_t row_stride,
+                   void* workspace, int64_t workspace_bytes, int dtype, void* stream);
+
+/* Bytes of workspace for such a call (0: none); -1 for sizes it refuses. */
+int64_t ako_sample_workspace(int64_t rows, int64_t vocab);
 
 /*
  * Launch-shape override for tuning sweeps and tests (no counterpart in the

@@ -118,7 +118,7 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         _int,
         [_ptr, _ptr, _ptr, _f32, _ptr, ctypes.c_int32, _ptr, _f32, _ptr, _f32, _ptr, _i64, _i64, _i64, _ptr, _i64, _int, _ptr],
     ),
-    "ako_sample_workspace": (_i64, [_i64, _i64]),
+    "ako_sample_workspace": (_i64, [_i64, _i64, _int]),
     "ako_set_tuning": (_int, [_int, _int, _int]),
     "ako_time_next_launch": (_int, [_ptr, _ptr]),
 }

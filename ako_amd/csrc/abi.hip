@@ -1187,12 +1187,16 @@ int64_t ako_paged_select_workspace(const ako_paged_t* cache, int64_t q_heads, in
 // --------------------------------------------------------------- sampling --
 static constexpr int64_t kMaxVocab = int64_t(1) << 22;
 
-int64_t ako_sample_workspace(int64_t rows, int64_t vocab) {
+int64_t ako_sample_workspace(int64_t rows, int64_t vocab, int dtype) {
+  if (!valid_dtype(dtype)) {
+    fail(AKO_ERR_UNSUPPORTED, "ako_sample_workspace: unknown dtype code %d", dtype);
+    return -1;
+  }
   if (rows < 0 || rows > kMaxInt || vocab < 1 || vocab > kMaxVocab) {
     fail(AKO_ERR_INVALID_ARGUMENT, "ako_sample_workspace: rows must be 0 to 2^31-1 and vocab 1 to %lld", (long long)kMaxVocab);
     return -1;
   }
-  return rows == 0 ? 0 : ako::sample_workspace(rows, vocab);
+  return rows == 0 ? 0 : ako::sample_workspace(rows, vocab, dtype);
 }
 
 int ako_sample_fwd(const void* logits, const float* uniform, const float* temperature, float temperature_all,
@@ -1214,7 +1218,7 @@ int ako_sample_fwd(const void* logits, const float* uniform, const float* temper
   if (row_stride < 0) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: negative row stride", fn);
   const Span in = span_2d(logits, rows, vocab, row_stride, ako::dtype_bytes(dtype));
   const Span o = span_2d(out, 1, rows, rows, 8);
-  const int64_t need = ako::sample_workspace(rows, vocab);
+  const int64_t need = ako::sample_workspace(rows, vocab, dtype);
   if (workspace_bytes < need || (need > 0 && (!workspace || !aligned(workspace, 16))))
     return fail(AKO_ERR_INVALID_ARGUMENT, "%s: needs a 16-byte aligned workspace of %lld bytes, got %lld", fn,
                 (long long)need, (long long)workspace_bytes);

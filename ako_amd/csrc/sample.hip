@@ -12,7 +12,7 @@
 // a row's sum stays below 2^62: sums of whole numbers do not depend on
 // their order, so histograms are built with LDS atomics, and the token is the same on every run and
 // for every way of dividing the work. A weight is off by 2^-(S+1) of the largest, 2^-46 at
-// 131072 tokens; tokens below that count as ruled out, as those with logits of -infinity
+// 131072 tokens, and by 2^-47 of itself; tokens below the former count as ruled out, as those with logits of -infinity
 // or NaN do.
 //
 // An element's place in the descending order is a 64-bit number that no other
@@ -88,21 +88,6 @@ __device__ __forceinline__ SampleSpace* space_of(const SampleDev& a, int64_t n) 
   return reinterpret_cast<SampleSpace*>(a.space) + n;
 }
 
-// What a row's threads share.
-struct SampleLds {
-  uint64_t hist[kBins];     // weights by bin of depth, or of place
-  uint64_t regions[kBins];  // weights by part of the row
-  uint64_t list[kList];
-  unsigned count[kBins];    // elements by bin of place
-  double pow2[128];         // 2^(j / 128)
-  uint64_t wave_sum[kWaves];
-  SampleFound found[kWaves];
-  uint64_t lo, hi;          // of the elements of a bin
-  unsigned n;               // elements of a bin
-  int bin;
-  uint64_t before;
-};
-
 // The row's own numbers, the same in all threads.
 struct SampleRow {
   double top64, per_unit;  // the largest finite logit, and log2(e) / T (0 where all that count weigh the same)
@@ -112,6 +97,22 @@ struct SampleRow {
   float tail;              // elements below here weigh less than 1 - top_p of all together
   float per_bin;           // bins of a unit of logits
   double bits;             // S
+};
+
+// What a row's threads share.
+struct SampleLds {
+  uint64_t hist[kBins];     // weights by bin of depth, or of place
+  uint64_t regions[kBins];  // weights by part of the row
+  uint64_t list[kList];
+  unsigned count[kBins];    // elements by bin of place
+  double pow2[128];         // 2^(j / 128)
+  uint64_t wave_sum[kWaves];
+  SampleRow row;
+  SampleFound found[kWaves];
+  uint64_t lo, hi;          // of the elements of a bin
+  unsigned n;               // elements of a bin
+  int bin;
+  uint64_t before;
 };
 
 // 2^(S - t), t log2 units below the largest, rounded to a whole number: 2^(j / 128) from a table
@@ -169,23 +170,25 @@ struct Row {
     }
     return p;
   }
-  // f(packet, index of its first element); all threads take part in every call. The next round's
-  // packet is on its way while this one is worked on.
+  // f(packet, index of its first element); all threads take part in every call. kAtOnce rounds' packets
+  // are on their way together.
   template <typename F>
   __device__ __forceinline__ void each_packet(F f) const {
+    constexpr int kAtOnce = HELD ? 4 : 16 / E;
     const int n = rounds();
-    P next;
-    if (!HELD) next = packet(0);
 #pragma unroll 1
-    for (int k = 0; k < n; ++k) {
-      P p;
-      if (HELD) {
-        p = held[k * THREADS + threadIdx.x];
-      } else {
-        p = next;
-        if (k + 1 < n) next = packet(k + 1);
+    for (int k0 = 0; k0 < n; k0 += kAtOnce) {
+      P p[kAtOnce];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        if (HELD) p[u] = held[(k0 + u) * THREADS + threadIdx.x];
+        else if (k0 + u < n) p[u] = packet(k0 + u);
       }
-      f(p, index(k));
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        if (k0 + u >= n) break;
+        f(p[u], index(k0 + u));
+      }
     }
   }
   // The same for the first pass, from memory: four rounds at a time.
@@ -302,15 +305,42 @@ struct Bins {
   }
 };
 
+// One element a lane, the same in every wavefront (0 behind the n-th): how many of the others are greater, and the sum
+// of their weights. The wavefronts compare with a sixteenth of the others each.
+struct Ranked {
+  int rank;
+  uint64_t before;
+};
+__device__ __forceinline__ Ranked rank_small(SampleLds& l, int n, uint64_t p, uint64_t w) {
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  __syncthreads();
+  if (wave == 0) l.count[lane] = l.hist[lane] = 0;
+  __syncthreads();
+  unsigned rank = 0;
+  uint64_t before = 0;
+#pragma unroll
+  for (int k = 0; k < kWave / kWaves; ++k) {
+    const int j = k * kWaves + wave;
+    const bool above = j < n && lane64(p, j) > p;
+    rank += above;
+    before += above ? lane64(w, j) : 0;
+  }
+  if (rank != 0) {
+    atomicAdd(&l.count[lane], rank);
+    add64(&l.hist[lane], before);
+  }
+  __syncthreads();
+  return Ranked{static_cast<int>(l.count[lane]), l.hist[lane]};
+}
+
 // The element of the list that covers `target` when the weights are laid end to end in descending
 // order of place; the target lies inside. weight(place): 0 for those that do not count.
 template <typename F>
 __device__ __forceinline__ uint64_t find_in_list(SampleLds& l, int n, uint64_t lo, uint64_t hi, uint64_t target, F weight) {
   const int lane = threadIdx.x % kWave;
-  if (n <= kWave) {  // one element a lane, every wavefront by itself
+  if (n <= kWave) {
     const uint64_t p = lane < n ? l.list[lane] : 0, w = lane < n ? weight(p) : 0;
-    uint64_t before = 0;
-    for (int j = 0; j < n; ++j) before += lane64(p, j) > p ? lane64(w, j) : 0;
+    const uint64_t before = rank_small(l, n, p, w).before;
     const uint64_t hit = __ballot(before <= target && target < before + w);
     return hit != 0 ? lane64(p, __builtin_ctzll(hit)) : lo;
   }
@@ -384,33 +414,22 @@ __device__ __forceinline__ uint64_t last_unit(float top_p, uint64_t total) {
   return want >= 1.0 ? (want < static_cast<double>(total) ? static_cast<uint64_t>(want) : total) - 1 : 0;
 }
 
-// All that is left to do for a list of up to 64 elements among which are all that may stay, one a
-// lane of one wavefront.
-__device__ __forceinline__ void draw_small(const SampleLds& l, const SampleRow& r, int n, int top_k, float top_p, float u, int64_t* out) {
+// All that is left to do for a list of up to 64 elements among which are all that may stay.
+__device__ __forceinline__ void draw_small(SampleLds& l, const SampleRow& r, int n, int top_k, float top_p, float u, int64_t* out) {
   const int lane = threadIdx.x % kWave;
   const uint64_t p = lane < n ? l.list[lane] : 0, w = lane < n ? weight_of(l, r, value_at(p)) : 0;
-  int rank = 0;
-  uint64_t before = 0;
-  for (int j = 0; j < n; ++j) {
-    const bool above = lane64(p, j) > p;
-    rank += above;
-    before += above ? lane64(w, j) : 0;
+  const Ranked at = rank_small(l, n, p, w);
+  bool stays = lane < n && at.rank < top_k;
+  if (top_p < 1.0f) {
+    const uint64_t last = __ballot(lane < n && at.rank == min(top_k, n) - 1);
+    stays = stays && at.before <= last_unit(top_p, lane64(at.before + w, __builtin_ctzll(last | uint64_t(1) << 63)));
   }
-  bool stays = lane < n && rank < top_k;
-  const uint64_t last = __ballot(lane < n && rank == min(top_k, n) - 1);
-  const uint64_t total = lane64(before + w, __builtin_ctzll(last | uint64_t(1) << 63));
-  if (top_p < 1.0f) stays = stays && before <= last_unit(top_p, total);
   stays = stays && value_at(p) >= r.keep;
-  const uint64_t kept = __ballot(stays);
-  uint64_t sum = 0, upto = 0;
-  for (int j = 0; j < n; ++j) {
-    if (!(kept >> j & 1)) continue;
-    const uint64_t x = lane64(w, j);
-    sum += x;
-    upto += static_cast<unsigned>(lane64(p, j)) > static_cast<unsigned>(p) ? x : 0;  // a lower index
-  }
-  const uint64_t target = drawn(u, sum);
-  if (stays && upto <= target && target < upto + w) *out = index_at(p);
+  // By index: the greater an index's complement, the earlier.
+  const uint64_t mine = stays ? w : 0, total = lane64(scan_lanes(mine), kWave - 1);
+  const uint64_t upto = rank_small(l, n, stays ? static_cast<unsigned>(p) : 0, mine).before;
+  const uint64_t target = drawn(u, total);
+  if (threadIdx.x < kWave && stays && upto <= target && target < upto + w) *out = index_at(p);
 }
 
 // A row's settings; values that a tensor should not hold count as the nearest that it may.
@@ -436,12 +455,13 @@ __device__ __forceinline__ SampleRow row_of(const SampleDev& a, const Settings& 
   r.per_unit = top < __builtin_inff() ? 1.4426950408889634074 / static_cast<double>(set.temperature) : 0.0;
   r.bits = a.weight_bits;
   const bool flat = !(r.per_unit > 0.0);
-  const auto below_top = [&](double units) {  // the logit so many log2 units down
-    return flat ? (top < __builtin_inff() ? -kMost : top) : __builtin_fmaxf(static_cast<float>(r.top64 - units / r.per_unit), -kMost);
+  // The logit so many log2 units down: a bound that only has to be the same everywhere.
+  const auto below_top = [&](float units) {
+    return flat ? (top < __builtin_inff() ? -kMost : top) : __builtin_fmaxf(top - units / static_cast<float>(r.per_unit), -kMost);
   };
-  r.floor = below_top(r.bits + 1);
-  // As many tokens weigh less than 2^-t of the largest each as there are: together less than 1 - set.top_p for this t.
-  r.tail = set.top_p < 1.0f ? below_top(fmin(64.0, static_cast<double>(__builtin_log2f(static_cast<float>(a.vocab) / (1.0f - __builtin_fmaxf(set.top_p, 0.0f)))) + 1.01)) : 0.0f;
+  r.floor = below_top(static_cast<float>(a.weight_bits + 1));
+  // As many tokens weigh less than 2^-t of the largest each as there are: together less than 1 - top_p for this t.
+  r.tail = set.top_p < 1.0f ? below_top(__builtin_fminf(64.0f, __builtin_log2f(static_cast<float>(a.vocab) / (1.0f - __builtin_fmaxf(set.top_p, 0.0f))) + 1.01f)) : 0.0f;
   r.keep = -kMost;
   if (set.min_p >= 1.0f) {
     r.keep = top;
@@ -514,7 +534,16 @@ __global__ __launch_bounds__(kPartThreads) void sample_top(SampleDev a) {
 struct PartLds {
   uint64_t hist[kBins];
   double pow2[128];
+  SampleRow row;
 };
+// The row's numbers, formed once for the workgroup: in every wavefront they would take as long as the rest.
+template <typename Lds>
+__device__ __forceinline__ void share_row(Lds& l, const SampleDev& a, const Settings& set, float top, float low) {
+  if (threadIdx.x < kWave) {
+    const SampleRow r = row_of(a, set, top, low);
+    if (threadIdx.x == 0) l.row = r;
+  }
+}
 __device__ __forceinline__ void add_to_row(const uint64_t* bins, uint64_t* row) {
   for (int i = threadIdx.x; i < kBins; i += kPartThreads)
     if (bins[i] != 0) add64(&row[i], bins[i]);
@@ -530,9 +559,10 @@ __global__ __launch_bounds__(kPartThreads) void sample_bins(SampleDev a) {
   if (set.greedy || !(f.top > -__builtin_inff())) return;
   for (int i = threadIdx.x; i < kBins; i += kPartThreads) l.hist[i] = 0;
   if (threadIdx.x < 128) l.pow2[threadIdx.x] = a.pow2[threadIdx.x];
-  const SampleRow r = row_of(a, set, f.top, f.low);
+  share_row(l, a, set, f.top, f.low);
   const auto row = part_of_row<T, kPartThreads>(a, n, start);
   __syncthreads();
+  const SampleRow r = l.row;
   if (set.top_k > 0) {
     row.each([&](float x, int) {
       if (x >= r.floor) add64(&l.hist[bin_of(r, x)], 1);
@@ -579,7 +609,7 @@ __global__ __launch_bounds__(kPartThreads) void sample_list(SampleDev a) {
   const bool counts = set.top_k > 0;
   if (set.greedy || !(f.top > -__builtin_inff()) || !(counts || set.top_p < 1.0f)) return;
   if (threadIdx.x < 128) l.pow2[threadIdx.x] = a.pow2[threadIdx.x];
-  const SampleRow r = row_of(a, set, f.top, f.low);
+  share_row(l, a, set, f.top, f.low);
   SampleSpace* const space = space_of(a, n);
   // The bin that covers the target, found by every part of the row.
   uint64_t bins[PER], mine = 0;
@@ -610,6 +640,7 @@ __global__ __launch_bounds__(kPartThreads) void sample_list(SampleDev a) {
   }
   __syncthreads();
   const int bin = found_bin;
+  const SampleRow r = l.row;
   if (bin < 0 || (counts && found_before + found_in > kList)) return;  // no more than top_k, or too many for the list
   part_of_row<T, kPartThreads>(a, n, start).each_packet([&](const auto& p, int i) {
     uint64_t sum = 0;
@@ -684,13 +715,14 @@ __global__ __launch_bounds__(kThreads) void sample_rows(SampleDev a) {
   clear(l.regions);
   clear(l.hist);
   clear(l.count);
-  __syncthreads();
   if (set.greedy || !(top > -__builtin_inff())) {
     if (threadIdx.x == 0) a.out[n] = top > -__builtin_inff() ? at : -1;
     return;
   }
 
-  const SampleRow r = row_of(a, set, top, low);
+  share_row(l, a, set, top, low);
+  __syncthreads();
+  const SampleRow r = l.row;
 
   // The last element that stays, and its value and index.
   uint64_t least = 0;
@@ -808,7 +840,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows(SampleDev a) {
         lo = hi - lo > width ? hi - width : lo;
       }
       if (counts && listed && held <= kWave) {
-        if (wave == 0) draw_small(l, r, held, top_k, top_p, u, a.out + n);
+        draw_small(l, r, held, top_k, top_p, u, a.out + n);
         return;
       }
     }
@@ -873,13 +905,20 @@ __global__ __launch_bounds__(kThreads) void sample_rows(SampleDev a) {
 namespace {
 
 // Workgroups of a row, and tokens of each: 4096 tokens or more, as many as fill the chip with a few rows. Rows that one
-// workgroup keeps in LDS, and many of them, are not divided.
+// workgroup keeps in LDS are not divided (32000 tokens in 16 bits with top_k 50: 25 us, divided 34), nor are more rows than
+// compute units. Longer rows, one workgroup a row and divided, in us (131072 tokens in 32 bits):
+//   rows            1          64         128        256
+//   no settings    65 / 21    69 / 35    75 / 51    81 / 79
+//   top_k 50       69 / 30    75 / 60    83 / 77    91 / 107
+//   top_p 0.9     110 / 42   141 / 76   151 / 100  157 / 152
+//   greedy         16 / 12    17 / 18    22 / 25    25 / 35
+// and 159 / 138 for 256 rows of mixed settings, where the undivided call takes as long as its slowest row.
 struct Parts {
   int parts, chunk;
 };
-Parts parts_of(int64_t rows, int64_t vocab) {
+Parts parts_of(int64_t rows, int64_t vocab, int dtype) {
   constexpr int64_t kStep = 2048;  // a multiple of the regions
-  if (vocab <= 8192 || rows > 1024) return Parts{1, static_cast<int>(vocab)};
+  if (vocab * dtype_bytes(dtype) <= kHeldBytes || rows > 256) return Parts{1, static_cast<int>(vocab)};
   const int64_t most = std::min<int64_t>(kMaxParts, std::max<int64_t>(1, 2048 / rows));
   const int64_t chunk = std::max<int64_t>(4096, ceil_div(ceil_div(vocab, most), kStep) * kStep);
   return Parts{static_cast<int>(ceil_div(vocab, chunk)), static_cast<int>(chunk)};
@@ -904,8 +943,8 @@ hipError_t launch_rows(const SampleDev& d, int64_t rows, hipStream_t stream) {
 
 }  // namespace
 
-int64_t sample_workspace(int64_t rows, int64_t vocab) {
-  return parts_of(rows, vocab).parts > 1 ? rows * static_cast<int64_t>(sizeof(SampleSpace)) : 0;
+int64_t sample_workspace(int64_t rows, int64_t vocab, int dtype) {
+  return parts_of(rows, vocab, dtype).parts > 1 ? rows * static_cast<int64_t>(sizeof(SampleSpace)) : 0;
 }
 
 hipError_t launch_sample(const SampleArgs& a, hipStream_t stream) {
@@ -921,7 +960,7 @@ hipError_t launch_sample(const SampleArgs& a, hipStream_t stream) {
   d.region_log2 = std::max(7, log2 - 11);  // at most kBins parts, of 16 lanes' packets or more
   for (int j = 0; j < 128; ++j) d.pow2[j] = std::exp2(j / 128.0);
   d.stride = a.stride;
-  const Parts p = parts_of(a.rows, a.vocab);
+  const Parts p = parts_of(a.rows, a.vocab, a.dtype);
   d.space = static_cast<unsigned char*>(a.workspace);
   d.parts = p.parts;
   d.chunk = p.chunk;

@@ -763,7 +763,7 @@ at::Tensor sample(const at::Tensor& logits, const at::Tensor& uniform, const py:
   if (!m.rows && !(m.all >= 0 && m.all <= 1)) value_error(pre + "min_p must be 0 to 1, got " + number(m.all));
   const at::Tensor x = logits.stride(1) == 1 || vocab == 1 ? logits : logits.contiguous();
   at::Tensor out = at::empty({rows}, logits.options().dtype(at::kLong)), space;
-  const int64_t need = std::max<int64_t>(0, ako_sample_workspace(rows, vocab));
+  const int64_t need = std::max<int64_t>(0, ako_sample_workspace(rows, vocab, dt));
   if (need > 0) space = at::empty({need}, logits.options().dtype(at::kByte));
   check(on_device(index, [&](hipStream_t s) {
           return ako_sample_fwd(x.data_ptr(), static_cast<const float*>(uniform.data_ptr()), t.ptr<float>(),

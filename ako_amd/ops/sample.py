@@ -143,7 +143,7 @@ def sample_hip_ctypes(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_
     x = logits if logits.stride(1) == 1 or vocab == 1 else logits.contiguous()
     out = torch.empty(rows, dtype=torch.int64, device=logits.device)
     both = lambda v, none: (v.data_ptr(), none) if torch.is_tensor(v) else (None, v)  # noqa: E731
-    need = max(0, lib().ako_sample_workspace(rows, vocab))
+    need = max(0, lib().ako_sample_workspace(rows, vocab, DT[logits.dtype]))
     space = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
     top_k = top_k if torch.is_tensor(top_k) else min(int(top_k), 2**31 - 1)
     status = call(index, lib().ako_sample_fwd, x.data_ptr(), uniform.data_ptr(), *both(temperature, 0.0), *both(top_k, 0),

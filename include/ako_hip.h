@@ -402,7 +402,7 @@ int ako_sample_fwd(const void* logits, const float* uniform, const float* temper
                    void* workspace, int64_t workspace_bytes, int dtype, void* stream);
 
 /* Bytes of workspace for such a call (0: none); -1 for sizes it refuses. */
-int64_t ako_sample_workspace(int64_t rows, int64_t vocab);
+int64_t ako_sample_workspace(int64_t rows, int64_t vocab, int dtype);
 
 /*
  * Launch-shape override for tuning sweeps and tests (no counterpart in the

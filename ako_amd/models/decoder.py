@@ -18,7 +18,10 @@ maximum length (``max_len``); appending then writes into the slab instead
 of re-concatenating the whole cache on every step as ``torch.cat`` does
 (``decoder.py:84-93``); the returned views are the same. ``PagedKVCache`` keeps
 keys and values in pages, in the model's type or in 8 bits; a step on it
-rotates, stores and attends through ``rope_qk_paged`` and ``paged_attention``.
+rotates, stores and attends through ``rope_qk_paged`` and ``paged_attention``,
+over all that is stored or over the blocks that ``paged_select`` chooses. With
+``ModelConfig.qk_norm`` every head of q and k has its RMSNorm before the rotation.
+``CausalLM.generate`` draws tokens through ``sample``.
 """
 
 from __future__ import annotations
@@ -30,11 +33,13 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from ako_amd.ops.paged import new_pages, paged_attention, paged_read, rope_qk_paged
+from ako_amd.ops.paged import new_pages, paged_attention, paged_means, paged_read, paged_select, rope_qk_paged
+from ako_amd.ops.qk_norm import rmsnorm_rope_qk
 from ako_amd.ops.rmsnorm import rmsnorm, rmsnorm_residual
 from ako_amd.ops.rmsnorm_ref import rmsnorm_ref
 from ako_amd.ops.rope import rope, rope_qk, rope_qk_cache
 from ako_amd.ops.rope_ref import build_rope_tables, rope_ref
+from ako_amd.ops.sample import sample
 from ako_amd.ops.swiglu import swiglu
 
 Backend = Literal["ako", "torch"]
@@ -63,6 +68,8 @@ class ModelConfig:
     #: three. gate and up stay separate: one 22016-row GEMV ran slower (201 us
     #: against 163 us for the pair).
     fused_qkv: bool = True
+    #: RMSNorm of every head of q and k, with one weight of ``head_dim`` for each of the two.
+    qk_norm: bool = False
 
     @property
     def head_dim(self) -> int:
@@ -234,20 +241,35 @@ class PagedKVCache:
     ``dtype`` or, with ``torch.float8_e4m3fn``, in 8 bits with one power-of-two
     scale per 32 elements; all layers share the block table. ``window`` and
     ``sinks`` limit what a token attends to: the last ``window`` positions and the
-    first ``sinks``. Lengths live on the device (``seq_lens``), so a step has static
-    shapes and can be captured and replayed; ``host_len`` mirrors them.
+    first ``sinks``. ``count`` limits it to that many pages for each key head: the ``first``
+    first, the ``last`` last and of the others those that ``paged_select`` chooses by
+    the means of their keys, which every step keeps up to date. Lengths live on the
+    device (``seq_lens``), so a step has static shapes and can be captured and replayed;
+    ``host_len`` mirrors them.
     """
 
     def __init__(self, n_layers: int, batch: int, kv_heads: int, head_dim: int, max_len: int, *,
                  dtype: torch.dtype, device: torch.device | str, page_size: int = 64,
-                 window: int | None = None, sinks: int = 0) -> None:
+                 window: int | None = None, sinks: int = 0, count: int | None = None, first: int = 1,
+                 last: int = 1) -> None:
+        if count is not None and (window is not None or sinks):
+            raise ValueError("a choice of pages leaves no room for a window or sinks")
+        if count is not None and (first < 0 or last < 1 or count < first + last):
+            raise ValueError("first must be at least 0, last at least 1 and count at least their sum, "
+                             f"got {first}, {last} and {count}")
         width = -(-max_len // page_size)
         self.n_layers = n_layers
         self.max_len = max_len
         self.window = window
         self.sinks = sinks
+        self.count = count
+        self.first = first
+        self.last = last
         self.pools = [new_pages(batch * width, kv_heads, page_size, head_dim, dtype, device=device)
                       for _ in range(n_layers)]
+        #: The means of the keys of full pages, one tensor for each layer, where pages are chosen.
+        self.means = [torch.zeros(batch * width, kv_heads, head_dim, dtype=torch.float32, device=device)
+                      for _ in range(n_layers if count is not None else 0)]
         self.block_table = torch.arange(batch * width, dtype=torch.int32, device=device).view(batch, width)
         self.seq_lens = torch.zeros(batch, dtype=torch.int32, device=device)
         self.host_len = 0
@@ -272,12 +294,20 @@ class PagedKVCache:
         self.host_len -= tokens
 
     def attend(self, layer_idx: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
-               sin: torch.Tensor, style: str) -> torch.Tensor:
-        """Rotate q and k, store k and v at the step's positions, and attend over all that is stored."""
+               sin: torch.Tensor, style: str, *, q_weight: torch.Tensor | None = None,
+               k_weight: torch.Tensor | None = None, eps: float = 1e-6) -> torch.Tensor:
+        """Rotate q and k (after their norms, with weights), store k and v at the step's positions, and attend
+        over what is stored."""
         kp, vp, ks, vs = self.pools[layer_idx]
         where = (kp, vp, self.block_table, self.seq_lens)
-        q = rope_qk_paged(q, k, v, cos, sin, *where, style, k_scales=ks, v_scales=vs)
-        return paged_attention(q, *where, k_scales=ks, v_scales=vs, window=self.window, sinks=self.sinks)
+        q = rope_qk_paged(q, k, v, cos, sin, *where, style, k_scales=ks, v_scales=vs, q_weight=q_weight,
+                          k_weight=k_weight, eps=eps)
+        blocks = None
+        if self.count is not None:
+            means = paged_means(kp, self.means[layer_idx], self.block_table, self.seq_lens, q.shape[1], k_scales=ks)
+            blocks = paged_select(q, means, self.block_table, self.seq_lens, kp.shape[2], self.count,
+                                  first=self.first, last=self.last)
+        return paged_attention(q, *where, k_scales=ks, v_scales=vs, window=self.window, sinks=self.sinks, blocks=blocks)
 
     def read(self, layer_idx: int, dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """This layer's filled keys and values as dense ``(batch, length, kv_heads, head_dim)`` tensors."""
@@ -317,12 +347,13 @@ def _zero_position(device: torch.device) -> torch.Tensor:
     return t
 
 
-def _fused_cache_rope(backend: Backend, override: KernelOverride | None) -> bool:
+def _fused_cache_rope(backend: Backend, override: KernelOverride | None, config: ModelConfig) -> bool:
     """Whether a static-cache decode step rotates q/k and appends k/v to the
     cache in one call (``rope_qk_cache``) instead of RoPE plus two copies.
-    Forcing a ``rope`` or ``rope_qk`` kernel keeps the unfused path."""
+    Forcing a ``rope`` or ``rope_qk`` kernel keeps the unfused path, and so do
+    norms of q and k, which come first."""
     o = override or {}
-    return backend == "ako" and not o.get("rope") and not o.get("rope_qk")
+    return backend == "ako" and not config.qk_norm and not o.get("rope") and not o.get("rope_qk")
 
 
 class Attention(nn.Module):
@@ -344,6 +375,8 @@ class Attention(nn.Module):
             self.k_proj = nn.Linear(config.hidden_dim, kv_dim, bias=False)
             self.v_proj = nn.Linear(config.hidden_dim, kv_dim, bias=False)
         self.o_proj = nn.Linear(config.hidden_dim, config.hidden_dim, bias=False)
+        self.q_norm_weight = nn.Parameter(torch.ones(config.head_dim)) if config.qk_norm else None
+        self.k_norm_weight = nn.Parameter(torch.ones(config.head_dim)) if config.qk_norm else None
 
     def _load_from_state_dict(self, state_dict, prefix, *args, **kwargs):
         """State dicts of either layout load into either: three ``q/k/v_proj``
@@ -395,10 +428,11 @@ class Attention(nn.Module):
         q, k, v = self.project_qkv(x)
         if isinstance(kv_cache, PagedKVCache):
             # cos/sin are the full tables; positions are read on the device.
-            attn = kv_cache.attend(layer_idx, q, k, v, cos, sin, cfg.rope_style)
+            attn = kv_cache.attend(layer_idx, q, k, v, cos, sin, cfg.rope_style, q_weight=self.q_norm_weight,
+                                   k_weight=self.k_norm_weight, eps=cfg.eps)
             return self.o_proj(attn.reshape(batch, seq_len, cfg.hidden_dim))
         if (isinstance(kv_cache, StaticKVCache) and seq_len == 1
-                and _fused_cache_rope(self.backend, self.kernel_override)):
+                and _fused_cache_rope(self.backend, self.kernel_override, cfg)):
             # cos/sin are the full tables here; the position is read on the device.
             q = rope_qk_cache(q, k, v, cos, sin, kv_cache.pos, kv_cache.k[layer_idx],
                               kv_cache.v[layer_idx], cfg.rope_style)
@@ -409,7 +443,7 @@ class Attention(nn.Module):
             attn = F.scaled_dot_product_attention(q.transpose(1, 2), kh, vh, attn_mask=kv_cache.mask)
             return self.o_proj(attn.transpose(1, 2).reshape(batch, seq_len, cfg.hidden_dim))
         if (isinstance(kv_cache, KVCache) and kv_cache.max_len is not None
-                and _fused_cache_rope(self.backend, self.kernel_override)):
+                and _fused_cache_rope(self.backend, self.kernel_override, cfg)):
             # Preallocated host-tracked cache: rotate q and write rotated k and v
             # into the slab from the first free slot on, in one call. cos/sin are
             # the rows of positions [start, start + seq), so position 0 of the
@@ -418,10 +452,17 @@ class Attention(nn.Module):
             q = rope_qk_cache(q, k, v, cos, sin, _zero_position(q.device), kc, vc, cfg.rope_style)
             k, v = kv_cache.advance(layer_idx, seq_len)
             return self._attend(q, k, v, batch, seq_len)
-        if self.backend == "ako" and not (self.kernel_override or {}).get("rope"):
+        override = self.kernel_override or {}
+        fused_norm = cfg.qk_norm and self.backend == "ako" and not override.get("rope") and not override.get("rope_qk")
+        if cfg.qk_norm and not fused_norm:
+            q, _ = _norm(self.backend, q, None, self.q_norm_weight, cfg.eps, override)
+            k, _ = _norm(self.backend, k, None, self.k_norm_weight, cfg.eps, override)
+        if fused_norm:
+            q, k = rmsnorm_rope_qk(q, k, self.q_norm_weight, self.k_norm_weight, cos, sin, cfg.eps, cfg.rope_style)
+        elif self.backend == "ako" and not override.get("rope"):
             # One dispatched op (a single launch on the HIP path) for both tensors.
             q, k = rope_qk(q, k, cos, sin, cfg.rope_style,
-                           kernel=(self.kernel_override or {}).get("rope_qk"))
+                           kernel=override.get("rope_qk"))
         else:
             q = _rope(self.backend, q, cos, sin, cfg.rope_style, self.kernel_override)
             k = _rope(self.backend, k, cos, sin, cfg.rope_style, self.kernel_override)
@@ -539,7 +580,7 @@ class DecoderStack(nn.Module):
                 raise
         if static_step:
             full = self.rope_tables(self.config.max_seq_len, device=x.device)
-            if _fused_cache_rope(self.backend, self.kernel_override):
+            if _fused_cache_rope(self.backend, self.kernel_override, self.config):
                 cos, sin = full  # the fused cache RoPE picks row pos itself
             else:
                 cos, sin = kv_cache.rope_rows(*full)
@@ -570,12 +611,13 @@ class DecoderStack(nn.Module):
                              max_len, dtype=p.dtype, device=p.device)
 
     def new_paged_cache(self, max_len: int, *, batch: int = 1, page_size: int = 64, quantized: bool = False,
-                        window: int | None = None, sinks: int = 0) -> PagedKVCache:
+                        window: int | None = None, sinks: int = 0, count: int | None = None, first: int = 1,
+                        last: int = 1) -> PagedKVCache:
         """A paged cache in the model's type, or with ``quantized`` in 8 bits."""
         p = next(self.parameters())
         return PagedKVCache(self.config.n_layers, batch, self.config.n_kv_heads, self.config.head_dim, max_len,
                             dtype=torch.float8_e4m3fn if quantized else p.dtype, device=p.device,
-                            page_size=page_size, window=window, sinks=sinks)
+                            page_size=page_size, window=window, sinks=sinks, count=count, first=first, last=last)
 
     def new_kv_cache(self, max_len: int | None = None) -> KVCache:
         return KVCache(n_layers=self.config.n_layers, max_len=max_len)
@@ -591,7 +633,7 @@ def build_stack(config: ModelConfig, *, backend: Backend = "ako", device: torch.
 
 
 class CausalLM(nn.Module):
-    """Token embedding -> ``DecoderStack`` -> LM head, with greedy decoding."""
+    """Token embedding -> ``DecoderStack`` -> LM head, with greedy and sampled decoding."""
 
     def __init__(self, config: ModelConfig, backend: Backend = "ako",
                  kernel_override: KernelOverride | None = None) -> None:
@@ -617,6 +659,28 @@ class CausalLM(nn.Module):
             out.append(nxt)
         return torch.cat(out, dim=1)
 
+    @torch.no_grad()
+    def generate(self, prompt: torch.Tensor, steps: int, *, temperature: float = 1.0, top_k: int = 0,
+                 top_p: float = 1.0, min_p: float = 0.0, generator: torch.Generator | None = None,
+                 kv_cache: KVCache | StaticKVCache | PagedKVCache | None = None) -> torch.Tensor:
+        """Prefill ``prompt (batch, seq)`` then ``steps`` tokens drawn by ``sample``; returns them.
+
+        The uniform numbers of all steps are drawn first, ``(steps, batch)``, from ``generator``
+        (of the prompt's device)."""
+        cache = kv_cache if kv_cache is not None else self.stack.new_kv_cache(prompt.shape[1] + steps)
+        uniform = torch.rand(steps, prompt.shape[0], generator=generator, device=prompt.device)
+        settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        ids, out = prompt, []
+        for u in uniform:
+            ids = _drawn(self.logits_last(ids, cache), u, settings)
+            out.append(ids)
+        return torch.cat(out, dim=1)
+
+
+def _drawn(logits: torch.Tensor, uniform: torch.Tensor, settings: dict[str, float]) -> torch.Tensor:
+    """``(batch, 1)`` tokens; 0 where no logit is above -infinity, for the embedding takes no -1."""
+    return sample(logits, uniform, **settings).clamp_(min=0).unsqueeze(1)
+
 
 class GraphedGreedy:
     """Greedy decoding with every decode step replayed from one HIP graph.
@@ -634,6 +698,8 @@ class GraphedGreedy:
                  cache: PagedKVCache | None = None) -> None:
         if prompt.shape[0] != 1:
             raise ValueError("graphed decoding is written for batch 1")
+        if steps < 2:
+            raise ValueError(f"graphed decoding needs at least 2 steps, got {steps}")
         self.model = model
         self.steps = steps
         self.prompt_len = prompt.shape[1]
@@ -645,13 +711,14 @@ class GraphedGreedy:
         self.cache = model.stack.new_static_cache(max_len) if cache is None else cache
         #: Device-side count of the positions held.
         self.position = self.cache.pos if cache is None else cache.seq_lens
-        self.ids = model.logits_last(prompt, self.cache).argmax(-1, keepdim=True)
+        self.slot = torch.zeros(1, dtype=torch.long, device=prompt.device)
+        self.ids = torch.zeros(1, 1, dtype=torch.long, device=prompt.device)
+        self._choose(model.logits_last(prompt, self.cache))
         self.history = torch.zeros(steps, dtype=torch.long, device=prompt.device)
         self.history[:1] = self.ids.view(1)
         # After a step, pos has advanced past the token just produced, whose
         # index in history is pos - prompt_len.
         self.base = torch.full((1,), self.prompt_len, dtype=torch.long, device=prompt.device)
-        self.slot = torch.zeros(1, dtype=torch.long, device=prompt.device)
 
         first = self.ids.clone()
         side = torch.cuda.Stream()
@@ -673,9 +740,13 @@ class GraphedGreedy:
 
     def _step(self) -> None:
         logits = self.model.logits_last(self.ids, self.cache)
-        torch.argmax(logits, -1, keepdim=True, out=self.ids)
         torch.sub(self.position, self.base, out=self.slot)
+        self._choose(logits)
         self.history.index_copy_(0, self.slot, self.ids.view(1))
+
+    def _choose(self, logits: torch.Tensor) -> None:
+        """The token for place ``slot`` of the history, into ``ids``."""
+        torch.argmax(logits, -1, keepdim=True, out=self.ids)
 
     @torch.no_grad()
     def run(self) -> torch.Tensor:
@@ -683,12 +754,27 @@ class GraphedGreedy:
         each replay advances the cache position and the slab holds exactly
         ``prompt + steps`` slots."""
         if self._ran:
-            raise RuntimeError("GraphedGreedy.run() decodes once; build a new runner for another pass")
+            raise RuntimeError(f"{type(self).__name__}.run() decodes once; build a new runner for another pass")
         self._ran = True
         for _ in range(self.steps - 1):
             self.graph.replay()
         self.cache.host_len = self.prompt_len + self.steps - 1
         return self.history.view(1, -1)
+
+
+class GraphedSampling(GraphedGreedy):
+    """``CausalLM.generate`` with every decode step replayed from one HIP graph: the same
+    tokens from a generator in the same state."""
+
+    def __init__(self, model: "CausalLM", prompt: torch.Tensor, steps: int, *, temperature: float = 1.0,
+                 top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, generator: torch.Generator | None = None,
+                 cache: PagedKVCache | None = None) -> None:
+        self.settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        self.uniform = torch.rand(steps, 1, generator=generator, device=prompt.device).view(-1)
+        super().__init__(model, prompt, steps, cache=cache)
+
+    def _choose(self, logits: torch.Tensor) -> None:
+        self.ids.copy_(_drawn(logits, self.uniform.index_select(0, self.slot), self.settings))
 
 
 def build_lm(config: ModelConfig, *, backend: Backend = "ako", device: torch.device | str = "cpu",

@@ -1,0 +1,210 @@
+"""Norms of q and k, chosen pages and sampling in the decoder, alone and together."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+import ako_amd as ako
+from ako_amd.models.decoder import CausalLM, GraphedGreedy, GraphedSampling, ModelConfig, build_lm, build_stack
+
+SIZES = dict(hidden_dim=128, n_layers=2, n_heads=4, n_kv_heads=2, intermediate_dim=96, max_seq_len=96, vocab_size=300, eps=1e-5)
+gpu = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a GPU")]
+DEVICES = ["cpu", pytest.param("cuda", marks=gpu)]
+
+
+def stack(device: str, backend: str = "ako", dtype=torch.float32, override=None, **kw):
+    """A stack whose norm weights differ from one another."""
+    model = build_stack(ModelConfig(**{**SIZES, **kw}), seed=3, device=device, backend=backend, dtype=dtype, kernel_override=override)
+    gen = torch.Generator().manual_seed(4)
+    with torch.no_grad():
+        for name, p in model.named_parameters():
+            if name.endswith(("q_norm_weight", "k_norm_weight")):
+                p.copy_(1 + 0.5 * torch.randn(p.shape, generator=gen))
+    return model
+
+
+def hidden(batch: int, tokens: int, device: str) -> torch.Tensor:
+    return torch.randn(batch, tokens, SIZES["hidden_dim"], generator=torch.Generator().manual_seed(1)).to(device)
+
+
+def close(a: torch.Tensor, b: torch.Tensor) -> None:
+    """fp32 results of two orders of the same sums. Through two layers the rows of 128 pass about
+    fifteen products of up to 128 terms, norms and softmaxes, each off by at most 128 half steps (2^-17) of its
+    largest terms, which the norms hold near 1: 15 * 2^-17 < 2^-13 each way."""
+    assert (a.double().cpu() - b.double().cpu()).abs().max() <= 2 * 2.0 ** -13 * max(1.0, b.abs().max().item())
+
+
+def plain_attention(attn, x: torch.Tensor) -> torch.Tensor:
+    """The module's own formula in 64 bits on the CPU."""
+    cfg = attn.config
+    x = x.double().cpu()
+    n, s, _ = x.shape
+    w = {k: v.double().cpu() for k, v in attn.state_dict().items()}
+    q, k, v = (x @ w["qkv_proj.weight"].T).split([cfg.hidden_dim, attn.kv_dim, attn.kv_dim], -1)
+    q, k, v = (t.view(n, s, -1, cfg.head_dim) for t in (q, k, v))
+    if cfg.qk_norm:
+        q, k = (t / (t.square().mean(-1, keepdim=True) + cfg.eps).sqrt() * w[name] for t, name in ((q, "q_norm_weight"), (k, "k_norm_weight")))
+    half = cfg.head_dim // 2
+    angle = torch.arange(s).double()[:, None] / cfg.rope_base ** (torch.arange(half).double() / half)
+    cos, sin = angle.cos()[:, None], angle.sin()[:, None]
+    q, k = (torch.cat((t[..., :half] * cos - t[..., half:] * sin, t[..., half:] * cos + t[..., :half] * sin), -1) for t in (q, k))
+    k, v = (t.repeat_interleave(cfg.n_heads // cfg.n_kv_heads, 2) for t in (k, v))
+    score = torch.einsum("bqhd,bkhd->bhqk", q, k) / math.sqrt(cfg.head_dim)
+    p = score.masked_fill(torch.ones(s, s, dtype=torch.bool).triu(1), -math.inf).softmax(-1)
+    return torch.einsum("bhqk,bkhd->bqhd", p, v).reshape(n, s, -1) @ w["o_proj.weight"].T
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("backend,override", [("torch", None), ("ako", None), ("ako", {"rope": "rope_ref"}),
+                                              ("ako", {"rope_qk": "rope_qk_ref"})])
+def test_a_layer_with_norms_is_its_formula(backend: str, override, device: str) -> None:
+    model = stack(device, backend, override=override, qk_norm=True)
+    attn, x = model.layers[0].attention, hidden(2, 11, device)
+    with torch.no_grad():
+        close(attn(x, *model.rope_tables(11, device=device)), plain_attention(attn, x))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fused_qkv", [True, False])
+@pytest.mark.parametrize("cache", ["dense", "slab", "static", "paged"])
+def test_every_cache_gives_the_same_with_norms(cache: str, fused_qkv: bool, device: str) -> None:
+    """A prompt, a chunk (where the cache takes one) and single tokens against the whole sequence at once."""
+    model = stack(device, qk_norm=True, fused_qkv=fused_qkv)
+    x = hidden(2, 20, device)
+    new = {"dense": lambda: model.new_kv_cache(), "slab": lambda: model.new_kv_cache(20),
+           "static": lambda: model.new_static_cache(20, batch=2), "paged": lambda: model.new_paged_cache(20, batch=2, page_size=4)}[cache]()
+    with torch.no_grad():
+        want = model(x)
+        cuts = [0, 13, *range(14, 21)] if cache != "paged" else [0, 6, 13, *range(14, 21)]
+        got = torch.cat([model(x[:, a:b], kv_cache=new) for a, b in zip(cuts, cuts[1:])], 1)
+    close(got, want)
+
+
+def test_only_norms_bring_weights() -> None:
+    plain, normed = stack("cpu").state_dict(), stack("cpu", qk_norm=True).state_dict()
+    extra = set(normed) - set(plain)
+    assert not set(plain) - set(normed) and len(extra) == 4
+    assert all(name.endswith(("q_norm_weight", "k_norm_weight")) and normed[name].shape == (32,) for name in extra)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("quantized", [False, True])
+def test_pages_enough_for_all_are_no_choice(quantized: bool, device: str) -> None:
+    model = stack(device)
+    x = hidden(2, 30, device)
+    with torch.no_grad():
+        every, chosen = (model.new_paged_cache(30, batch=2, page_size=4, quantized=quantized, **kw) for kw in ({}, {"count": 8}))
+        for a, b in ((0, 9), (9, 22), (22, 23), (23, 30)):
+            close(model(x[:, a:b], kv_cache=chosen), model(x[:, a:b], kv_cache=every))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_step_attends_to_the_pages_that_its_means_choose(device: str, monkeypatch) -> None:
+    """The choice and the attention of each layer of a step, from what the cache holds."""
+    model = stack(device, qk_norm=True)
+    x = hidden(2, 40, device)
+    cache = model.new_paged_cache(40, batch=2, page_size=4, count=3)
+    seen = []
+    from ako_amd.models import decoder
+
+    def attention(q, *where, blocks, **kw):
+        out = ako.paged_attention(q, *where, blocks=blocks, **kw)
+        seen.append((q, where, blocks, out))
+        return out
+
+    monkeypatch.setattr(decoder, "paged_attention", attention)
+    with torch.no_grad():
+        for a, b in ((0, 21), (21, 39), (39, 40)):
+            model(x[:, a:b], kv_cache=cache)
+            for layer, (q, (kp, vp, table, lens), blocks, out) in enumerate(seen):
+                k, v = (t.double().cpu() for t in cache.read(layer))
+                means = F.pad(k, (0, 0, 0, 0, 0, -k.shape[1] % 4)).unflatten(1, (-1, 4)).mean(2)
+                for n in range(2):
+                    for i in range(b - a):
+                        own = (a + i) // 4
+                        for head in range(2):
+                            group = q[n, i, 2 * head:2 * head + 2].double().cpu()
+                            got = [j for j in blocks[n, i, head].tolist() if j >= 0]
+                            if own < 3:
+                                assert got == list(range(own + 1))
+                            else:
+                                score = means[n, 1:own, head] @ group.sum(0)
+                                # Means are 32-bit sums of four: off by less than 2^-21 of their terms.
+                                slack = 2.0 ** -21 * group.sum(0).abs().sum() * k[n, :, head].abs().max()
+                                assert got[0] == 0 and got[2] == own and score[got[1] - 1] >= score.max() - slack
+                            keys = [j for j in range(a + i + 1) if j // 4 in got]
+                            p = (group @ k[n, keys, head].T / math.sqrt(32)).softmax(-1)
+                            close(out[n, i, 2 * head:2 * head + 2], p @ v[n, keys, head])
+            seen.clear()
+
+
+def test_refusals() -> None:
+    model = stack("cpu")
+    for kw, match in ((dict(count=3, window=4), "window or sinks"), (dict(count=3, sinks=1), "window or sinks"),
+                      (dict(count=1), "at least their sum"), (dict(count=3, last=0), "at least their sum"), (dict(count=3, first=-1), "at least")):
+        with pytest.raises(ValueError, match=match):
+            model.new_paged_cache(20, page_size=4, **kw)
+    lm = build_lm(ModelConfig(**SIZES), dtype=torch.float32)
+    with pytest.raises(ValueError, match="top_p"):
+        lm.generate(torch.zeros(1, 3, dtype=torch.long), 2, top_p=1.5)
+    for runner in (GraphedGreedy, GraphedSampling):
+        with pytest.raises(ValueError, match="at least 2 steps"):
+            runner(lm, torch.zeros(1, 3, dtype=torch.long), 1)
+
+
+def language_model(device: str, dtype=torch.float32, **kw) -> CausalLM:
+    return build_lm(ModelConfig(**{**SIZES, **kw}), dtype=dtype, seed=5, device=device, init_std=0.2)
+
+
+def prompt_on(device: str, batch: int = 1) -> torch.Tensor:
+    return torch.randint(0, 300, (batch, 9), generator=torch.Generator().manual_seed(0)).to(device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_generated_tokens_are_those_of_each_steps_logits(device: str) -> None:
+    """Temperature 0 and top_k 1 are greedy decoding; any settings are ``sample`` of every step's logits."""
+    model, prompt = language_model(device), prompt_on(device, 3)
+    greedy = model.generate_greedy(prompt, 6)
+    assert torch.equal(model.generate(prompt, 6, temperature=0.0), greedy)
+    assert torch.equal(model.generate(prompt, 6, top_k=1), greedy)
+    gen = torch.Generator(device).manual_seed(7)
+    settings = dict(temperature=0.8, top_k=40, top_p=0.9, min_p=0.01)
+    got = model.generate(prompt, 6, generator=gen, **settings)
+    uniform = torch.rand(6, 3, generator=torch.Generator(device).manual_seed(7), device=device)
+    cache, ids = model.stack.new_kv_cache(15), prompt
+    with torch.no_grad():
+        for i in range(6):
+            ids = ako.sample(model.logits_last(ids, cache), uniform[i], **settings)[:, None]
+            assert torch.equal(got[:, i:i + 1], ids)
+    assert len(set(got.flatten().tolist())) > 3  # not one token over and over
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_logits_without_a_token_give_the_first(device: str, monkeypatch) -> None:
+    model = language_model(device)
+    monkeypatch.setattr(model.lm_head, "forward", lambda h: torch.full((h.shape[0], 300), float("nan"), device=h.device))
+    assert model.generate(prompt_on(device), 3).tolist() == [[0, 0, 0]]
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a GPU")
+@pytest.mark.parametrize("cache", ["static", "paged", "chosen", "chosen mx8"])
+@pytest.mark.parametrize("qk_norm", [False, True])
+def test_replayed_sampling_is_eager_sampling(cache: str, qk_norm: bool) -> None:
+    model, prompt = language_model("cuda", torch.float16, qk_norm=qk_norm), prompt_on("cuda")
+    new = {"static": lambda: None, "paged": lambda: model.stack.new_paged_cache(40, page_size=16),
+           "chosen": lambda: model.stack.new_paged_cache(40, page_size=4, count=4),
+           "chosen mx8": lambda: model.stack.new_paged_cache(40, page_size=4, count=4, quantized=True)}[cache]
+    settings = dict(temperature=0.9, top_p=0.95, top_k=100)
+    gen = lambda: torch.Generator("cuda").manual_seed(11)  # noqa: E731
+    with torch.no_grad():
+        want = model.generate(prompt, 30, generator=gen(), kv_cache=new() or model.stack.new_static_cache(39), **settings)
+        runner = GraphedSampling(model, prompt, 30, generator=gen(), cache=new(), **settings)
+        assert torch.equal(runner.run(), want)
+        with pytest.raises(RuntimeError, match="GraphedSampling"):
+            runner.run()
+    assert len(set(want.flatten().tolist())) > 5

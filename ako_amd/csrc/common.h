@@ -161,6 +161,14 @@ __device__ __forceinline__ float lane_group_sum(float v, int log2) {
   return v;
 }
 
+// 1 / sqrt(sum * inv_dim + eps), to about half a step: the instruction's result, off by up to a step, and one
+// correction r += r (1 - v r^2) / 2 with v r in two parts. 0 and infinities keep the instruction's.
+__device__ __forceinline__ float inverse_rms(float sum, float inv_dim, float eps) {
+  const float v = __builtin_fmaf(sum, inv_dim, eps), r = rsqrtf(v), h = v * r;
+  const float off = __builtin_fmaf(-h, r, 1.0f) - __builtin_fmaf(v, r, -h) * r;
+  return __builtin_fabsf(off) < 1.0f ? __builtin_fmaf(0.5f * r, off, r) : r;
+}
+
 // ---- workgroup order over the XCDs ------------------------------------------
 // Workgroups are dispatched round-robin over the 8 XCDs (workgroup b runs on
 // XCD b % 8). block_order hands each XCD runs of `chunk` consecutive blocks:

@@ -136,7 +136,7 @@ __global__ __launch_bounds__(256) void paged_write(WriteDev a) {
       weights(e0, f);
       if (LAYOUT != kInterleaved) weights(PAIR ? e0 + half : upper ? e0 - half : e0 + half, f2);
     }
-    ss = rsqrtf(lane_group_sum(ss, a.head_log2) * a.inv_dim + a.eps);
+    ss = inverse_rms(lane_group_sum(ss, a.head_log2), a.inv_dim, a.eps);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       f[i] = to_f32(own[i]) * ss * f[i];
@@ -145,6 +145,8 @@ __global__ __launch_bounds__(256) void paged_write(WriteDev a) {
   }
   const auto value = [&](int i) { return NORM ? f[i] : to_f32(own[i]); };
   const auto partner = [&](int i) { return NORM ? f2[i] : to_f32(other[i]); };
+  // a b + c d: of norms, which are not rounded before, in two roundings, as in rmsnorm_rope_qk; else in three, as in rope.
+  const auto two_products = [](float a, float b, float c, float d) { return NORM ? __builtin_fmaf(a, b, c * d) : a * b + c * d; };
 
   const TokenPlace at = token_place(a.c, token);
   int slot = 0, page = -1;
@@ -161,8 +163,8 @@ __global__ __launch_bounds__(256) void paged_write(WriteDev a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float o = value(i), p = partner(i);
-        r[i] = upper ? p * n[i] + o * c[i] : o * c[i] - p * n[i];
-        r2[i] = o * n[i] + p * c[i];
+        r[i] = upper ? two_products(p, n[i], o, c[i]) : two_products(o, c[i], -p, n[i]);
+        r2[i] = two_products(o, n[i], p, c[i]);
       }
     } else {
       float c[4], n[4];
@@ -172,8 +174,8 @@ __global__ __launch_bounds__(256) void paged_write(WriteDev a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float o = value(2 * i), p = value(2 * i + 1);
-        r[2 * i] = o * c[i] - p * n[i];
-        r[2 * i + 1] = o * n[i] + p * c[i];
+        r[2 * i] = two_products(o, c[i], -p, n[i]);
+        r[2 * i + 1] = two_products(o, n[i], p, c[i]);
       }
     }
   } else {

@@ -3,7 +3,7 @@
 //   y = (x * rsqrt(sum(x^2) / head_dim + eps)) * w      for each head, w per element
 //   (a, b) -> (a c - b n, a n + b c)                    for each rotated pair of y
 //
-// in 32 bits, each product rounded by itself, the result rounded once to the
+// in 32 bits, a rotated element in two roundings, the result rounded once to the
 // storage type: nothing is rounded between the norm and the rotation, as it is
 // where two operators follow each other.
 //
@@ -78,7 +78,7 @@ __global__ __launch_bounds__(256) void norm_rope(NormRopeDev a) {
     if (live && i >= fresh) ss = __builtin_fmaf(x0[i], x0[i], ss);
     if (live && (NEOX ? i : E + i) >= fresh) ss = __builtin_fmaf(x1[i], x1[i], ss);
   }
-  const float r = rsqrtf(lane_group_sum(ss, a.lanes_log2) * a.inv_dim + a.eps);
+  const float r = inverse_rms(lane_group_sum(ss, a.lanes_log2), a.inv_dim, a.eps);
 #pragma unroll
   for (int i = 0; i < E; ++i) {
     x0[i] = x0[i] * r * w0[i];
@@ -88,16 +88,16 @@ __global__ __launch_bounds__(256) void norm_rope(NormRopeDev a) {
   if constexpr (NEOX || E == 1) {
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      y0.e[i] = from_f32<T>(x0[i] * c[i] - x1[i] * n[i]);
-      y1.e[i] = from_f32<T>(x0[i] * n[i] + x1[i] * c[i]);
+      y0.e[i] = from_f32<T>(__builtin_fmaf(x0[i], c[i], -(x1[i] * n[i])));
+      y1.e[i] = from_f32<T>(__builtin_fmaf(x0[i], n[i], x1[i] * c[i]));
     }
   } else {
 #pragma unroll
     for (int i = 0; i < E; i += 2) {
-      y0.e[i] = from_f32<T>(x0[i] * c[i / 2] - x0[i + 1] * n[i / 2]);
-      y0.e[i + 1] = from_f32<T>(x0[i] * n[i / 2] + x0[i + 1] * c[i / 2]);
-      y1.e[i] = from_f32<T>(x1[i] * c[E / 2 + i / 2] - x1[i + 1] * n[E / 2 + i / 2]);
-      y1.e[i + 1] = from_f32<T>(x1[i] * n[E / 2 + i / 2] + x1[i + 1] * c[E / 2 + i / 2]);
+      y0.e[i] = from_f32<T>(__builtin_fmaf(x0[i], c[i / 2], -(x0[i + 1] * n[i / 2])));
+      y0.e[i + 1] = from_f32<T>(__builtin_fmaf(x0[i], n[i / 2], x0[i + 1] * c[i / 2]));
+      y1.e[i] = from_f32<T>(__builtin_fmaf(x1[i], c[E / 2 + i / 2], -(x1[i + 1] * n[E / 2 + i / 2])));
+      y1.e[i + 1] = from_f32<T>(__builtin_fmaf(x1[i], n[E / 2 + i / 2], x1[i + 1] * c[E / 2 + i / 2]));
     }
   }
   if (!live) return;

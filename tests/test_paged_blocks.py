@@ -242,7 +242,8 @@ def test_c_entries_refuse_what_they_cannot_do() -> None:
                   (dict(out=LENS), "overlap"), (dict(mstr=I3(-1, 1, 0)), "negative")):
         assert select(cache(), **kw) == INVALID and m in _native.last_error(), kw
     for kw in (dict(size=16), dict(ws=None), dict(ws=WS + 8)):
-        assert select(long, **kw) == INVALID and "workspace" in _native.last_error()
+        assert select(cache(pages=64, width=1 << 16), **kw) == INVALID and "workspace" in _native.last_error()
+    assert lib.ako_paged_select_workspace(ctypes.addressof(long), 4, 3, F16) == 0  # a tile's scores fit in LDS
     assert select(cache(kv_heads=4, width=1 << 27, page=1), ws=WS) == INVALID and "2^28" in _native.last_error()
     assert lib.ako_paged_select_workspace(ctypes.addressof(cache(kv_heads=3)), 4, 3, F16) == -1
     for kw, m in ((dict(m=None), "null"), (dict(mstr=None), "null"), (dict(mstr=I3(64, 64, 0)), "rows of the means"), (dict(m=LENS), "overlap"),

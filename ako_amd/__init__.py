@@ -6,8 +6,9 @@ benchmark-driven selector, and the gfx950 HIP kernels race the PyTorch
 baselines as ``backend="hip"`` candidates. ``rope_qk_cache`` (RoPE of q and k
 plus the KV-cache append in one launch) is an addition of this package; it
 writes the caches in place, so it is called directly rather than selected.
-So are the operations on a paged cache: ``rope_qk_paged``, ``paged_read`` and
-``paged_attention``.
+So are the operations on a paged cache, ``rope_qk_paged``, ``paged_read``,
+``paged_attention``, ``paged_means`` and ``paged_select``, and the two that have no
+candidate to race, ``rmsnorm_rope_qk`` and ``sample``.
 """
 
 __version__ = "0.1.0"

@@ -1,5 +1,8 @@
 // Attention of a step's tokens over the blocks of a paged cache that are listed for each of
 // them, on gfx950: attn_rows with BLOCKS (paged_rows.h), and how a call is cut up.
+//
+// 16 tokens of 4096 keys of 8 key heads in 8 bits, 138 MB: 40 us with the join, 3.5 TB/s. 2048 tokens, each with 1024 keys of
+// its own choosing: 420 us, 5.3 GB from L2 at 12.6 TB/s; four tokens share a tile, but hardly any blocks.
 
 #include "paged_rows.h"
 

@@ -12,7 +12,7 @@
 // lane. Bound by HBM on long prompts: 4 x 2048 tokens into e4m3 pages, 186 MB, in
 // 37.5 us, 5.0 TB/s (a copy of that size reaches 6.5); 69 MB of such pages and
 // what comes of them in 15.0, 4.6 TB/s, calls one after the other. One step's 1.6 MB is
-// launch latency: 2.8 us replayed from a graph.
+// launch latency: 2.8 us replayed from a graph. With norms 3.3, and 1464 ragged tokens into e4m3 pages 11.4.
 
 #include <algorithm>
 

@@ -10,6 +10,10 @@
 // Scores are formed in 64 bits, on the matrix cores: which of two blocks is the k-th
 // hangs on the last bits of their scores, and so it is the same for every order of the
 // sums, every batch and every division of the work up to errors of 2^-50 or so.
+//
+// 16 rows of 1024 blocks of 8 key heads take 27 us, 64 MB of means, 2.4 TB/s: single rows, by vector
+// arithmetic. 2048 rows of 512 blocks take 81: 53 for the scores, on the matrix cores at half their 64-bit
+// rate (29 us at 71 TFLOP/s), and 28 for the choice.
 
 #include <algorithm>
 #include <limits>
@@ -46,7 +50,8 @@ struct MeansDev {
 // A workgroup looks at `tile` token rows for those at the last slot of their page, and takes
 // their pages one after the other: each wavefront a quarter of the slots, a kilobyte per load and
 // eight loads in flight, added up in the order of the slots' residues and then of
-// the wavefronts. Bound by HBM where pages are many.
+// the wavefronts. Bound by HBM where pages are many: 69 MB of bfloat16 pages in 17.1 us, 4.0 TB/s (a wavefront
+// to a page took 48).
 template <typename T, bool MX>
 __global__ __launch_bounds__(256) void paged_means(MeansDev a) {
   __shared__ float part[4][kWave][9];  // 9: lanes' rows on different banks
@@ -135,7 +140,7 @@ typedef double f64x4 __attribute__((ext_vector_type(4)));
 // Up to 16 token rows by 16 blocks per wavefront and step. The matrix instruction takes four elements of
 // the inner dimension from the four groups of 16 lanes; which four is only a name, so group g
 // holds packet 4 i + g of a row in its i-th 16 bytes, and a load takes 64 bytes in a row of each of 16 means. (With a quarter of the row
-// in each group, a load touched 64 lines, which the L1 did not hold until the eighth: 4 times as long.) The rows' sums of
+// in each group a load touched 64 lines, which the L1 did not hold until the eighth: 38 us against 31 for 16 rows of 1024 blocks.) The rows' sums of
 // queries stay in registers. Rows of a tile that belong to different sequences are
 // done one sequence after the other.
 template <typename T, int DP>

@@ -1196,7 +1196,7 @@ int64_t ako_sample_workspace(int64_t rows, int64_t vocab, int dtype) {
     fail(AKO_ERR_INVALID_ARGUMENT, "ako_sample_workspace: rows must be 0 to 2^31-1 and vocab 1 to %lld", (long long)kMaxVocab);
     return -1;
   }
-  return rows == 0 ? 0 : ako::sample_workspace(rows, vocab, dtype);
+  return rows == 0 ? 0 : ako::sample_workspace(rows, vocab);
 }
 
 int ako_sample_fwd(const void* logits, const float* uniform, const float* temperature, float temperature_all,
@@ -1218,7 +1218,7 @@ int ako_sample_fwd(const void* logits, const float* uniform, const float* temper
   if (row_stride < 0) return fail(AKO_ERR_INVALID_ARGUMENT, "%s: negative row stride", fn);
   const Span in = span_2d(logits, rows, vocab, row_stride, ako::dtype_bytes(dtype));
   const Span o = span_2d(out, 1, rows, rows, 8);
-  const int64_t need = ako::sample_workspace(rows, vocab, dtype);
+  const int64_t need = ako::sample_workspace(rows, vocab);
   if (workspace_bytes < need || (need > 0 && (!workspace || !aligned(workspace, 16))))
     return fail(AKO_ERR_INVALID_ARGUMENT, "%s: needs a 16-byte aligned workspace of %lld bytes, got %lld", fn,
                 (long long)need, (long long)workspace_bytes);

@@ -283,7 +283,7 @@ struct SampleArgs {
   void* workspace;  // sample_workspace bytes
   int dtype;
 };
-int64_t sample_workspace(int64_t rows, int64_t vocab, int dtype);
+int64_t sample_workspace(int64_t rows, int64_t vocab);
 hipError_t launch_sample(const SampleArgs& a, hipStream_t stream);
 
 }  // namespace ako

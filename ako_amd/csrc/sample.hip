@@ -908,21 +908,23 @@ __global__ __launch_bounds__(kThreads) void sample_rows(SampleDev a) {
 
 namespace {
 
-// Workgroups of a row, and tokens of each: 4096 tokens or more, as many as fill the chip with a few rows. Rows that one
-// workgroup keeps in LDS are not divided (32000 tokens in 16 bits with top_k 50: 25 us, divided 34), nor are more rows than
-// compute units. Longer rows, one workgroup a row and divided, in us (131072 tokens in 32 bits):
-//   rows            1          64         128        256
-//   no settings    65 / 21    69 / 35    75 / 51    81 / 79
-//   top_k 50       69 / 30    75 / 60    83 / 77    91 / 107
-//   top_p 0.9     110 / 42   141 / 76   151 / 100  157 / 152
-//   greedy         16 / 12    17 / 18    22 / 25    25 / 35
-// and 159 / 138 for 256 rows of mixed settings, where the undivided call takes as long as its slowest row.
+// Workgroups of a row, and tokens of each: 4096 tokens or more, as many as fill the chip with a few rows. Dividing costs
+// launches and a second look at every row, and gains where rows are long and leave compute units idle: rows of more than
+// 32768 tokens, one for every 512 tokens of a row at most, and no more than compute units. One workgroup a row and
+// divided, in us:
+//   tokens            131072, 32 bits                             50000, 16 bits         32000, 32 bits
+//   rows              1          64         128        256        1          128        1          64         256
+//   no settings      65 / 21    69 / 35    75 / 51    81 / 79    30 / 20    32 / 30    24 / 21    25 / 23    29 / 38
+//   top_k 50         69 / 30    75 / 60    83 / 77    91 / 107   34 / 29    36 / 52    27 / 30    28 / 37    32 / 65
+//   top_p 0.9       110 / 42   141 / 76   151 / 100  157 / 152   61 / 31    70 / 69    39 / 34    47 / 45    51 / 74
+//   greedy           16 / 12    17 / 18    22 / 25    25 / 35     9 / 12    10 / 16    14 / 12     9 / 13    11 / 19
+// and 159 / 138 for 256 rows of 131072 with mixed settings, where the undivided call takes as long as its slowest row.
 struct Parts {
   int parts, chunk;
 };
-Parts parts_of(int64_t rows, int64_t vocab, int dtype) {
+Parts parts_of(int64_t rows, int64_t vocab) {
   constexpr int64_t kStep = 2048;  // a multiple of the regions
-  if (vocab * dtype_bytes(dtype) <= kHeldBytes || rows > 256) return Parts{1, static_cast<int>(vocab)};
+  if (vocab <= 32768 || rows > std::min<int64_t>(256, vocab / 512)) return Parts{1, static_cast<int>(vocab)};
   const int64_t most = std::min<int64_t>(kMaxParts, std::max<int64_t>(1, 2048 / rows));
   const int64_t chunk = std::max<int64_t>(4096, ceil_div(ceil_div(vocab, most), kStep) * kStep);
   return Parts{static_cast<int>(ceil_div(vocab, chunk)), static_cast<int>(chunk)};
@@ -947,8 +949,8 @@ hipError_t launch_rows(const SampleDev& d, int64_t rows, hipStream_t stream) {
 
 }  // namespace
 
-int64_t sample_workspace(int64_t rows, int64_t vocab, int dtype) {
-  return parts_of(rows, vocab, dtype).parts > 1 ? rows * static_cast<int64_t>(sizeof(SampleSpace)) : 0;
+int64_t sample_workspace(int64_t rows, int64_t vocab) {
+  return parts_of(rows, vocab).parts > 1 ? rows * static_cast<int64_t>(sizeof(SampleSpace)) : 0;
 }
 
 hipError_t launch_sample(const SampleArgs& a, hipStream_t stream) {
@@ -964,7 +966,7 @@ hipError_t launch_sample(const SampleArgs& a, hipStream_t stream) {
   d.region_log2 = std::max(7, log2 - 11);  // at most kBins parts, of 16 lanes' packets or more
   for (int j = 0; j < 128; ++j) d.pow2[j] = std::exp2(j / 128.0);
   d.stride = a.stride;
-  const Parts p = parts_of(a.rows, a.vocab, a.dtype);
+  const Parts p = parts_of(a.rows, a.vocab);
   d.space = static_cast<unsigned char*>(a.workspace);
   d.parts = p.parts;
   d.chunk = p.chunk;

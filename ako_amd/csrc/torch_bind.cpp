@@ -643,7 +643,7 @@ at::Tensor paged_select(const at::Tensor& q, const at::Tensor& k_means, const at
   const int64_t heads = q.size(-2), kv_heads = k_means.size(1);
   if (heads % kv_heads)
     p.refuse(std::to_string(heads) + " query heads are no multiple of " + std::to_string(kv_heads) + " key heads");
-  if (first < 0 || last < 1 || count < first + last)
+  if (first < 0 || last < 1 || count - last < first)
     p.refuse("first must be at least 0, last at least 1 and count at least their sum, got " + std::to_string(first) + ", " +
              std::to_string(last) + " and " + std::to_string(count));
   const at::Tensor qv = head_view(q);

@@ -667,6 +667,8 @@ class CausalLM(nn.Module):
 
         The uniform numbers of all steps are drawn first, ``(steps, batch)``, from ``generator``
         (of the prompt's device)."""
+        if steps < 1:
+            raise ValueError(f"generation needs at least 1 step, got {steps}")
         cache = kv_cache if kv_cache is not None else self.stack.new_kv_cache(prompt.shape[1] + steps)
         uniform = torch.rand(steps, prompt.shape[0], generator=generator, device=prompt.device)
         settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)

@@ -151,6 +151,8 @@ def test_refusals() -> None:
     lm = build_lm(ModelConfig(**SIZES), dtype=torch.float32)
     with pytest.raises(ValueError, match="top_p"):
         lm.generate(torch.zeros(1, 3, dtype=torch.long), 2, top_p=1.5)
+    with pytest.raises(ValueError, match="at least 1 step"):
+        lm.generate(torch.zeros(1, 3, dtype=torch.long), 0)
     for runner in (GraphedGreedy, GraphedSampling):
         with pytest.raises(ValueError, match="at least 2 steps"):
             runner(lm, torch.zeros(1, 3, dtype=torch.long), 1)

@@ -286,3 +286,26 @@ def test_streams_and_captured_calls() -> None:
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a GPU")
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_the_token_does_not_depend_on_the_division(dtype) -> None:
+    """Rows of 40000 tokens are divided over workgroups up to 78 of them at once, and whole from 79 on."""
+    gen = torch.Generator("cuda").manual_seed(3)
+    x = (torch.randn(79, 40000, generator=gen, device="cuda") * 3).to(dtype)
+    x[::5] = x[::5].round()  # many equal ones
+    x[3, 1:] = -math.inf
+    x[4] = math.nan
+    x[5] = 1.5  # more alike than a list holds
+    u = torch.rand(79, generator=gen, device="cuda")
+    for kw in ({}, dict(temperature=0.0), dict(top_k=50), dict(top_k=5000), dict(top_p=0.9), dict(top_k=1000, top_p=0.5), dict(min_p=0.02),
+               dict(temperature=torch.linspace(0, 2, 79, device="cuda"), top_p=torch.linspace(0, 1, 79, device="cuda"),
+                    top_k=torch.arange(79, dtype=torch.int32, device="cuda") * 40)):
+        whole = ako.sample(x, u, **kw)
+        part = {k: v[:78] if torch.is_tensor(v) else v for k, v in kw.items()}
+        assert torch.equal(ako.sample(x[:78], u[:78], **part), whole[:78]), kw
+        one = {k: v[7:8] if torch.is_tensor(v) else v for k, v in kw.items()}
+        assert torch.equal(ako.sample(x[7:8], u[7:8], **one), whole[7:8]), kw
+        assert whole[4] == -1 and whole[3] == 0

@@ -41,7 +41,8 @@ def rmsnorm_rope_qk(
 
     q and k are ``(batch, seq, heads, head_dim)`` with head counts of their own, the
     weights ``(head_dim,)``, ``cos``/``sin`` the ``(seq, head_dim / 2)`` rows of the
-    positions. ``head_dim`` is even, at most 512.
+    positions. ``head_dim`` is even, at most 512. There is no backward pass: on a GPU
+    the results carry no gradient.
     """
     args = (q, k, q_weight, k_weight, cos, sin, eps, style)
     if q.is_cuda and not hip_disabled():

@@ -161,6 +161,24 @@ __device__ __forceinline__ float lane_group_sum(float v, int log2) {
   return v;
 }
 
+// The same in 64 bits.
+template <int CTRL>
+__device__ __forceinline__ double dpp_mov64(double v) {
+  const uint64_t x = __builtin_bit_cast(uint64_t, v);
+  const unsigned lo = __builtin_amdgcn_mov_dpp(static_cast<int>(static_cast<unsigned>(x)), CTRL, 0xF, 0xF, false);
+  const unsigned hi = __builtin_amdgcn_mov_dpp(static_cast<int>(x >> 32), CTRL, 0xF, 0xF, false);
+  return __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+}
+__device__ __forceinline__ double lane_group_sum(double v, int log2) {
+  if (log2 > 0) v += dpp_mov64<0xB1>(v);
+  if (log2 > 1) v += dpp_mov64<0x4E>(v);
+  if (log2 > 2) v += dpp_mov64<0x141>(v);
+  if (log2 > 3) v += dpp_mov64<0x140>(v);
+  if (log2 > 4) v += __shfl_xor(v, 16);
+  if (log2 > 5) v += __shfl_xor(v, 32);
+  return v;
+}
+
 // 1 / sqrt(sum * inv_dim + eps), to about half a step: the instruction's result, off by up to a step, and one
 // correction r += r (1 - v r^2) / 2 with v r in two parts. 0 and infinities keep the instruction's.
 __device__ __forceinline__ float inverse_rms(float sum, float inv_dim, float eps) {

@@ -15,6 +15,7 @@
 // launch latency: 2.8 us replayed from a graph. With norms 3.3, and 1464 ragged tokens into e4m3 pages 11.4.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.h"
 
@@ -77,6 +78,15 @@ __device__ __forceinline__ void put(const PagedDev& c, bool is_v, int page, int 
   }
 }
 
+// In 32 bits, with an odd last bit where any were lost: a later rounding to fewer bits then goes as from all of them.
+__device__ __forceinline__ float to_odd(double x) {
+  const float f = static_cast<float>(x);
+  const double back = f;
+  unsigned b = __builtin_bit_cast(unsigned, f);
+  if (back != x && !(b & 1)) b += __builtin_fabs(x) > __builtin_fabs(back) ? 1u : ~0u;
+  return x == x && __builtin_fabs(back) < __builtin_inf() ? __builtin_bit_cast(float, b) : f;
+}
+
 // q, k and v of a token are numbered through as heads, and a head's lanes
 // rounded up to a multiple of four for e4m3 pages, so that a 32-element block is
 // a quad of lanes and its maximum two DPP steps.
@@ -117,15 +127,20 @@ __global__ __launch_bounds__(256) void paged_write(WriteDev a) {
     if (LAYOUT == kOwnNeox && !is_v) other = load_eight<T>(x + (upper ? e0 - half : e0 + half));
   }
 
-  // NORM: the factors of the lane's own elements and of their partners.
-  [[maybe_unused]] float f[8], f2[8];
+  // NORM: the lane's own elements, normed, and their partners. EXACT: which 8-bit value a key is rounded to, and at
+  // times its block's scale, hangs on last bits, so normed keys are formed in 64 bits, and in 32 bits only the last
+  // bit stands for all behind it (1464 ragged tokens: 11.4 us in 32 bits throughout, where some three of 1.5 million stored keys were the neighbours of the
+  // formula's).
+  constexpr bool EXACT = NORM && MX;
+  [[maybe_unused]] float f[8], f2[8], w1[8], w2[8];
+  [[maybe_unused]] double inverse = 0.0;
   if constexpr (NORM) {
-    float ss = 0.0f;
+    std::conditional_t<EXACT, double, float> ss = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float o = to_f32(own[i]), p = to_f32(other[i]);
-      ss = __builtin_fmaf(o, o, ss);
-      if (PAIR) ss = __builtin_fmaf(p, p, ss);
+      const decltype(ss) o = to_f32(own[i]), p = to_f32(other[i]);
+      ss = __builtin_elementwise_fma(o, o, ss);
+      if (PAIR) ss = __builtin_elementwise_fma(p, p, ss);
     }
     const auto weights = [&](int e, float (&w)[8]) {
       const void* const base = is_q ? a.qw : a.kw;
@@ -133,16 +148,25 @@ __global__ __launch_bounds__(256) void paged_write(WriteDev a) {
       else load_f32<T, 8>(static_cast<const T*>(base) + e, w);
     };
     if (live && !is_v) {
-      weights(e0, f);
-      if (LAYOUT != kInterleaved) weights(PAIR ? e0 + half : upper ? e0 - half : e0 + half, f2);
+      weights(e0, w1);
+      if (LAYOUT != kInterleaved) weights(PAIR ? e0 + half : upper ? e0 - half : e0 + half, w2);
     }
-    ss = inverse_rms(lane_group_sum(ss, a.head_log2), a.inv_dim, a.eps);
+    ss = lane_group_sum(ss, a.head_log2);
+    float r;
+    if constexpr (EXACT) {
+      inverse = 1.0 / sqrt(ss / a.head_dim + a.eps);
+      r = static_cast<float>(inverse);
+    } else {
+      r = inverse_rms(ss, a.inv_dim, a.eps);
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      f[i] = to_f32(own[i]) * ss * f[i];
-      f2[i] = to_f32(other[i]) * ss * f2[i];
+      f[i] = to_f32(own[i]) * r * w1[i];
+      f2[i] = to_f32(other[i]) * r * w2[i];
     }
   }
+  [[maybe_unused]] const auto exact = [&](int i) { return to_f32(own[i]) * inverse * w1[i]; };
+  [[maybe_unused]] const auto exact_partner = [&](int i) { return to_f32(other[i]) * inverse * w2[i]; };
   const auto value = [&](int i) { return NORM ? f[i] : to_f32(own[i]); };
   const auto partner = [&](int i) { return NORM ? f2[i] : to_f32(other[i]); };
   // a b + c d: of norms, which are not rounded before, in two roundings, as in rmsnorm_rope_qk; else in three, as in rope.
@@ -166,6 +190,16 @@ __global__ __launch_bounds__(256) void paged_write(WriteDev a) {
         r[i] = upper ? two_products(p, n[i], o, c[i]) : two_products(o, c[i], -p, n[i]);
         r2[i] = two_products(o, n[i], p, c[i]);
       }
+      if constexpr (EXACT) {
+        if (!is_q) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const double o = exact(i), p = exact_partner(i);
+            r[i] = to_odd(upper ? p * n[i] + o * c[i] : o * c[i] - p * n[i]);
+            r2[i] = to_odd(o * n[i] + p * c[i]);
+          }
+        }
+      }
     } else {
       float c[4], n[4];
       const int64_t row = at.pos * a.st + e0 / 2;
@@ -176,6 +210,16 @@ __global__ __launch_bounds__(256) void paged_write(WriteDev a) {
         const float o = value(2 * i), p = value(2 * i + 1);
         r[2 * i] = two_products(o, c[i], -p, n[i]);
         r[2 * i + 1] = two_products(o, n[i], p, c[i]);
+      }
+      if constexpr (EXACT) {
+        if (!is_q) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const double o = exact(2 * i), p = exact(2 * i + 1);
+            r[2 * i] = to_odd(o * c[i] - p * n[i]);
+            r[2 * i + 1] = to_odd(o * n[i] + p * c[i]);
+          }
+        }
       }
     }
   } else {

@@ -12,7 +12,7 @@
 // lane. Bound by HBM on long prompts: 4 x 2048 tokens into e4m3 pages, 186 MB, in
 // 37.5 us, 5.0 TB/s (a copy of that size reaches 6.5); 69 MB of such pages and
 // what comes of them in 15.0, 4.6 TB/s, calls one after the other. One step's 1.6 MB is
-// launch latency: 2.8 us replayed from a graph. With norms 3.3, and 1464 ragged tokens into e4m3 pages 11.4.
+// launch latency: 2.8 us replayed from a graph. With norms 3.3, and 1464 ragged tokens into e4m3 pages 15.6.
 
 #include <algorithm>
 #include <type_traits>
@@ -50,6 +50,7 @@ struct WriteDev {
   const void* kw;
   int w_f32, head_log2;           // 2^head_log2 lanes per head
   float eps, inv_dim;
+  double inv_dim64;
 };
 
 // Eight values of a row of the key or value pages; for e4m3 also their block's
@@ -129,7 +130,7 @@ __global__ __launch_bounds__(256) void paged_write(WriteDev a) {
 
   // NORM: the lane's own elements, normed, and their partners. EXACT: which 8-bit value a key is rounded to, and at
   // times its block's scale, hangs on last bits, so normed keys are formed in 64 bits, and in 32 bits only the last
-  // bit stands for all behind it (1464 ragged tokens: 11.4 us in 32 bits throughout, where some three of 1.5 million stored keys were the neighbours of the
+  // bit stands for all behind it (1464 ragged tokens: 15.6 us, and 11.4 in 32 bits throughout, where some three of 1.5 million stored keys were the neighbours of the
   // formula's).
   constexpr bool EXACT = NORM && MX;
   [[maybe_unused]] float f[8], f2[8], w1[8], w2[8];
@@ -154,7 +155,10 @@ __global__ __launch_bounds__(256) void paged_write(WriteDev a) {
     ss = lane_group_sum(ss, a.head_log2);
     float r;
     if constexpr (EXACT) {
-      inverse = 1.0 / sqrt(ss / a.head_dim + a.eps);
+      // From 23 bits to 45 in one step; sums whose root 32 bits do not hold take the long way.
+      const double v = __builtin_fma(ss, a.inv_dim64, static_cast<double>(a.eps)), y = rsqrtf(static_cast<float>(v));
+      const double off = __builtin_fma(-v * y, y, 1.0);
+      inverse = __builtin_fabs(off) < 0x1p-16 ? __builtin_fma(0.5 * y, off, y) : 1.0 / sqrt(v);
       r = static_cast<float>(inverse);
     } else {
       r = inverse_rms(ss, a.inv_dim, a.eps);
@@ -343,6 +347,7 @@ hipError_t run_write(const PagedWriteArgs& a, hipStream_t stream) {
     d.w_f32 = a.w_dtype == kF32;
     d.eps = a.eps;
     d.inv_dim = 1.0f / static_cast<float>(d.head_dim);
+    d.inv_dim64 = 1.0 / d.head_dim;
   }
   d.lanes = (d.q_heads + 2 * d.kv_heads) * d.per_head;
   const int block = block_size(d.lanes);

@@ -32,6 +32,7 @@
 
 #include "common.h"
 #include "launch.h"
+#include "row_rounds.h"
 
 namespace ako {
 
@@ -144,7 +145,6 @@ __device__ __forceinline__ int bin_of(const SampleRow& r, float x) {
 
 // The row in packets of 16 bytes, read again for every pass or (HELD) kept in LDS after the
 // first. What is left behind the last whole packet comes as packets of one element, in a round of its own.
-constexpr int kHeldBytes = 1 << 16;
 template <typename T, bool HELD, int THREADS = kThreads>
 struct Row {
   static constexpr int E = 16 / static_cast<int>(sizeof(T));
@@ -154,12 +154,10 @@ struct Row {
   P* held;          // HELD: round k's packets from place k * THREADS on
 
   __device__ __forceinline__ Row(const T* row, int vocab, P* lds) : x(row), whole(vocab / E), rest(vocab % E), held(lds) {}
-  __device__ __forceinline__ int rounds() const { return (whole + THREADS - 1) / THREADS + (rest > 0); }
-  // The index of the first element of this thread's packet; in the round behind the whole packets that of its only one.
+  __device__ __forceinline__ int rounds() const { return rounds_of(whole, rest, THREADS); }
+  // The index of the first element of this thread's packet.
   __device__ __forceinline__ int index(int round) const {
-    const int i = round * THREADS + static_cast<int>(threadIdx.x);
-    if (rest == 0 || round + 1 < rounds()) return i * E;
-    return whole * E + (static_cast<int>(threadIdx.x) < rest ? static_cast<int>(threadIdx.x) : 0);
+    return index_in_round<E>(whole, rest, THREADS, round, static_cast<int>(threadIdx.x));
   }
   // -infinity behind the end.
   __device__ __forceinline__ P packet(int round) const {
@@ -179,40 +177,20 @@ struct Row {
   template <typename F>
   __device__ __forceinline__ void each_packet(F f) const {
     constexpr int kAtOnce = HELD ? 4 : 16 / E;
-    const int n = rounds();
-#pragma unroll 1
-    for (int k0 = 0; k0 < n; k0 += kAtOnce) {
-      P p[kAtOnce];
-#pragma unroll
-      for (int u = 0; u < kAtOnce; ++u) {
-        if (HELD) p[u] = held[(k0 + u) * THREADS + threadIdx.x];
-        else if (k0 + u < n) p[u] = packet(k0 + u);
-      }
-#pragma unroll
-      for (int u = 0; u < kAtOnce; ++u) {
-        if (k0 + u >= n) break;
-        f(p[u], index(k0 + u));
-      }
-    }
+    P p[kAtOnce];
+    in_groups<kAtOnce, HELD>(rounds(), [&](int u, int k) { p[u] = HELD ? held[k * THREADS + threadIdx.x] : packet(k); },
+                             [&](int u, int k) { f(p[u], index(k)); });
   }
   // The same for the first pass, from memory: four rounds at a time.
   template <typename F>
   __device__ __forceinline__ void first_pass(F f) const {
-    const int n = rounds();
-#pragma unroll 1
-    for (int k0 = 0; k0 < n; k0 += 4) {
-      P p[4];
+    P p[4];
+    in_groups<4, false>(rounds(), [&](int u, int k) { p[u] = packet(k); },
+                        [&](int u, int k) {
+                          if (HELD) held[k * THREADS + threadIdx.x] = p[u];
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (k0 + u < n) p[u] = packet(k0 + u);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (k0 + u >= n) break;
-        if (HELD) held[(k0 + u) * THREADS + threadIdx.x] = p[u];
-#pragma unroll
-        for (int e = 0; e < E; ++e) f(to_f32(p[u].e[e]), index(k0 + u) + e);
-      }
-    }
+                          for (int e = 0; e < E; ++e) f(to_f32(p[u].e[e]), index(k) + e);
+                        });
   }
   // f(element, index).
   template <typename F>
@@ -680,7 +658,7 @@ template <typename T, bool HELD, bool SPLIT>
 __global__ __launch_bounds__(kThreads) void sample_rows(SampleDev a) {
   using R = Row<T, HELD>;
   __shared__ SampleLds l;
-  __shared__ typename R::P held_row[HELD ? kHeldBytes / 16 + kThreads : 1];  // and the round behind the whole packets
+  __shared__ typename R::P held_row[HELD ? held_places(kThreads) : 1];  // and the round behind the whole packets
   const int64_t n = blockIdx.x;
   const R row(static_cast<const T*>(a.x) + n * a.stride, a.vocab, held_row);
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;

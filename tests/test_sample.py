@@ -309,3 +309,12 @@ def test_the_token_does_not_depend_on_the_division(dtype) -> None:
         one = {k: v[7:8] if torch.is_tensor(v) else v for k, v in kw.items()}
         assert torch.equal(ako.sample(x[7:8], u[7:8], **one), whole[7:8]), kw
         assert whole[4] == -1 and whole[3] == 0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype,vocab", [(torch.float16, 24577), (torch.float16, 24601), (torch.bfloat16, 32001), (torch.bfloat16, 32767),
+                                         (torch.float32, 12289), (torch.float32, 12301), (torch.float32, 16383)])
+def test_rows_of_four_rounds_and_a_rest(dtype, vocab: int, device: str) -> None:
+    """Kept in LDS with more than three rounds of packets and elements behind the last whole one."""
+    for kw in ({}, dict(top_k=5), dict(top_k=5000), dict(top_p=0.7), dict(top_k=6000, top_p=0.8), dict(min_p=0.01)):
+        check(*rows(5, vocab, dtype, device, vocab), **kw)

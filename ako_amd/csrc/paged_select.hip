@@ -19,6 +19,7 @@
 #include <limits>
 
 #include "paged.h"
+#include "select_rule.h"
 
 namespace ako {
 
@@ -498,8 +499,8 @@ __global__ __launch_bounds__(WAVES* kWave, DP <= 128 ? (SCORES > 8192 ? WAVES / 
   }
 }
 
-// Workgroups of a launch, at most, for a call of many rows: work-items stay below 2^32.
-constexpr int64_t kSlice = int64_t(1) << 22;
+// Workgroups of 256 of a launch, at most, for a call of many rows.
+constexpr int64_t kSlice = slice_groups(256);
 
 hipError_t launch_paged_means(const PagedMeansArgs& a, hipStream_t stream) {
   MeansDev d{};
@@ -559,14 +560,13 @@ int64_t slice_rows(const PagedSelectArgs& a) {
 
 template <typename T, int DP>
 void launch_tile_dim(const SelectDev& d, bool few, dim3 grid, hipStream_t stream) {
-  // Few workgroups, each of a whole row: 16 wavefronts to have more of it in flight, where the registers allow.
-  constexpr int kOneWaves = DP <= 128 ? 16 : 8;
+  constexpr int kOneWaves = tile_threads(DP, true) / kWave, kTileWaves = tile_threads(DP, false) / kWave;
   if (d.tile == 1) {
     if (few) AKO_LAUNCH((select_tile<T, DP, kFewScores, kOneWaves, true>), grid, dim3(kOneWaves * kWave), 0, stream, d);
     else AKO_LAUNCH((select_tile<T, DP, kMostScores, kOneWaves, true>), grid, dim3(kOneWaves * kWave), 0, stream, d);
   } else {
-    if (few) AKO_LAUNCH((select_tile<T, DP, kFewScores, 8, false>), grid, dim3(8 * kWave), 0, stream, d);
-    else AKO_LAUNCH((select_tile<T, DP, kMostScores, 8, false>), grid, dim3(8 * kWave), 0, stream, d);
+    if (few) AKO_LAUNCH((select_tile<T, DP, kFewScores, kTileWaves, false>), grid, dim3(kTileWaves * kWave), 0, stream, d);
+    else AKO_LAUNCH((select_tile<T, DP, kMostScores, kTileWaves, false>), grid, dim3(kTileWaves * kWave), 0, stream, d);
   }
 }
 template <typename T>
@@ -612,7 +612,7 @@ hipError_t launch_paged_select(const PagedSelectArgs& a, hipStream_t stream) {
   d.tile = tile_rows(a);
   const bool scored = d.width > a.count;
   if (scored && in_lds(a)) {
-    const int64_t rows = std::max<int64_t>(1, 2 * kSlice / a.c.kv_heads) * d.tile;
+    const int64_t rows = tile_slice(a.c.head_dim, d.tile, a.c.kv_heads);
     const bool few = d.tile * a.c.table_width <= kFewScores;
     for (int64_t t = 0; t < a.c.tokens; t += rows) {
       d.token0 = static_cast<int>(t);

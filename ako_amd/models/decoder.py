@@ -670,7 +670,7 @@ class CausalLM(nn.Module):
         if steps < 1:
             raise ValueError(f"generation needs at least 1 step, got {steps}")
         cache = kv_cache if kv_cache is not None else self.stack.new_kv_cache(prompt.shape[1] + steps)
-        uniform = torch.rand(steps, prompt.shape[0], generator=generator, device=prompt.device)
+        uniform = torch.rand(steps, prompt.shape[0], generator=generator, dtype=torch.float32, device=prompt.device)
         settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
         ids, out = prompt, []
         for u in uniform:
@@ -772,7 +772,7 @@ class GraphedSampling(GraphedGreedy):
                  top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, generator: torch.Generator | None = None,
                  cache: PagedKVCache | None = None) -> None:
         self.settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
-        self.uniform = torch.rand(steps, 1, generator=generator, device=prompt.device).view(-1)
+        self.uniform = torch.rand(steps, 1, generator=generator, dtype=torch.float32, device=prompt.device).view(-1)
         super().__init__(model, prompt, steps, cache=cache)
 
     def _choose(self, logits: torch.Tensor) -> None:

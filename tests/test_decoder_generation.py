@@ -210,3 +210,29 @@ def test_replayed_sampling_is_eager_sampling(cache: str, qk_norm: bool) -> None:
         with pytest.raises(RuntimeError, match="GraphedSampling"):
             runner.run()
     assert len(set(want.flatten().tolist())) > 5
+
+
+@pytest.fixture
+def half_by_default():
+    """A program whose new tensors are float16 unless it says otherwise, as for building its model."""
+    torch.set_default_dtype(torch.float16)
+    yield
+    torch.set_default_dtype(torch.float32)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_drawing_does_not_hang_on_the_default_type(device: str, half_by_default) -> None:
+    model, prompt = language_model(device), prompt_on(device, 2)
+    got = model.generate(prompt, 3, generator=torch.Generator(device).manual_seed(7))
+    torch.set_default_dtype(torch.float32)
+    assert torch.equal(got, model.generate(prompt, 3, generator=torch.Generator(device).manual_seed(7)))
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a GPU")
+def test_replayed_drawing_does_not_hang_on_the_default_type(half_by_default) -> None:
+    model, prompt = language_model("cuda", torch.float16), prompt_on("cuda")
+    with torch.no_grad():
+        got = GraphedSampling(model, prompt, 4, generator=torch.Generator("cuda").manual_seed(7)).run()
+        torch.set_default_dtype(torch.float32)
+        assert torch.equal(got, GraphedSampling(model, prompt, 4, generator=torch.Generator("cuda").manual_seed(7)).run())

@@ -100,8 +100,8 @@ def sample_ref(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) 
     rows, vocab = logits.shape
 
     def column(v, dtype=torch.float32):
-        if not torch.is_tensor(v):
-            v = torch.full((rows,), min(v, 2**31 - 1) if dtype != torch.float32 else v, dtype=dtype, device=logits.device)
+        if not torch.is_tensor(v):  # numbers past float32's largest are infinite, as for the kernel
+            v = torch.full((rows,), min(v, 2**31 - 1) if dtype != torch.float32 else v, dtype=torch.float64, device=logits.device).to(dtype)
         return v[:, None].double() if dtype == torch.float32 else v[:, None].long()
 
     t, k, p, low = column(temperature), column(top_k, torch.int32), column(top_p), column(min_p)

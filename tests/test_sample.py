@@ -318,3 +318,13 @@ def test_rows_of_four_rounds_and_a_rest(dtype, vocab: int, device: str) -> None:
     """Kept in LDS with more than three rounds of packets and elements behind the last whole one."""
     for kw in ({}, dict(top_k=5), dict(top_k=5000), dict(top_p=0.7), dict(top_k=6000, top_p=0.8), dict(min_p=0.01)):
         check(*rows(5, vocab, dtype, device, vocab), **kw)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_numbers_that_float32_does_not_hold(device: str) -> None:
+    """They are rounded to it: past its largest to infinity, next to 0 and 1 to those."""
+    x, u = rows(6, 500, torch.float32, device, 12)
+    assert torch.equal(ako.sample(x, u, temperature=1e39), ako.sample(x, u, temperature=math.inf))
+    assert torch.equal(ako.sample(x, u, temperature=1e-50), ako.sample(x, u, temperature=0.0))
+    assert torch.equal(ako.sample(x, u, top_p=1 - 1e-12, min_p=1e-60), ako.sample(x, u))
+    assert torch.equal(ako.sample(x, u, top_k=10 ** 30), ako.sample(x, u))

@@ -11,6 +11,7 @@ on a GPU it runs the HIP kernel (and raises if the library cannot be loaded, unl
 from __future__ import annotations
 
 import ctypes
+import warnings
 
 import torch
 
@@ -42,10 +43,13 @@ def rmsnorm_rope_qk(
     q and k are ``(batch, seq, heads, head_dim)`` with head counts of their own, the
     weights ``(head_dim,)``, ``cos``/``sin`` the ``(seq, head_dim / 2)`` rows of the
     positions. ``head_dim`` is even, at most 512. There is no backward pass: on a GPU
-    the results carry no gradient.
+    the results carry no gradient, with a warning where one could be expected of them.
     """
     args = (q, k, q_weight, k_weight, cos, sin, eps, style)
     if q.is_cuda and not hip_disabled():
+        if torch.is_grad_enabled() and any(t.requires_grad for t in args[:4]):
+            warnings.warn("rmsnorm_rope_qk has no backward pass on a GPU: no gradient goes from its results to q, k "
+                          "or the weights; call it under torch.no_grad() where none is wanted", stacklevel=2)
         return rmsnorm_rope_qk_hip(*args)
     return rmsnorm_rope_qk_ref(*args)
 

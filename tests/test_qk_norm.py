@@ -303,3 +303,49 @@ def test_captured_steps_follow_the_lengths() -> None:
             page, slot = int(s.table[i, p // 4]), p % 4
             assert torch.equal(s.k_pages[page, :, slot], pages[page, :, slot])
         s.k_pages.copy_(pages)
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a GPU")
+@pytest.mark.parametrize("which", range(4))
+def test_gradients_that_are_not_formed_are_told_of(which: int) -> None:
+    """The results are the same and carry no gradient; nothing is said where none can be expected."""
+    import warnings
+
+    args = [*inputs(1, 3, 2, 1, 32, torch.float32, "cuda"), *tables(3, 32, "cuda")]
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        want = ako.rmsnorm_rope_qk(*args)
+        args[which] = args[which].detach().requires_grad_()
+        with torch.no_grad():
+            ako.rmsnorm_rope_qk(*args)
+    with pytest.warns(UserWarning, match="no backward pass"):
+        got = ako.rmsnorm_rope_qk(*args)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b) and not a.requires_grad
+
+
+def test_gradients_on_a_cpu_are_the_formulas() -> None:
+    import warnings
+
+    args = [*inputs(1, 2, 2, 1, 8, torch.float32, "cpu"), *tables(2, 8)]
+    args[:4] = [t.double().requires_grad_() for t in args[:4]]
+
+    def turned(q, k, qw, kw):
+        out = []
+        for x, w in ((q, qw), (k, kw)):
+            y = x / (x.square().mean(-1, keepdim=True) + EPS).sqrt() * w
+            a, b = y.chunk(2, -1)
+            c, n = (t.double()[:, None] for t in args[4:])
+            out.append(torch.cat((a * c - b * n, a * n + b * c), -1))
+        return out
+
+    seeds = [torch.randn(t.shape, generator=torch.Generator().manual_seed(i), dtype=torch.float64) for i, t in enumerate(args[:2])]
+    want = torch.autograd.grad(turned(*args[:4]), args[:4], seeds)
+    low = [t.detach().float().requires_grad_() for t in args[:4]]
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        got = torch.autograd.grad(ako.rmsnorm_rope_qk(*low, *args[4:]), low, [s.float() for s in seeds])
+    for a, b in zip(got, want):
+        # Sums of at most 16 products of four 32-bit factors, each of some size around 1: 16 * 8 half steps.
+        assert (a.double() - b).abs().max() <= 128 * 2.0 ** -24 * max(1.0, b.abs().max().item())

@@ -469,7 +469,15 @@ __device__ __forceinline__ Row<T, false, THREADS> part_of_row(const SampleDev& a
   return Row<T, false, THREADS>(static_cast<const T*>(a.x) + n * a.stride + start, min(a.chunk, a.vocab - start), nullptr);
 }
 
-// The largest logit, the first that has it and the least that is not ruled out, over the lanes of a wavefront.
+// The largest logit, the first that has it and the least that is not ruled out, with one more logit. By comparisons, which
+// no NaN passes: a maximum with a signalling NaN is NaN, and one of 16 bits arrives here as it was.
+__device__ __forceinline__ void look_at(SampleFound& f, float x, int i) {
+  f.at = x > f.top ? i : f.at;
+  f.top = x > f.top ? x : f.top;
+  f.low = x < f.low && x > -__builtin_inff() ? x : f.low;
+}
+
+// The same over the lanes of a wavefront.
 __device__ __forceinline__ void join_found(SampleFound& f) {
 #pragma unroll
   for (int k = 1; k < kWave; k *= 2) {
@@ -498,9 +506,7 @@ __global__ __launch_bounds__(kPartThreads) void sample_top(SampleDev a) {
   if (part == 0 && threadIdx.x == 0) space->n = 0;
   SampleFound f{-__builtin_inff(), __builtin_inff(), a.vocab};
   part_of_row<T, kPartThreads>(a, n, start).first_pass([&](float x, int i) {
-    f.at = x > f.top ? start + i : f.at;
-    f.top = __builtin_fmaxf(f.top, x);
-    f.low = __builtin_fminf(f.low, x > -__builtin_inff() ? x : __builtin_inff());
+    look_at(f, x, start + i);
   });
   join_found(f);
   if (threadIdx.x % kWave == 0) waves[threadIdx.x / kWave] = f;
@@ -677,12 +683,8 @@ __global__ __launch_bounds__(kThreads) void sample_rows(SampleDev a) {
     low = f.low;
     at = f.at;
   } else {
-    row.first_pass([&](float x, int i) {
-      at = x > top ? i : at;
-      top = __builtin_fmaxf(top, x);
-      low = __builtin_fminf(low, x > -__builtin_inff() ? x : __builtin_inff());
-    });
     SampleFound f{top, low, at};
+    row.first_pass([&](float x, int i) { look_at(f, x, i); });
     join_found(f);
     if (lane == 0) l.found[wave] = f;
     __syncthreads();

@@ -328,3 +328,25 @@ def test_numbers_that_float32_does_not_hold(device: str) -> None:
     assert torch.equal(ako.sample(x, u, temperature=1e-50), ako.sample(x, u, temperature=0.0))
     assert torch.equal(ako.sample(x, u, top_p=1 - 1e-12, min_p=1e-60), ako.sample(x, u))
     assert torch.equal(ako.sample(x, u, top_k=10 ** 30), ako.sample(x, u))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_signalling_nan_is_ruled_out_too(dtype, device: str) -> None:
+    """NaN of either sign whose first mantissa bit is clear, in rows in LDS, whole in memory and divided."""
+    bits, quiet = {torch.float32: (torch.int32, 0x400000), torch.float16: (torch.int16, 0x200), torch.bfloat16: (torch.int16, 0x40)}[dtype]
+    inf = torch.tensor([math.inf, -math.inf], dtype=dtype).view(bits)
+    for n, v in ((6, 50), (6, 5000), (6, 70000), (100, 33000)):
+        x, u = rows(n, v, dtype, "cpu", v)
+        raw, clean = x.clone().view(bits), x.clone()
+        for k in range(2):
+            at = torch.randint(0, v, (v // 7,), generator=torch.Generator().manual_seed(k))
+            raw[:, at], clean[:, at] = inf[k] + 1, -math.inf
+        raw[4], clean[4] = inf[0] + 1, -math.inf
+        raw[5], clean[5] = inf[1] + quiet - 1, -math.inf
+        raw[5, 3], clean[5, 3] = x.view(bits)[5, 3], x[5, 3]
+        y = raw.view(dtype).to(device)
+        assert torch.equal(y.cpu().view(bits), raw)
+        for kw in ({}, dict(temperature=0.0), dict(top_k=7), dict(top_p=0.5), dict(top_k=30, top_p=0.9, min_p=0.01)):
+            got = ako.sample(y, u.to(device), **kw)
+            assert torch.equal(got, ako.sample(clean.to(device), u.to(device), **kw)) and got[4:6].tolist() == [-1, 3]

@@ -700,6 +700,9 @@ __global__ __launch_bounds__(WAVES* kWave, DP * sizeof(T) <= 128 && !MX ? 3 : DP
       for (int d = 0; d < DP / 16; ++d) o[d] *= keep;
       m = mn;
     }
+    // The second product takes the weights in the rows' type, as its matrix instruction does: each is rounded once, by up to
+    // half a step of that type, as the output is after it. 2048 tokens of 1024 listed keys in bfloat16 are 1.72e-3 of
+    // their size from 64 bits, with 32-bit weights 1.68e-3. The weights' own sum takes them in 32 bits.
     const float from = base - Mfma<T>::kShift;
     Pack<T, E> p;
     float pf[NB][4];

@@ -8,8 +8,9 @@
 // heads. Of equal scores the lowest block comes first.
 //
 // Scores are formed in 64 bits, on the matrix cores: which of two blocks is the k-th
-// hangs on the last bits of their scores, and so it is the same for every order of the
-// sums, every batch and every division of the work up to errors of 2^-50 or so.
+// hangs on the last bits of their scores. Single rows, by vector arithmetic, add up in another order than several, so
+// the choice is the same for every batch and every division of the work but where two scores are closer than some
+// 2^-50 of the size of their terms.
 //
 // 16 rows of 1024 blocks of 8 key heads take 27 us, 64 MB of means, 2.4 TB/s: single rows, by vector
 // arithmetic. 2048 rows of 512 blocks take 81: 53 for the scores, on the matrix cores at half their 64-bit
@@ -547,7 +548,8 @@ int tile_rows(const PagedSelectArgs& a) {
   return tile;
 }
 
-// Whether a tile's scores stay in LDS.
+// Whether a tile's scores stay in LDS: one launch then, and no scores in memory. On either side of the border, 8 key heads of 128:
+// 2048 rows of 896 / 897 blocks take 172 / 216 us, 512 rows 46 / 100, 16 rows, a single tile, 47 / 23.
 constexpr int kFewScores = 8192, kMostScores = 14336;
 bool in_lds(const PagedSelectArgs& a) { return tile_rows(a) * a.c.table_width <= kMostScores; }
 

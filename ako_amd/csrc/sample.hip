@@ -890,8 +890,10 @@ namespace {
 
 // Workgroups of a row, and tokens of each: 4096 tokens or more, as many as fill the chip with a few rows. Dividing costs
 // launches and a second look at every row, and gains where rows are long and leave compute units idle: rows of more than
-// 32768 tokens, one for every 512 tokens of a row at most, and no more than compute units. One workgroup a row and
-// divided, in us:
+// 32768 tokens, one for every 512 tokens of a row at most, and no more than compute units. What the host knows of a call's
+// settings has no part in it. It loses where rows fill the chip and all have settings of a short chain: at the border,
+// 256 rows of 131072, with top_k 50 and for greedy rows, whose later launches have nothing to do. One workgroup a
+// row and divided, in us:
 //   tokens            131072, 32 bits                             50000, 16 bits         32000, 32 bits
 //   rows              1          64         128        256        1          128        1          64         256
 //   no settings      65 / 21    69 / 35    75 / 51    81 / 79    30 / 20    32 / 30    24 / 21    25 / 23    29 / 38

@@ -693,7 +693,8 @@ class GraphedGreedy:
     and the next step is captured. Each replay reads the token in ``ids``,
     writes the next one back into ``ids`` and into ``history``, and advances
     the device-side position, so decoding needs no host work per token
-    beyond the replay call.
+    beyond the replay call. ``steps`` is at least 2: the first token is the prefill's,
+    and the step that is captured writes the second into ``history``.
     """
 
     def __init__(self, model: "CausalLM", prompt: torch.Tensor, steps: int, *,

@@ -56,7 +56,8 @@ def rope_qk_paged(
 
     ``cos``/``sin`` hold the rows of positions 0, 1, .... With e4m3 pages
     (``k_scales``, ``v_scales``) keys and values are quantised as they are
-    written, the keys straight from the 32-bit rotation. Padding rows of the
+    written, the keys straight from the rotation, which is in 32 bits (after norms,
+    in 64 for the keys). Padding rows of the
     result are zero; a row whose position has no page, or no table row, is not
     stored and its row of the result is NaN. The rows of a step must have slots
     of their own: pages that sequences share are full ones.
@@ -133,8 +134,10 @@ def paged_select(
     A row may take the blocks up to its own. If they are more than ``count``, it takes the ``first``
     first and the ``last`` last of them, and of the others those whose mean key has the largest product with
     the sum of the queries that share the key head; of equal ones the lowest. Scores are formed in
-    64 bits, so the choice does not depend on how the work was divided. Blocks without a
-    page are not taken; padding rows take none.
+    64 bits, and the order of their sums hangs on how many rows a call has: the choice is the same for
+    every division of the work, but where two scores are closer than some 2^-50 of the size of their terms
+    (equal means have equal scores in any order, and so have sums that 64 bits hold exactly). Every call
+    repeats itself. Blocks without a page are not taken; padding rows take none.
     """
     if q.is_cuda and not hip_disabled():
         return paged_select_hip(q, k_means, block_table, seq_lens, page_size, count, first, last, cu_seqlens)

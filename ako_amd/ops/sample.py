@@ -20,8 +20,9 @@ NaN as 0 and above 1 as 1; uniform numbers below 0 or NaN count as 0, and from 1
 token kept.
 
 On a GPU this runs the HIP kernel (and raises if the library cannot be loaded,
-unless ``AKO_HIP_DISABLE=1``), on a CPU the sorts below. The token does not depend
-on the batch around a row.
+unless ``AKO_HIP_DISABLE=1``), on a CPU the sorts below. The kernel's weights are whole
+multiples of 2^-51 of the largest (2^-45 at 131072 tokens), and what is below half of that is ruled
+out; its token does not depend on the batch around a row.
 """
 
 from __future__ import annotations

@@ -362,7 +362,9 @@ int ako_paged_means_fwd(const ako_paged_t* cache, float* means, const int64_t* m
  * than count, else count of them: the first `first`, the last `last` up to its own,
  * and of the others those with the largest scores
  *   sum over the heads h that read key head `head` of q[row][h] . means[page][head],
- * of equal ones the lowest blocks (64-bit sums; NaN counts as -infinity). first >= 0,
+ * of equal ones the lowest blocks (64-bit sums, in an order that hangs on how many rows a
+ * sequence has: scores closer than some 2^-50 of the size of their terms may change places with it; NaN counts as
+ * -infinity). first >= 0,
  * last >= 1, count >= first + last. Rows that are padding get -1 only. Of the cache, the pages, scales and their
  * strides are not used and page_dtype is dtype, that of q. workspace
  * holds ako_paged_select_workspace bytes, 16-byte aligned, that nothing else uses until the

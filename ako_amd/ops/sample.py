@@ -120,6 +120,7 @@ def sample_ref(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) 
     before = wo.cumsum(-1) - wo
     keep = (before < p * wo.sum(-1, keepdim=True)) | ~(p < 1)
     keep &= (wo >= low.clamp(max=1.0)) | ~(low > 0)
+    keep &= ~(low >= 1) | (torch.gather(x, 1, index) == top)  # next to the largest weights round to 1
     keep = torch.where(draw, (keep & (wo > 0)) | (rank == 0), rank == 0)
     kept = torch.zeros_like(w).scatter_(1, index, torch.where(keep, wo, 0.0))
     upto = kept.cumsum(-1)

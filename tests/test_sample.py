@@ -350,3 +350,15 @@ def test_signalling_nan_is_ruled_out_too(dtype, device: str) -> None:
         for kw in ({}, dict(temperature=0.0), dict(top_k=7), dict(top_p=0.5), dict(top_k=30, top_p=0.9, min_p=0.01)):
             got = ako.sample(y, u.to(device), **kw)
             assert torch.equal(got, ako.sample(clean.to(device), u.to(device), **kw)) and got[4:6].tolist() == [-1, 3]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_min_p_of_one_keeps_the_largest_alone(dtype, device: str) -> None:
+    """Also of logits so close that their weights are 1 in 64 bits."""
+    least = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    x = torch.arange(40, dtype=torch.float64).mul(least).to(dtype).flip(0).roll(7).expand(5, -1).contiguous().to(device)
+    x[:, 20] = x[:, 7]  # and one more like the largest
+    u = torch.tensor([0.0, 0.3, 0.499, 0.501, 0.999], device=device)
+    for kw in (dict(min_p=1.0), dict(min_p=torch.ones(5, device=device)), dict(min_p=1.0, top_p=0.9), dict(min_p=1.0, temperature=30.0)):
+        assert ako.sample(x, u, **kw).tolist() == [7, 7, 7, 20, 20]
